@@ -212,6 +212,159 @@ int nut_kv_read_positions(const nut_kvcache *kv, size_t begin, size_t end,
 int nut_kv_write_positions(nut_kvcache *kv, size_t begin, size_t end,
                            const float *keys, const float *values);
 
+/* ----------------------------------------------------- paged KV cache -- */
+
+/* A cache of one layer's K and V rows for several sequences at once, in
+ * pages of page_size rows that the caller hands out (no reference
+ * counterpart: KVCache holds one sequence, contiguously). The memory is the
+ * caller's; these structs are views of it. Nothing here allocates, every
+ * call only launches kernels on `stream` (so it can be captured into a
+ * graph), and every workspace is the caller's: calls that may run at the
+ * same time, or graphs that may be replayed at the same time, need
+ * workspaces of their own. Device pointers are the device's that
+ * nut_set_device selected.
+ *
+ * Arguments that the host sees are checked (NUT_EINVAL). What only the
+ * device sees is checked in the kernels: a page outside [0, pages), or a
+ * sequence longer than max_length, is not read or written; it sets a bit of
+ * *d_status, which nut_paged_check turns into NUT_EOUTOFRANGE. */
+enum { NUT_F32 = 0, NUT_F16 = 1, NUT_BF16 = 2 };
+
+typedef struct nut_paged_kv {
+    /* Row `slot` of page p for KV head h starts at element
+     * p page_stride + h head_stride + slot slot_stride of both. Strides of 0,
+     * 0, 0 mean packed, [pages][kv_heads][page_size][head_dim]. Rows must
+     * start at multiples of 16 bytes and must not overlap. */
+    void *d_keys, *d_values;
+    /* [pages][kv_heads][2][head_dim] of `type`, packed: the smallest, then
+     * the largest component of a page's keys. NULL: none are kept, and
+     * nut_paged_select refuses the view. */
+    void *d_bounds;
+    size_t pages, page_size, kv_heads;
+    size_t head_dim; /* a multiple of 8, up to 256 */
+    size_t page_stride, head_stride, slot_stride;
+    int type;      /* NUT_F32, NUT_F16 or NUT_BF16 */
+    int *d_status; /* one word, zeroed by the caller once; NULL: none */
+} nut_paged_kv;
+
+/* The sequences of a call: sequence b holds d_lengths[b] rows (0 to
+ * max_length), row i in page d_pages[b table_stride + i / page_size], slot
+ * i % page_size. Sequences may share pages that are only read. */
+typedef struct nut_paged_batch {
+    const int *d_pages;
+    size_t table_stride; /* table_stride page_size >= max_length */
+    const int *d_lengths;
+    size_t batch, max_length;
+} nut_paged_batch;
+
+/* What eviction goes by, [batch][kv_heads][stride] each: the attention
+ * weight that a row has gathered, and the position that its token had in
+ * the text. stride >= max_length. */
+typedef struct nut_paged_history {
+    float *d_weights;
+    int *d_positions;
+    size_t stride;
+} nut_paged_history;
+
+/* Puts new rows behind the rows that the sequences hold. d_keys and d_values
+ * hold `rows` fp32 rows: row r's head h at element r row_stride +
+ * h head_stride (multiples of 4; 0, 0: packed [rows][kv_heads][head_dim]).
+ * Sequence b gets rows d_starts[b] to d_starts[b + 1] (at most max_new;
+ * source rows that no sequence names are left out), or one row, row b, where
+ * d_starts is NULL. Rows are rounded to the cache's type (to nearest, ties
+ * to even), the page bounds widened, and where history is given the rows'
+ * weights set to 0 and their positions to d_first_positions[b] onwards (NULL:
+ * d_lengths[b] onwards). d_new_lengths (may be NULL, must not be d_lengths)
+ * gets the lengths with the new rows; max_length is the most that it may
+ * say. A sequence that would pass max_length gets no row and keeps its
+ * length. No two sequences may append to one page. */
+int nut_paged_append(const nut_paged_kv *kv, const nut_paged_batch *seqs,
+                     const float *d_keys, const float *d_values, size_t rows,
+                     size_t row_stride, size_t head_stride,
+                     const int *d_starts, size_t max_new,
+                     const nut_paged_history *history,
+                     const int *d_first_positions, int *d_new_lengths,
+                     void *stream);
+/* nut_paged_append from a nut_kvcache, such as nut_prefill leaves: its rows
+ * [begin, end) of `layer` go behind the one sequence of `seqs`. */
+int nut_paged_append_cache(const nut_paged_kv *kv,
+                           const nut_paged_batch *seqs,
+                           const nut_kvcache *source, size_t layer,
+                           size_t begin, size_t end,
+                           const nut_paged_history *history,
+                           const int *d_first_positions, int *d_new_lengths,
+                           void *stream);
+
+/* Attention of one new token a sequence: for every head h of `heads` (a
+ * multiple of kv_heads; head h reads KV head h / (heads / kv_heads)),
+ * out = softmax(scale q . k) v over the sequence's rows, fp32
+ * [batch][heads][head_dim]; query rows of a sequence at d_query +
+ * b query_stride (0: packed; a multiple of 4). d_lse (may be NULL) gets the
+ * log of each softmax's denominator, [batch][heads]. A sequence without rows,
+ * or a head whose scores are all minus infinity, gets zeros and minus
+ * infinity.
+ *
+ * history (may be NULL): every row's weight grows by its attention weight,
+ * summed over the heads that share its KV head; the positions are not read.
+ *
+ * d_selected (may be NULL): [batch][kv_heads][top], only the rows of these
+ * pages of the sequence's table are read (indexes into its table row, as
+ * nut_paged_select writes them; -1 for none, and one behind the sequence's
+ * rows has no row; a page named twice counts twice). Not together with
+ * history.
+ *
+ * The workspace (16-byte aligned) needs nut_paged_attention_workspace bytes,
+ * top = 0 standing for no selection; (size_t)-1 for arguments that the call
+ * would refuse. */
+size_t nut_paged_attention_workspace(const nut_paged_kv *kv,
+                                     const nut_paged_batch *seqs,
+                                     size_t heads, size_t top, int weighted);
+int nut_paged_attention(const nut_paged_kv *kv, const nut_paged_batch *seqs,
+                        const float *d_query, size_t query_stride,
+                        size_t heads, float scale, const int *d_selected,
+                        size_t top, const nut_paged_history *history,
+                        float *d_out, float *d_lse, void *d_workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* Chooses the pages that a new token's attention reads: for each sequence
+ * and KV head the `first` first and the `last` last pages and the best others,
+ * `top` in all (first + last <= top), in ascending order, then -1. A page's
+ * score is the largest, over the heads that share the KV head, of
+ * sum_d max(q_d lo_d, q_d hi_d): no row of the page has a larger q . k. Sums
+ * in 64 bits, ties to the lower page; a score that is not a number ranks
+ * first. The workspace (16-byte aligned) needs nut_paged_select_workspace
+ * bytes. */
+size_t nut_paged_select_workspace(const nut_paged_kv *kv,
+                                  const nut_paged_batch *seqs, size_t heads,
+                                  size_t top);
+int nut_paged_select(const nut_paged_kv *kv, const nut_paged_batch *seqs,
+                     const float *d_query, size_t query_stride, size_t heads,
+                     size_t top, size_t first, size_t last, int *d_selected,
+                     void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* Cuts every sequence down to `budget` rows, each KV head by its own
+ * weights: rows at positions below `first` and the rows at the `last` last
+ * positions stay (first + last <= budget), and of the others those of the
+ * largest weight, ties to the lower row, a weight that is not a number below
+ * all others. Rows that stay beyond the budget move, with their weights and
+ * positions, into the places of rows that go, both in ascending order;
+ * nothing else moves. The bounds of a page that rows move into are widened.
+ * d_new_lengths (must not be d_lengths) gets min(length, budget). Positions
+ * are distinct and not negative. Pages that hold rows below the budget must
+ * not be shared. The workspace (16-byte aligned) needs
+ * nut_paged_evict_workspace bytes. */
+size_t nut_paged_evict_workspace(const nut_paged_kv *kv,
+                                 const nut_paged_batch *seqs, size_t budget);
+int nut_paged_evict(const nut_paged_kv *kv, const nut_paged_batch *seqs,
+                    const nut_paged_history *history, size_t budget,
+                    size_t first, size_t last, int *d_new_lengths,
+                    void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* Waits for the device, then raises what the view's status word holds
+ * (NUT_EOUTOFRANGE: "paged cache: page out of range", "paged cache: length
+ * out of range", "paged cache: rows out of range") and clears it. */
+int nut_paged_check(const nut_paged_kv *kv);
+
 /* -------------------------------------------------------- token loop -- */
 
 /* decode_quantized_token (src/quant_model.cpp:158-206): one token through

@@ -24,6 +24,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libnutllm_hip.so")
 
 INT8, INT4 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 PATH_AUTO, PATH_STEPS, PATH_TOKEN = 0, 1, 2
 
 
@@ -158,6 +159,20 @@ _SIGS = {
                                        C.c_uint32, _P, _P, _P]),
     "nut_kv_read_positions": (C.c_int, [_P, _SZ, _SZ, _P, _P]),
     "nut_kv_write_positions": (C.c_int, [_P, _SZ, _SZ, _P, _P]),
+    "nut_paged_append": (C.c_int, [_P, _P, _P, _P, _SZ, _SZ, _SZ, _P, _SZ, _P,
+                                   _P, _P, _P]),
+    "nut_paged_append_cache": (C.c_int, [_P, _P, _P, _SZ, _SZ, _SZ, _P, _P,
+                                         _P, _P]),
+    "nut_paged_attention_workspace": (_SZ, [_P, _P, _SZ, _SZ, C.c_int]),
+    "nut_paged_attention": (C.c_int, [_P, _P, _P, _SZ, _SZ, C.c_float, _P,
+                                      _SZ, _P, _P, _P, _P, _SZ, _P]),
+    "nut_paged_select_workspace": (_SZ, [_P, _P, _SZ, _SZ]),
+    "nut_paged_select": (C.c_int, [_P, _P, _P, _SZ, _SZ, _SZ, _SZ, _SZ, _P,
+                                   _P, _SZ, _P]),
+    "nut_paged_evict_workspace": (_SZ, [_P, _P, _SZ]),
+    "nut_paged_evict": (C.c_int, [_P, _P, _P, _SZ, _SZ, _SZ, _P, _P, _SZ,
+                                  _P]),
+    "nut_paged_check": (C.c_int, [_P]),
 }
 
 
@@ -464,6 +479,153 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+
+def _raw(buffer):
+    """Address of a device buffer (an object with `ptr`), None for none."""
+    if buffer is None:
+        return None
+    return buffer.ptr.value if isinstance(buffer.ptr, C.c_void_p) else buffer.ptr
+
+
+class _PagedKV(C.Structure):
+    _fields_ = [("d_keys", _P), ("d_values", _P), ("d_bounds", _P),
+                ("pages", _SZ), ("page_size", _SZ), ("kv_heads", _SZ),
+                ("head_dim", _SZ), ("page_stride", _SZ),
+                ("head_stride", _SZ), ("slot_stride", _SZ),
+                ("type", C.c_int), ("d_status", _P)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [("d_pages", _P), ("table_stride", _SZ), ("d_lengths", _P),
+                ("batch", _SZ), ("max_length", _SZ)]
+
+
+class _PagedHistory(C.Structure):
+    _fields_ = [("d_weights", _P), ("d_positions", _P), ("stride", _SZ)]
+
+
+class PagedBatch:
+    """The sequences of a paged cache's call (nut_paged_batch): their page
+    table [batch][table_stride] and lengths [batch], int32 device buffers;
+    max_length bounds the lengths."""
+
+    def __init__(self, pages, table_stride, lengths, batch, max_length):
+        self._keep = (pages, lengths)
+        self.batch, self.max_length = int(batch), int(max_length)
+        self.view = _PagedBatch(_raw(pages), table_stride, _raw(lengths),
+                                batch, max_length)
+        self.ref = C.addressof(self.view)
+
+
+class PagedHistory:
+    """What eviction goes by (nut_paged_history): gathered weights (fp32) and
+    positions (int32), [batch][kv_heads][stride] device buffers."""
+
+    def __init__(self, weights, positions, stride):
+        self._keep = (weights, positions)
+        self.view = _PagedHistory(_raw(weights), _raw(positions), stride)
+        self.ref = C.addressof(self.view)
+
+
+def _ref(view):
+    return None if view is None else view.ref
+
+
+def _bytes(count):
+    if count == C.c_size_t(-1).value:
+        check(1)
+    return count
+
+
+class PagedKV:
+    """One layer's paged K/V cache (nut_paged_kv): a view of device buffers
+    that the caller holds. dtype is F32, F16 or BF16; strides are
+    (page, head, slot) in elements, None for packed
+    [pages][kv_heads][page_size][head_dim]. Every buffer is an object with
+    `ptr` (and `nbytes`, where a workspace or new rows are passed), such as a
+    DeviceArray. Calls are asynchronous on `stream` and allocate nothing."""
+
+    def __init__(self, keys, values, pages, page_size, kv_heads, head_dim,
+                 dtype, strides=None, bounds=None, status=None):
+        self._keep = (keys, values, bounds, status)
+        self.kv_heads, self.head_dim = int(kv_heads), int(head_dim)
+        self.page_size, self.pages, self.dtype = int(page_size), int(pages), dtype
+        self._scale = max(1, self.head_dim) ** -0.5
+        self.view = _PagedKV(_raw(keys), _raw(values), _raw(bounds), pages,
+                             page_size, kv_heads, head_dim,
+                             *(strides or (0, 0, 0)), dtype, _raw(status))
+        self.ref = C.addressof(self.view)
+
+    def append(self, seqs, keys, values, new_lengths=None, *, starts=None,
+               max_new=1, history=None, first_positions=None, row_stride=0,
+               head_stride=0, stream=None):
+        """nut_paged_append: fp32 rows [rows][kv_heads][head_dim] behind the
+        sequences, rows starts[b] to starts[b + 1] for sequence b (one each
+        without starts)."""
+        row = row_stride or self.kv_heads * self.head_dim or 1
+        used = (self.kv_heads - 1) * (head_stride or self.head_dim) + self.head_dim
+        held = min(keys.nbytes, values.nbytes) // 4
+        rows = (held - used) // row + 1 if held >= used else 0
+        check(lib().nut_paged_append(
+            self.ref, seqs.ref, _raw(keys), _raw(values), rows, row_stride,
+            head_stride, _raw(starts), max_new, _ref(history),
+            _raw(first_positions), _raw(new_lengths), stream))
+
+    def append_cache(self, seqs, source, layer, begin, end, new_lengths=None,
+                     *, history=None, first_positions=None, stream=None):
+        """nut_paged_append_cache: rows [begin, end) of a KVCache's layer
+        behind the one sequence of seqs."""
+        check(lib().nut_paged_append_cache(
+            self.ref, seqs.ref, source.handle, layer, begin, end,
+            _ref(history), _raw(first_positions), _raw(new_lengths), stream))
+
+    def attention_workspace(self, seqs, heads, top=0, weighted=False):
+        return _bytes(lib().nut_paged_attention_workspace(
+            self.ref, seqs.ref, heads, top, int(weighted)))
+
+    def attention(self, seqs, query, out, heads, *, scale=None,
+                  query_stride=0, selected=None, top=0, history=None,
+                  lse=None, workspace=None, stream=None):
+        """nut_paged_attention: one new token's attention for each sequence,
+        fp32 query and out [batch][heads][head_dim]; scale None is
+        1 / sqrt(head_dim)."""
+        check(lib().nut_paged_attention(
+            self.ref, seqs.ref, _raw(query), query_stride, heads,
+            self._scale if scale is None else scale, _raw(selected),
+            top, _ref(history), _raw(out), _raw(lse), _raw(workspace),
+            0 if workspace is None else workspace.nbytes, stream))
+
+    def select_workspace(self, seqs, heads, top):
+        return _bytes(lib().nut_paged_select_workspace(self.ref, seqs.ref,
+                                                       heads, top))
+
+    def select(self, seqs, query, selected, heads, top, *, first=1, last=1,
+               query_stride=0, workspace=None, stream=None):
+        """nut_paged_select: the `top` pages of each sequence and KV head that
+        bound q . k highest, int32 [batch][kv_heads][top]."""
+        check(lib().nut_paged_select(
+            self.ref, seqs.ref, _raw(query), query_stride, heads, top, first,
+            last, _raw(selected), _raw(workspace),
+            0 if workspace is None else workspace.nbytes, stream))
+
+    def evict_workspace(self, seqs, budget):
+        return _bytes(lib().nut_paged_evict_workspace(self.ref, seqs.ref,
+                                                      budget))
+
+    def evict(self, seqs, history, new_lengths, budget, *, first=0, last=0,
+              workspace=None, stream=None):
+        """nut_paged_evict: every sequence down to `budget` rows by gathered
+        weight, the `first` first and `last` last positions kept."""
+        check(lib().nut_paged_evict(
+            self.ref, seqs.ref, _ref(history), budget, first, last,
+            _raw(new_lengths), _raw(workspace),
+            0 if workspace is None else workspace.nbytes, stream))
+
+    def check(self):
+        """nut_paged_check: waits, then raises OutOfRange for a page, length
+        or row that an earlier call could not follow."""
+        check(lib().nut_paged_check(self.ref))
 
 
 class DeviceModel:

@@ -1,0 +1,294 @@
+"""The paged KV cache's operators against their definitions in 64 bits: sizes
+at the edges of pages and tiles, empty sequences, every type and layout, NaN in
+the slots behind a sequence's end, workspaces that start as NaN. Tolerances are
+derived in paged_case.Case.expect_attention; what is moved or chosen is
+compared bit for bit."""
+import numpy as np
+import pytest
+
+from paged_case import Case, decode, encode, same
+
+pytestmark = pytest.mark.gpu
+
+EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300]
+
+
+def query_of(case, heads, seed=1, sigma=1.5):
+    rng = np.random.default_rng(seed)
+    return (rng.standard_normal((case.batch, heads, case.dim)) * sigma).astype(np.float32)
+
+
+def check_attention(case, heads, query, **kw):
+    out, lse, weights, tol, tol_w = case.expect_attention(query, heads,
+                                                          selected=kw.get("selected"))
+    got, got_lse = case.attention(query, heads, **kw)
+    err = np.abs(got - out) / np.where(tol > 0, tol, 1)
+    print(f"worst error {err.max():.3f} of its bound", flush=True)
+    assert np.all(np.abs(got - out) <= tol)
+    empty = np.isneginf(lse)
+    assert np.array_equal(np.isneginf(got_lse), empty)
+    # the logarithm's argument errs as a weight does, and its result is rounded
+    assert np.all(np.abs(got_lse - lse)[~empty] <=
+                  (tol_w + 2.0 ** -22 * (1 + np.abs(lse)))[~empty])
+    return weights, tol_w
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page,slot_major", [
+    (4, 2, 16, 16, False), (8, 2, 64, 16, False), (2, 2, 128, 32, True), (32, 4, 64, 64, False),
+    (6, 2, 80, 24, True), (3, 1, 8, 1, False), (5, 1, 40, 7, False), (34, 2, 24, 128, True),
+    (4, 1, 256, 16, False), (16, 1, 136, 5, True),
+])
+def test_attention(gpu, kind, heads, kv, dim, page, slot_major):
+    case = Case(kind, EDGES, kv, dim, page, seed=dim + page, slot_major=slot_major).upload()
+    check_attention(case, heads, query_of(case, heads))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lengths", [[1500], [2049, 1, 0, 1024, 1023, 1025], [5000, 4097]])
+def test_attention_split_lengths(gpu, kind, lengths):
+    case = Case(kind, lengths, 1, 64, 48, seed=3).upload()
+    check_attention(case, 4, query_of(case, 4, sigma=3.0))
+
+
+def test_attention_long(gpu):
+    """A length that many runs share, with a table wider than the sequence."""
+    case = Case("f16", [20011], 1, 16, 64, seed=5, max_length=33000).upload()
+    check_attention(case, 3, query_of(case, 3))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_attention_large_and_small_values(gpu, kind):
+    """Scores of hundreds either way, a row that takes all the weight, queries
+    far from one; without the log-sum-exp."""
+    case = Case(kind, [5, 77, 260], 2, 32, 16, seed=8, sigma=30.0)
+    case.upload()
+    q = query_of(case, 4, sigma=20.0)
+    out, _, _, tol, _ = case.expect_attention(q, 4)
+    got, lse = case.attention(q, 4, lse=False)
+    assert np.all(np.abs(got - out) <= tol) and np.all(lse == 7.0)
+    for power in (-60, 40):
+        q = query_of(case, 4) * np.float32(2.0 ** power)
+        scale = float(2.0 ** -power / 8)
+        out, _, _, tol, _ = case.expect_attention(q, 4, scale=scale)
+        got, _ = case.attention(q, 4, scale=scale)
+        assert np.all(np.abs(got - out) <= tol)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_attention_infinite_keys(gpu, kind):
+    """Rows whose score is minus infinity weigh nothing, a sequence of such
+    rows alone gives zeros; a NaN key shows in its own KV head only."""
+    case = Case(kind, [40, 3, 33], 2, 32, 16, seed=9)
+    q = np.abs(query_of(case, 4)) + np.float32(0.1)
+    inf = encode(np.array(-np.inf), kind)
+    plain = Case(kind, [40, 3, 33], 2, 32, 16, seed=9)
+    for i in (0, 17, 39):  # sequence 0: these rows
+        case.keys[case.table[0, i // 16], :, i % 16, 5] = inf
+    for i in range(3):     # sequence 1: all rows
+        case.keys[case.table[1, 0], :, i, 5] = inf
+    case.keys[case.table[2, 1], 1, 3, 0] = encode(np.array(np.nan), kind)
+    case.upload()
+    got, lse = case.attention(q, 4)
+    assert np.all(got[1] == 0) and np.all(np.isneginf(lse[1]))
+    assert np.all(np.isnan(got[2, 2:])) and np.all(np.isfinite(got[2, :2]))
+    keep = [i for i in range(40) if i not in (0, 17, 39)]
+    for h in range(4):
+        k, v = (plain.rows(p, 0, h // 2)[keep] for p in (plain.keys, plain.values))
+        s = k @ q[0, h].astype(np.float64) * 32 ** -0.5
+        p = np.exp(s - s.max())
+        want, size = (p / p.sum()) @ v, (p / p.sum()) @ np.abs(v)
+        _, _, _, _, tol_w = plain.expect_attention(q, 4)
+        assert np.all(np.abs(got[0, h] - want) <= tol_w[0, h] * size)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 64, 16), (3, 3, 128, 32), (34, 2, 24, 9)])
+def test_attention_gathers_weights(gpu, kind, heads, kv, dim, page):
+    lengths = [0, 1, 33, 128, 700, 1300]
+    case = Case(kind, lengths, kv, dim, page, seed=11).upload()
+    before = case.weights.copy()
+    q = query_of(case, heads)
+    weights, tol_w = check_attention(case, heads, q, history=case.history)
+    case.attention(q, heads, history=case.history, lse=False)  # a second token
+    got = case.fetch("weights").astype(np.float64)
+    group = heads // kv
+    for b, n in enumerate(lengths):
+        rel = tol_w[b].reshape(kv, group).max(1)[:, None]
+        # two additions to the weight that was there, each rounded once
+        want = before[b] + 2 * weights[b]
+        bound = 2 * weights[b] * (rel + group * 2.0 ** -24) + 2 * 2.0 ** -24 * want + 1e-37
+        assert np.all(np.abs(got[b] - want) <= bound)
+        assert same(case.fetch("weights")[b, :, n:], before[b, :, n:])
+    assert same(case.fetch("positions"), case.positions)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page,top,first,last", [
+    (8, 2, 64, 16, 8, 1, 2), (2, 2, 128, 8, 5, 0, 0), (32, 4, 64, 4, 31, 1, 1),
+    (6, 2, 80, 24, 4, 0, 1), (34, 2, 24, 3, 16, 16, 0), (4, 1, 256, 16, 1, 0, 1),
+])
+def test_select_and_sparse_attention(gpu, kind, heads, kv, dim, page, top, first, last):
+    lengths = [0, 1, page * top, page * top + 1, 500, 1203]
+    case = Case(kind, lengths, kv, dim, page, seed=13, slot_major=top == 5).upload()
+    q = query_of(case, heads)
+    want = case.expect_select(q, heads, top, first, last)
+    got = case.select(q, heads, top, first, last)
+    assert np.array_equal(got, want)
+    check_attention(case, heads, q, selected=got, top=top)
+
+
+def test_select_ties_and_many_pages(gpu):
+    """Pages of equal bounds go by their index; more pages than threads."""
+    case = Case("bf16", [9000, 777], 2, 16, 1, seed=17)
+    case.keys[:] = encode(np.round(decode(case.keys, "bf16")), "bf16")
+    case.bounds[:, :, 0] = case.bounds[:, :, 1] = case.keys[:, :, 0]
+    case.upload()
+    q = np.round(query_of(case, 4))
+    for top, first, last in ((64, 1, 2), (700, 0, 0), (1, 0, 0)):
+        assert np.array_equal(case.select(q, 4, top, first, last),
+                              case.expect_select(q, 4, top, first, last))
+    case.bounds[:] = encode(np.float32(1.0), "bf16")
+    case.upload()
+    assert np.array_equal(case.select(q, 4, 64, 1, 2), case.expect_select(q, 4, 64, 1, 2))
+
+
+def test_select_not_a_number_first(gpu):
+    case = Case("f32", [320], 1, 16, 16, seed=19)
+    case.bounds[case.table[0, 7], 0, 1, 3] = np.nan
+    case.upload()
+    got = case.select(query_of(case, 2), 2, 2, 0, 1)
+    assert got.tolist() == [[[7, 19]]]
+
+
+def test_sparse_attention_of_a_callers_selection(gpu):
+    """A page twice counts twice; -1 anywhere, and pages behind the sequence's
+    end, count nothing; a page no table row has is reported."""
+    case = Case("f32", [100, 100, 100], 1, 32, 16, seed=21).upload()
+    q = query_of(case, 2)
+    chosen = np.array([[[3, -1, 3, 0]], [[-1, -1, -1, -1]], [[6, 1, -1, -1]]], np.int32)
+    check_attention(case, 2, q, selected=chosen, top=4)
+    case.paged.check()
+    chosen[1, 0, 2] = 1 << 30
+    out, _ = case.attention(q, 2, selected=chosen, top=4)
+    assert np.all(out[1] == 0)
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kv,dim,page,budget,first,last,slot_major", [
+    (2, 64, 16, 100, 4, 16, False), (3, 80, 24, 64, 0, 0, True), (1, 8, 1, 33, 1, 32, False),
+    (2, 16, 300, 260, 0, 7, False), (2, 128, 128, 1, 0, 1, False), (1, 256, 7, 500, 0, 500, True),
+])
+def test_evict(gpu, kind, kv, dim, page, budget, first, last, slot_major):
+    lengths = [0, 1, budget - 1, budget, budget + 1, budget + 40, 3 * budget + 5]
+    case = Case(kind, lengths, kv, dim, page, seed=23, slot_major=slot_major)
+    # heavy tails, rows without weight, positions as earlier evictions leave them
+    case.weights[:] = np.exp(3 * case.rng.standard_normal(case.weights.shape))
+    case.weights[case.rng.random(case.weights.shape) < 0.2] = 0.0
+    for b in range(case.batch):
+        for h in range(kv):
+            case.positions[b, h] = 3 * case.rng.permutation(case.max_length)
+    check_evict(case, budget, first, last)
+
+
+def check_evict(case, budget, first=0, last=0):
+    case.upload()
+    new = case.expect_evict(budget, first, last)
+    case.evict(budget, first, last)
+    assert np.array_equal(case.new_lengths(), new)
+    for name in ("weights", "positions", "bounds"):
+        assert same(case.fetch(name), getattr(case, name)), name
+    for name in ("keys", "values"):
+        assert same(case.pool(name), getattr(case, name)), name
+    case.paged.check()
+
+
+def test_evict_ties_and_not_numbers(gpu):
+    case = Case("f16", [900, 450], 2, 16, 16, seed=25)
+    case.weights[0] = 0.5                     # all equal: the first rows stay
+    case.weights[1] = np.round(case.weights[1] * 4) / 4
+    case.weights[1, 0, ::3] = np.nan          # below all others
+    case.weights[1, 1, ::5] = np.inf
+    case.weights[1, 1, 1::5] = -np.inf
+    case.weights[1, 1, 2::5] = -0.0
+    check_evict(case, 300, 2, 10)
+
+
+def test_evict_long(gpu):
+    """Many more rows than threads, and twice in a row."""
+    case = Case("bf16", [20000, 15001], 1, 8, 64, seed=27)
+    case.weights[:] = np.exp(case.rng.standard_normal(case.weights.shape))
+    check_evict(case, 4096, 4, 512)
+    case.lengths = case.new_lengths()
+    check_evict(case, 4000, 4, 512)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kv,dim,page,slot_major", [
+    (2, 64, 16, False), (4, 128, 32, True), (1, 8, 1, False), (3, 80, 24, False),
+    (2, 256, 300, True)])
+def test_append_ragged(gpu, kind, kv, dim, page, slot_major):
+    lengths = [0, 1, 15, 16, 17, 250, 3, 0]
+    counts = [1, 40, 1, 16, 0, 333, 2, 0]
+    case = Case(kind, lengths, kv, dim, page, seed=29, slot_major=slot_major, room=340).upload()
+    rows = sum(counts) + 5  # source rows behind the last sequence's
+    k = case.rng.standard_normal((rows, kv, dim)).astype(np.float32)
+    v = case.rng.standard_normal((rows, kv, dim)).astype(np.float32)
+    firsts = np.arange(1000, 1000 + 50 * len(counts), 50, dtype=np.int32)
+    starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    new = case.expect_append(k, v, counts, firsts=firsts)
+    A = gpu.DeviceArray
+    case.paged.append(case.seqs, A(like=k), A(like=v), case.d["new_lengths"], starts=A(like=starts),
+                      max_new=333, history=case.history, first_positions=A(like=firsts))
+    gpu.synchronize()
+    check_append(case, new)
+
+
+def check_append(case, new):
+    assert np.array_equal(case.new_lengths(), new)
+    for name in ("weights", "positions", "bounds"):
+        assert same(case.fetch(name), getattr(case, name)), name
+    for name in ("keys", "values"):
+        assert same(case.pool(name), getattr(case, name)), name
+    case.paged.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kv,dim", [(2, 16), (4, 64), (1, 40), (32, 128), (2, 256)])
+def test_append_tokens(gpu, kind, kv, dim):
+    """One row each, out of fused rows [q | k | v], with rounding ties, values
+    beyond fp16, signed zeros, subnormals and infinities among the values."""
+    case = Case(kind, [0, 5, 15, 16, 63], kv, dim, 16, seed=31, room=1).upload()
+    fused = case.rng.standard_normal((case.batch, 3, kv, dim)).astype(np.float32)
+    odd = np.array([1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8, 1 + 2.0 ** -11, 1 + 3 * 2.0 ** -11, -0.0,
+                    70000.0, 65519.9, 2.0 ** -25, 3 * 2.0 ** -25, 1e-40, np.inf, -np.inf,
+                    3.4e38, -1.0], np.float32)
+    flat = fused[:, 2].reshape(case.batch, -1).copy()
+    flat[1, :14], flat[2, -14:] = odd, odd
+    fused[:, 2] = flat.reshape(case.batch, kv, dim)
+    whole = gpu.DeviceArray(like=fused)
+
+    class Part:
+        def __init__(self, i):
+            self.ptr = whole.ptr.value + 4 * i * kv * dim
+            self.nbytes = whole.nbytes - 4 * i * kv * dim
+
+    new = case.expect_append(fused[:, 1], fused[:, 2], [1] * 5)
+    case.paged.append(case.seqs, Part(1), Part(2), case.d["new_lengths"], history=case.history,
+                      row_stride=3 * kv * dim, head_stride=dim)
+    gpu.synchronize()
+    check_append(case, new)
+
+
+def test_append_not_a_number_shows_in_the_bounds(gpu):
+    case = Case("f32", [3, 0], 1, 16, 8, seed=33, room=2).upload()
+    k = np.ones((2, 1, 16), np.float32)
+    k[0, 0, 4] = k[1, 0, 5] = np.nan
+    A = gpu.DeviceArray
+    case.paged.append(case.seqs, A(like=k), A(like=k), case.d["new_lengths"])
+    gpu.synchronize()
+    for b, d in ((0, 4), (1, 5)):
+        nan = np.isnan(case.fetch("bounds")[case.table[b, 0], 0])
+        assert np.all(nan[:, d]) and nan.sum() == 2

@@ -1,0 +1,363 @@
+"""The paged KV cache's operators as a serving loop uses them: a model's prompt
+moved into pages, tokens appended, read, weighed and evicted; in captured
+graphs, on other streams, far into a large pool; and what they do with page
+tables, lengths and row counts that they cannot follow."""
+import numpy as np
+import pytest
+import torch
+
+from nutllm_amd import workloads as W
+from paged_case import Case, same
+
+pytestmark = pytest.mark.gpu
+
+
+def query_of(case, heads, seed=1):
+    rng = np.random.default_rng(seed)
+    return rng.standard_normal((case.batch, heads, case.dim)).astype(np.float32)
+
+
+def near(case, heads, query, got, **kw):
+    out, lse, weights, tol, _ = case.expect_attention(query, heads, **kw)
+    assert np.all(np.abs(got - out) <= tol)
+    return weights
+
+
+class Tensor:
+    """A torch tensor as a device buffer."""
+
+    def __init__(self, t):
+        self.t, self.ptr, self.nbytes = t, t.data_ptr(), t.numel() * t.element_size()
+
+
+def test_prompt_into_pages(gpu):
+    """nut_prefill's K and V rows, layer by layer, behind what a sequence
+    holds; attention over them."""
+    cfg = W.make_config("step_gqa2", max_seq=96)
+    model = W.build("step_gqa2", 0, 3, 96)
+    dev, cache = model.to_device(), gpu.KVCache(cfg)
+    dev.prefill(cache, W.synth_tokens(5, cfg.vocab_size, 70))
+    keys, values = cache.read_positions(0, 70)
+    for layer in range(cfg.layers):
+        for begin, end in ((0, 70), (9, 42), (70, 70)):
+            case = Case("f32", [5], cfg.kv_heads, cfg.head_dim, 16, seed=layer, room=70).upload()
+            new = case.expect_append(keys[layer, :, begin:end].transpose(1, 0, 2),
+                                     values[layer, :, begin:end].transpose(1, 0, 2),
+                                     [end - begin])
+            case.paged.append_cache(case.seqs, cache, layer, begin, end, case.d["new_lengths"],
+                                    history=case.history)
+            gpu.synchronize()
+            assert np.array_equal(case.new_lengths(), new)
+            for name in ("keys", "values"):
+                assert same(case.pool(name), getattr(case, name))
+            for name in ("bounds", "weights", "positions"):
+                assert same(case.fetch(name), getattr(case, name))
+            case.d["lengths"].upload(new)
+            case.lengths = new
+            q = query_of(case, 4)
+            near(case, 4, q, case.attention(q, 4)[0])
+    for layer, begin, end in ((cfg.layers, 0, 1), (0, 5, 4), (0, 0, 71)):
+        with pytest.raises(gpu.OutOfRange):
+            case.paged.append_cache(case.seqs, cache, layer, begin, end)
+    other = Case("f32", [5], cfg.kv_heads + 1, cfg.head_dim, 16, room=70).upload()
+    with pytest.raises(gpu.InvalidArgument, match="cache configuration mismatch"):
+        other.paged.append_cache(other.seqs, cache, 0, 0, 1)
+    cache.close(), dev.close()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_serving_loop(gpu, kind):
+    """Ragged prompts, then tokens one at a time: append, attention that
+    gathers weights, and an eviction to the budget whenever a sequence passes
+    it; the host follows with the device's weights, which decide."""
+    budget, heads, kv, dim = 40, 8, 2, 64
+    case = Case(kind, [0, 0, 0], kv, dim, 16, seed=41, max_length=budget + 60).upload()
+    case.bounds[:] = 0
+    case.upload()
+    rng, A = np.random.default_rng(7), gpu.DeviceArray
+    counts, text = [50, 1, 37], np.zeros(3, np.int32)
+    for step in range(14):
+        rows = sum(counts)
+        k = rng.standard_normal((rows, kv, dim)).astype(np.float32)
+        v = rng.standard_normal((rows, kv, dim)).astype(np.float32)
+        starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        new = case.expect_append(k, v, counts, firsts=text)
+        case.paged.append(case.seqs, A(like=k), A(like=v), case.d["new_lengths"],
+                          starts=A(like=starts) if step == 0 else None, max_new=max(counts),
+                          history=case.history, first_positions=A(like=text))
+        gpu.synchronize()
+        assert np.array_equal(case.new_lengths(), new)
+        text += np.array(counts, np.int32)
+        case.lengths = new
+        case.d["lengths"].upload(new)
+        q = query_of(case, heads, step)
+        grown = near(case, heads, q, case.attention(q, heads, history=case.history)[0])
+        weights = case.fetch("weights")
+        assert np.allclose(weights, case.weights + grown, rtol=1e-4, atol=1e-6)
+        case.weights = weights
+        if np.any(new > budget):
+            new = case.expect_evict(budget, 2, 8)
+            case.evict(budget, 2, 8)
+            assert np.array_equal(case.new_lengths(), new)
+            case.lengths = new
+            case.d["lengths"].upload(new)
+        for name in ("weights", "positions", "bounds"):
+            assert same(case.fetch(name), getattr(case, name)), name
+        for name in ("keys", "values"):
+            assert same(case.pool(name), getattr(case, name)), name
+        chosen = case.select(q, heads, 2, 0, 1)
+        assert np.array_equal(chosen, case.expect_select(q, heads, 2, 0, 1))
+        near(case, heads, q, case.attention(q, heads, selected=chosen, top=2)[0], selected=chosen)
+        counts = [1, 1, 1]
+    case.paged.check()
+
+
+def test_captured_step(gpu):
+    """A decode step (append, weighted attention, selection, attention over
+    it, eviction) in two graphs with workspaces of their own, replayed in turn
+    with other work between; each replay sees the inputs of its time."""
+    heads, budget, top = 4, 100, 3
+    case = Case("f16", [90, 130, 60], 2, 64, 16, seed=43, room=8).upload()
+    A, stream, graphs = gpu.DeviceArray, torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    k, v = (torch.zeros(3, 2, 64, device="cuda") for _ in range(2))
+    q = torch.zeros(3, heads, 64, device="cuda")
+    after = gpu.PagedBatch(case.d["table"], case.width, case.d["new_lengths"], 3, case.max_length)
+    cut = A(like=np.zeros(3, np.int32))
+    for _ in range(2):
+        sparse = torch.zeros(3, heads, 64, device="cuda")
+        out, chosen = torch.zeros_like(sparse), torch.zeros(3, 2, top, dtype=torch.int32,
+                                                            device="cuda")
+        sizes = (case.paged.attention_workspace(after, heads, weighted=True),
+                 case.paged.select_workspace(after, heads, top),
+                 case.paged.attention_workspace(after, heads, top=top),
+                 case.paged.evict_workspace(after, budget))
+        space = [Tensor(torch.full((max(1, n),), 255, dtype=torch.uint8, device="cuda"))
+                 for n in sizes]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            at = torch.cuda.current_stream().cuda_stream
+            case.paged.append(case.seqs, Tensor(k), Tensor(v), case.d["new_lengths"],
+                              history=case.history, stream=at)
+            case.paged.attention(after, Tensor(q), Tensor(out), heads, history=case.history,
+                                 workspace=space[0], stream=at)
+            case.paged.select(after, Tensor(q), Tensor(chosen), heads, top, workspace=space[1],
+                              stream=at)
+            case.paged.attention(after, Tensor(q), Tensor(sparse), heads,
+                                 selected=Tensor(chosen), top=top, workspace=space[2], stream=at)
+            case.paged.evict(after, case.history, cut, budget, first=1, last=5,
+                             workspace=space[3], stream=at)
+        graphs.append((graph, out, chosen, sparse, space))
+    rng = np.random.default_rng(3)
+    for turn in range(6):
+        graph, out, chosen, sparse, _ = graphs[turn % 2]
+        new = [torch.from_numpy(rng.standard_normal(t.shape).astype(np.float32)) for t in (k, v, q)]
+        for t, n in zip((k, v, q), new):
+            t.copy_(n)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        case.lengths = case.expect_append(new[0].numpy(), new[1].numpy(), [1, 1, 1])
+        query = new[2].numpy()
+        near(case, heads, query, out.cpu().numpy())
+        want = case.expect_select(query, heads, top, 1, 1)
+        assert np.array_equal(chosen.cpu().numpy(), want)
+        near(case, heads, query, sparse.cpu().numpy(), selected=want)
+        # the weights that decided, from the device: those below the budget
+        # moved with their rows, so the plan is made from a copy of the state
+        # before the move: the rows beyond the budget are where they were
+        moved = case.fetch("weights")
+        lengths = cut.download(np.int32, 3)
+        assert np.array_equal(lengths, np.minimum(case.lengths, budget))
+        at = case.fetch("positions")
+        for b in range(3):
+            n, m = int(case.lengths[b]), int(lengths[b])
+            for h in range(2):
+                there = {int(p): i for i, p in enumerate(case.positions[b, h, :n])}
+                assert len({int(p) for p in at[b, h, :m]}) == m
+                kept = [there[int(p)] for p in at[b, h, :m]]
+                for i, j in enumerate(kept):
+                    assert i == j or j >= budget
+                    to, of = (case.table[b, x // 16] for x in (i, j))
+                    for name in ("keys", "values"):
+                        pool = getattr(case, name)
+                        pool[to, h, i % 16] = pool[of, h, j % 16]
+        case.weights, case.positions = moved, at
+        case.bounds = case.fetch("bounds")
+        for name in ("keys", "values"):
+            assert same(case.pool(name), getattr(case, name)), name
+        case.lengths = lengths
+        case.d["lengths"].upload(lengths)
+        torch.cuda.synchronize()
+    case.paged.check()
+
+
+def test_two_calls_at_once(gpu):
+    """Calls on two streams with workspaces of their own."""
+    case = Case("bf16", [900, 1500], 2, 64, 16, seed=45).upload()
+    q = [query_of(case, 8, s) for s in (1, 2)]
+    need = case.paged.attention_workspace(case.seqs, 8)
+    work = [gpu.DeviceArray(like=np.full(max(1, need), 255, np.uint8)) for _ in q]
+    dq = [gpu.DeviceArray(like=x) for x in q]
+    out = [gpu.DeviceArray(4 * 2 * 8 * 64) for _ in q]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, a, o, w in zip(streams, dq, out, work):
+            case.paged.attention(case.seqs, a, o, 8, workspace=w, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for x, o in zip(q, out):
+        near(case, 8, x, o.download(np.float32, 2 * 8 * 64).reshape(2, 8, 64))
+
+
+def test_same_answer_every_time(gpu):
+    """Nothing depends on the order in which workgroups run."""
+    case = Case("f16", [3000, 700], 2, 64, 16, seed=47).upload()
+    q = query_of(case, 8)
+    first = case.attention(q, 8)
+    for _ in range(3):
+        again = case.attention(q, 8)
+        assert same(again[0], first[0]) and same(again[1], first[1])
+
+
+@pytest.mark.parametrize("slot_major", [False, True])
+def test_far_into_a_large_pool(gpu, slot_major):
+    """Byte and element offsets beyond 32 bits: append, bounds, selection,
+    attention and eviction with pages at both ends of a 12 GB pool."""
+    kv, dim, ps, pages = 2, 64, 16, 1 << 20
+    stride = kv * ps * dim + (64 if slot_major else 0)
+    keys, values = (torch.empty(pages * stride, dtype=torch.float32, device="cuda")
+                    for _ in range(2))
+    bounds = torch.zeros(pages, kv, 2, dim, device="cuda")
+    strides = (stride, dim, kv * dim) if slot_major else (stride, ps * dim, dim)
+    paged = gpu.PagedKV(Tensor(keys), Tensor(values), pages, ps, kv, dim, gpu.F32,
+                        strides=strides, bounds=Tensor(bounds))
+    table = np.array([[pages - 1, 0, pages // 2 + 1, pages - 2]], np.int32)
+    case = Case("f32", [0], kv, dim, ps, seed=49, max_length=64)
+    case.pages, case.table = 4, np.arange(4, dtype=np.int32)[None]
+    n = 60
+    k, v = (case.rng.standard_normal((n, kv, dim)).astype(np.float32) for _ in range(2))
+    A = gpu.DeviceArray
+    d_table, d_len, d_new = A(like=table), A(like=np.zeros(1, np.int32)), A(4)
+    weights, positions = A(like=case.weights), A(like=case.positions)
+    history = gpu.PagedHistory(weights, positions, 64)
+    seqs = gpu.PagedBatch(d_table, 4, d_len, 1, 64)
+    paged.append(seqs, A(like=k), A(like=v), d_new, starts=A(like=np.array([0, n], np.int32)),
+                 max_new=n, history=history)
+    case.lengths = case.expect_append(k, v, [n])
+    after = gpu.PagedBatch(d_table, 4, d_new, 1, 64)
+    q = query_of(case, 4)
+    dq, out, chosen = A(like=q), A(4 * 4 * dim), A(4 * 2 * kv)
+    space = A(1 << 20)
+    paged.select(after, dq, chosen, 4, 2, first=0, last=1, workspace=space)
+    paged.attention(after, dq, out, 4, selected=chosen, top=2, workspace=space)
+    gpu.synchronize()
+    want = case.expect_select(q, 4, 2, 0, 1)
+    assert np.array_equal(chosen.download(np.int32, 2 * kv).reshape(1, kv, 2), want)
+    near(case, 4, q, out.download(np.float32, 4 * dim).reshape(1, 4, dim), selected=want)
+    paged.attention(after, dq, out, 4, workspace=space)
+    gpu.synchronize()
+    near(case, 4, q, out.download(np.float32, 4 * dim).reshape(1, 4, dim))
+    case.weights = case.rng.random(case.weights.shape).astype(np.float32)
+    weights.upload(case.weights)
+    case.lengths = case.expect_evict(20)
+    paged.evict(after, history, d_len, 20, workspace=space)
+    paged.attention(seqs, dq, out, 4, workspace=space)
+    gpu.synchronize()
+    near(case, 4, q, out.download(np.float32, 4 * dim).reshape(1, 4, dim))
+
+
+@pytest.mark.parametrize("bad", [-1, 1 << 30, 9])
+def test_pages_that_the_cache_has_not(gpu, bad):
+    """A bad entry's rows count nothing and are not written; entries behind a
+    sequence's end are not read; the call says so once."""
+    case = Case("f32", [40, 40], 1, 32, 16, seed=51, max_length=64, spare=1).upload()
+    assert case.pages == 9
+    q = query_of(case, 2)
+    table = case.table.copy()
+    table[0, 1] = bad     # rows 16 to 31
+    table[:, 3] = bad     # behind the end: no matter
+    case.d["table"].upload(table)
+    got, lse = case.attention(q, 2)
+    out, want_lse, _, tol, _ = case.expect_attention(q, 2)
+    assert np.all(np.abs(got[1] - out[1]) <= tol[1])
+    few = Case("f32", [40, 40], 1, 32, 16, seed=51, max_length=64, spare=1)
+    rows = np.r_[0:16, 32:40]
+    k, v = few.rows(few.keys, 0, 0)[rows], few.rows(few.values, 0, 0)[rows]
+    for h in range(2):
+        s = k @ q[0, h].astype(np.float64) * 32 ** -0.5
+        p = np.exp(s - s.max())
+        assert np.all(np.abs(got[0, h] - (p / p.sum()) @ v) <= 1e-5)
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+    case.paged.check()  # said once
+    # a selection does not choose it before a page that there is
+    table[0, 0] = bad
+    case.d["table"].upload(table)
+    assert case.select(q, 2, 1, 0, 0)[0, 0].tolist() == [2]
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+    # rows to be appended or moved there are left out; the others arrive
+    case.d["table"].upload(case.table)
+    before = case.pool("keys").copy()
+    table = case.table.copy()
+    table[0, 2] = bad
+    case.d["table"].upload(table)
+    ones = gpu.DeviceArray(like=np.ones((2, 1, 32), np.float32))
+    case.paged.append(case.seqs, ones, ones, case.d["new_lengths"])
+    gpu.synchronize()
+    before[case.table[1, 2], 0, 8] = 1.0
+    assert same(case.pool("keys"), before)
+    case.evict(30)
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+
+
+def test_lengths_and_counts_out_of_range(gpu):
+    """A length below zero or over max_length holds no rows; appends that do
+    not fit leave a sequence as it is."""
+    case = Case("f32", [20, 20, 20, 20], 1, 32, 16, seed=53, max_length=32).upload()
+    q = query_of(case, 2)
+    case.d["lengths"].upload(np.array([20, -1, 33, 0], np.int32))
+    got, lse = case.attention(q, 2)
+    assert np.all(got[1:] == 0) and np.all(np.isneginf(lse[1:])) and np.all(np.isfinite(lse[0]))
+    with pytest.raises(gpu.OutOfRange, match="length out of range"):
+        case.paged.check()
+    assert np.all(case.select(q, 2, 4, 1, 1)[1:] == -1)
+    with pytest.raises(gpu.OutOfRange, match="length out of range"):
+        case.paged.check()
+    case.evict(10)
+    assert case.new_lengths().tolist() == [10, -1, 33, 0]
+    with pytest.raises(gpu.OutOfRange, match="length out of range"):
+        case.paged.check()
+    case = Case("f32", [20, 20, 20, 20], 1, 32, 16, seed=53, max_length=32).upload()
+    A, rows = gpu.DeviceArray, np.ones((40, 1, 32), np.float32)
+    before = case.pool("keys").copy()
+    for starts in ([0, 13, 13, 13, 13],   # 33 rows of at most 32
+                   [0, -1, -1, -1, -1], [5, 4, 4, 4, 4], [0, 14, 14, 14, 14],
+                   [38, 41, 41, 41, 41], [-3, 0, 0, 0, 0]):
+        case.paged.append(case.seqs, A(like=rows), A(like=rows), case.d["new_lengths"],
+                          starts=A(like=np.array(starts, np.int32)), max_new=13,
+                          history=case.history)
+        gpu.synchronize()
+        assert case.new_lengths().tolist() == [20] * 4
+        assert same(case.pool("keys"), before)
+        with pytest.raises(gpu.OutOfRange, match="out of range"):
+            case.paged.check()
+    assert same(case.fetch("weights"), case.weights)
+
+
+def test_allocates_nothing(gpu):
+    case = Case("bf16", [300, 40], 2, 64, 16, seed=55, room=1).upload()
+    q = gpu.DeviceArray(like=query_of(case, 4))
+    out, rows = gpu.DeviceArray(4 * 2 * 4 * 64), gpu.DeviceArray(4 * 2 * 2 * 64)
+    chosen, space = gpu.DeviceArray(4 * 2 * 2 * 3), gpu.DeviceArray(1 << 20)
+    before = gpu.device_allocations()
+    case.paged.append(case.seqs, rows, rows, case.d["new_lengths"], history=case.history)
+    case.paged.attention(case.seqs, q, out, 4, history=case.history, workspace=space)
+    case.paged.select(case.seqs, q, chosen, 4, 3, workspace=space)
+    case.paged.attention(case.seqs, q, out, 4, selected=chosen, top=3, workspace=space)
+    case.paged.evict(case.seqs, case.history, case.d["new_lengths"], 50, workspace=space)
+    gpu.synchronize()
+    assert gpu.device_allocations() == before
