@@ -1,5 +1,26 @@
 // paged_attention.hip — attention of one new token a sequence over a paged
 // KV cache.
+//
+// A workgroup takes a run of one sequence's rows for one KV head and up to 16
+// of the query heads that share it, and reads each row once. Its four waves
+// take tiles of the run in turn, each with a softmax of its own (running
+// maximum and sum); they are joined at the end, and the runs by join_kernel.
+//
+// Everything between a tile's loads and its products stays in the lane that
+// it was loaded into. With lane = 16 j + c, the matrix instruction for
+// S = K Q^T (rows: keys, columns: heads) takes row c's components from lane
+// (j, c) and leaves the scores of keys 4 j + i (i = 0..3) and head c there.
+// The one for O^T = V^T P^T sums over keys in an order of our choice, so lane
+// (j, c) supplies exactly those keys: P needs no exchange, and lane (j, c)
+// loads V rows 4 j + i, components c G .. c G + G - 1 (G = head dim / 16),
+// whose t-th is row c of output tile t. Only the running maximum crosses lanes.
+//
+// Products are exact. fp32 rows run on v_mfma_f32_16x16x4f32; 16-bit rows on
+// the 16x16x32 forms, with the fp32 operand (the query, the weights) split
+// into limbs of the rows' type whose sum it is: three bfloat16 limbs (8 bits
+// each, all 24), or two fp16 limbs (22 bits and more, the query scaled by a
+// power of two so that its largest component lies in [2^13, 2^14), weights in
+// [0, 2^14]). Accumulation is fp32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -12,105 +33,593 @@ namespace nut {
 
 namespace {
 
-template <int TYPE> __device__ __forceinline__ float component(const char *row, uint32_t d)
+constexpr int kWaves = 4;
+constexpr uint32_t kMostRows = 1024; // of a run
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct AttendArgs {
+    PagedView kv;
+    PagedSeqs s;
+    const float *query;
+    size_t query_stride;
+    uint32_t heads, group;
+    float scale; // times log2(e)
+    const int *selected;
+    uint32_t top;
+    float *out, *lse;
+    uint32_t chunk, chunks, tiles;
+    float *parts;  // [batch][heads][chunks][head_dim], unnormalised
+    float2 *stats; // [batch][heads][chunks]: exponent they refer to, sum
+    float *scores; // [batch][heads][chunks * chunk], base 2; nullptr: not kept
+};
+
+template <int TYPE>
+__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c)
 {
-    if constexpr (TYPE == NUT_F32)
-        return reinterpret_cast<const float *>(row)[d];
-    const uint32_t bits = reinterpret_cast<const uint16_t *>(row)[d];
-    return TYPE == NUT_BF16 ? from_bf16(bits) : from_f16(bits);
+    if constexpr (TYPE == NUT_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A workgroup per (sequence, query head), 256 rows at a time: a thread per
-// row takes its score, then a thread per component adds the weighted values.
-template <int TYPE>
-__global__ __launch_bounds__(256) void attend_kernel(PagedView kv, PagedSeqs s,
-                                                     const float *__restrict__ query,
-                                                     size_t query_stride, uint32_t heads,
-                                                     float scale,
-                                                     const int *__restrict__ selected,
-                                                     uint32_t top, float *__restrict__ out,
-                                                     float *__restrict__ lse,
-                                                     float *__restrict__ scores,
-                                                     size_t score_stride)
+// The limbs of eight fp32 values as matrix operands. A value that is not
+// finite is its first limb alone.
+template <int TYPE, int LIMBS>
+__device__ __forceinline__ void split(const float (&x)[8], u32x4 (&limb)[LIMBS])
 {
-    __shared__ float q[256], p[256], red[8];
-    __shared__ size_t at[256];
-    const uint32_t hq = blockIdx.x % heads, b = blockIdx.x / heads;
-    const uint32_t h = hq / (heads / kv.kv_heads), t = threadIdx.x;
-    const uint32_t n = paged_length(kv, s, b, t == 0 && hq == 0);
-    if (t < kv.head_dim)
-        q[t] = query[b * query_stride + size_t(hq) * kv.head_dim + t] * scale;
-    const uint32_t total = selected == nullptr ? n : top * kv.page_size;
-    float most = -INFINITY, sum = 0.0f, acc = 0.0f;
-    for (uint32_t base = 0; base < total; base += 256) {
-        __syncthreads();
-        const uint32_t i = base + t;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        float a = x[2 * w], b = x[2 * w + 1];
+#pragma unroll
+        for (int l = 0; l < LIMBS; l++) {
+            if constexpr (TYPE == NUT_BF16) {
+                // the upper half of the bits: what is cut off is the rest, exactly
+                const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+                limb[l][w] = __builtin_amdgcn_perm(ub, ua, 0x07060302);
+                a -= __uint_as_float(ua & 0xffff0000u);
+                b -= __uint_as_float(ub & 0xffff0000u);
+            } else {
+                const uint32_t ha = to_f16(a), hb = to_f16(b);
+                limb[l][w] = ha | (hb << 16);
+                a -= from_f16(ha);
+                b -= from_f16(hb);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float max_over_rows(float v)
+{
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// One wave's softmax over the tiles it has seen, for the head of its lane:
+// weights are 2^(score - ref), ref = most - 14 for fp16 rows and most else
+// (0 before the first score that is not minus infinity).
+template <int TYPE, int HD> struct Softmax {
+    static constexpr int G = HD / 16;
+    static constexpr float kShift = TYPE == NUT_F16 ? 14.0f : 0.0f;
+    float most = -INFINITY, ref = 0.0f, sum = 0.0f;
+    f32x4 o[G];
+
+    __device__ __forceinline__ Softmax()
+    {
+#pragma unroll
+        for (int t = 0; t < G; t++)
+            o[t] = f32x4{0, 0, 0, 0};
+    }
+    // Raises the running maximum; what was summed is scaled to it.
+    __device__ __forceinline__ void raise(float tile)
+    {
+        const float now = fmaxf(most, tile);
+        if (__any(now > most)) {
+            const float to = now == -INFINITY ? 0.0f : now - kShift;
+            const float f = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
+            // a sum that is not a number stays one
+            sum = most == -INFINITY ? sum : sum * f;
+#pragma unroll
+            for (int t = 0; t < G; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    o[t][i] = most == -INFINITY ? o[t][i] : o[t][i] * f;
+            most = now, ref = to;
+        }
+    }
+};
+
+// The rows of one tile in registers: 32 rows of 16 bits or 16 of 32.
+template <int TYPE, int HD> struct Tile {
+    static constexpr int G = HD / 16;
+    static constexpr bool kWide = TYPE == NUT_F32;
+    static constexpr int kRows = kWide ? 16 : 32;
+    static constexpr int kScores = kRows / 4;            // of a lane
+    static constexpr int kKeys = kWide ? HD / 16 : HD / 16; // 16-byte pieces of K
+    static constexpr int kWords = kWide ? G : G / 2;     // of a V row
+    u32x4 k[kKeys];
+    uint32_t v[kScores][kWords];
+    uint32_t gone; // bits of the lane's scores whose row is masked
+
+    // FULL: the head dim is HD; else components beyond it count zero.
+    template <bool FULL>
+    __device__ __forceinline__ void load(const PagedView &kv, const size_t *at, int lane)
+    {
+        const int j = lane >> 4, c = lane & 15;
+        constexpr int kSize = kWide ? 4 : 2;
+        constexpr int kParts = kWide ? HD / 16 : HD / 32; // pieces of a row's 16 j .. 16 j + 15
+#pragma unroll
+        for (int sub = 0; sub < kRows / 16; sub++) {
+            const size_t row = at[16 * sub + c];
+            const char *p = kv.keys + (row == kNoRow ? 0 : row);
+#pragma unroll
+            for (int n = 0; n < kParts; n++) {
+                const uint32_t byte = n * 64 + j * 16;
+                const bool in = FULL || byte < kv.head_dim * kSize;
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(p + (in ? byte : 0));
+                k[sub * kParts + n] = in ? x : u32x4{0, 0, 0, 0};
+            }
+        }
+        gone = 0;
+#pragma unroll
+        for (int r = 0; r < kScores; r++) {
+            const size_t row = at[16 * (r / 4) + 4 * j + r % 4];
+            gone |= uint32_t(row == kNoRow) << r;
+            const char *p = kv.values + (row == kNoRow ? 0 : row);
+            constexpr int kPiece = kWords < 4 ? kWords : 4;
+#pragma unroll
+            for (int w = 0; w < kWords; w += kPiece) {
+                const uint32_t byte = (c * kWords + w) * 4;
+                const char *q = p + (FULL || byte < kv.head_dim * kSize ? byte : 0);
+                if constexpr (kPiece == 1) {
+                    v[r][w] = *reinterpret_cast<const uint32_t *>(q);
+                } else if constexpr (kPiece == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(q);
+                    v[r][w] = x[0], v[r][w + 1] = x[1];
+                } else {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(q);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[r][w + e] = x[e];
+                }
+            }
+        }
+    }
+};
+
+// The query of the lane's head as a matrix operand, scaled to base 2.
+template <int TYPE, int HD> struct Query {
+    static constexpr int kLimbs = TYPE == NUT_F32 ? 1 : TYPE == NUT_F16 ? 2 : 3;
+    static constexpr int kParts = TYPE == NUT_F32 ? HD / 16 : HD / 32;
+    u32x4 x[kParts][kLimbs];
+    int exponent = 0; // scores come out divided by 2^exponent
+
+    __device__ __forceinline__ void load(const float *q, bool valid, uint32_t head_dim,
+                                         float scale, int lane)
+    {
+        const int j = lane >> 4;
+        constexpr int kEach = TYPE == NUT_F32 ? 4 : 8;
+        float v[kParts][kEach];
+        float most = 0.0f;
+#pragma unroll
+        for (int n = 0; n < kParts; n++) {
+            const uint32_t d = n * 4 * kEach + j * kEach;
+#pragma unroll
+            for (int e = 0; e < kEach; e += 4) {
+                float4 f = make_float4(0, 0, 0, 0);
+                if (valid && d + e < head_dim)
+                    f = *reinterpret_cast<const float4 *>(q + d + e);
+                v[n][e] = f.x * scale, v[n][e + 1] = f.y * scale;
+                v[n][e + 2] = f.z * scale, v[n][e + 3] = f.w * scale;
+            }
+#pragma unroll
+            for (int e = 0; e < kEach; e++)
+                most = fmaxf(most, fabsf(v[n][e]));
+        }
+        if constexpr (TYPE == NUT_F32) {
+#pragma unroll
+            for (int n = 0; n < kParts; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    x[n][0][e] = __float_as_uint(v[n][e]);
+        } else {
+            most = max_over_rows(most);
+            if (TYPE == NUT_F16 && most > 0.0f && most < INFINITY)
+                exponent = ilogbf(most) - 13;
+#pragma unroll
+            for (int n = 0; n < kParts; n++) {
+                bool odd = false;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[n][e] = TYPE == NUT_F16 ? ldexpf(v[n][e], -exponent) : v[n][e];
+                    if (v[n][e] != v[n][e]) // cut to its upper half, a NaN may look infinite
+                        v[n][e] = __uint_as_float(0x7fc00000u);
+                    odd = odd || !(fabsf(v[n][e]) < INFINITY);
+                }
+                split<TYPE, kLimbs>(v[n], x[n]);
+                if (odd) { // inf - inf is not a limb
+#pragma unroll
+                    for (int l = 1; l < kLimbs; l++)
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            const uint32_t lo = fabsf(v[n][2 * w]) < INFINITY ? 0xffffu : 0;
+                            const uint32_t hi = fabsf(v[n][2 * w + 1]) < INFINITY ? 0xffff0000u : 0;
+                            x[n][l][w] &= lo | hi;
+                        }
+                }
+            }
+        }
+    }
+};
+
+template <int TYPE, int HD>
+__device__ __forceinline__ void attend(const Tile<TYPE, HD> &tile, const Query<TYPE, HD> &q,
+                                       Softmax<TYPE, HD> &sm, float *scores)
+{
+    using T = Tile<TYPE, HD>;
+    constexpr int G = T::G;
+    float s[T::kScores];
+    if constexpr (T::kWide) {
+        f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < T::kKeys; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(tile.k[n][e]),
+                                                           __uint_as_float(q.x[n][0][e]), acc, 0,
+                                                           0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            s[i] = acc[i];
+    } else {
+        constexpr int kParts = HD / 32;
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < kParts; n++)
+#pragma unroll
+                for (int l = Query<TYPE, HD>::kLimbs - 1; l >= 0; l--)
+                    acc = product<TYPE>(tile.k[sub * kParts + n], q.x[n][l], acc);
+            const bool odd = acc[0] + acc[1] + acc[2] + acc[3] != acc[0] + acc[1] + acc[2] + acc[3];
+            if (__any(odd)) {
+                // An infinite key: the first limb's product has the sum's sign, a
+                // later limb of zero, or of the other sign, makes it no number.
+                f32x4 first{0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < kParts; n++)
+                    first = product<TYPE>(tile.k[sub * kParts + n], q.x[n][0], first);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[i] = acc[i] != acc[i] ? first[i] : acc[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                s[4 * sub + i] = TYPE == NUT_F16 ? ldexpf(acc[i], q.exponent) : acc[i];
+        }
+    }
+    const bool masked = __any(tile.gone != 0);
+    if (masked) {
+#pragma unroll
+        for (int r = 0; r < T::kScores; r++)
+            s[r] = tile.gone >> r & 1 ? -INFINITY : s[r];
+    }
+    if (scores != nullptr) {
+#pragma unroll
+        for (int sub = 0; sub < T::kRows / 16; sub++)
+            *reinterpret_cast<float4 *>(scores + 16 * sub) =
+                make_float4(s[4 * sub], s[4 * sub + 1], s[4 * sub + 2], s[4 * sub + 3]);
+    }
+    float most = s[0];
+#pragma unroll
+    for (int r = 1; r < T::kScores; r++)
+        most = fmaxf(most, s[r]);
+    sm.raise(max_over_rows(most));
+    float p[8];
+#pragma unroll
+    for (int r = 0; r < T::kScores; r++) {
+        p[r] = __builtin_amdgcn_exp2f(s[r] - sm.ref);
+        sm.sum += p[r];
+    }
+    uint32_t v[T::kScores][T::kWords];
+#pragma unroll
+    for (int r = 0; r < T::kScores; r++)
+#pragma unroll
+        for (int w = 0; w < T::kWords; w++) // a masked row may hold NaN, and 0 NaN is NaN
+            v[r][w] = masked && (tile.gone >> r & 1) ? 0 : tile.v[r][w];
+    if constexpr (T::kWide) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < G; t++)
+                sm.o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][t]), p[r],
+                                                               sm.o[t], 0, 0, 0);
+    } else {
+        constexpr int kLimbs = Query<TYPE, HD>::kLimbs;
+        u32x4 limb[kLimbs];
+        split<TYPE, kLimbs>(p, limb);
+#pragma unroll
+        for (int t = 0; t < G; t++) {
+            u32x4 x; // component t of the eight rows
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                x[w] = __builtin_amdgcn_perm(v[2 * w + 1][t / 2], v[2 * w][t / 2],
+                                             t % 2 ? 0x07060302 : 0x05040100);
+#pragma unroll
+            for (int l = kLimbs - 1; l >= 0; l--)
+                sm.o[t] = product<TYPE>(x, limb[l], sm.o[t]);
+        }
+    }
+}
+
+template <int TYPE, int HD, bool FULL>
+__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a)
+{
+    using T = Tile<TYPE, HD>;
+    constexpr int G = T::G;
+    __shared__ size_t at[kMostRows];
+    __shared__ float joint[2][HD / 4 + 3][kWave];
+    const PagedView &kv = a.kv;
+    uint32_t id = blockIdx.x;
+    const uint32_t c = id % a.chunks;
+    id /= a.chunks;
+    const uint32_t tile16 = id % a.tiles;
+    id /= a.tiles;
+    const uint32_t h = id % kv.kv_heads, b = id / kv.kv_heads;
+    const uint32_t n = paged_length(kv, a.s, b, threadIdx.x == 0 && c == 0 && h == 0);
+    const uint32_t total = a.selected == nullptr ? n : a.top * kv.page_size;
+    const uint32_t begin = c * a.chunk;
+    if (begin >= total && c != 0)
+        return;
+    const uint32_t count = min(total - begin, a.chunk);
+    const int tiles = int((count + T::kRows - 1) / T::kRows);
+
+    // where the run's rows begin, so that pages need not fit tiles
+    for (uint32_t i = threadIdx.x; i < uint32_t(tiles) * T::kRows; i += 64 * kWaves) {
         size_t row = kNoRow;
-        if (i < total) {
-            int index = int(i / kv.page_size);
-            const uint32_t slot = i % kv.page_size;
-            if (selected != nullptr) {
-                index = selected[(size_t(b) * kv.kv_heads + h) * top + index];
-                if (index < -1 || index >= int((s.max_length - 1) / kv.page_size + 1))
+        if (i < count) {
+            int index = int((begin + i) / kv.page_size);
+            const uint32_t slot = (begin + i) % kv.page_size;
+            if (a.selected != nullptr) {
+                index = a.selected[(size_t(b) * kv.kv_heads + h) * a.top + index];
+                if (index < -1 || index >= int((a.s.max_length - 1) / kv.page_size + 1))
                     paged_flag(kv.status, kBadPage);
             }
             if (index >= 0 && uint64_t(index) * kv.page_size + slot < n)
-                row = paged_row(kv, s, b, uint32_t(index), slot, h);
+                row = paged_row(kv, a.s, b, uint32_t(index), slot, h);
         }
-        float score = -INFINITY;
-        if (row != kNoRow) {
-            score = 0.0f;
-            for (uint32_t d = 0; d < kv.head_dim; d++)
-                score = fmaf(q[d], component<TYPE>(kv.keys + row, d), score);
-        }
-        if (scores != nullptr && i < total)
-            scores[(size_t(b) * heads + hq) * score_stride + i] = score;
-        float top_here = wave_max(score);
-        if (t % kWave == 0)
-            red[t / kWave] = top_here;
-        __syncthreads();
-        top_here = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float now = fmaxf(most, top_here);
-        const float ref = now == -INFINITY ? 0.0f : now;
-        const float keep = most == -INFINITY ? 0.0f : expf(most - ref);
-        p[t] = expf(score - ref);
-        at[t] = row;
-        const float here = wave_sum(p[t]);
-        if (t % kWave == 0)
-            red[4 + t / kWave] = here;
-        __syncthreads();
-        sum = sum * keep + red[4] + red[5] + red[6] + red[7];
-        acc *= keep;
-        if (t < kv.head_dim)
-            for (uint32_t j = 0; j < min(256u, total - base); j++)
-                if (at[j] != kNoRow)
-                    acc = fmaf(p[j], component<TYPE>(kv.values + at[j], t), acc);
-        most = now;
+        at[i] = row;
     }
-    if (t < kv.head_dim)
-        out[(size_t(b) * heads + hq) * kv.head_dim + t] = sum == 0.0f ? 0.0f : acc / sum;
-    if (t == 0 && lse != nullptr)
-        lse[size_t(b) * heads + hq] = sum == 0.0f ? -INFINITY : most + logf(sum);
+
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int j = lane >> 4, column = lane & 15;
+    const uint32_t mine = tile16 * 16 + column;
+    const bool valid = mine < a.group;
+    const uint32_t head = h * a.group + (valid ? mine : 0);
+    Query<TYPE, HD> q;
+    q.load(a.query + b * a.query_stride + size_t(head) * kv.head_dim, valid, kv.head_dim, a.scale,
+           lane);
+    const size_t row = size_t(b) * a.heads + head;
+    float *scores = a.scores != nullptr && valid
+                        ? a.scores + row * a.chunks * a.chunk + begin + 4 * j
+                        : nullptr;
+    Softmax<TYPE, HD> sm;
+    __syncthreads();
+
+    const auto scores_of = [&](int t) {
+        return scores == nullptr ? nullptr : scores + t * T::kRows;
+    };
+    if constexpr (HD == 256) {
+        // one tile fills the registers
+        Tile<TYPE, HD> x;
+        for (int t = wave; t < tiles; t += kWaves) {
+            x.template load<FULL>(kv, at + t * T::kRows, lane);
+            attend<TYPE, HD>(x, q, sm, scores_of(t));
+        }
+    } else {
+        // two tiles in registers, the next one's loads in flight while one is used
+        Tile<TYPE, HD> x, y;
+        if (wave < tiles)
+            x.template load<FULL>(kv, at + wave * T::kRows, lane);
+        for (int t = wave; t < tiles; t += 2 * kWaves) {
+            if (t + kWaves < tiles)
+                y.template load<FULL>(kv, at + (t + kWaves) * T::kRows, lane);
+            attend<TYPE, HD>(x, q, sm, scores_of(t));
+            if (t + kWaves < tiles) {
+                if (t + 2 * kWaves < tiles)
+                    x.template load<FULL>(kv, at + (t + 2 * kWaves) * T::kRows, lane);
+                attend<TYPE, HD>(y, q, sm, scores_of(t + kWaves));
+            }
+        }
+    }
+    sm.sum += __shfl_xor(sm.sum, 16);
+    sm.sum += __shfl_xor(sm.sum, 32);
+
+    // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
+#pragma unroll
+    for (int step = kWaves / 2; step > 0; step /= 2) {
+        if (wave >= step && wave < 2 * step) {
+            float(*to)[kWave] = joint[wave - step];
+            to[0][lane] = sm.most, to[1][lane] = sm.ref, to[2][lane] = sm.sum;
+#pragma unroll
+            for (int t = 0; t < G; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    to[3 + 4 * t + i][lane] = sm.o[t][i];
+        }
+        __syncthreads();
+        if (wave < step) {
+            const float(*from)[kWave] = joint[wave];
+            const float most = from[0][lane];
+            sm.raise(most);
+            const float f = most == -INFINITY ? 1.0f
+                                              : __builtin_amdgcn_exp2f(from[1][lane] - sm.ref);
+            sm.sum = fmaf(from[2][lane], f, sm.sum);
+#pragma unroll
+            for (int t = 0; t < G; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    sm.o[t][i] = fmaf(from[3 + 4 * t + i][lane], f, sm.o[t][i]);
+        }
+        __syncthreads();
+    }
+    if (wave != 0 || !valid)
+        return;
+    const bool whole = a.parts == nullptr;
+    float f = 1.0f;
+    if (whole)
+        f = sm.sum == 0.0f ? 0.0f : 1.0f / sm.sum;
+    float *out = whole ? a.out + row * kv.head_dim : a.parts + (row * a.chunks + c) * kv.head_dim;
+    float flat[HD / 4]; // components 4 j G .. 4 j G + 4 G - 1 of the head
+#pragma unroll
+    for (int t = 0; t < G; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            flat[i * G + t] = sm.o[t][i] * f;
+#pragma unroll
+    for (int d = 0; d < HD / 4; d += 4)
+        if (FULL || uint32_t(j * (HD / 4) + d) < kv.head_dim)
+            *reinterpret_cast<float4 *>(out + j * (HD / 4) + d) =
+                make_float4(flat[d], flat[d + 1], flat[d + 2], flat[d + 3]);
+    if (j != 0)
+        return;
+    if (!whole)
+        a.stats[row * a.chunks + c] =
+            make_float2(sm.sum == 0.0f ? -INFINITY : sm.ref, sm.sum);
+    else if (a.lse != nullptr)
+        a.lse[row] = sm.sum == 0.0f ? -INFINITY
+                                    : (sm.ref + log2f(sm.sum)) * 0.69314718055994531f;
 }
 
-__global__ __launch_bounds__(256) void weigh_kernel(PagedView kv, PagedSeqs s, uint32_t heads,
-                                                    const float *__restrict__ scores,
-                                                    const float *__restrict__ lse,
-                                                    size_t score_stride, float *weights,
-                                                    size_t stride, uint32_t blocks)
+// The first batch x heads workgroups join a head's runs; the others, one per
+// (sequence, KV head, 1,024 rows), add the weights of theirs. Runs without a
+// row hold ref = -inf, and their sums are not read.
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, PagedHistory history,
+                                                   uint32_t joins, uint32_t blocks)
 {
-    const uint32_t c = blockIdx.x % blocks, h = blockIdx.x / blocks % kv.kv_heads;
-    const uint32_t b = blockIdx.x / blocks / kv.kv_heads, i = c * 256 + threadIdx.x;
-    const uint32_t group = heads / kv.kv_heads;
-    if (i >= paged_length(kv, s, b, false))
+    __shared__ float red[64];
+    __shared__ float acc[256][4];
+    const PagedView &kv = a.kv;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if (blockIdx.x < joins) {
+        const uint32_t row = blockIdx.x, b = row / a.heads;
+        const uint32_t n = paged_length(kv, a.s, b, false);
+        const uint32_t total = a.selected == nullptr ? n : a.top * kv.page_size;
+        const uint32_t runs = (total + a.chunk - 1) / a.chunk;
+        const float2 *stats = a.stats + size_t(row) * a.chunks;
+        float most = -INFINITY;
+        for (uint32_t i = threadIdx.x; i < runs; i += 256)
+            most = fmaxf(most, stats[i].x);
+        most = wave_max(most);
+        if (lane == 0)
+            red[wave] = most;
+        __syncthreads();
+        most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const uint32_t tpr = kv.head_dim / 4, part = threadIdx.x % tpr, g = threadIdx.x / tpr;
+        const uint32_t groups = 256 / tpr;
+        float sum = 0.0f;
+        f32x4 o{0, 0, 0, 0};
+        if (g < groups)
+            for (uint32_t i = g; i < runs; i += groups) {
+                const float2 st = stats[i];
+                if (st.x == -INFINITY)
+                    continue;
+                const float f = __builtin_amdgcn_exp2f(st.x - most);
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(
+                    a.parts + (size_t(row) * a.chunks + i) * kv.head_dim + part * 4);
+                sum = fmaf(st.y, f, sum);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o[e] = fmaf(x[e], f, o[e]);
+            }
+        *reinterpret_cast<f32x4 *>(acc[threadIdx.x]) = o;
+        __syncthreads();
+        for (uint32_t i = 1; g == 0 && i < groups; i++)
+            o += *reinterpret_cast<const f32x4 *>(acc[i * tpr + part]);
+        __syncthreads();
+        acc[threadIdx.x][0] = sum;
+        __syncthreads();
+        if (g != 0)
+            return;
+        for (uint32_t i = 1; i < groups; i++)
+            sum += acc[i * tpr + part][0];
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        *reinterpret_cast<f32x4 *>(a.out + size_t(row) * kv.head_dim + part * 4) = o * f;
+        if (part == 0 && a.lse != nullptr)
+            a.lse[row] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
         return;
-    float w = 0.0f;
-    for (uint32_t j = 0; j < group; j++) {
-        const size_t head = size_t(b) * heads + h * group + j;
-        if (lse[head] != -INFINITY)
-            w += expf(scores[head * score_stride + i] - lse[head]);
     }
-    weights[(size_t(b) * kv.kv_heads + h) * stride + i] += w;
+    const uint32_t id = blockIdx.x - joins, c = id % blocks, h = id / blocks % kv.kv_heads;
+    const uint32_t b = id / blocks / kv.kv_heads;
+    const uint32_t n = paged_length(kv, a.s, b, false), first = c * 1024;
+    if (first >= n)
+        return;
+    const uint32_t runs = (n + a.chunk - 1) / a.chunk;
+    float grown[4] = {0, 0, 0, 0};
+    for (uint32_t base = 0; base < a.group; base += 64) {
+        const uint32_t here = min(64u, a.group - base);
+        const size_t row = size_t(b) * a.heads + h * a.group + base;
+        __syncthreads();
+        for (uint32_t g = wave; g < here; g += 4) {
+            const float2 *stats = a.stats + (row + g) * a.chunks;
+            float most = -INFINITY;
+            for (uint32_t i = lane; i < runs; i += kWave)
+                most = fmaxf(most, stats[i].x);
+            most = wave_max(most);
+            float sum = 0.0f;
+            for (uint32_t i = lane; i < runs; i += kWave)
+                if (stats[i].x != -INFINITY)
+                    sum = fmaf(stats[i].y, __builtin_amdgcn_exp2f(stats[i].x - most), sum);
+            sum = wave_sum(sum);
+            // no weight where nothing has any
+            if (lane == 0)
+                red[g] = sum == 0.0f ? INFINITY : most + log2f(sum);
+        }
+        __syncthreads();
+        for (uint32_t g = 0; g < here; g++) {
+            const float *scores = a.scores + (row + g) * a.chunks * a.chunk + first;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (first + e * 256 + threadIdx.x < n)
+                    grown[e] += __builtin_amdgcn_exp2f(scores[e * 256 + threadIdx.x] - red[g]);
+        }
+    }
+    float *weights = history.weights + (size_t(b) * kv.kv_heads + h) * history.stride + first;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (first + e * 256 + threadIdx.x < n)
+            weights[e * 256 + threadIdx.x] += grown[e];
+}
+
+template <int TYPE, int HD>
+void attend_as(const AttendArgs &a, dim3 grid, hipStream_t stream)
+{
+    const auto kernel = a.kv.head_dim == HD ? attend_kernel<TYPE, HD, true>
+                                            : attend_kernel<TYPE, HD, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, a);
+}
+
+template <int TYPE> void attend_in(const AttendArgs &a, dim3 grid, hipStream_t stream)
+{
+    if (a.kv.head_dim <= 32)
+        attend_as<TYPE, 32>(a, grid, stream);
+    else if (a.kv.head_dim <= 64)
+        attend_as<TYPE, 64>(a, grid, stream);
+    else if (a.kv.head_dim <= 128)
+        attend_as<TYPE, 128>(a, grid, stream);
+    else
+        attend_as<TYPE, 256>(a, grid, stream);
 }
 
 } // namespace
@@ -118,11 +627,23 @@ __global__ __launch_bounds__(256) void weigh_kernel(PagedView kv, PagedSeqs s, u
 AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_t heads,
                              uint32_t top, bool weighted)
 {
-    (void)kv, (void)top;
+    const auto aligned = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
     AttentionPlan plan{};
-    plan.stats = 0;
-    plan.scores = (size_t(seqs.batch) * heads * sizeof(float) + 255) / 256 * 256;
-    plan.bytes = weighted ? plan.scores + size_t(seqs.batch) * heads * seqs.max_length * 4 : 0;
+    const uint32_t group = heads / kv.kv_heads, rows = top == 0 ? seqs.max_length
+                                                                : top * kv.page_size;
+    plan.tiles = (group + 15) / 16;
+    plan.chunk = kMostRows;
+    while (plan.chunk > 128 && uint64_t(seqs.batch) * kv.kv_heads * plan.tiles *
+                                       ((rows + plan.chunk - 1) / plan.chunk) <
+                                   1024)
+        plan.chunk /= 2;
+    plan.chunks = (rows + plan.chunk - 1) / plan.chunk;
+    if (plan.chunks == 1 && !weighted)
+        return plan;
+    const size_t runs = size_t(seqs.batch) * heads * plan.chunks;
+    plan.stats = aligned(runs * kv.head_dim * sizeof(float));
+    plan.scores = plan.stats + aligned(runs * sizeof(float2));
+    plan.bytes = plan.scores + (weighted ? aligned(runs * plan.chunk * sizeof(float)) : 0);
     return plan;
 }
 
@@ -133,23 +654,31 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
 {
     const bool weighted = history.weights != nullptr;
     const AttentionPlan plan = plan_attention(kv, seqs, heads, top, weighted);
-    float *scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
-    if (weighted && lse == nullptr)
-        lse = reinterpret_cast<float *>(workspace);
-    const auto kernel = kv.type == NUT_F32   ? attend_kernel<NUT_F32>
-                        : kv.type == NUT_F16 ? attend_kernel<NUT_F16>
-                                             : attend_kernel<NUT_BF16>;
-    hipLaunchKernelGGL(kernel, paged_grid(uint64_t(seqs.batch) * heads, 256), dim3(256), 0, stream,
-                       kv, seqs, query, query_stride, heads, scale, selected, top, out, lse,
-                       scores, size_t(seqs.max_length));
+    const bool split = plan.bytes != 0;
+    AttendArgs a{kv, seqs, query, query_stride, heads, heads / kv.kv_heads,
+                 scale * 1.4426950408889634f, selected, top, out, lse, plan.chunk, plan.chunks,
+                 plan.tiles, nullptr, nullptr, nullptr};
+    if (split) {
+        a.parts = reinterpret_cast<float *>(workspace);
+        a.stats = reinterpret_cast<float2 *>(workspace + plan.stats);
+        a.scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
+    }
+    const dim3 grid = paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks,
+                                 64 * kWaves);
+    const uint32_t blocks = weighted ? (seqs.max_length + 1023) / 1024 : 0;
+    const uint64_t joins = uint64_t(seqs.batch) * heads;
+    const dim3 join = paged_grid(joins + uint64_t(seqs.batch) * kv.kv_heads * blocks, 256);
+    if (kv.type == NUT_F32)
+        attend_in<NUT_F32>(a, grid, stream);
+    else if (kv.type == NUT_F16)
+        attend_in<NUT_F16>(a, grid, stream);
+    else
+        attend_in<NUT_BF16>(a, grid, stream);
     check_launch("paged attention");
-    if (!weighted)
+    if (!split)
         return;
-    const uint32_t blocks = (seqs.max_length + 255) / 256;
-    hipLaunchKernelGGL(weigh_kernel,
-                       paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
-                       stream, kv, seqs, heads, scores, lse, size_t(seqs.max_length),
-                       history.weights, history.stride, blocks);
+    hipLaunchKernelGGL(join_kernel, join, dim3(256), 0, stream, a, history, uint32_t(joins),
+                       blocks);
     check_launch("paged attention");
 }
 
