@@ -33,7 +33,6 @@ namespace nut {
 
 namespace {
 
-constexpr int kWaves = 4;
 constexpr uint32_t kMostRows = 1024; // of a run
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -176,7 +175,8 @@ template <int TYPE, int HD> struct Tile {
             const size_t row = at[16 * (r / 4) + 4 * j + r % 4];
             gone |= uint32_t(row == kNoRow) << r;
             const char *p = kv.values + (row == kNoRow ? 0 : row);
-            constexpr int kPiece = kWords < 4 ? kWords : 4;
+            // pieces of a power of two words divide a row of 8 n components
+            constexpr int kPiece = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;
 #pragma unroll
             for (int w = 0; w < kWords; w += kPiece) {
                 const uint32_t byte = (c * kWords + w) * 4;
@@ -201,16 +201,14 @@ template <int TYPE, int HD> struct Tile {
 template <int TYPE, int HD> struct Query {
     static constexpr int kLimbs = TYPE == NUT_F32 ? 1 : TYPE == NUT_F16 ? 2 : 3;
     static constexpr int kParts = TYPE == NUT_F32 ? HD / 16 : HD / 32;
+    static constexpr int kEach = TYPE == NUT_F32 ? 4 : 8;
+    float v[kParts][kEach]; // as it was read
     u32x4 x[kParts][kLimbs];
     int exponent = 0; // scores come out divided by 2^exponent
 
-    __device__ __forceinline__ void load(const float *q, bool valid, uint32_t head_dim,
-                                         float scale, int lane)
+    __device__ __forceinline__ void fetch(const float *q, bool valid, uint32_t head_dim, int lane)
     {
         const int j = lane >> 4;
-        constexpr int kEach = TYPE == NUT_F32 ? 4 : 8;
-        float v[kParts][kEach];
-        float most = 0.0f;
 #pragma unroll
         for (int n = 0; n < kParts; n++) {
             const uint32_t d = n * 4 * kEach + j * kEach;
@@ -219,13 +217,20 @@ template <int TYPE, int HD> struct Query {
                 float4 f = make_float4(0, 0, 0, 0);
                 if (valid && d + e < head_dim)
                     f = *reinterpret_cast<const float4 *>(q + d + e);
-                v[n][e] = f.x * scale, v[n][e + 1] = f.y * scale;
-                v[n][e + 2] = f.z * scale, v[n][e + 3] = f.w * scale;
+                v[n][e] = f.x, v[n][e + 1] = f.y, v[n][e + 2] = f.z, v[n][e + 3] = f.w;
             }
-#pragma unroll
-            for (int e = 0; e < kEach; e++)
-                most = fmaxf(most, fabsf(v[n][e]));
         }
+    }
+    __device__ __forceinline__ void convert(float scale)
+    {
+        float most = 0.0f;
+#pragma unroll
+        for (int n = 0; n < kParts; n++)
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                v[n][e] *= scale;
+                most = fmaxf(most, fabsf(v[n][e]));
+            }
         if constexpr (TYPE == NUT_F32) {
 #pragma unroll
             for (int n = 0; n < kParts; n++)
@@ -362,244 +367,318 @@ __device__ __forceinline__ void attend(const Tile<TYPE, HD> &tile, const Query<T
     }
 }
 
+// Where row i of a run lies: page `index` of the sequence (-1: none, -2: one
+// that no table row has), and what the table says of it.
+struct Place {
+    int index, page;
+    uint32_t slot;
+};
+
+__device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t b, uint32_t h, uint32_t i,
+                                          uint32_t most, uint32_t pages)
+{
+    Place p{-1, -1, 0};
+    if (i >= most)
+        return p;
+    p.index = int(i / a.kv.page_size);
+    p.slot = i - uint32_t(p.index) * a.kv.page_size;
+    if (a.selected != nullptr) {
+        p.index = a.selected[(size_t(b) * a.kv.kv_heads + h) * a.top + p.index];
+        if (p.index < -1 || p.index >= int(pages))
+            p.index = -2;
+    }
+    if (p.index >= 0)
+        p.page = a.s.table[size_t(b) * a.s.table_stride + p.index];
+    return p;
+}
+
+// Waves of a workgroup: their sums have to fit its 64 KB of shared memory.
+template <int HD> constexpr int kWavesOf = HD == 256 ? 2 : 4;
+
 template <int TYPE, int HD, bool FULL>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a)
+__global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
 {
     using T = Tile<TYPE, HD>;
-    constexpr int G = T::G;
-    __shared__ size_t at[kMostRows];
-    __shared__ float joint[2][HD / 4 + 3][kWave];
+    constexpr int G = T::G, kWaves = kWavesOf<HD>, kThreads = 64 * kWaves;
+    constexpr int kStride = HD + 4; // of a head's sums: 16 lanes' rows on all banks
+    // the rows' offsets, and when they are done with the waves' sums
+    __shared__ union Shared {
+        size_t at[kMostRows];
+        float o[kWaves][16][kStride];
+    } lds;
+    __shared__ float stat[3][kWaves][16];
     const PagedView &kv = a.kv;
-    uint32_t id = blockIdx.x;
-    const uint32_t c = id % a.chunks;
-    id /= a.chunks;
+    // A sequence's runs one after another, begun one further for each: workgroups
+    // go to the 8 XCDs in turn, and if every sequence's runs began alike, the
+    // late runs, which short sequences have not, would all be one XCD's.
+    uint32_t id = blockIdx.x / a.chunks;
+    const uint32_t c = (blockIdx.x + id) % a.chunks;
     const uint32_t tile16 = id % a.tiles;
     id /= a.tiles;
     const uint32_t h = id % kv.kv_heads, b = id / kv.kv_heads;
-    const uint32_t n = paged_length(kv, a.s, b, threadIdx.x == 0 && c == 0 && h == 0);
-    const uint32_t total = a.selected == nullptr ? n : a.top * kv.page_size;
     const uint32_t begin = c * a.chunk;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int j = lane >> 4, column = lane & 15;
+    const uint32_t first = tile16 * 16, here = min(16u, a.group - first);
+    const bool valid = uint32_t(column) < here;
+    const size_t row = size_t(b) * a.heads + h * a.group + first;
+    const size_t mine = row + (valid ? column : 0);
+    Query<TYPE, HD> q;
+    q.fetch(a.query + b * a.query_stride + (mine - size_t(b) * a.heads) * kv.head_dim, valid,
+            kv.head_dim, lane);
+
+    // Where the run's rows begin, so that pages need not fit tiles. The first
+    // entries of the table are fetched beside the length, not after it: what
+    // lies behind the length is not used.
+    const uint32_t most = a.selected == nullptr ? a.s.max_length : a.top * kv.page_size;
+    const uint32_t pages = (a.s.max_length - 1) / kv.page_size + 1;
+    Place place = place_of(a, b, h, begin + threadIdx.x, most, pages);
+    const uint32_t n = paged_length(kv, a.s, b, threadIdx.x == 0 && c == 0 && h == 0);
+    asm volatile("" : "+v"(place.page));
+    const uint32_t total = a.selected == nullptr ? n : most;
     if (begin >= total && c != 0)
         return;
     const uint32_t count = min(total - begin, a.chunk);
     const int tiles = int((count + T::kRows - 1) / T::kRows);
-
-    // where the run's rows begin, so that pages need not fit tiles
-    for (uint32_t i = threadIdx.x; i < uint32_t(tiles) * T::kRows; i += 64 * kWaves) {
+    for (uint32_t i = threadIdx.x; i < uint32_t(tiles) * T::kRows; i += kThreads) {
+        if (i >= kThreads)
+            place = place_of(a, b, h, begin + i, most, pages);
         size_t row = kNoRow;
-        if (i < count) {
-            int index = int((begin + i) / kv.page_size);
-            const uint32_t slot = (begin + i) % kv.page_size;
-            if (a.selected != nullptr) {
-                index = a.selected[(size_t(b) * kv.kv_heads + h) * a.top + index];
-                if (index < -1 || index >= int((a.s.max_length - 1) / kv.page_size + 1))
-                    paged_flag(kv.status, kBadPage);
-            }
-            if (index >= 0 && uint64_t(index) * kv.page_size + slot < n)
-                row = paged_row(kv, a.s, b, uint32_t(index), slot, h);
+        if (i < count && place.index < -1)
+            paged_flag(kv.status, kBadPage);
+        if (i < count && place.index >= 0 &&
+            uint64_t(place.index) * kv.page_size + place.slot < n) {
+            if (place.page >= 0 && uint32_t(place.page) < kv.pages)
+                row = size_t(place.page) * kv.page_stride + h * kv.head_stride +
+                      place.slot * kv.slot_stride;
+            else
+                paged_flag(kv.status, kBadPage);
         }
-        at[i] = row;
+        lds.at[i] = row;
     }
 
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int j = lane >> 4, column = lane & 15;
-    const uint32_t mine = tile16 * 16 + column;
-    const bool valid = mine < a.group;
-    const uint32_t head = h * a.group + (valid ? mine : 0);
-    Query<TYPE, HD> q;
-    q.load(a.query + b * a.query_stride + size_t(head) * kv.head_dim, valid, kv.head_dim, a.scale,
-           lane);
-    const size_t row = size_t(b) * a.heads + head;
     float *scores = a.scores != nullptr && valid
-                        ? a.scores + row * a.chunks * a.chunk + begin + 4 * j
+                        ? a.scores + mine * a.chunks * a.chunk + begin + 4 * j
                         : nullptr;
     Softmax<TYPE, HD> sm;
     __syncthreads();
-
-    const auto scores_of = [&](int t) {
-        return scores == nullptr ? nullptr : scores + t * T::kRows;
-    };
-    if constexpr (HD == 256) {
-        // one tile fills the registers
-        Tile<TYPE, HD> x;
-        for (int t = wave; t < tiles; t += kWaves) {
-            x.template load<FULL>(kv, at + t * T::kRows, lane);
-            attend<TYPE, HD>(x, q, sm, scores_of(t));
-        }
-    } else {
-        // two tiles in registers, the next one's loads in flight while one is used
-        Tile<TYPE, HD> x, y;
-        if (wave < tiles)
-            x.template load<FULL>(kv, at + wave * T::kRows, lane);
-        for (int t = wave; t < tiles; t += 2 * kWaves) {
-            if (t + kWaves < tiles)
-                y.template load<FULL>(kv, at + (t + kWaves) * T::kRows, lane);
-            attend<TYPE, HD>(x, q, sm, scores_of(t));
-            if (t + kWaves < tiles) {
-                if (t + 2 * kWaves < tiles)
-                    x.template load<FULL>(kv, at + (t + 2 * kWaves) * T::kRows, lane);
-                attend<TYPE, HD>(y, q, sm, scores_of(t + kWaves));
-            }
-        }
+    // One tile in registers a wave: the other waves of the SIMD (four and more
+    // up to 64 components) keep loads in flight. A second tile in registers
+    // cost their places: 378 us for 337 where both were measured.
+    Tile<TYPE, HD> x;
+    if (wave < tiles)
+        x.template load<FULL>(kv, lds.at + wave * T::kRows, lane);
+    q.convert(a.scale);
+    for (int t = wave; t < tiles;) {
+        attend<TYPE, HD>(x, q, sm, scores == nullptr ? nullptr : scores + t * T::kRows);
+        t += kWaves;
+        if (t < tiles)
+            x.template load<FULL>(kv, lds.at + t * T::kRows, lane);
     }
     sm.sum += __shfl_xor(sm.sum, 16);
     sm.sum += __shfl_xor(sm.sum, 32);
 
-    // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
+    // The waves' sums side by side; then a thread per four components adds them.
+    __syncthreads();
+    if (j == 0)
+        stat[0][wave][column] = sm.most, stat[1][wave][column] = sm.ref,
+        stat[2][wave][column] = sm.sum;
+    {
+        float flat[HD / 4]; // components 4 j G .. 4 j G + 4 G - 1 of the lane's head
 #pragma unroll
-    for (int step = kWaves / 2; step > 0; step /= 2) {
-        if (wave >= step && wave < 2 * step) {
-            float(*to)[kWave] = joint[wave - step];
-            to[0][lane] = sm.most, to[1][lane] = sm.ref, to[2][lane] = sm.sum;
+        for (int t = 0; t < G; t++)
 #pragma unroll
-            for (int t = 0; t < G; t++)
+            for (int i = 0; i < 4; i++)
+                flat[i * G + t] = sm.o[t][i];
+        float *to = lds.o[wave][column] + j * (HD / 4);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    to[3 + 4 * t + i][lane] = sm.o[t][i];
-        }
-        __syncthreads();
-        if (wave < step) {
-            const float(*from)[kWave] = joint[wave];
-            const float most = from[0][lane];
-            sm.raise(most);
-            const float f = most == -INFINITY ? 1.0f
-                                              : __builtin_amdgcn_exp2f(from[1][lane] - sm.ref);
-            sm.sum = fmaf(from[2][lane], f, sm.sum);
-#pragma unroll
-            for (int t = 0; t < G; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    sm.o[t][i] = fmaf(from[3 + 4 * t + i][lane], f, sm.o[t][i]);
-        }
-        __syncthreads();
+        for (int d = 0; d < HD / 4; d += 4)
+            *reinterpret_cast<f32x4 *>(to + d) =
+                f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
     }
-    if (wave != 0 || !valid)
-        return;
-    const bool whole = a.parts == nullptr;
-    float f = 1.0f;
-    if (whole)
-        f = sm.sum == 0.0f ? 0.0f : 1.0f / sm.sum;
-    float *out = whole ? a.out + row * kv.head_dim : a.parts + (row * a.chunks + c) * kv.head_dim;
-    float flat[HD / 4]; // components 4 j G .. 4 j G + 4 G - 1 of the head
+    __syncthreads();
+    const uint32_t parts = kv.head_dim / 4;
+    for (uint32_t i = threadIdx.x; i < here * parts; i += kThreads) {
+        const uint32_t head = i / parts, d = i % parts * 4;
+        float most = stat[0][0][head];
 #pragma unroll
-    for (int t = 0; t < G; t++)
+        for (int w = 1; w < kWaves; w++)
+            most = fmaxf(most, stat[0][w][head]);
+        const float ref = most == -INFINITY ? 0.0f : most - Softmax<TYPE, HD>::kShift;
+        float sum = 0.0f;
+        f32x4 o{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            flat[i * G + t] = sm.o[t][i] * f;
+        for (int w = 0; w < kWaves; w++) {
+            // what no row of a finite score reached is zero, or not a number
+            const float f = stat[0][w][head] == -INFINITY
+                                ? 1.0f
+                                : __builtin_amdgcn_exp2f(stat[1][w][head] - ref);
+            sum = fmaf(stat[2][w][head], f, sum);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&lds.o[w][head][d]);
 #pragma unroll
-    for (int d = 0; d < HD / 4; d += 4)
-        if (FULL || uint32_t(j * (HD / 4) + d) < kv.head_dim)
-            *reinterpret_cast<float4 *>(out + j * (HD / 4) + d) =
-                make_float4(flat[d], flat[d + 1], flat[d + 2], flat[d + 3]);
-    if (j != 0)
-        return;
-    if (!whole)
-        a.stats[row * a.chunks + c] =
-            make_float2(sm.sum == 0.0f ? -INFINITY : sm.ref, sm.sum);
-    else if (a.lse != nullptr)
-        a.lse[row] = sm.sum == 0.0f ? -INFINITY
-                                    : (sm.ref + log2f(sm.sum)) * 0.69314718055994531f;
+            for (int e = 0; e < 4; e++)
+                o[e] = fmaf(y[e], f, o[e]);
+        }
+        const size_t at = row + head;
+        if (a.parts != nullptr) {
+            *reinterpret_cast<f32x4 *>(a.parts + (at * a.chunks + c) * kv.head_dim + d) = o;
+            if (d == 0)
+                a.stats[at * a.chunks + c] = make_float2(sum == 0.0f ? -INFINITY : ref, sum);
+        } else {
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<f32x4 *>(a.out + at * kv.head_dim + d) = o * f;
+            if (d == 0 && a.lse != nullptr)
+                a.lse[at] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
+        }
+    }
 }
 
-// The first batch x heads workgroups join a head's runs; the others, one per
-// (sequence, KV head, 1,024 rows), add the weights of theirs. Runs without a
-// row hold ref = -inf, and their sums are not read.
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, PagedHistory history,
-                                                   uint32_t joins, uint32_t blocks)
+// One head's runs joined: tpr = head_dim / 4 threads hold four components each,
+// and the workgroup's groups of tpr threads take runs in turn. The first
+// run of a group is fetched beside the length, before it is known to count.
+__device__ __forceinline__ void join_head(const AttendArgs &a, uint32_t row, float *red,
+                                          f32x4 *acc)
 {
-    __shared__ float red[64];
-    __shared__ float acc[256][4];
     const PagedView &kv = a.kv;
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    if (blockIdx.x < joins) {
-        const uint32_t row = blockIdx.x, b = row / a.heads;
-        const uint32_t n = paged_length(kv, a.s, b, false);
-        const uint32_t total = a.selected == nullptr ? n : a.top * kv.page_size;
-        const uint32_t runs = (total + a.chunk - 1) / a.chunk;
-        const float2 *stats = a.stats + size_t(row) * a.chunks;
-        float most = -INFINITY;
-        for (uint32_t i = threadIdx.x; i < runs; i += 256)
-            most = fmaxf(most, stats[i].x);
-        most = wave_max(most);
+    const uint32_t waves = blockDim.x / kWave, tpr = kv.head_dim / 4;
+    const uint32_t part = threadIdx.x % tpr, g = threadIdx.x / tpr, groups = blockDim.x / tpr;
+    const float2 *stats = a.stats + size_t(row) * a.chunks;
+    const f32x4 *parts =
+        reinterpret_cast<const f32x4 *>(a.parts + size_t(row) * a.chunks * kv.head_dim) + part;
+    float2 own{-INFINITY, 0.0f};
+    if (threadIdx.x < a.chunks)
+        own = stats[threadIdx.x];
+    f32x4 ahead{0, 0, 0, 0};
+    if (g < groups && g < a.chunks)
+        ahead = parts[g * tpr];
+    const uint32_t n = paged_length(kv, a.s, row / a.heads, false);
+    asm volatile("" : "+v"(own.x), "+v"(own.y), "+v"(ahead));
+    const uint32_t total = a.selected == nullptr ? n : a.top * kv.page_size;
+    const uint32_t runs = (total + a.chunk - 1) / a.chunk;
+
+    // Runs that no row of a finite score reached hold ref = -inf: their sums
+    // are not read.
+    float most = threadIdx.x < runs ? own.x : -INFINITY;
+    for (uint32_t i = threadIdx.x + blockDim.x; i < runs; i += blockDim.x)
+        most = fmaxf(most, stats[i].x);
+    most = wave_max(most);
+    if (waves > 1) {
         if (lane == 0)
             red[wave] = most;
         __syncthreads();
-        most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const uint32_t tpr = kv.head_dim / 4, part = threadIdx.x % tpr, g = threadIdx.x / tpr;
-        const uint32_t groups = 256 / tpr;
-        float sum = 0.0f;
-        f32x4 o{0, 0, 0, 0};
-        if (g < groups)
-            for (uint32_t i = g; i < runs; i += groups) {
-                const float2 st = stats[i];
-                if (st.x == -INFINITY)
-                    continue;
-                const float f = __builtin_amdgcn_exp2f(st.x - most);
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(
-                    a.parts + (size_t(row) * a.chunks + i) * kv.head_dim + part * 4);
-                sum = fmaf(st.y, f, sum);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    o[e] = fmaf(x[e], f, o[e]);
-            }
-        *reinterpret_cast<f32x4 *>(acc[threadIdx.x]) = o;
-        __syncthreads();
-        for (uint32_t i = 1; g == 0 && i < groups; i++)
-            o += *reinterpret_cast<const f32x4 *>(acc[i * tpr + part]);
-        __syncthreads();
-        acc[threadIdx.x][0] = sum;
-        __syncthreads();
-        if (g != 0)
-            return;
-        for (uint32_t i = 1; i < groups; i++)
-            sum += acc[i * tpr + part][0];
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-        *reinterpret_cast<f32x4 *>(a.out + size_t(row) * kv.head_dim + part * 4) = o * f;
-        if (part == 0 && a.lse != nullptr)
-            a.lse[row] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
-        return;
+        for (uint32_t w = 0; w < waves; w++)
+            most = fmaxf(most, red[w]);
     }
-    const uint32_t id = blockIdx.x - joins, c = id % blocks, h = id / blocks % kv.kv_heads;
-    const uint32_t b = id / blocks / kv.kv_heads;
-    const uint32_t n = paged_length(kv, a.s, b, false), first = c * 1024;
-    if (first >= n)
-        return;
-    const uint32_t runs = (n + a.chunk - 1) / a.chunk;
-    float grown[4] = {0, 0, 0, 0};
-    for (uint32_t base = 0; base < a.group; base += 64) {
-        const uint32_t here = min(64u, a.group - base);
-        const size_t row = size_t(b) * a.heads + h * a.group + base;
-        __syncthreads();
-        for (uint32_t g = wave; g < here; g += 4) {
-            const float2 *stats = a.stats + (row + g) * a.chunks;
-            float most = -INFINITY;
-            for (uint32_t i = lane; i < runs; i += kWave)
-                most = fmaxf(most, stats[i].x);
-            most = wave_max(most);
-            float sum = 0.0f;
-            for (uint32_t i = lane; i < runs; i += kWave)
-                if (stats[i].x != -INFINITY)
-                    sum = fmaf(stats[i].y, __builtin_amdgcn_exp2f(stats[i].x - most), sum);
-            sum = wave_sum(sum);
-            // no weight where nothing has any
-            if (lane == 0)
-                red[g] = sum == 0.0f ? INFINITY : most + log2f(sum);
-        }
-        __syncthreads();
-        for (uint32_t g = 0; g < here; g++) {
-            const float *scores = a.scores + (row + g) * a.chunks * a.chunk + first;
+    float sum = 0.0f;
+    f32x4 o{0, 0, 0, 0};
+    if (g < groups)
+        for (uint32_t i = g; i < runs; i += groups) {
+            const float2 st = stats[i];
+            const f32x4 x = i == g ? ahead : parts[i * tpr];
+            if (st.x == -INFINITY)
+                continue;
+            const float f = __builtin_amdgcn_exp2f(st.x - most);
+            sum = fmaf(st.y, f, sum);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (first + e * 256 + threadIdx.x < n)
-                    grown[e] += __builtin_amdgcn_exp2f(scores[e * 256 + threadIdx.x] - red[g]);
+                o[e] = fmaf(x[e], f, o[e]);
         }
+    acc[2 * threadIdx.x] = o;
+    acc[2 * threadIdx.x + 1][0] = sum;
+    __syncthreads();
+    if (g != 0)
+        return;
+    for (uint32_t i = 1; i < groups; i++) {
+        o += acc[2 * (i * tpr + part)];
+        sum += acc[2 * (i * tpr + part) + 1][0];
     }
-    float *weights = history.weights + (size_t(b) * kv.kv_heads + h) * history.stride + first;
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<f32x4 *>(a.out + size_t(row) * kv.head_dim + part * 4) = o * f;
+    if (part == 0 && a.lse != nullptr)
+        a.lse[row] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
+}
+
+// The weights of four rows a thread, over the heads that share them, 8 at a
+// time: 8 lanes a head find its maximum and sum from the runs, while the
+// scores are on their way.
+__device__ __forceinline__ void weigh_rows(const AttendArgs &a, const PagedHistory &history,
+                                           uint32_t b, uint32_t h, uint32_t first, float *base)
+{
+    constexpr int kHeads = 8;
+    const PagedView &kv = a.kv;
+    const uint32_t n = paged_length(kv, a.s, b, false);
+    if (first >= n)
+        return;
+    const uint32_t runs = (n + a.chunk - 1) / a.chunk, span = a.chunks * a.chunk;
+    float grown[4] = {0, 0, 0, 0};
+    for (uint32_t g = 0; g < a.group; g += kHeads) {
+        const uint32_t here = min(uint32_t(kHeads), a.group - g);
+        const size_t row = size_t(b) * a.heads + h * a.group + g;
+        float s[kHeads][4];
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (first + e * 256 + threadIdx.x < n)
-            weights[e * 256 + threadIdx.x] += grown[e];
+        for (int k = 0; k < kHeads; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t i = first + e * blockDim.x + threadIdx.x;
+                s[k][e] = uint32_t(k) < here && i < n ? a.scores[(row + k) * span + i] : -INFINITY;
+            }
+        __syncthreads();
+        for (uint32_t k = threadIdx.x / 8; k < here; k += blockDim.x / 8) {
+            float most = -INFINITY, sum = 0.0f;
+            for (uint32_t i = threadIdx.x % 8; i < runs; i += 8) {
+                const float2 st = a.stats[(row + k) * a.chunks + i];
+                if (st.x == -INFINITY)
+                    continue;
+                const float now = fmaxf(most, st.x);
+                sum = sum * __builtin_amdgcn_exp2f(most - now) +
+                      st.y * __builtin_amdgcn_exp2f(st.x - now);
+                most = now;
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                const float m = __shfl_xor(most, o), z = __shfl_xor(sum, o);
+                const float now = fmaxf(most, m);
+                if (now != -INFINITY)
+                    sum = (most == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f(most - now)) +
+                          (m == -INFINITY ? 0.0f : z * __builtin_amdgcn_exp2f(m - now));
+                most = now;
+            }
+            // no weight where nothing has any
+            if (threadIdx.x % 8 == 0)
+                base[k] = most == -INFINITY ? INFINITY : most + log2f(sum);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kHeads; k++)
+            if (uint32_t(k) < here)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    grown[e] += __builtin_amdgcn_exp2f(s[k][e] - base[k]);
+    }
+    float *weights = history.weights + (size_t(b) * kv.kv_heads + h) * history.stride;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t i = first + e * blockDim.x + threadIdx.x;
+        if (i < n)
+            weights[i] += grown[e];
+    }
+}
+
+// The first batch x heads workgroups join a head's runs; the others, `blocks`
+// for each sequence and KV head, add the weights of 4 rows a thread.
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, PagedHistory history,
+                                                   uint32_t joins, uint32_t blocks)
+{
+    __shared__ float red[8];
+    __shared__ f32x4 acc[512];
+    if (blockIdx.x < joins) {
+        join_head(a, blockIdx.x, red, acc);
+    } else {
+        const uint32_t id = blockIdx.x - joins, h = id / blocks % a.kv.kv_heads;
+        weigh_rows(a, history, id / blocks / a.kv.kv_heads, h, id % blocks * 4 * blockDim.x, red);
+    }
 }
 
 template <int TYPE, int HD>
@@ -607,7 +686,7 @@ void attend_as(const AttendArgs &a, dim3 grid, hipStream_t stream)
 {
     const auto kernel = a.kv.head_dim == HD ? attend_kernel<TYPE, HD, true>
                                             : attend_kernel<TYPE, HD, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWavesOf<HD>), 0, stream, a);
 }
 
 template <int TYPE> void attend_in(const AttendArgs &a, dim3 grid, hipStream_t stream)
@@ -616,6 +695,8 @@ template <int TYPE> void attend_in(const AttendArgs &a, dim3 grid, hipStream_t s
         attend_as<TYPE, 32>(a, grid, stream);
     else if (a.kv.head_dim <= 64)
         attend_as<TYPE, 64>(a, grid, stream);
+    else if (a.kv.head_dim <= 96)
+        attend_as<TYPE, 96>(a, grid, stream);
     else if (a.kv.head_dim <= 128)
         attend_as<TYPE, 128>(a, grid, stream);
     else
@@ -664,10 +745,12 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
         a.scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
     }
     const dim3 grid = paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks,
-                                 64 * kWaves);
-    const uint32_t blocks = weighted ? (seqs.max_length + 1023) / 1024 : 0;
+                                 256);
+    // a wave joins up to 16 runs of a head
+    const uint32_t threads = plan.chunks <= 16 ? 64 : 256;
+    const uint32_t blocks = weighted ? (seqs.max_length + 4 * threads - 1) / (4 * threads) : 0;
     const uint64_t joins = uint64_t(seqs.batch) * heads;
-    const dim3 join = paged_grid(joins + uint64_t(seqs.batch) * kv.kv_heads * blocks, 256);
+    const dim3 join = paged_grid(joins + uint64_t(seqs.batch) * kv.kv_heads * blocks, threads);
     if (kv.type == NUT_F32)
         attend_in<NUT_F32>(a, grid, stream);
     else if (kv.type == NUT_F16)
@@ -677,7 +760,7 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
     check_launch("paged attention");
     if (!split)
         return;
-    hipLaunchKernelGGL(join_kernel, join, dim3(256), 0, stream, a, history, uint32_t(joins),
+    hipLaunchKernelGGL(join_kernel, join, dim3(threads), 0, stream, a, history, uint32_t(joins),
                        blocks);
     check_launch("paged attention");
 }
