@@ -148,10 +148,15 @@ template <int TYPE, int HD> struct Tile {
     static constexpr int kWords = kWide ? G : G / 2;     // of a V row
     u32x4 k[kKeys];
     uint32_t v[kScores][kWords];
-    uint32_t gone; // bits of the lane's scores whose row is masked
 
-    // FULL: the head dim is HD; else components beyond it count zero.
-    template <bool FULL>
+    template <bool NT, typename V> static __device__ __forceinline__ V fetch(const char *p)
+    {
+        const V *q = reinterpret_cast<const V *>(p);
+        return NT ? __builtin_nontemporal_load(q) : *q;
+    }
+    // FULL: the head dim is HD; else components beyond it count zero. NT: past
+    // the caches' replacement.
+    template <bool FULL, bool NT>
     __device__ __forceinline__ void load(const PagedView &kv, const size_t *at, int lane)
     {
         const int j = lane >> 4, c = lane & 15;
@@ -159,22 +164,18 @@ template <int TYPE, int HD> struct Tile {
         constexpr int kParts = kWide ? HD / 16 : HD / 32; // pieces of a row's 16 j .. 16 j + 15
 #pragma unroll
         for (int sub = 0; sub < kRows / 16; sub++) {
-            const size_t row = at[16 * sub + c];
-            const char *p = kv.keys + (row == kNoRow ? 0 : row);
+            const char *p = kv.keys + at[16 * sub + c];
 #pragma unroll
             for (int n = 0; n < kParts; n++) {
                 const uint32_t byte = n * 64 + j * 16;
                 const bool in = FULL || byte < kv.head_dim * kSize;
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(p + (in ? byte : 0));
+                const u32x4 x = fetch<NT, u32x4>(p + (in ? byte : 0));
                 k[sub * kParts + n] = in ? x : u32x4{0, 0, 0, 0};
             }
         }
-        gone = 0;
 #pragma unroll
         for (int r = 0; r < kScores; r++) {
-            const size_t row = at[16 * (r / 4) + 4 * j + r % 4];
-            gone |= uint32_t(row == kNoRow) << r;
-            const char *p = kv.values + (row == kNoRow ? 0 : row);
+            const char *p = kv.values + at[16 * (r / 4) + 4 * j + r % 4];
             // pieces of a power of two words divide a row of 8 n components
             constexpr int kPiece = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;
 #pragma unroll
@@ -182,12 +183,12 @@ template <int TYPE, int HD> struct Tile {
                 const uint32_t byte = (c * kWords + w) * 4;
                 const char *q = p + (FULL || byte < kv.head_dim * kSize ? byte : 0);
                 if constexpr (kPiece == 1) {
-                    v[r][w] = *reinterpret_cast<const uint32_t *>(q);
+                    v[r][w] = fetch<NT, uint32_t>(q);
                 } else if constexpr (kPiece == 2) {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(q);
+                    const u32x2 x = fetch<NT, u32x2>(q);
                     v[r][w] = x[0], v[r][w + 1] = x[1];
                 } else {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(q);
+                    const u32x4 x = fetch<NT, u32x4>(q);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         v[r][w + e] = x[e];
@@ -223,13 +224,14 @@ template <int TYPE, int HD> struct Query {
     }
     __device__ __forceinline__ void convert(float scale)
     {
-        float most = 0.0f;
+        float most = 0.0f, odd = 0.0f;
 #pragma unroll
         for (int n = 0; n < kParts; n++)
 #pragma unroll
             for (int e = 0; e < kEach; e++) {
                 v[n][e] *= scale;
                 most = fmaxf(most, fabsf(v[n][e]));
+                odd = fmaf(v[n][e], 0.0f, odd); // not a number after one that is not finite
             }
         if constexpr (TYPE == NUT_F32) {
 #pragma unroll
@@ -238,38 +240,48 @@ template <int TYPE, int HD> struct Query {
                 for (int e = 0; e < 4; e++)
                     x[n][0][e] = __float_as_uint(v[n][e]);
         } else {
-            most = max_over_rows(most);
-            if (TYPE == NUT_F16 && most > 0.0f && most < INFINITY)
-                exponent = ilogbf(most) - 13;
+            if constexpr (TYPE == NUT_F16) {
+                most = max_over_rows(most);
+                if (most > 0.0f && most < INFINITY)
+                    exponent = ilogbf(most) - 13;
 #pragma unroll
-            for (int n = 0; n < kParts; n++) {
-                bool odd = false;
+                for (int n = 0; n < kParts; n++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    v[n][e] = TYPE == NUT_F16 ? ldexpf(v[n][e], -exponent) : v[n][e];
-                    if (v[n][e] != v[n][e]) // cut to its upper half, a NaN may look infinite
-                        v[n][e] = __uint_as_float(0x7fc00000u);
-                    odd = odd || !(fabsf(v[n][e]) < INFINITY);
-                }
+                    for (int e = 0; e < 8; e++)
+                        v[n][e] = ldexpf(v[n][e], -exponent);
+            }
+            const bool rare = __any(odd != odd);
+            if (rare) { // cut to its upper half, a NaN may look infinite
+#pragma unroll
+                for (int n = 0; n < kParts; n++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        v[n][e] = v[n][e] != v[n][e] ? __uint_as_float(0x7fc00000u) : v[n][e];
+            }
+#pragma unroll
+            for (int n = 0; n < kParts; n++)
                 split<TYPE, kLimbs>(v[n], x[n]);
-                if (odd) { // inf - inf is not a limb
+            if (rare) { // inf - inf is not a limb
 #pragma unroll
-                    for (int l = 1; l < kLimbs; l++)
+                for (int n = 0; n < kParts; n++)
 #pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const uint32_t lo = fabsf(v[n][2 * w]) < INFINITY ? 0xffffu : 0;
-                            const uint32_t hi = fabsf(v[n][2 * w + 1]) < INFINITY ? 0xffff0000u : 0;
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t lo = fabsf(v[n][2 * w]) < INFINITY ? 0xffffu : 0;
+                        const uint32_t hi = fabsf(v[n][2 * w + 1]) < INFINITY ? 0xffff0000u : 0;
+#pragma unroll
+                        for (int l = 1; l < kLimbs; l++)
                             x[n][l][w] &= lo | hi;
-                        }
-                }
+                    }
             }
         }
     }
 };
 
+// `gone`: bit r set where row r of the tile is masked, the same in every lane.
 template <int TYPE, int HD>
-__device__ __forceinline__ void attend(const Tile<TYPE, HD> &tile, const Query<TYPE, HD> &q,
-                                       Softmax<TYPE, HD> &sm, float *scores)
+__device__ __forceinline__ void attend(Tile<TYPE, HD> &tile, uint32_t gone,
+                                       const Query<TYPE, HD> &q, Softmax<TYPE, HD> &sm,
+                                       float *scores, int lane)
 {
     using T = Tile<TYPE, HD>;
     constexpr int G = T::G;
@@ -313,11 +325,16 @@ __device__ __forceinline__ void attend(const Tile<TYPE, HD> &tile, const Query<T
                 s[4 * sub + i] = TYPE == NUT_F16 ? ldexpf(acc[i], q.exponent) : acc[i];
         }
     }
-    const bool masked = __any(tile.gone != 0);
-    if (masked) {
+    if (gone != 0) { // a masked row may hold NaN, and 0 NaN is NaN
+        const uint32_t mine = gone >> (4 * (lane >> 4));
 #pragma unroll
-        for (int r = 0; r < T::kScores; r++)
-            s[r] = tile.gone >> r & 1 ? -INFINITY : s[r];
+        for (int r = 0; r < T::kScores; r++) {
+            const bool out = mine >> (16 * (r / 4) + r % 4) & 1;
+            s[r] = out ? -INFINITY : s[r];
+#pragma unroll
+            for (int w = 0; w < T::kWords; w++)
+                tile.v[r][w] = out ? 0 : tile.v[r][w];
+        }
     }
     if (scores != nullptr) {
 #pragma unroll
@@ -336,12 +353,7 @@ __device__ __forceinline__ void attend(const Tile<TYPE, HD> &tile, const Query<T
         p[r] = __builtin_amdgcn_exp2f(s[r] - sm.ref);
         sm.sum += p[r];
     }
-    uint32_t v[T::kScores][T::kWords];
-#pragma unroll
-    for (int r = 0; r < T::kScores; r++)
-#pragma unroll
-        for (int w = 0; w < T::kWords; w++) // a masked row may hold NaN, and 0 NaN is NaN
-            v[r][w] = masked && (tile.gone >> r & 1) ? 0 : tile.v[r][w];
+    const auto &v = tile.v;
     if constexpr (T::kWide) {
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -380,7 +392,7 @@ __device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t b, uint3
     Place p{-1, -1, 0};
     if (i >= most)
         return p;
-    p.index = int(i / a.kv.page_size);
+    p.index = int(page_of(a.kv, i));
     p.slot = i - uint32_t(p.index) * a.kv.page_size;
     if (a.selected != nullptr) {
         p.index = a.selected[(size_t(b) * a.kv.kv_heads + h) * a.top + p.index];
@@ -395,7 +407,7 @@ __device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t b, uint3
 // Waves of a workgroup: their sums have to fit its 64 KB of shared memory.
 template <int HD> constexpr int kWavesOf = HD == 256 ? 2 : 4;
 
-template <int TYPE, int HD, bool FULL>
+template <int TYPE, int HD, bool FULL, bool NT>
 __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
 {
     using T = Tile<TYPE, HD>;
@@ -407,15 +419,14 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
         float o[kWaves][16][kStride];
     } lds;
     __shared__ float stat[3][kWaves][16];
+    __shared__ uint32_t gone[kMostRows / 32]; // bit per row: masked
     const PagedView &kv = a.kv;
     // A sequence's runs one after another, begun one further for each: workgroups
     // go to the 8 XCDs in turn, and if every sequence's runs began alike, the
     // late runs, which short sequences have not, would all be one XCD's.
-    uint32_t id = blockIdx.x / a.chunks;
-    const uint32_t c = (blockIdx.x + id) % a.chunks;
-    const uint32_t tile16 = id % a.tiles;
-    id /= a.tiles;
-    const uint32_t h = id % kv.kv_heads, b = id / kv.kv_heads;
+    const uint32_t b = blockIdx.z, h = a.tiles == 1 ? blockIdx.y : blockIdx.y / a.tiles;
+    const uint32_t tile16 = blockIdx.y - h * a.tiles;
+    uint32_t c = (blockIdx.x + blockIdx.y + gridDim.y * b) % a.chunks;
     const uint32_t begin = c * a.chunk;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -432,7 +443,7 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
     // entries of the table are fetched beside the length, not after it: what
     // lies behind the length is not used.
     const uint32_t most = a.selected == nullptr ? a.s.max_length : a.top * kv.page_size;
-    const uint32_t pages = (a.s.max_length - 1) / kv.page_size + 1;
+    const uint32_t pages = page_of(kv, a.s.max_length - 1) + 1;
     Place place = place_of(a, b, h, begin + threadIdx.x, most, pages);
     const uint32_t n = paged_length(kv, a.s, b, threadIdx.x == 0 && c == 0 && h == 0);
     asm volatile("" : "+v"(place.page));
@@ -441,21 +452,26 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
         return;
     const uint32_t count = min(total - begin, a.chunk);
     const int tiles = int((count + T::kRows - 1) / T::kRows);
-    for (uint32_t i = threadIdx.x; i < uint32_t(tiles) * T::kRows; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < (count + kWave - 1) / kWave * kWave; i += kThreads) {
         if (i >= kThreads)
             place = place_of(a, b, h, begin + i, most, pages);
-        size_t row = kNoRow;
+        size_t at = 0;
+        bool out = true;
         if (i < count && place.index < -1)
             paged_flag(kv.status, kBadPage);
         if (i < count && place.index >= 0 &&
             uint64_t(place.index) * kv.page_size + place.slot < n) {
-            if (place.page >= 0 && uint32_t(place.page) < kv.pages)
-                row = size_t(place.page) * kv.page_stride + h * kv.head_stride +
-                      place.slot * kv.slot_stride;
+            out = place.page < 0 || uint32_t(place.page) >= kv.pages;
+            if (!out)
+                at = size_t(place.page) * kv.page_stride + h * kv.head_stride +
+                     place.slot * kv.slot_stride;
             else
                 paged_flag(kv.status, kBadPage);
         }
-        lds.at[i] = row;
+        lds.at[i] = at;
+        const uint64_t masked = __ballot(out);
+        if (lane % 32 == 0)
+            gone[i / 32] = uint32_t(masked >> lane);
     }
 
     float *scores = a.scores != nullptr && valid
@@ -468,13 +484,15 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
     // cost their places: 378 us for 337 where both were measured.
     Tile<TYPE, HD> x;
     if (wave < tiles)
-        x.template load<FULL>(kv, lds.at + wave * T::kRows, lane);
+        x.template load<FULL, NT>(kv, lds.at + wave * T::kRows, lane);
     q.convert(a.scale);
     for (int t = wave; t < tiles;) {
-        attend<TYPE, HD>(x, q, sm, scores == nullptr ? nullptr : scores + t * T::kRows);
+        const uint32_t word = gone[t * T::kRows / 32] >> (t * T::kRows % 32);
+        attend<TYPE, HD>(x, __builtin_amdgcn_readfirstlane(T::kWide ? word & 0xffffu : word), q, sm,
+                         scores == nullptr ? nullptr : scores + t * T::kRows, lane);
         t += kWaves;
         if (t < tiles)
-            x.template load<FULL>(kv, lds.at + t * T::kRows, lane);
+            x.template load<FULL, NT>(kv, lds.at + t * T::kRows, lane);
     }
     sm.sum += __shfl_xor(sm.sum, 16);
     sm.sum += __shfl_xor(sm.sum, 32);
@@ -498,7 +516,7 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
                 f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
     }
     __syncthreads();
-    const uint32_t parts = kv.head_dim / 4;
+    const uint32_t parts = FULL ? HD / 4 : kv.head_dim / 4;
     for (uint32_t i = threadIdx.x; i < here * parts; i += kThreads) {
         const uint32_t head = i / parts, d = i % parts * 4;
         float most = stat[0][0][head];
@@ -681,26 +699,35 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, PagedHistory hi
     }
 }
 
+// Rows beyond this many bytes go past the caches' replacement: nothing of them
+// is there when the next call comes, and HBM is read faster without it. Three
+// caches in turn, us a call without and with, by MB of a call's rows: bfloat16
+// 33 15.3 16.3, 66 19.8 21.7, 131 33.3 30.6, 524 108 96, fp16 131 32.9 33.4, 262
+// 54 52, 2,097 359 328, fp32 131 32 30, 2,097 372 334.
+constexpr uint64_t kPastCaches = 128ull << 20;
+
 template <int TYPE, int HD>
-void attend_as(const AttendArgs &a, dim3 grid, hipStream_t stream)
+void attend_as(const AttendArgs &a, dim3 grid, uint64_t bytes, hipStream_t stream)
 {
-    const auto kernel = a.kv.head_dim == HD ? attend_kernel<TYPE, HD, true>
-                                            : attend_kernel<TYPE, HD, false>;
+    const auto kernel = a.kv.head_dim != HD    ? attend_kernel<TYPE, HD, false, false>
+                        : bytes >= kPastCaches ? attend_kernel<TYPE, HD, true, true>
+                                               : attend_kernel<TYPE, HD, true, false>;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * kWavesOf<HD>), 0, stream, a);
 }
 
-template <int TYPE> void attend_in(const AttendArgs &a, dim3 grid, hipStream_t stream)
+template <int TYPE>
+void attend_in(const AttendArgs &a, dim3 grid, uint64_t bytes, hipStream_t stream)
 {
     if (a.kv.head_dim <= 32)
-        attend_as<TYPE, 32>(a, grid, stream);
+        attend_as<TYPE, 32>(a, grid, bytes, stream);
     else if (a.kv.head_dim <= 64)
-        attend_as<TYPE, 64>(a, grid, stream);
+        attend_as<TYPE, 64>(a, grid, bytes, stream);
     else if (a.kv.head_dim <= 96)
-        attend_as<TYPE, 96>(a, grid, stream);
+        attend_as<TYPE, 96>(a, grid, bytes, stream);
     else if (a.kv.head_dim <= 128)
-        attend_as<TYPE, 128>(a, grid, stream);
+        attend_as<TYPE, 128>(a, grid, bytes, stream);
     else
-        attend_as<TYPE, 256>(a, grid, stream);
+        attend_as<TYPE, 256>(a, grid, bytes, stream);
 }
 
 } // namespace
@@ -713,11 +740,21 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     const uint32_t group = heads / kv.kv_heads, rows = top == 0 ? seqs.max_length
                                                                 : top * kv.page_size;
     plan.tiles = (group + 15) / 16;
+    // Runs as long as leave 512 workgroups: of 32 ragged sequences of up to 2,048
+    // bfloat16 rows, 13.5 us in runs of 512 (512 workgroups), 14.2 in runs of 256
+    // and 16.0 in runs of 1,024; of 7 of up to 5,001 fp32 rows 20.0 in runs of 128
+    // and 20.9 in runs of 256 and 512 (210 workgroups).
     plan.chunk = kMostRows;
     while (plan.chunk > 128 && uint64_t(seqs.batch) * kv.kv_heads * plan.tiles *
                                        ((rows + plan.chunk - 1) / plan.chunk) <
-                                   1024)
+                                   512)
         plan.chunk /= 2;
+    // Keys of up to 64 KB are one run whatever the number of workgroups: the
+    // join's launch costs more. One sequence of 64 components, one run and
+    // split: 256 fp32 rows 6.9 and 8.6 us, 512 10.3 and 8.6; 512 bfloat16 rows
+    // 7.2 and 8.4, 1,000 10.6 and 8.5.
+    if (rows <= kMostRows && uint64_t(rows) * kv.head_dim * paged_element(kv.type) <= 65536)
+        plan.chunk = kMostRows;
     plan.chunks = (rows + plan.chunk - 1) / plan.chunk;
     if (plan.chunks == 1 && !weighted)
         return plan;
@@ -744,19 +781,24 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
         a.stats = reinterpret_cast<float2 *>(workspace + plan.stats);
         a.scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
     }
-    const dim3 grid = paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks,
-                                 256);
+    paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks, 512);
+    require(seqs.batch <= 65535 && uint64_t(kv.kv_heads) * plan.tiles <= 65535, NUT_EINVAL,
+            "paged cache: more rows than one launch covers");
+    const dim3 grid(plan.chunks, kv.kv_heads * plan.tiles, seqs.batch);
     // a wave joins up to 16 runs of a head
     const uint32_t threads = plan.chunks <= 16 ? 64 : 256;
     const uint32_t blocks = weighted ? (seqs.max_length + 4 * threads - 1) / (4 * threads) : 0;
     const uint64_t joins = uint64_t(seqs.batch) * heads;
     const dim3 join = paged_grid(joins + uint64_t(seqs.batch) * kv.kv_heads * blocks, threads);
+    const uint64_t rows = top == 0 ? seqs.max_length : uint64_t(top) * kv.page_size;
+    const uint64_t bytes = rows * seqs.batch * kv.kv_heads * kv.head_dim * 2 *
+                           paged_element(kv.type);
     if (kv.type == NUT_F32)
-        attend_in<NUT_F32>(a, grid, stream);
+        attend_in<NUT_F32>(a, grid, bytes, stream);
     else if (kv.type == NUT_F16)
-        attend_in<NUT_F16>(a, grid, stream);
+        attend_in<NUT_F16>(a, grid, bytes, stream);
     else
-        attend_in<NUT_BF16>(a, grid, stream);
+        attend_in<NUT_BF16>(a, grid, bytes, stream);
     check_launch("paged attention");
     if (!split)
         return;
