@@ -117,39 +117,71 @@ __global__ __launch_bounds__(256) void append_kernel(
 
 // ------------------------------------------------------ the k-th largest --
 
-constexpr int kBits = 11, kBins = 1 << kBits;
+constexpr int kBits = 8, kBins = 1 << kBits;
 
 struct RankScratch {
     uint32_t bins[kBins];
     uint32_t wave[16], more[16];
+    uint32_t any[16][2], all[16][2];
     uint32_t bin, above, count;
-    unsigned long long any, all;
 };
+
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ uint32_t dpp_bits(uint32_t v, uint32_t fill)
+{
+    return uint32_t(__builtin_amdgcn_update_dpp(int(fill), int(v), CTRL, ROWS, 0xF, false));
+}
+
+// Bits that any (all) lanes of the wave have, in lane 63.
+__device__ __forceinline__ uint32_t any_bits(uint32_t v)
+{
+    v |= dpp_bits<kDppQuadSwap1>(v, 0);
+    v |= dpp_bits<kDppQuadSwap2>(v, 0);
+    v |= dpp_bits<kDppRowHalfMirror>(v, 0);
+    v |= dpp_bits<kDppRowMirror>(v, 0);
+    v |= dpp_bits<kDppRowBcast15, 0xA>(v, 0);
+    return v | dpp_bits<kDppRowBcast31, 0xC>(v, 0);
+}
+
+__device__ __forceinline__ uint32_t all_bits(uint32_t v) { return ~any_bits(~v); }
 
 // Finds, for keys get(0) to get(n - 1) and 1 <= k < n, the threshold T and
 // the number of ties such that the k largest keys, ties to the lowest index,
 // are the keys over T and the first `ties` keys equal to T. A radix search
-// from the first bit in which the keys differ, 11 bits a pass, which ends at
-// the first digit whose keys are all taken (scores differ in their leading
-// bits: two or three passes). Every thread of the workgroup calls it.
+// from the first bit in which the keys differ, 8 bits a pass (a bin a thread),
+// which ends at the first digit whose keys are all taken: two or three passes
+// of scores that differ in their leading bits. Every thread of the workgroup,
+// 256 of them or more, calls it; it begins and ends at a barrier.
 template <typename K, typename Get>
 __device__ __forceinline__ void kth_largest(Get get, uint32_t n, uint32_t k, RankScratch &sc,
                                             K &threshold, uint32_t &ties)
 {
+    constexpr int kWidth = 8 * sizeof(K);
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const uint32_t waves = blockDim.x / kWave;
-    if (threadIdx.x == 0)
-        sc.any = 0, sc.all = ~0ull;
-    __syncthreads();
     K any = 0, all = K(~K(0));
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const K key = get(i);
         any |= key, all &= key;
     }
-    atomicOr(&sc.any, (unsigned long long)any);
-    atomicAnd(&sc.all, (unsigned long long)all);
+#pragma unroll
+    for (int w = 0; w < kWidth / 32; w++) {
+        const uint32_t o = any_bits(uint32_t(any >> (32 * w)));
+        const uint32_t a = all_bits(uint32_t(all >> (32 * w)));
+        if (lane == kWave - 1)
+            sc.any[wave][w] = o, sc.all[wave][w] = a;
+    }
+    if (threadIdx.x < kBins)
+        sc.bins[threadIdx.x] = 0;
     __syncthreads();
-    any = K(sc.any), all = K(sc.all);
+    any = 0, all = K(~K(0));
+    for (uint32_t w = 0; w < blockDim.x / kWave; w++) {
+        K o = 0, a = 0;
+#pragma unroll
+        for (int p = 0; p < kWidth / 32; p++)
+            o |= K(sc.any[w][p]) << (32 * p), a |= K(sc.all[w][p]) << (32 * p);
+        any |= o, all &= a;
+    }
     const K differ = any ^ all;
     if (differ == 0) {
         threshold = any;
@@ -157,56 +189,50 @@ __device__ __forceinline__ void kth_largest(Get get, uint32_t n, uint32_t k, Ran
         __syncthreads();
         return;
     }
-    int shift = 64 - __clzll((unsigned long long)differ); // bits still open
-    K prefix = shift >= int(8 * sizeof(K)) ? K(0) : K(any >> shift << shift);
+    int open = 64 - __clzll((unsigned long long)differ); // bits not yet decided
+    K prefix = open >= kWidth ? K(0) : K(any >> open << open);
     uint32_t left = k;
     while (true) {
-        const int width = min(kBits, shift), top = shift;
-        shift -= width;
-        for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x)
-            sc.bins[i] = 0;
-        __syncthreads();
+        const int shift = max(0, open - kBits);
+        const uint32_t mask = (1u << (open - shift)) - 1;
         for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
             const K key = get(i);
-            const K open = key ^ prefix;
-            if (top >= int(8 * sizeof(K)) || (open >> top) == 0)
-                atomicAdd(&sc.bins[uint32_t(key >> shift) & ((1u << width) - 1)], 1u);
+            if (open >= kWidth || (K(key ^ prefix) >> open) == 0)
+                atomicAdd(&sc.bins[uint32_t(key >> shift) & mask], 1u);
         }
         __syncthreads();
-        // thread t owns `own` bins, from the highest down
-        const uint32_t own = kBins / blockDim.x, high = kBins - 1 - threadIdx.x * own;
-        uint32_t sum = 0;
-        for (uint32_t i = 0; i < own; i++)
-            sum += sc.bins[high - i];
-        uint32_t scan = sum;
+        // thread t owns bin 255 - t: a scan from the highest bin down
+        uint32_t own = 0, scan = 0;
+        if (threadIdx.x < kBins) {
+            own = scan = sc.bins[kBins - 1 - threadIdx.x];
 #pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const uint32_t up = __shfl_up(scan, o);
-            scan += lane >= uint32_t(o) ? up : 0;
+            for (int o = 1; o < kWave; o <<= 1) {
+                const uint32_t up = __shfl_up(scan, o);
+                scan += lane >= uint32_t(o) ? up : 0;
+            }
+            if (lane == kWave - 1)
+                sc.wave[wave] = scan;
         }
-        if (lane == kWave - 1)
-            sc.wave[wave] = scan;
         __syncthreads();
-        for (uint32_t w = 0; w < wave; w++)
-            scan += sc.wave[w];
-        if (scan >= left && scan - sum < left) {
-            uint32_t above = scan - sum, i = 0;
-            while (above + sc.bins[high - i] < left)
-                above += sc.bins[high - i++];
-            sc.bin = high - i, sc.above = above, sc.count = sc.bins[high - i];
+        if (threadIdx.x < kBins) {
+            for (uint32_t w = 0; w < wave; w++)
+                scan += sc.wave[w];
+            if (scan >= left && scan - own < left)
+                sc.bin = kBins - 1 - threadIdx.x, sc.above = scan - own, sc.count = own;
+            sc.bins[kBins - 1 - threadIdx.x] = 0; // for the next pass
         }
         __syncthreads();
         prefix |= K(sc.bin) << shift;
         left -= sc.above;
         const bool whole = sc.count == left;
-        __syncthreads();
         if (whole || shift == 0) {
             threshold = prefix;
             ties = whole ? 0xffffffffu : left;
+            __syncthreads();
             return;
         }
+        open = shift;
     }
-    (void)waves;
 }
 
 // Lanes below this one in a ballot.
@@ -245,7 +271,7 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
     const uint32_t b = id / blocks / kv.kv_heads;
     const uint32_t n = paged_length(kv, s, b, threadIdx.x == 0 && h == 0 && c == 0);
-    const uint32_t count = n / kv.page_size + (n % kv.page_size != 0);
+    const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
     if (c * per_block >= count)
         return;
     const uint32_t end = min(count, (c + 1) * per_block);
@@ -309,7 +335,10 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     }
 }
 
-// A workgroup per (sequence, KV head): the `top` best of its pages.
+// A workgroup per (sequence, KV head): the `top` best of its pages. Up to kKept
+// scores are read once.
+constexpr uint32_t kKept = 4096;
+
 __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSeqs s,
                                                            const uint64_t *__restrict__ scores,
                                                            uint32_t width, uint32_t top,
@@ -318,7 +347,7 @@ __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSe
 {
     const uint32_t id = blockIdx.x, h = id % kv.kv_heads, b = id / kv.kv_heads;
     const uint32_t n = paged_length(kv, s, b, false);
-    const uint32_t count = n / kv.page_size + (n % kv.page_size != 0);
+    const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
     int *out = selected + (size_t(b) * kv.kv_heads + h) * top;
     if (count <= top) {
         for (uint32_t i = threadIdx.x; i < top; i += blockDim.x)
@@ -326,10 +355,15 @@ __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSe
         return;
     }
     __shared__ RankScratch sc;
+    __shared__ uint64_t keys[kKept];
     const uint64_t *mine = scores + (size_t(b) * kv.kv_heads + h) * width;
-    const auto get = [&](uint32_t i) -> uint64_t {
+    const auto key_of = [&](uint32_t i) -> uint64_t {
         return i < first || i >= count - last ? ~0ull : mine[i];
     };
+    if (count <= kKept)
+        for (uint32_t i = threadIdx.x; i < count; i += blockDim.x)
+            keys[i] = key_of(i);
+    const auto get = [&](uint32_t i) -> uint64_t { return count <= kKept ? keys[i] : key_of(i); };
     uint64_t threshold;
     uint32_t ties;
     kth_largest<uint64_t>(get, count, top, sc, threshold, ties);
@@ -378,33 +412,52 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return key; // at least ~0xff800000 = 0x007fffff, over a NaN's
 }
 
+constexpr uint32_t kKeptRows = 8192;
+
 // A workgroup per (sequence, KV head) decides what stays: moves[i] of a row
 // i below the budget is -1 where it stays and its rank among the holes where
-// it goes; from[r] is the r-th row that stays beyond the budget.
-__global__ __launch_bounds__(1024) void plan_eviction_kernel(PagedView kv, PagedSeqs s,
-                                                             PagedHistory history,
-                                                             uint32_t budget, uint32_t first,
-                                                             uint32_t last, int *new_lengths,
-                                                             int *__restrict__ moves,
-                                                             int *__restrict__ from)
+// it goes; from[r] is the r-th row that stays beyond the budget. Weights and
+// positions of up to kKeptRows rows are read once, eight rows a thread at a
+// time, and live on as keys in shared memory.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, PagedSeqs s,
+                                                                PagedHistory history,
+                                                                uint32_t budget, uint32_t first,
+                                                                uint32_t last, int *new_lengths,
+                                                                int *__restrict__ moves,
+                                                                int *__restrict__ from)
 {
     const uint32_t id = blockIdx.x, h = id % kv.kv_heads, b = id / kv.kv_heads;
     const bool leader = threadIdx.x == 0 && h == 0;
-    const uint32_t n = paged_length(kv, s, b, leader);
-    if (leader) {
-        const int was = s.lengths[b];
-        new_lengths[b] = n > budget ? int(budget) : was;
-    }
-    if (n <= budget)
-        return;
-    __shared__ RankScratch sc;
-    __shared__ int newest_of[16];
     const size_t at = (size_t(b) * kv.kv_heads + h) * history.stride;
     const float *weights = history.weights + at;
     const int *positions = history.positions + at;
+    // the first rows beside the length, which max_length bounds
+    constexpr int kEach = 8;
+    float w[kEach];
+    int p[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const uint32_t i = e * THREADS + threadIdx.x;
+        w[e] = i < s.max_length ? weights[i] : 0.0f;
+        p[e] = i < s.max_length ? positions[i] : 0;
+    }
+    const uint32_t n = paged_length(kv, s, b, leader);
+    if (leader)
+        new_lengths[b] = n > budget ? int(budget) : s.lengths[b];
+    if (n <= budget)
+        return;
+    __shared__ RankScratch sc;
+    __shared__ int newest_of[THREADS / kWave];
+    __shared__ uint32_t keys[kKeptRows < kEach * THREADS ? kKeptRows : kEach * THREADS];
+    constexpr uint32_t kHeld = sizeof keys / sizeof keys[0];
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     int newest = -1;
-    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+        if (e * THREADS + threadIdx.x < n)
+            newest = max(newest, p[e]);
+    for (uint32_t i = kEach * THREADS + threadIdx.x; i < n; i += THREADS)
         newest = max(newest, positions[i]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
@@ -412,31 +465,38 @@ __global__ __launch_bounds__(1024) void plan_eviction_kernel(PagedView kv, Paged
     if (lane == 0)
         newest_of[wave] = newest;
     __syncthreads();
-    for (uint32_t w = 0; w < blockDim.x / kWave; w++)
-        newest = max(newest, newest_of[w]);
+    for (uint32_t v = 0; v < THREADS / kWave; v++)
+        newest = max(newest, newest_of[v]);
     const int64_t recent = int64_t(newest) - int64_t(last);
+    const auto key_of = [&](int position, float weight) -> uint32_t {
+        return position < int64_t(first) || position > recent ? 0xffffffffu : weight_key(weight);
+    };
+    if (n <= kHeld)
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const uint32_t i = e * THREADS + threadIdx.x;
+            if (i < n)
+                keys[i] = key_of(p[e], w[e]);
+        }
     const auto get = [&](uint32_t i) -> uint32_t {
-        const int p = positions[i];
-        return p < int64_t(first) || p > recent ? 0xffffffffu : weight_key(weights[i]);
+        return n <= kHeld ? keys[i] : key_of(positions[i], weights[i]);
     };
     uint32_t threshold, ties;
     kth_largest<uint32_t>(get, n, budget, sc, threshold, ties);
 
-    const uint32_t run = (n + blockDim.x - 1) / blockDim.x * kWave;
+    // each wave takes a run of rows: its ties first, then its holes and rows to
+    // move, then their places
+    const uint32_t run = (n + THREADS - 1) / THREADS * kWave;
     const uint32_t begin = min(n, wave * run), end = min(n, begin + run);
     uint32_t equal = 0;
-    for (uint32_t i = begin + lane; i < end; i += kWave)
-        equal += get(i) == threshold;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        equal += __shfl_xor(equal, o);
+    for (uint32_t base = begin; base < end; base += kWave)
+        equal += __popcll(__ballot(base + lane < end && get(base + lane) == threshold));
     if (lane == 0)
         sc.more[wave] = equal;
     __syncthreads();
     uint32_t seen = 0;
-    for (uint32_t w = 0; w < wave; w++)
-        seen += sc.more[w];
-    // walk the run twice: count its holes and its rows to move, then place them
+    for (uint32_t v = 0; v < wave; v++)
+        seen += sc.more[v];
     uint32_t holes = 0, moved = 0;
     int *move = moves + (size_t(b) * kv.kv_heads + h) * budget;
     int *source = from + (size_t(b) * kv.kv_heads + h) * budget;
@@ -465,96 +525,113 @@ __global__ __launch_bounds__(1024) void plan_eviction_kernel(PagedView kv, Paged
                 sc.wave[wave] = holes, sc.bins[wave] = moved;
             __syncthreads();
             holes = moved = 0;
-            for (uint32_t w = 0; w < wave; w++)
-                holes += sc.wave[w], moved += sc.bins[w];
+            for (uint32_t v = 0; v < wave; v++)
+                holes += sc.wave[v], moved += sc.bins[v];
         }
     }
 }
 
-// A workgroup per (sequence, KV head, page below the budget) fetches what
-// moves into the page. Sources lie beyond the budget and are only read, so
+// A workgroup per (sequence, KV head, `span` rows below the budget: whole
+// pages) fetches what moves there, 256 rows of the plan at a time: a thread a
+// row finds where it comes from and lists it, then head_dim / 8 threads a row
+// copy what is listed. Sources lie beyond the budget and are only read, so
 // the order of workgroups does not matter.
 template <int TYPE>
 __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs s,
                                                         PagedHistory history, uint32_t budget,
-                                                        uint32_t pages,
+                                                        uint32_t span, uint32_t blocks,
                                                         const int *__restrict__ moves,
                                                         const int *__restrict__ from)
 {
-    const uint32_t id = blockIdx.x, c = id % pages, h = id / pages % kv.kv_heads;
-    const uint32_t b = id / pages / kv.kv_heads;
+    constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
+    const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
+    const uint32_t b = id / blocks / kv.kv_heads;
+    const size_t row = size_t(b) * kv.kv_heads + h, at = row * history.stride;
+    const int *move = moves + row * budget, *source = from + row * budget;
+    const uint32_t first = c * span, last = min(budget, first + span);
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t tpr = kv.head_dim / 8, part = threadIdx.x % tpr, group = threadIdx.x / tpr;
+    const uint32_t groups = 256 / tpr, column = part * 8 * kSize;
+    __shared__ size_t to[256], of[256];
+    __shared__ uint32_t page[256];
+    __shared__ uint32_t listed[4];
+    int rank = first + threadIdx.x < last ? move[first + threadIdx.x] : -1;
     const uint32_t n = paged_length(kv, s, b, false);
     if (n <= budget)
         return;
-    const uint32_t ps = kv.page_size, first = c * ps, end = min(budget - first, ps);
-    const size_t row = size_t(b) * kv.kv_heads + h, at = row * history.stride;
-    const int *move = moves + row * budget + first, *source = from + row * budget;
-    const size_t page = paged_row(kv, s, b, c, 0, h);
-    const uint32_t tpr = kv.head_dim / 8, part = threadIdx.x % tpr, group = threadIdx.x / tpr;
-    const uint32_t groups = 256 / tpr;
-    const size_t size = TYPE == NUT_F32 ? 4 : 2, column = part * 8 * size;
-    __shared__ int sources[256];
-    __shared__ float low[256][8], high[256][8];
-    float lo[8], hi[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        lo[i] = INFINITY, hi[i] = -INFINITY;
-    bool some = false;
-    for (uint32_t w = 0; w < end; w += 256) {
-        const uint32_t slot = w + threadIdx.x;
-        const int rank = slot < end ? move[slot] : -1;
-        const int src = rank < 0 ? -1 : source[rank];
-        if (src >= 0) {
-            history.weights[at + first + slot] = history.weights[at + src];
-            history.positions[at + first + slot] = history.positions[at + src];
+    for (uint32_t base = first; base < last; base += 256) {
+        const uint32_t i = base + threadIdx.x;
+        if (base != first)
+            rank = i < last ? move[i] : -1;
+        size_t here = kNoRow, there = kNoRow;
+        const uint32_t index = page_of(kv, min(i, last - 1));
+        if (rank >= 0) {
+            const uint32_t from_row = uint32_t(source[rank]);
+            history.weights[at + i] = history.weights[at + from_row];
+            history.positions[at + i] = history.positions[at + from_row];
+            const uint32_t from_page = page_of(kv, from_row);
+            here = paged_row(kv, s, b, index, i - index * kv.page_size, h);
+            there = paged_row(kv, s, b, from_page, from_row - from_page * kv.page_size, h);
         }
-        sources[threadIdx.x] = src;
-        if (__syncthreads_or(src >= 0) && page != kNoRow && group < groups) {
-            for (uint32_t r = group; r < min(end - w, 256u); r += groups) {
-                const int i = sources[r];
-                if (i < 0)
-                    continue;
-                const size_t there = paged_row(kv, s, b, uint32_t(i) / ps, uint32_t(i) % ps, h);
-                if (there == kNoRow)
-                    continue;
-                some = true;
-                const size_t here = page + size_t(w + r) * kv.slot_stride + column;
-                const uint4 *k = reinterpret_cast<const uint4 *>(kv.keys + there + column);
-                const uint4 *v = reinterpret_cast<const uint4 *>(kv.values + there + column);
-                uint4 *to_k = reinterpret_cast<uint4 *>(kv.keys + here);
-                uint4 *to_v = reinterpret_cast<uint4 *>(kv.values + here);
-                float x[8];
-                load8<TYPE>(kv.keys + there + column, x);
+        const bool go = here != kNoRow && there != kNoRow;
+        const uint64_t going = __ballot(go);
+        if (lane == 0)
+            listed[wave] = __popcll(going);
+        __syncthreads();
+        uint32_t place = rank_in(going), count = 0;
+        for (uint32_t w = 0; w < 4; w++) {
+            place += w < wave ? listed[w] : 0;
+            count += listed[w];
+        }
+        if (go)
+            to[place] = here, of[place] = there, page[place] = index;
+        __syncthreads();
+        if (group < groups)
+            for (uint32_t r = group; r < count; r += 2 * groups) {
+                // two rows in flight
+                const uint32_t r2 = min(r + groups, count - 1);
+                uint4 k[2][kSize / 2], v[2][kSize / 2];
 #pragma unroll
-                for (int j = 0; j < int(size / 2); j++)
-                    to_k[j] = k[j], to_v[j] = v[j];
+                for (int e = 0; e < int(kSize / 2); e++) {
+                    k[0][e] = reinterpret_cast<const uint4 *>(kv.keys + of[r] + column)[e];
+                    v[0][e] = reinterpret_cast<const uint4 *>(kv.values + of[r] + column)[e];
+                    k[1][e] = reinterpret_cast<const uint4 *>(kv.keys + of[r2] + column)[e];
+                    v[1][e] = reinterpret_cast<const uint4 *>(kv.values + of[r2] + column)[e];
+                }
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    lo[j] = lower(lo[j], x[j]), hi[j] = upper(hi[j], x[j]);
+                for (int e = 0; e < int(kSize / 2); e++) {
+                    reinterpret_cast<uint4 *>(kv.keys + to[r] + column)[e] = k[0][e];
+                    reinterpret_cast<uint4 *>(kv.values + to[r] + column)[e] = v[0][e];
+                    if (r + groups < count) {
+                        reinterpret_cast<uint4 *>(kv.keys + to[r2] + column)[e] = k[1][e];
+                        reinterpret_cast<uint4 *>(kv.values + to[r2] + column)[e] = v[1][e];
+                    }
+                }
             }
+        if (kv.bounds != nullptr && count != 0) {
+            // head_dim / 8 threads a page widen its bounds by what moved in: the
+            // list is in the order of rows, so a page's entries are a run of it
+            if (group < groups)
+                for (uint32_t r = group; r < count; r += groups) {
+                    if (r != 0 && page[r - 1] == page[r])
+                        continue; // not a page's first
+                    char *bounds = kv.bounds +
+                                   (size_t(s.table[size_t(b) * s.table_stride + page[r]]) *
+                                        kv.kv_heads + h) * 2 * kv.head_dim * kSize + column;
+                    float lo[8], hi[8], x[8];
+                    load8<TYPE>(bounds, lo);
+                    load8<TYPE>(bounds + kv.head_dim * kSize, hi);
+                    for (uint32_t e = r; e < count && page[e] == page[r]; e++) {
+                        load8<TYPE>(kv.keys + of[e] + column, x);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            lo[j] = lower(lo[j], x[j]), hi[j] = upper(hi[j], x[j]);
+                    }
+                    store8<TYPE>(bounds, lo);
+                    store8<TYPE>(bounds + kv.head_dim * kSize, hi);
+                }
         }
         __syncthreads();
-    }
-    if (kv.bounds == nullptr || !__syncthreads_or(some))
-        return;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        low[threadIdx.x][i] = lo[i], high[threadIdx.x][i] = hi[i];
-    __syncthreads();
-    if (threadIdx.x < tpr) {
-        char *bounds = kv.bounds + (size_t(s.table[size_t(b) * s.table_stride + c]) *
-                                        kv.kv_heads + h) * 2 * kv.head_dim * size;
-        float a[8], z[8];
-        load8<TYPE>(bounds + column, a);
-        load8<TYPE>(bounds + kv.head_dim * size + column, z);
-        for (uint32_t g = 0; g < groups; g++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                a[i] = lower(a[i], low[g * tpr + part][i]);
-                z[i] = upper(z[i], high[g * tpr + part][i]);
-            }
-        store8<TYPE>(bounds + column, a);
-        store8<TYPE>(bounds + kv.head_dim * size + column, z);
     }
 }
 
@@ -570,7 +647,7 @@ void scores_for(const PagedView &kv, const PagedSeqs &seqs, const float *query,
     while (lanes * 8 < kv.head_dim)
         lanes *= 2;
     const uint32_t width = pages_of(kv, seqs.max_length), group = heads / kv.kv_heads;
-    const uint32_t per_block = 256 / lanes * 4, blocks = (width + per_block - 1) / per_block;
+    const uint32_t per_block = 256 / lanes, blocks = (width + per_block - 1) / per_block;
     const dim3 grid = paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256);
     const auto kernel = group == 1   ? page_scores_kernel<TYPE, 1>
                         : group == 2 ? page_scores_kernel<TYPE, 2>
@@ -634,17 +711,21 @@ void launch_paged_evict(const PagedView &kv, const PagedSeqs &seqs, const PagedH
     int *moves = reinterpret_cast<int *>(workspace);
     int *from = reinterpret_cast<int *>(workspace + evict_workspace(kv, seqs, budget) / 2);
     const uint64_t heads = uint64_t(seqs.batch) * kv.kv_heads;
-    hipLaunchKernelGGL(plan_eviction_kernel, paged_grid(heads, 1024), dim3(1024), 0, stream, kv, seqs, history,
+    // eight rows a thread of the smaller workgroup
+    const uint32_t threads = seqs.max_length <= 2048 ? 256 : 1024;
+    hipLaunchKernelGGL(threads == 256 ? plan_eviction_kernel<256> : plan_eviction_kernel<1024>,
+                       paged_grid(heads, threads), dim3(threads), 0, stream, kv, seqs, history,
                        budget, first, last, new_lengths, moves, from);
     check_launch("paged evict");
     if (budget >= seqs.max_length)
         return;
-    const uint32_t pages = pages_of(kv, budget);
+    const uint32_t span = kv.page_size >= 256 ? kv.page_size : 256 / kv.page_size * kv.page_size;
+    const uint32_t blocks = (budget - 1) / span + 1;
     const auto kernel = kv.type == NUT_F32   ? move_rows_kernel<NUT_F32>
                         : kv.type == NUT_F16 ? move_rows_kernel<NUT_F16>
                                              : move_rows_kernel<NUT_BF16>;
-    hipLaunchKernelGGL(kernel, paged_grid(heads * pages, 256), dim3(256), 0, stream, kv, seqs, history,
-                       budget, pages, moves, from);
+    hipLaunchKernelGGL(kernel, paged_grid(heads * blocks, 256), dim3(256), 0, stream, kv, seqs,
+                       history, budget, span, blocks, moves, from);
     check_launch("paged evict");
 }
 
