@@ -145,6 +145,29 @@ __device__ __forceinline__ uint32_t any_bits(uint32_t v)
 
 __device__ __forceinline__ uint32_t all_bits(uint32_t v) { return ~any_bits(~v); }
 
+// The largest of a wave's values, none below -1, in lane 63.
+__device__ __forceinline__ int largest(int v)
+{
+    v = max(v, int(dpp_bits<kDppQuadSwap1>(v, ~0u)));
+    v = max(v, int(dpp_bits<kDppQuadSwap2>(v, ~0u)));
+    v = max(v, int(dpp_bits<kDppRowHalfMirror>(v, ~0u)));
+    v = max(v, int(dpp_bits<kDppRowMirror>(v, ~0u)));
+    v = max(v, int(dpp_bits<kDppRowBcast15, 0xA>(v, ~0u)));
+    return max(v, int(dpp_bits<kDppRowBcast31, 0xC>(v, ~0u)));
+}
+
+// Sum of this lane's value and those of the lanes below it.
+__device__ __forceinline__ uint32_t running_sum(uint32_t v)
+{
+    constexpr int kRowShift = 0x110; // lane i of a row of 16 from lane i - n
+    v += dpp_bits<kRowShift + 1>(v, 0);
+    v += dpp_bits<kRowShift + 2>(v, 0);
+    v += dpp_bits<kRowShift + 4>(v, 0);
+    v += dpp_bits<kRowShift + 8>(v, 0);
+    v += dpp_bits<kDppRowBcast15, 0xA>(v, 0);
+    return v + dpp_bits<kDppRowBcast31, 0xC>(v, 0);
+}
+
 // Finds, for keys get(0) to get(n - 1) and 1 <= k < n, the threshold T and
 // the number of ties such that the k largest keys, ties to the lowest index,
 // are the keys over T and the first `ties` keys equal to T. A radix search
@@ -204,12 +227,8 @@ __device__ __forceinline__ void kth_largest(Get get, uint32_t n, uint32_t k, Ran
         // thread t owns bin 255 - t: a scan from the highest bin down
         uint32_t own = 0, scan = 0;
         if (threadIdx.x < kBins) {
-            own = scan = sc.bins[kBins - 1 - threadIdx.x];
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const uint32_t up = __shfl_up(scan, o);
-                scan += lane >= uint32_t(o) ? up : 0;
-            }
+            own = sc.bins[kBins - 1 - threadIdx.x];
+            scan = running_sum(own);
             if (lane == kWave - 1)
                 sc.wave[wave] = scan;
         }
@@ -244,6 +263,9 @@ __device__ __forceinline__ uint32_t rank_in(uint64_t mask)
 
 // ---------------------------------------------------------------- select --
 
+// Pages a lane scores: more where the query's conversions weigh more.
+template <int TYPE, int GH> constexpr int kPagesOf = GH < 4 ? 1 : TYPE == NUT_F32 ? 2 : 4;
+
 // Order-preserving image of a score; a NaN ranks above every number, the
 // pages that are always read above both.
 __device__ __forceinline__ uint64_t score_key(double v)
@@ -259,26 +281,55 @@ __device__ __forceinline__ uint64_t score_key(double v)
 //   sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (hi_d + lo_d) / 2
 //                                        + |q_d| (hi_d - lo_d) / 2,
 // two multiply-adds a component in 64 bits: the answer is whole numbers, and
-// 32 bits would let rounding choose among near pages. GH heads at a time.
+// 32 bits would let rounding choose among near pages. GH heads at a time, and
+// kPages pages a lane, all fetched before the first is used.
 template <int TYPE, int GH>
 __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeqs s,
                                                           const float *__restrict__ query,
                                                           size_t query_stride, uint32_t heads,
-                                                          uint32_t lanes, uint32_t per_block,
-                                                          uint32_t blocks, uint32_t width,
+                                                          uint32_t lanes, uint32_t blocks,
+                                                          uint32_t width,
                                                           uint64_t *__restrict__ scores)
 {
+    constexpr int kPages = kPagesOf<TYPE, GH>, kSize = TYPE == NUT_F32 ? 4 : 2;
+    constexpr int kWords = kSize / 2; // 16-byte words of eight components
     const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
     const uint32_t b = id / blocks / kv.kv_heads;
+    const uint32_t step = 256 / lanes, begin = c * step * kPages + threadIdx.x / lanes;
+    const uint32_t group = heads / kv.kv_heads, part = threadIdx.x & (lanes - 1);
+    const bool works = part * 8 < kv.head_dim;
+    // the table beside the length: what lies behind it is not used
+    int page[kPages];
+#pragma unroll
+    for (int k = 0; k < kPages; k++)
+        page[k] = begin + k * step < width
+                      ? s.table[size_t(b) * s.table_stride + begin + k * step]
+                      : -1;
     const uint32_t n = paged_length(kv, s, b, threadIdx.x == 0 && h == 0 && c == 0);
     const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
-    if (c * per_block >= count)
+    if (c * step * kPages >= count)
         return;
-    const uint32_t end = min(count, (c + 1) * per_block);
-    const uint32_t group = heads / kv.kv_heads, part = threadIdx.x % lanes;
-    const size_t size = TYPE == NUT_F32 ? 4 : 2;
-    const bool works = part * 8 < kv.head_dim;
-    uint64_t *out = scores + (size_t(b) * kv.kv_heads + h) * width;
+    uint4 low[kPages][kWords], high[kPages][kWords];
+#pragma unroll
+    for (int k = 0; k < kPages; k++) {
+        const bool good = page[k] >= 0 && uint32_t(page[k]) < kv.pages;
+        if (!good && begin + k * step < count)
+            paged_flag(kv.status, kBadPage);
+        const bool read = good && works && begin + k * step < count;
+        const uint4 *at = reinterpret_cast<const uint4 *>(
+            kv.bounds + (size_t(good ? page[k] : 0) * kv.kv_heads + h) * 2 * kv.head_dim * kSize +
+            part * 8 * kSize);
+#pragma unroll
+        for (int w = 0; w < kWords; w++) {
+            low[k][w] = read ? at[w] : make_uint4(0, 0, 0, 0);
+            high[k][w] = read ? at[w + kv.head_dim / 8 * kWords] : make_uint4(0, 0, 0, 0);
+        }
+        page[k] = good ? page[k] : -1;
+    }
+    uint64_t best[kPages];
+#pragma unroll
+    for (int k = 0; k < kPages; k++)
+        best[k] = 0;
     for (uint32_t g = 0; g < group; g += GH) {
         double q[GH][8];
 #pragma unroll
@@ -293,45 +344,71 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
             for (int i = 0; i < 8; i++)
                 q[j][i] = double(v[i]);
         }
-        for (uint32_t p = c * per_block + threadIdx.x / lanes; p < end; p += 256 / lanes) {
-            const int page = s.table[size_t(b) * s.table_stride + p];
-            const bool good = page >= 0 && uint32_t(page) < kv.pages;
-            if (!good && part == 0)
-                paged_flag(kv.status, kBadPage);
-            double mid[8], half[8];
-            {
-                float lo[8] = {0, 0, 0, 0, 0, 0, 0, 0}, hi[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (good && works) {
-                    const char *at = kv.bounds + (size_t(page) * kv.kv_heads + h) * 2 *
-                                                     kv.head_dim * size + part * 8 * size;
-                    load8<TYPE>(at, lo);
-                    load8<TYPE>(at + kv.head_dim * size, hi);
-                }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    mid[i] = 0.5 * (double(hi[i]) + double(lo[i]));
-                    half[i] = 0.5 * (double(hi[i]) - double(lo[i]));
+        for (int k = 0; k < kPages; k++) {
+            // one page's sums at a time, and its bounds widened anew for each
+            // four heads: kept in 64 bits they would fill the registers
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int w = 0; w < kWords; w++)
+                asm volatile("" : "+v"(low[k][w].x), "+v"(low[k][w].y), "+v"(low[k][w].z),
+                             "+v"(low[k][w].w), "+v"(high[k][w].x), "+v"(high[k][w].y),
+                             "+v"(high[k][w].z), "+v"(high[k][w].w));
+            float lo[8], hi[8];
+            load8<TYPE>(reinterpret_cast<const char *>(low[k]), lo);
+            load8<TYPE>(reinterpret_cast<const char *>(high[k]), hi);
+            double sum[GH];
+#pragma unroll
+            for (int j = 0; j < GH; j++)
+                sum[j] = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const double mid = 0.5 * (double(hi[i]) + double(lo[i]));
+                const double half = 0.5 * (double(hi[i]) - double(lo[i]));
+#pragma unroll
+                for (int j = 0; j < GH; j++)
+                    sum[j] = fma(fabs(q[j][i]), half, fma(q[j][i], mid, sum[j]));
+            }
+            // sums over the page's lanes: while a lane holds several heads it
+            // trades half of them for the other half's part, then it adds
+            uint32_t mine = g, held = GH;
+#pragma unroll
+            for (int i = 0; i < 5; i++) {
+                const uint32_t o = 1u << i;
+                if (o >= lanes)
+                    break;
+                if ((GH >> i) > 1) {
+                    const int rest = (GH >> i) / 2;
+                    const bool upper_half = part & o;
+#pragma unroll
+                    for (int j = 0; j < rest; j++) {
+                        const double give = upper_half ? sum[j] : sum[j + rest];
+                        const double keep = upper_half ? sum[j + rest] : sum[j];
+                        sum[j] = keep + __shfl_xor(give, int(o));
+                    }
+                    mine += upper_half ? rest : 0;
+                    held = rest;
+                } else {
+                    sum[0] += __shfl_xor(sum[0], int(o));
                 }
             }
-            uint64_t best = 0;
 #pragma unroll
             for (int j = 0; j < GH; j++) {
-                double sum = 0.0;
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    sum = fma(fabs(q[j][i]), half[i], fma(q[j][i], mid[i], sum));
-                for (uint32_t o = 1; o < lanes; o <<= 1)
-                    sum += __shfl_xor(sum, int(o));
-                const uint64_t key = score_key(sum);
-                if (g + j < group && key > best)
-                    best = key;
-            }
-            if (part == 0) {
-                if (!good)
-                    best = 0;
-                out[p] = g == 0 ? best : (best > out[p] ? best : out[p]);
+                const uint64_t key = score_key(sum[j]);
+                if (uint32_t(j) < held && mine + j < group && key > best[k])
+                    best[k] = key;
             }
         }
+    }
+    uint64_t *out = scores + (size_t(b) * kv.kv_heads + h) * width;
+#pragma unroll
+    for (int k = 0; k < kPages; k++) {
+        for (uint32_t o = 1; o < lanes; o <<= 1) {
+            const uint64_t other = __shfl_xor((unsigned long long)best[k], int(o));
+            best[k] = other > best[k] ? other : best[k];
+        }
+        if (part == 0 && begin + k * step < count) // a bad page below all others
+            out[begin + k * step] = page[k] < 0 ? 0 : best[k];
     }
 }
 
@@ -346,24 +423,34 @@ __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSe
                                                            int *__restrict__ selected)
 {
     const uint32_t id = blockIdx.x, h = id % kv.kv_heads, b = id / kv.kv_heads;
+    const uint64_t *mine = scores + (size_t(b) * kv.kv_heads + h) * width;
+    // the first scores beside the length: those behind it are not used
+    constexpr uint32_t kEach = 4;
+    uint64_t early[kEach];
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; e++)
+        early[e] = e * 256 + threadIdx.x < width ? mine[e * 256 + threadIdx.x] : 0;
     const uint32_t n = paged_length(kv, s, b, false);
     const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
     int *out = selected + (size_t(b) * kv.kv_heads + h) * top;
     if (count <= top) {
-        for (uint32_t i = threadIdx.x; i < top; i += blockDim.x)
+        for (uint32_t i = threadIdx.x; i < top; i += 256)
             out[i] = i < count ? int(i) : -1;
         return;
     }
     __shared__ RankScratch sc;
     __shared__ uint64_t keys[kKept];
-    const uint64_t *mine = scores + (size_t(b) * kv.kv_heads + h) * width;
-    const auto key_of = [&](uint32_t i) -> uint64_t {
-        return i < first || i >= count - last ? ~0ull : mine[i];
+    const auto key_of = [&](uint32_t i, uint64_t score) -> uint64_t {
+        return i < first || i >= count - last ? ~0ull : score;
     };
-    if (count <= kKept)
-        for (uint32_t i = threadIdx.x; i < count; i += blockDim.x)
-            keys[i] = key_of(i);
-    const auto get = [&](uint32_t i) -> uint64_t { return count <= kKept ? keys[i] : key_of(i); };
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; e++)
+        keys[e * 256 + threadIdx.x] = key_of(e * 256 + threadIdx.x, early[e]);
+    for (uint32_t i = kEach * 256 + threadIdx.x; i < min(count, kKept); i += 256)
+        keys[i] = key_of(i, mine[i]);
+    const auto get = [&](uint32_t i) -> uint64_t {
+        return i < kKept ? keys[i] : key_of(i, mine[i]);
+    };
     uint64_t threshold;
     uint32_t ties;
     kth_largest<uint64_t>(get, count, top, sc, threshold, ties);
@@ -373,13 +460,11 @@ __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSe
     const uint32_t run = (count + blockDim.x - 1) / blockDim.x * kWave;
     const uint32_t begin = min(count, wave * run), end = min(count, begin + run);
     uint32_t over = 0, equal = 0;
-    for (uint32_t i = begin + lane; i < end; i += kWave) {
-        const uint64_t key = get(i);
-        over += key > threshold, equal += key == threshold;
+    for (uint32_t base = begin; base < end; base += kWave) {
+        const uint64_t key = base + lane < end ? get(base + lane) : 0;
+        over += __popcll(__ballot(base + lane < end && key > threshold));
+        equal += __popcll(__ballot(base + lane < end && key == threshold));
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        over += __shfl_xor(over, o), equal += __shfl_xor(equal, o);
     if (lane == 0)
         sc.wave[wave] = over, sc.more[wave] = equal;
     __syncthreads();
@@ -414,9 +499,9 @@ __device__ __forceinline__ uint32_t weight_key(float w)
 
 constexpr uint32_t kKeptRows = 8192;
 
-// A workgroup per (sequence, KV head) decides what stays: moves[i] of a row
-// i below the budget is -1 where it stays and its rank among the holes where
-// it goes; from[r] is the r-th row that stays beyond the budget. Weights and
+// A workgroup per (sequence, KV head) decides what stays: to[r] is the r-th
+// row below the budget that goes, from[r] the r-th beyond it that stays, and
+// counts how many there are. Weights and
 // positions of up to kKeptRows rows are read once, eight rows a thread at a
 // time, and live on as keys in shared memory.
 template <int THREADS>
@@ -424,8 +509,9 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
                                                                 PagedHistory history,
                                                                 uint32_t budget, uint32_t first,
                                                                 uint32_t last, int *new_lengths,
-                                                                int *__restrict__ moves,
-                                                                int *__restrict__ from)
+                                                                int *__restrict__ to,
+                                                                int *__restrict__ from,
+                                                                int *__restrict__ counts)
 {
     const uint32_t id = blockIdx.x, h = id % kv.kv_heads, b = id / kv.kv_heads;
     const bool leader = threadIdx.x == 0 && h == 0;
@@ -445,8 +531,11 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
     const uint32_t n = paged_length(kv, s, b, leader);
     if (leader)
         new_lengths[b] = n > budget ? int(budget) : s.lengths[b];
-    if (n <= budget)
+    if (n <= budget) {
+        if (threadIdx.x == 0)
+            counts[id] = 0;
         return;
+    }
     __shared__ RankScratch sc;
     __shared__ int newest_of[THREADS / kWave];
     __shared__ uint32_t keys[kKeptRows < kEach * THREADS ? kKeptRows : kEach * THREADS];
@@ -459,10 +548,8 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
             newest = max(newest, p[e]);
     for (uint32_t i = kEach * THREADS + threadIdx.x; i < n; i += THREADS)
         newest = max(newest, positions[i]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        newest = max(newest, __shfl_xor(newest, o));
-    if (lane == 0)
+    newest = largest(newest);
+    if (lane == kWave - 1)
         newest_of[wave] = newest;
     __syncthreads();
     for (uint32_t v = 0; v < THREADS / kWave; v++)
@@ -498,8 +585,7 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
     for (uint32_t v = 0; v < wave; v++)
         seen += sc.more[v];
     uint32_t holes = 0, moved = 0;
-    int *move = moves + (size_t(b) * kv.kv_heads + h) * budget;
-    int *source = from + (size_t(b) * kv.kv_heads + h) * budget;
+    int *hole_at = to + size_t(id) * budget, *source = from + size_t(id) * budget;
     for (int pass = 0; pass < 2; pass++) {
         uint32_t met = seen;
         for (uint32_t base = begin; base < end; base += kWave) {
@@ -511,9 +597,9 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
             const uint64_t hole = __ballot(i < end && i < budget && !kept);
             const uint64_t goes = __ballot(kept && i >= budget);
             if (pass == 1) {
-                if (i < end && i < budget)
-                    move[i] = kept ? -1 : int(holes + rank_in(hole));
-                else if (kept)
+                if (i < end && i < budget && !kept)
+                    hole_at[holes + rank_in(hole)] = int(i);
+                else if (kept && i >= budget)
                     source[moved + rank_in(goes)] = int(i);
             }
             holes += __popcll(hole);
@@ -524,114 +610,113 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
             if (lane == 0)
                 sc.wave[wave] = holes, sc.bins[wave] = moved;
             __syncthreads();
+            if (threadIdx.x == THREADS - kWave)
+                counts[id] = int(moved);
             holes = moved = 0;
             for (uint32_t v = 0; v < wave; v++)
                 holes += sc.wave[v], moved += sc.bins[v];
+            if (threadIdx.x == THREADS - kWave)
+                counts[id] += int(moved);
         }
     }
 }
 
-// A workgroup per (sequence, KV head, `span` rows below the budget: whole
-// pages) fetches what moves there, 256 rows of the plan at a time: a thread a
-// row finds where it comes from and lists it, then head_dim / 8 threads a row
-// copy what is listed. Sources lie beyond the budget and are only read, so
-// the order of workgroups does not matter.
+// A workgroup per (sequence, KV head, 256 entries of its list): a thread an
+// entry finds where the row lies and takes its weight and position along, then
+// head_dim / 8 threads a row copy rows. Sources lie beyond the budget and are
+// only read, so the order of workgroups does not matter; the bounds of a page
+// whose entries begin in one workgroup's part and end in another's are the
+// first one's.
 template <int TYPE>
 __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs s,
                                                         PagedHistory history, uint32_t budget,
-                                                        uint32_t span, uint32_t blocks,
-                                                        const int *__restrict__ moves,
-                                                        const int *__restrict__ from)
+                                                        uint32_t blocks,
+                                                        const int *__restrict__ to,
+                                                        const int *__restrict__ from,
+                                                        const int *__restrict__ counts)
 {
     constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
-    const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
-    const uint32_t b = id / blocks / kv.kv_heads;
-    const size_t row = size_t(b) * kv.kv_heads + h, at = row * history.stride;
-    const int *move = moves + row * budget, *source = from + row * budget;
-    const uint32_t first = c * span, last = min(budget, first + span);
-    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t id = blockIdx.x, c = id % blocks, row = id / blocks;
+    const uint32_t h = row % kv.kv_heads, b = row / kv.kv_heads;
+    const size_t at = row * history.stride;
+    to += size_t(row) * budget, from += size_t(row) * budget;
     const uint32_t tpr = kv.head_dim / 8, part = threadIdx.x % tpr, group = threadIdx.x / tpr;
     const uint32_t groups = 256 / tpr, column = part * 8 * kSize;
-    __shared__ size_t to[256], of[256];
-    __shared__ uint32_t page[256];
-    __shared__ uint32_t listed[4];
-    int rank = first + threadIdx.x < last ? move[first + threadIdx.x] : -1;
-    const uint32_t n = paged_length(kv, s, b, false);
-    if (n <= budget)
+    __shared__ size_t here[256], there[256];
+    const uint32_t first = c * 256, r0 = first + threadIdx.x;
+    // the list beside its length: what lies behind it is not used
+    int dst = r0 < budget ? to[r0] : 0, src = r0 < budget ? from[r0] : 0;
+    const uint32_t total = uint32_t(counts[row]);
+    asm volatile("" : "+v"(dst), "+v"(src));
+    if (first >= total)
         return;
-    for (uint32_t base = first; base < last; base += 256) {
-        const uint32_t i = base + threadIdx.x;
-        if (base != first)
-            rank = i < last ? move[i] : -1;
-        size_t here = kNoRow, there = kNoRow;
-        const uint32_t index = page_of(kv, min(i, last - 1));
-        if (rank >= 0) {
-            const uint32_t from_row = uint32_t(source[rank]);
-            history.weights[at + i] = history.weights[at + from_row];
-            history.positions[at + i] = history.positions[at + from_row];
-            const uint32_t from_page = page_of(kv, from_row);
-            here = paged_row(kv, s, b, index, i - index * kv.page_size, h);
-            there = paged_row(kv, s, b, from_page, from_row - from_page * kv.page_size, h);
-        }
-        const bool go = here != kNoRow && there != kNoRow;
-        const uint64_t going = __ballot(go);
-        if (lane == 0)
-            listed[wave] = __popcll(going);
-        __syncthreads();
-        uint32_t place = rank_in(going), count = 0;
-        for (uint32_t w = 0; w < 4; w++) {
-            place += w < wave ? listed[w] : 0;
-            count += listed[w];
-        }
-        if (go)
-            to[place] = here, of[place] = there, page[place] = index;
-        __syncthreads();
-        if (group < groups)
-            for (uint32_t r = group; r < count; r += 2 * groups) {
-                // two rows in flight
-                const uint32_t r2 = min(r + groups, count - 1);
-                uint4 k[2][kSize / 2], v[2][kSize / 2];
+    const uint32_t count = min(256u, total - first);
+    if (r0 < total) {
+        const uint32_t to_page = page_of(kv, dst), from_page = page_of(kv, src);
+        const float w = history.weights[at + src];
+        const int p = history.positions[at + src];
+        const size_t x = paged_row(kv, s, b, to_page, dst - to_page * kv.page_size, h);
+        const size_t y = paged_row(kv, s, b, from_page, src - from_page * kv.page_size, h);
+        history.weights[at + dst] = w;
+        history.positions[at + dst] = p;
+        here[threadIdx.x] = y == kNoRow ? kNoRow : x;
+        there[threadIdx.x] = x == kNoRow ? kNoRow : y;
+    }
+    __syncthreads();
+    if (group >= groups)
+        return;
+    for (uint32_t r = group; r < count; r += 2 * groups) {
+        // two rows in flight
+        uint4 k[2][kSize / 2], v[2][kSize / 2];
+        size_t x[2];
 #pragma unroll
-                for (int e = 0; e < int(kSize / 2); e++) {
-                    k[0][e] = reinterpret_cast<const uint4 *>(kv.keys + of[r] + column)[e];
-                    v[0][e] = reinterpret_cast<const uint4 *>(kv.values + of[r] + column)[e];
-                    k[1][e] = reinterpret_cast<const uint4 *>(kv.keys + of[r2] + column)[e];
-                    v[1][e] = reinterpret_cast<const uint4 *>(kv.values + of[r2] + column)[e];
-                }
+        for (int i = 0; i < 2; i++) {
+            const uint32_t e = min(r + i * groups, count - 1);
+            const size_t y = there[e] == kNoRow ? 0 : there[e];
+            x[i] = r + i * groups < count ? here[e] : kNoRow;
 #pragma unroll
-                for (int e = 0; e < int(kSize / 2); e++) {
-                    reinterpret_cast<uint4 *>(kv.keys + to[r] + column)[e] = k[0][e];
-                    reinterpret_cast<uint4 *>(kv.values + to[r] + column)[e] = v[0][e];
-                    if (r + groups < count) {
-                        reinterpret_cast<uint4 *>(kv.keys + to[r2] + column)[e] = k[1][e];
-                        reinterpret_cast<uint4 *>(kv.values + to[r2] + column)[e] = v[1][e];
-                    }
-                }
+            for (int w = 0; w < int(kSize / 2); w++) {
+                k[i][w] = reinterpret_cast<const uint4 *>(kv.keys + y + column)[w];
+                v[i][w] = reinterpret_cast<const uint4 *>(kv.values + y + column)[w];
             }
-        if (kv.bounds != nullptr && count != 0) {
-            // head_dim / 8 threads a page widen its bounds by what moved in: the
-            // list is in the order of rows, so a page's entries are a run of it
-            if (group < groups)
-                for (uint32_t r = group; r < count; r += groups) {
-                    if (r != 0 && page[r - 1] == page[r])
-                        continue; // not a page's first
-                    char *bounds = kv.bounds +
-                                   (size_t(s.table[size_t(b) * s.table_stride + page[r]]) *
-                                        kv.kv_heads + h) * 2 * kv.head_dim * kSize + column;
-                    float lo[8], hi[8], x[8];
-                    load8<TYPE>(bounds, lo);
-                    load8<TYPE>(bounds + kv.head_dim * kSize, hi);
-                    for (uint32_t e = r; e < count && page[e] == page[r]; e++) {
-                        load8<TYPE>(kv.keys + of[e] + column, x);
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            lo[j] = lower(lo[j], x[j]), hi[j] = upper(hi[j], x[j]);
-                    }
-                    store8<TYPE>(bounds, lo);
-                    store8<TYPE>(bounds + kv.head_dim * kSize, hi);
-                }
         }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (x[i] != kNoRow)
+#pragma unroll
+                for (int w = 0; w < int(kSize / 2); w++) {
+                    reinterpret_cast<uint4 *>(kv.keys + x[i] + column)[w] = k[i][w];
+                    reinterpret_cast<uint4 *>(kv.values + x[i] + column)[w] = v[i][w];
+                }
+    }
+    if (kv.bounds == nullptr)
+        return;
+    // head_dim / 8 threads a page: the list is in the order of rows, so a page's
+    // entries are a run of it
+    for (uint32_t r = group; r < count; r += groups) {
+        const uint32_t page = page_of(kv, to[first + r]);
+        if (first + r != 0 && page_of(kv, to[first + r - 1]) == page)
+            continue; // not its first
+        if (paged_row(kv, s, b, page, 0, h) == kNoRow)
+            continue;
+        char *bounds = kv.bounds + (size_t(s.table[size_t(b) * s.table_stride + page]) *
+                                        kv.kv_heads + h) * 2 * kv.head_dim * kSize + column;
+        float lo[8], hi[8];
+        load8<TYPE>(bounds, lo);
+        load8<TYPE>(bounds + kv.head_dim * kSize, hi);
+        for (uint32_t e = first + r; e < total && page_of(kv, to[e]) == page; e++) {
+            const uint32_t from_page = page_of(kv, from[e]);
+            const size_t y = paged_row(kv, s, b, from_page, from[e] - from_page * kv.page_size, h);
+            if (y == kNoRow)
+                continue;
+            float x[8];
+            load8<TYPE>(kv.keys + y + column, x);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                lo[j] = lower(lo[j], x[j]), hi[j] = upper(hi[j], x[j]);
+        }
+        store8<TYPE>(bounds, lo);
+        store8<TYPE>(bounds + kv.head_dim * kSize, hi);
     }
 }
 
@@ -639,22 +724,30 @@ uint32_t pages_of(const PagedView &kv, uint32_t rows) { return (rows - 1) / kv.p
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <int TYPE>
-void scores_for(const PagedView &kv, const PagedSeqs &seqs, const float *query,
-                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
+template <int TYPE, int GH>
+void scores_of(const PagedView &kv, const PagedSeqs &seqs, const float *query,
+               size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
     uint32_t lanes = 1;
     while (lanes * 8 < kv.head_dim)
         lanes *= 2;
-    const uint32_t width = pages_of(kv, seqs.max_length), group = heads / kv.kv_heads;
-    const uint32_t per_block = 256 / lanes, blocks = (width + per_block - 1) / per_block;
-    const dim3 grid = paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256);
-    const auto kernel = group == 1   ? page_scores_kernel<TYPE, 1>
-                        : group == 2 ? page_scores_kernel<TYPE, 2>
-                        : group <= 4 ? page_scores_kernel<TYPE, 4>
-                                     : page_scores_kernel<TYPE, 8>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, kv, seqs, query, query_stride, heads,
-                       lanes, per_block, blocks, width, scores);
+    const uint32_t width = pages_of(kv, seqs.max_length);
+    const uint32_t per_block = 256 / lanes * kPagesOf<TYPE, GH>;
+    const uint32_t blocks = (width + per_block - 1) / per_block;
+    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH>),
+                       paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
+                       stream, kv, seqs, query, query_stride, heads, lanes, blocks, width, scores);
+}
+
+template <int TYPE>
+void scores_for(const PagedView &kv, const PagedSeqs &seqs, const float *query,
+                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
+{
+    const uint32_t group = heads / kv.kv_heads;
+    const auto run = group == 1   ? scores_of<TYPE, 1>
+                     : group == 2 ? scores_of<TYPE, 2>
+                                  : scores_of<TYPE, 4>;
+    run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 
 } // namespace
@@ -701,31 +794,33 @@ void launch_paged_select(const PagedView &kv, const PagedSeqs &seqs, const float
 
 size_t evict_workspace(const PagedView &kv, const PagedSeqs &seqs, uint32_t budget)
 {
-    return 2 * aligned(size_t(seqs.batch) * kv.kv_heads * budget * sizeof(int));
+    const size_t heads = size_t(seqs.batch) * kv.kv_heads;
+    return 2 * aligned(heads * budget * sizeof(int)) + aligned(heads * sizeof(int));
 }
 
 void launch_paged_evict(const PagedView &kv, const PagedSeqs &seqs, const PagedHistory &history,
                         uint32_t budget, uint32_t first, uint32_t last, int *new_lengths,
                         char *workspace, hipStream_t stream)
 {
-    int *moves = reinterpret_cast<int *>(workspace);
-    int *from = reinterpret_cast<int *>(workspace + evict_workspace(kv, seqs, budget) / 2);
     const uint64_t heads = uint64_t(seqs.batch) * kv.kv_heads;
+    const size_t list = aligned(heads * budget * sizeof(int));
+    int *to = reinterpret_cast<int *>(workspace);
+    int *from = reinterpret_cast<int *>(workspace + list);
+    int *counts = reinterpret_cast<int *>(workspace + 2 * list);
     // eight rows a thread of the smaller workgroup
     const uint32_t threads = seqs.max_length <= 2048 ? 256 : 1024;
     hipLaunchKernelGGL(threads == 256 ? plan_eviction_kernel<256> : plan_eviction_kernel<1024>,
                        paged_grid(heads, threads), dim3(threads), 0, stream, kv, seqs, history,
-                       budget, first, last, new_lengths, moves, from);
+                       budget, first, last, new_lengths, to, from, counts);
     check_launch("paged evict");
     if (budget >= seqs.max_length)
         return;
-    const uint32_t span = kv.page_size >= 256 ? kv.page_size : 256 / kv.page_size * kv.page_size;
-    const uint32_t blocks = (budget - 1) / span + 1;
+    const uint32_t most = std::min(budget, seqs.max_length - budget), blocks = (most + 255) / 256;
     const auto kernel = kv.type == NUT_F32   ? move_rows_kernel<NUT_F32>
                         : kv.type == NUT_F16 ? move_rows_kernel<NUT_F16>
                                              : move_rows_kernel<NUT_BF16>;
     hipLaunchKernelGGL(kernel, paged_grid(heads * blocks, 256), dim3(256), 0, stream, kv, seqs,
-                       history, budget, span, blocks, moves, from);
+                       history, budget, blocks, to, from, counts);
     check_launch("paged evict");
 }
 
