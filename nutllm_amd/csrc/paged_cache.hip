@@ -264,7 +264,61 @@ __device__ __forceinline__ uint32_t rank_in(uint64_t mask)
 // ---------------------------------------------------------------- select --
 
 // Pages a lane scores: more where the query's conversions weigh more.
-template <int TYPE, int GH> constexpr int kPagesOf = GH < 4 ? 1 : TYPE == NUT_F32 ? 2 : 4;
+template <int GH> constexpr uint32_t kPagesOf = GH <= 2 ? 1 : GH == 4 ? 2 : 4;
+
+// A partner's value among the lanes of a page: for O = 2 and 1 the lane O away,
+// for 8 and 4 the mirror image in 2 O lanes, which lies O away in the bit that
+// counts and has not been told apart in the others yet.
+template <int O> __device__ __forceinline__ uint32_t partner(uint32_t v)
+{
+    if constexpr (O == 16)
+        return __shfl_xor(v, 16);
+    else
+        return dpp_bits<(O == 8   ? kDppRowMirror
+                         : O == 4 ? kDppRowHalfMirror
+                         : O == 2 ? kDppQuadSwap2
+                                  : kDppQuadSwap1)>(v, 0);
+}
+
+template <int O> __device__ __forceinline__ uint64_t partner_bits(uint64_t v)
+{
+    return uint64_t(partner<O>(uint32_t(v >> 32))) << 32 | partner<O>(uint32_t(v));
+}
+
+// Sums over the 2 O lanes of a page: while a lane holds several heads it trades
+// half of them for the other half's part, then it adds. `head` becomes the
+// first head that is left, of HELD / (2 O) or one.
+template <int O, int HELD>
+__device__ __forceinline__ void sum_lanes(double *sum, uint32_t part, uint32_t &head)
+{
+    if constexpr (O > 0) {
+        if constexpr (HELD > 1) {
+            const bool up = part & O;
+#pragma unroll
+            for (int j = 0; j < HELD / 2; j++) {
+                const double give = up ? sum[j] : sum[j + HELD / 2];
+                const double keep = up ? sum[j + HELD / 2] : sum[j];
+                sum[j] = keep + __builtin_bit_cast(
+                                    double, partner_bits<O>(__builtin_bit_cast(uint64_t, give)));
+            }
+            head += up ? HELD / 2 : 0;
+            sum_lanes<O / 2, HELD / 2>(sum, part, head);
+        } else {
+            sum[0] += __builtin_bit_cast(
+                double, partner_bits<O>(__builtin_bit_cast(uint64_t, sum[0])));
+            sum_lanes<O / 2, 1>(sum, part, head);
+        }
+    }
+}
+
+template <int O> __device__ __forceinline__ uint64_t best_of_lanes(uint64_t v)
+{
+    if constexpr (O > 0) {
+        const uint64_t other = partner_bits<O>(v);
+        return best_of_lanes<O / 2>(other > v ? other : v);
+    }
+    return v;
+}
 
 // Order-preserving image of a score; a NaN ranks above every number, the
 // pages that are always read above both.
@@ -276,61 +330,71 @@ __device__ __forceinline__ uint64_t score_key(double v)
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// Scores of every page: `lanes` lanes (a power of two, head_dim / 8 of them
-// with work) hold eight components of a page's bounds each. For one page
-//   sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (hi_d + lo_d) / 2
-//                                        + |q_d| (hi_d - lo_d) / 2,
+// Scores of every page: LANES lanes, head_dim / 8 of them with work, hold eight
+// components of a page's bounds each. For one page
+//   2 sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (hi_d + lo_d)
+//                                          + |q_d| (hi_d - lo_d),
 // two multiply-adds a component in 64 bits: the answer is whole numbers, and
-// 32 bits would let rounding choose among near pages. GH heads at a time, and
-// kPages pages a lane, all fetched before the first is used.
-template <int TYPE, int GH>
+// 32 bits would let rounding choose among near pages. GH heads at a time, one
+// page of a lane after another with the next one's bounds on their way.
+template <int TYPE, int GH, uint32_t LANES>
 __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeqs s,
                                                           const float *__restrict__ query,
                                                           size_t query_stride, uint32_t heads,
-                                                          uint32_t lanes, uint32_t blocks,
-                                                          uint32_t width,
+                                                          uint32_t blocks, uint32_t width,
                                                           uint64_t *__restrict__ scores)
 {
-    constexpr int kPages = kPagesOf<TYPE, GH>, kSize = TYPE == NUT_F32 ? 4 : 2;
+    constexpr uint32_t kPages = kPagesOf<GH>, kSize = TYPE == NUT_F32 ? 4 : 2;
     constexpr int kWords = kSize / 2; // 16-byte words of eight components
     const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
     const uint32_t b = id / blocks / kv.kv_heads;
-    const uint32_t step = 256 / lanes, begin = c * step * kPages + threadIdx.x / lanes;
-    const uint32_t group = heads / kv.kv_heads, part = threadIdx.x & (lanes - 1);
+    constexpr uint32_t step = 256 / LANES;
+    const uint32_t mine = threadIdx.x / LANES, first = c * step * kPages;
+    const uint32_t group = heads / kv.kv_heads, part = threadIdx.x % LANES;
     const bool works = part * 8 < kv.head_dim;
+    __shared__ int pages[256 * kPages];
     // the table beside the length: what lies behind it is not used
-    int page[kPages];
+    int entry[kPages];
 #pragma unroll
-    for (int k = 0; k < kPages; k++)
-        page[k] = begin + k * step < width
-                      ? s.table[size_t(b) * s.table_stride + begin + k * step]
-                      : -1;
+    for (uint32_t k = 0; k < kPages; k++) {
+        const uint32_t i = k * 256 + threadIdx.x;
+        entry[k] = i < step * kPages && first + i < width
+                       ? s.table[size_t(b) * s.table_stride + first + i]
+                       : -1;
+    }
     const uint32_t n = paged_length(kv, s, b, threadIdx.x == 0 && h == 0 && c == 0);
     const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
-    if (c * step * kPages >= count)
+    if (first >= count)
         return;
-    uint4 low[kPages][kWords], high[kPages][kWords];
 #pragma unroll
-    for (int k = 0; k < kPages; k++) {
-        const bool good = page[k] >= 0 && uint32_t(page[k]) < kv.pages;
-        if (!good && begin + k * step < count)
-            paged_flag(kv.status, kBadPage);
-        const bool read = good && works && begin + k * step < count;
-        const uint4 *at = reinterpret_cast<const uint4 *>(
-            kv.bounds + (size_t(good ? page[k] : 0) * kv.kv_heads + h) * 2 * kv.head_dim * kSize +
-            part * 8 * kSize);
+    for (uint32_t k = 0; k < kPages; k++) {
+        const uint32_t i = k * 256 + threadIdx.x;
+        if (i < step * kPages) {
+            const bool good = entry[k] >= 0 && uint32_t(entry[k]) < kv.pages;
+            if (!good && first + i < count)
+                paged_flag(kv.status, kBadPage);
+            pages[i] = good ? entry[k] : -1;
+        }
+    }
+    __syncthreads();
+    const char *bounds = kv.bounds + size_t(h) * 2 * kv.head_dim * kSize + part * 8 * kSize;
+    const size_t page_bytes = size_t(kv.kv_heads) * 2 * kv.head_dim * kSize;
+    const auto fetch = [&](uint32_t k, uint4(&low)[kWords], uint4(&high)[kWords]) {
+        const int page = pages[mine + k * step];
+        const bool read = page >= 0 && works && first + mine + k * step < count;
+        const uint4 *at =
+            reinterpret_cast<const uint4 *>(bounds + size_t(read ? page : 0) * page_bytes);
 #pragma unroll
         for (int w = 0; w < kWords; w++) {
-            low[k][w] = read ? at[w] : make_uint4(0, 0, 0, 0);
-            high[k][w] = read ? at[w + kv.head_dim / 8 * kWords] : make_uint4(0, 0, 0, 0);
+            low[w] = read ? at[w] : make_uint4(0, 0, 0, 0);
+            high[w] = read ? at[w + kv.head_dim / 8 * kWords] : make_uint4(0, 0, 0, 0);
         }
-        page[k] = good ? page[k] : -1;
-    }
-    uint64_t best[kPages];
-#pragma unroll
-    for (int k = 0; k < kPages; k++)
-        best[k] = 0;
+    };
+    uint64_t *out = scores + (size_t(b) * kv.kv_heads + h) * width + first + mine;
+#pragma unroll 1
     for (uint32_t g = 0; g < group; g += GH) {
+        uint4 low[kWords], high[kWords], next_low[kWords], next_high[kWords];
+        fetch(0, low, high);
         double q[GH][8];
 #pragma unroll
         for (int j = 0; j < GH; j++) {
@@ -344,71 +408,46 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
             for (int i = 0; i < 8; i++)
                 q[j][i] = double(v[i]);
         }
-#pragma unroll
-        for (int k = 0; k < kPages; k++) {
-            // one page's sums at a time, and its bounds widened anew for each
-            // four heads: kept in 64 bits they would fill the registers
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int w = 0; w < kWords; w++)
-                asm volatile("" : "+v"(low[k][w].x), "+v"(low[k][w].y), "+v"(low[k][w].z),
-                             "+v"(low[k][w].w), "+v"(high[k][w].x), "+v"(high[k][w].y),
-                             "+v"(high[k][w].z), "+v"(high[k][w].w));
+#pragma unroll 1
+        for (uint32_t k = 0; k < kPages; k++) {
+            if (k + 1 < kPages)
+                fetch(k + 1, next_low, next_high);
             float lo[8], hi[8];
-            load8<TYPE>(reinterpret_cast<const char *>(low[k]), lo);
-            load8<TYPE>(reinterpret_cast<const char *>(high[k]), hi);
+            load8<TYPE>(reinterpret_cast<const char *>(low), lo);
+            load8<TYPE>(reinterpret_cast<const char *>(high), hi);
             double sum[GH];
 #pragma unroll
             for (int j = 0; j < GH; j++)
                 sum[j] = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const double mid = 0.5 * (double(hi[i]) + double(lo[i]));
-                const double half = 0.5 * (double(hi[i]) - double(lo[i]));
+                const double mid = double(hi[i]) + double(lo[i]);
+                const double half = double(hi[i]) - double(lo[i]);
 #pragma unroll
                 for (int j = 0; j < GH; j++)
                     sum[j] = fma(fabs(q[j][i]), half, fma(q[j][i], mid, sum[j]));
             }
-            // sums over the page's lanes: while a lane holds several heads it
-            // trades half of them for the other half's part, then it adds
-            uint32_t mine = g, held = GH;
+            uint32_t head = g;
+            sum_lanes<LANES / 2, GH>(sum, part, head);
+            constexpr int kLeft = GH > int(LANES) ? GH / int(LANES) : 1;
+            uint64_t best = 0;
 #pragma unroll
-            for (int i = 0; i < 5; i++) {
-                const uint32_t o = 1u << i;
-                if (o >= lanes)
-                    break;
-                if ((GH >> i) > 1) {
-                    const int rest = (GH >> i) / 2;
-                    const bool upper_half = part & o;
-#pragma unroll
-                    for (int j = 0; j < rest; j++) {
-                        const double give = upper_half ? sum[j] : sum[j + rest];
-                        const double keep = upper_half ? sum[j + rest] : sum[j];
-                        sum[j] = keep + __shfl_xor(give, int(o));
-                    }
-                    mine += upper_half ? rest : 0;
-                    held = rest;
-                } else {
-                    sum[0] += __shfl_xor(sum[0], int(o));
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < GH; j++) {
+            for (int j = 0; j < kLeft; j++) {
                 const uint64_t key = score_key(sum[j]);
-                if (uint32_t(j) < held && mine + j < group && key > best[k])
-                    best[k] = key;
+                if (head + j < group && key > best)
+                    best = key;
             }
-        }
-    }
-    uint64_t *out = scores + (size_t(b) * kv.kv_heads + h) * width;
+            best = best_of_lanes<LANES / 2>(best);
+            if (part == 0 && first + mine + k * step < count) {
+                uint64_t *to = out + k * step;
+                if (pages[mine + k * step] < 0)
+                    best = 0; // below every page that there is
+                *to = g == 0 || best > *to ? best : *to;
+            }
 #pragma unroll
-    for (int k = 0; k < kPages; k++) {
-        for (uint32_t o = 1; o < lanes; o <<= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)best[k], int(o));
-            best[k] = other > best[k] ? other : best[k];
+            for (int w = 0; w < kWords; w++)
+                low[w] = next_low[w], high[w] = next_high[w];
         }
-        if (part == 0 && begin + k * step < count) // a bad page below all others
-            out[begin + k * step] = page[k] < 0 ? 0 : best[k];
     }
 }
 
@@ -724,19 +763,27 @@ uint32_t pages_of(const PagedView &kv, uint32_t rows) { return (rows - 1) / kv.p
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+template <int TYPE, int GH, uint32_t LANES>
+void scores_by(const PagedView &kv, const PagedSeqs &seqs, const float *query,
+               size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
+{
+    const uint32_t width = pages_of(kv, seqs.max_length);
+    const uint32_t per_block = 256 / LANES * kPagesOf<GH>;
+    const uint32_t blocks = (width + per_block - 1) / per_block;
+    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH, LANES>),
+                       paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
+                       stream, kv, seqs, query, query_stride, heads, blocks, width, scores);
+}
+
 template <int TYPE, int GH>
 void scores_of(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
-    uint32_t lanes = 1;
-    while (lanes * 8 < kv.head_dim)
-        lanes *= 2;
-    const uint32_t width = pages_of(kv, seqs.max_length);
-    const uint32_t per_block = 256 / lanes * kPagesOf<TYPE, GH>;
-    const uint32_t blocks = (width + per_block - 1) / per_block;
-    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH>),
-                       paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
-                       stream, kv, seqs, query, query_stride, heads, lanes, blocks, width, scores);
+    const auto run = kv.head_dim <= 32    ? scores_by<TYPE, GH, 4>
+                     : kv.head_dim <= 64  ? scores_by<TYPE, GH, 8>
+                     : kv.head_dim <= 128 ? scores_by<TYPE, GH, 16>
+                                          : scores_by<TYPE, GH, 32>;
+    run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 
 template <int TYPE>
@@ -746,7 +793,8 @@ void scores_for(const PagedView &kv, const PagedSeqs &seqs, const float *query,
     const uint32_t group = heads / kv.kv_heads;
     const auto run = group == 1   ? scores_of<TYPE, 1>
                      : group == 2 ? scores_of<TYPE, 2>
-                                  : scores_of<TYPE, 4>;
+                     : group <= 4 ? scores_of<TYPE, 4>
+                                  : scores_of<TYPE, 8>;
     run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 
