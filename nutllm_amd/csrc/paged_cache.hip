@@ -120,10 +120,10 @@ __global__ __launch_bounds__(256) void append_kernel(
 constexpr int kBits = 8, kBins = 1 << kBits;
 
 struct RankScratch {
-    uint32_t bins[kBins];
-    uint32_t wave[16], more[16];
-    uint32_t any[16][2], all[16][2];
+    alignas(16) uint32_t bins[kBins];
+    uint32_t any[2], lacked[2]; // bits that some key has, and that some key lacks
     uint32_t bin, above, count;
+    uint32_t places[130]; // of each wave's run of 64 keys, and their sum
 };
 
 template <int CTRL, int ROWS = 0xF>
@@ -168,48 +168,80 @@ __device__ __forceinline__ uint32_t running_sum(uint32_t v)
     return v + dpp_bits<kDppRowBcast31, 0xC>(v, 0);
 }
 
-// Finds, for keys get(0) to get(n - 1) and 1 <= k < n, the threshold T and
-// the number of ties such that the k largest keys, ties to the lowest index,
-// are the keys over T and the first `ties` keys equal to T. A radix search
-// from the first bit in which the keys differ, 8 bits a pass (a bin a thread),
-// which ends at the first digit whose keys are all taken: two or three passes
-// of scores that differ in their leading bits. Every thread of the workgroup,
-// 256 of them or more, calls it; it begins and ends at a barrier.
-template <typename K, typename Get>
-__device__ __forceinline__ void kth_largest(Get get, uint32_t n, uint32_t k, RankScratch &sc,
-                                            K &threshold, uint32_t &ties)
+// Lanes below this one in a ballot.
+__device__ __forceinline__ uint32_t rank_in(uint64_t mask)
+{
+    return __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32),
+                                     __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+}
+
+// Keys 0 to n - 1 of a workgroup, EACH a thread in registers (key
+// e THREADS + thread), and segment after segment of so many, read anew each
+// time by `load`, where there are more.
+template <typename K, int THREADS, int EACH, typename Load> struct Keys {
+    static constexpr uint32_t kSegment = THREADS * EACH;
+    const Load &load;
+    uint32_t n;
+    K key[EACH];
+
+    __device__ __forceinline__ uint32_t index(uint32_t segment, int e) const
+    {
+        return segment + e * THREADS + threadIdx.x;
+    }
+    __device__ __forceinline__ void open(uint32_t segment)
+    {
+        if (n > kSegment)
+#pragma unroll
+            for (int e = 0; e < EACH; e++)
+                key[e] = index(segment, e) < n ? load(index(segment, e)) : K(0);
+    }
+    template <typename Use> __device__ __forceinline__ void each(Use use)
+    {
+        for (uint32_t segment = 0; segment < n; segment += kSegment) {
+            open(segment);
+#pragma unroll
+            for (int e = 0; e < EACH; e++)
+                if (index(segment, e) < n)
+                    use(key[e]);
+        }
+    }
+};
+
+// Finds the threshold T and the number of ties such that the k largest keys
+// (1 <= k < n), ties to the lowest index, are the keys over T and the first
+// `ties` keys equal to T. A radix search from the first bit in which the keys
+// differ, 8 bits a pass, which ends at the first digit whose keys are all
+// taken: two or three passes of scores that differ in their leading bits.
+// Every thread of the workgroup calls it, with sc.bins, any and lacked zero
+// and a barrier behind that; it ends at a barrier.
+template <typename K, int THREADS, int EACH, typename Load>
+__device__ __forceinline__ void kth_largest(Keys<K, THREADS, EACH, Load> &keys, uint32_t k,
+                                            RankScratch &sc, K &threshold, uint32_t &ties)
 {
     constexpr int kWidth = 8 * sizeof(K);
-    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t lane = threadIdx.x & (kWave - 1);
     K any = 0, all = K(~K(0));
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const K key = get(i);
-        any |= key, all &= key;
-    }
+    keys.each([&](K key) { any |= key, all &= key; });
 #pragma unroll
     for (int w = 0; w < kWidth / 32; w++) {
-        const uint32_t o = any_bits(uint32_t(any >> (32 * w)));
-        const uint32_t a = all_bits(uint32_t(all >> (32 * w)));
-        if (lane == kWave - 1)
-            sc.any[wave][w] = o, sc.all[wave][w] = a;
+        const uint32_t has = any_bits(uint32_t(any >> (32 * w)));
+        const uint32_t lacks = any_bits(uint32_t(~all >> (32 * w)));
+        if (lane == kWave - 1) {
+            atomicOr(&sc.any[w], has);
+            atomicOr(&sc.lacked[w], lacks);
+        }
     }
-    if (threadIdx.x < kBins)
-        sc.bins[threadIdx.x] = 0;
     __syncthreads();
-    any = 0, all = K(~K(0));
-    for (uint32_t w = 0; w < blockDim.x / kWave; w++) {
-        K o = 0, a = 0;
+    any = 0;
+    K differ = 0;
 #pragma unroll
-        for (int p = 0; p < kWidth / 32; p++)
-            o |= K(sc.any[w][p]) << (32 * p), a |= K(sc.all[w][p]) << (32 * p);
-        any |= o, all &= a;
+    for (int w = 0; w < kWidth / 32; w++) {
+        any |= K(sc.any[w]) << (32 * w);
+        differ |= K(sc.any[w] & sc.lacked[w]) << (32 * w);
     }
-    const K differ = any ^ all;
     if (differ == 0) {
         threshold = any;
         ties = k;
-        __syncthreads();
         return;
     }
     int open = 64 - __clzll((unsigned long long)differ); // bits not yet decided
@@ -218,47 +250,78 @@ __device__ __forceinline__ void kth_largest(Get get, uint32_t n, uint32_t k, Ran
     while (true) {
         const int shift = max(0, open - kBits);
         const uint32_t mask = (1u << (open - shift)) - 1;
-        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const K key = get(i);
+        keys.each([&](K key) {
             if (open >= kWidth || (K(key ^ prefix) >> open) == 0)
                 atomicAdd(&sc.bins[uint32_t(key >> shift) & mask], 1u);
-        }
+        });
         __syncthreads();
-        // thread t owns bin 255 - t: a scan from the highest bin down
-        uint32_t own = 0, scan = 0;
-        if (threadIdx.x < kBins) {
-            own = sc.bins[kBins - 1 - threadIdx.x];
-            scan = running_sum(own);
-            if (lane == kWave - 1)
-                sc.wave[wave] = scan;
-        }
-        __syncthreads();
-        if (threadIdx.x < kBins) {
-            for (uint32_t w = 0; w < wave; w++)
-                scan += sc.wave[w];
-            if (scan >= left && scan - own < left)
-                sc.bin = kBins - 1 - threadIdx.x, sc.above = scan - own, sc.count = own;
-            sc.bins[kBins - 1 - threadIdx.x] = 0; // for the next pass
+        if (threadIdx.x < kWave) {
+            // lane l holds bins 255 - 4 l down to 252 - 4 l: from the highest
+            uint4 *at = reinterpret_cast<uint4 *>(sc.bins) + (kWave - 1 - lane);
+            const uint4 bins = *at;
+            *at = make_uint4(0, 0, 0, 0); // for the next pass
+            const uint32_t own = bins.x + bins.y + bins.z + bins.w;
+            const uint32_t scan = running_sum(own);
+            if (scan >= left && scan - own < left) {
+                const uint32_t size[4] = {bins.w, bins.z, bins.y, bins.x};
+                uint32_t above = scan - own, bin = 255 - 4 * lane, count = size[0];
+#pragma unroll
+                for (int i = 1; i < 4; i++)
+                    if (above + count < left)
+                        above += count, bin--, count = size[i];
+                sc.bin = bin, sc.above = above, sc.count = count;
+            }
         }
         __syncthreads();
         prefix |= K(sc.bin) << shift;
         left -= sc.above;
-        const bool whole = sc.count == left;
-        if (whole || shift == 0) {
+        if (sc.count == left || shift == 0) {
             threshold = prefix;
-            ties = whole ? 0xffffffffu : left;
-            __syncthreads();
+            ties = sc.count == left ? 0xffffffffu : left;
             return;
         }
         open = shift;
+        // sc.bin and its neighbours are written again behind the next barrier
     }
 }
 
-// Lanes below this one in a ballot.
-__device__ __forceinline__ uint32_t rank_in(uint64_t mask)
+// place[e] becomes the number of set flags before flag e of this thread, in the
+// order of keys, `base` growing by all of them. Flags are counts of two kinds
+// in halves of a word. Every thread calls it; sc.places may be in use until
+// the first barrier only.
+template <int THREADS, int EACH>
+__device__ __forceinline__ void places_of(const uint32_t (&flag)[EACH], uint32_t (&place)[EACH],
+                                          uint32_t &base, RankScratch &sc)
 {
-    return __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32),
-                                     __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+    constexpr uint32_t kWaves = THREADS / kWave, kRuns = kWaves * EACH;
+    static_assert(kRuns <= 128, "two runs a lane");
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    uint32_t sum = 0; // of lane e's run
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const uint64_t low = __ballot(flag[e] & 0xffffu), high = __ballot(flag[e] >> 16);
+        place[e] = rank_in(low) | rank_in(high) << 16;
+        if (lane == uint32_t(e))
+            sum = __popcll(low) | uint32_t(__popcll(high)) << 16;
+    }
+    __syncthreads();
+    if (lane < EACH)
+        sc.places[lane * kWaves + wave] = sum;
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+        const uint32_t a = 2 * lane < kRuns ? sc.places[2 * lane] : 0;
+        const uint32_t z = 2 * lane + 1 < kRuns ? sc.places[2 * lane + 1] : 0;
+        const uint32_t scan = running_sum(a + z);
+        sc.places[2 * lane] = scan - a - z;
+        sc.places[2 * lane + 1] = scan - z;
+        if (lane == kWave - 1)
+            sc.places[128] = scan;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; e++)
+        place[e] += base + sc.places[e * kWaves + wave];
+    base += sc.places[128];
 }
 
 // ---------------------------------------------------------------- select --
@@ -451,24 +514,25 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     }
 }
 
-// A workgroup per (sequence, KV head): the `top` best of its pages. Up to kKept
-// scores are read once.
-constexpr uint32_t kKept = 4096;
-
+// A workgroup per (sequence, KV head): the `top` best of its pages.
 __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSeqs s,
                                                            const uint64_t *__restrict__ scores,
                                                            uint32_t width, uint32_t top,
                                                            uint32_t first, uint32_t last,
                                                            int *__restrict__ selected)
 {
+    constexpr int kEach = 8;
+    __shared__ RankScratch sc;
     const uint32_t id = blockIdx.x, h = id % kv.kv_heads, b = id / kv.kv_heads;
     const uint64_t *mine = scores + (size_t(b) * kv.kv_heads + h) * width;
     // the first scores beside the length: those behind it are not used
-    constexpr uint32_t kEach = 4;
     uint64_t early[kEach];
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; e++)
+    for (int e = 0; e < kEach; e++)
         early[e] = e * 256 + threadIdx.x < width ? mine[e * 256 + threadIdx.x] : 0;
+    sc.bins[threadIdx.x] = 0;
+    if (threadIdx.x < 2)
+        sc.any[threadIdx.x] = sc.lacked[threadIdx.x] = 0;
     const uint32_t n = paged_length(kv, s, b, false);
     const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
     int *out = selected + (size_t(b) * kv.kv_heads + h) * top;
@@ -477,51 +541,44 @@ __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSe
             out[i] = i < count ? int(i) : -1;
         return;
     }
-    __shared__ RankScratch sc;
-    __shared__ uint64_t keys[kKept];
     const auto key_of = [&](uint32_t i, uint64_t score) -> uint64_t {
         return i < first || i >= count - last ? ~0ull : score;
     };
+    const auto load = [&](uint32_t i) { return key_of(i, mine[i]); };
+    Keys<uint64_t, 256, kEach, decltype(load)> keys{load, count, {}};
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; e++)
-        keys[e * 256 + threadIdx.x] = key_of(e * 256 + threadIdx.x, early[e]);
-    for (uint32_t i = kEach * 256 + threadIdx.x; i < min(count, kKept); i += 256)
-        keys[i] = key_of(i, mine[i]);
-    const auto get = [&](uint32_t i) -> uint64_t {
-        return i < kKept ? keys[i] : key_of(i, mine[i]);
-    };
+    for (int e = 0; e < kEach; e++)
+        keys.key[e] = key_of(e * 256 + threadIdx.x, early[e]);
+    __syncthreads();
     uint64_t threshold;
     uint32_t ties;
-    kth_largest<uint64_t>(get, count, top, sc, threshold, ties);
+    kth_largest(keys, top, sc, threshold, ties);
 
-    // each wave writes what is kept of a run of pages of its own
-    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const uint32_t run = (count + blockDim.x - 1) / blockDim.x * kWave;
-    const uint32_t begin = min(count, wave * run), end = min(count, begin + run);
-    uint32_t over = 0, equal = 0;
-    for (uint32_t base = begin; base < end; base += kWave) {
-        const uint64_t key = base + lane < end ? get(base + lane) : 0;
-        over += __popcll(__ballot(base + lane < end && key > threshold));
-        equal += __popcll(__ballot(base + lane < end && key == threshold));
-    }
-    if (lane == 0)
-        sc.wave[wave] = over, sc.more[wave] = equal;
-    __syncthreads();
-    uint32_t at = 0, seen = 0;
-    for (uint32_t w = 0; w < wave; w++)
-        at += sc.wave[w], seen += sc.more[w];
-    at += min(seen, ties);
-    for (uint32_t base = begin; base < end; base += kWave) {
-        const uint32_t i = base + lane;
-        const uint64_t key = i < end ? get(i) : 0;
-        const bool tie = i < end && key == threshold;
-        const uint64_t tied = __ballot(tie);
-        const bool kept = i < end && (key > threshold || (tie && seen + rank_in(tied) < ties));
-        const uint64_t all = __ballot(kept);
-        if (kept)
-            out[at + rank_in(all)] = int(i);
-        at += __popcll(all);
-        seen += __popcll(tied);
+    uint32_t at = 0, met = 0;
+    for (uint32_t segment = 0; segment < count; segment += keys.kSegment) {
+        keys.open(segment);
+        uint32_t flag[kEach], place[kEach];
+        bool kept[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const bool in = keys.index(segment, e) < count;
+            kept[e] = in && keys.key[e] >= threshold;
+            flag[e] = in && keys.key[e] == threshold;
+        }
+        if (ties != 0xffffffffu) {
+            places_of<256, kEach>(flag, place, met, sc);
+#pragma unroll
+            for (int e = 0; e < kEach; e++)
+                kept[e] = kept[e] && (flag[e] == 0 || place[e] < ties);
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; e++)
+            flag[e] = kept[e];
+        places_of<256, kEach>(flag, place, at, sc);
+#pragma unroll
+        for (int e = 0; e < kEach; e++)
+            if (kept[e])
+                out[place[e]] = int(keys.index(segment, e));
     }
 }
 
@@ -536,13 +593,10 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return key; // at least ~0xff800000 = 0x007fffff, over a NaN's
 }
 
-constexpr uint32_t kKeptRows = 8192;
-
 // A workgroup per (sequence, KV head) decides what stays: to[r] is the r-th
 // row below the budget that goes, from[r] the r-th beyond it that stays, and
-// counts how many there are. Weights and
-// positions of up to kKeptRows rows are read once, eight rows a thread at a
-// time, and live on as keys in shared memory.
+// counts how many there are. Weights and positions of up to eight rows a
+// thread are read once.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, PagedSeqs s,
                                                                 PagedHistory history,
@@ -552,13 +606,15 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
                                                                 int *__restrict__ from,
                                                                 int *__restrict__ counts)
 {
+    constexpr int kEach = 8;
+    __shared__ RankScratch sc;
+    __shared__ int newest_of[THREADS / kWave];
     const uint32_t id = blockIdx.x, h = id % kv.kv_heads, b = id / kv.kv_heads;
     const bool leader = threadIdx.x == 0 && h == 0;
     const size_t at = (size_t(b) * kv.kv_heads + h) * history.stride;
     const float *weights = history.weights + at;
     const int *positions = history.positions + at;
     // the first rows beside the length, which max_length bounds
-    constexpr int kEach = 8;
     float w[kEach];
     int p[kEach];
 #pragma unroll
@@ -567,6 +623,10 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
         w[e] = i < s.max_length ? weights[i] : 0.0f;
         p[e] = i < s.max_length ? positions[i] : 0;
     }
+    if (threadIdx.x < kBins)
+        sc.bins[threadIdx.x] = 0;
+    if (threadIdx.x < 2)
+        sc.any[threadIdx.x] = sc.lacked[threadIdx.x] = 0;
     const uint32_t n = paged_length(kv, s, b, leader);
     if (leader)
         new_lengths[b] = n > budget ? int(budget) : s.lengths[b];
@@ -575,10 +635,6 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
             counts[id] = 0;
         return;
     }
-    __shared__ RankScratch sc;
-    __shared__ int newest_of[THREADS / kWave];
-    __shared__ uint32_t keys[kKeptRows < kEach * THREADS ? kKeptRows : kEach * THREADS];
-    constexpr uint32_t kHeld = sizeof keys / sizeof keys[0];
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     int newest = -1;
 #pragma unroll
@@ -591,73 +647,61 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
     if (lane == kWave - 1)
         newest_of[wave] = newest;
     __syncthreads();
-    for (uint32_t v = 0; v < THREADS / kWave; v++)
+    newest = newest_of[0];
+#pragma unroll
+    for (int v = 1; v < THREADS / kWave; v++)
         newest = max(newest, newest_of[v]);
     const int64_t recent = int64_t(newest) - int64_t(last);
     const auto key_of = [&](int position, float weight) -> uint32_t {
         return position < int64_t(first) || position > recent ? 0xffffffffu : weight_key(weight);
     };
-    if (n <= kHeld)
+    const auto load = [&](uint32_t i) { return key_of(positions[i], weights[i]); };
+    Keys<uint32_t, THREADS, kEach, decltype(load)> keys{load, n, {}};
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+        keys.key[e] = key_of(p[e], w[e]);
+    uint32_t threshold, ties;
+    kth_largest(keys, budget, sc, threshold, ties);
+
+    // holes in the lower halves of words, rows to move in the upper ones: each
+    // segment has at most 2^13 of them
+    uint32_t met = 0, holes = 0, moved = 0;
+    int *hole_at = to + size_t(id) * budget, *source = from + size_t(id) * budget;
+    for (uint32_t segment = 0; segment < n; segment += keys.kSegment) {
+        keys.open(segment);
+        uint32_t flag[kEach], place[kEach];
+        bool kept[kEach];
 #pragma unroll
         for (int e = 0; e < kEach; e++) {
-            const uint32_t i = e * THREADS + threadIdx.x;
-            if (i < n)
-                keys[i] = key_of(p[e], w[e]);
+            const bool in = keys.index(segment, e) < n;
+            kept[e] = in && keys.key[e] >= threshold;
+            flag[e] = in && keys.key[e] == threshold;
         }
-    const auto get = [&](uint32_t i) -> uint32_t {
-        return n <= kHeld ? keys[i] : key_of(positions[i], weights[i]);
-    };
-    uint32_t threshold, ties;
-    kth_largest<uint32_t>(get, n, budget, sc, threshold, ties);
-
-    // each wave takes a run of rows: its ties first, then its holes and rows to
-    // move, then their places
-    const uint32_t run = (n + THREADS - 1) / THREADS * kWave;
-    const uint32_t begin = min(n, wave * run), end = min(n, begin + run);
-    uint32_t equal = 0;
-    for (uint32_t base = begin; base < end; base += kWave)
-        equal += __popcll(__ballot(base + lane < end && get(base + lane) == threshold));
-    if (lane == 0)
-        sc.more[wave] = equal;
-    __syncthreads();
-    uint32_t seen = 0;
-    for (uint32_t v = 0; v < wave; v++)
-        seen += sc.more[v];
-    uint32_t holes = 0, moved = 0;
-    int *hole_at = to + size_t(id) * budget, *source = from + size_t(id) * budget;
-    for (int pass = 0; pass < 2; pass++) {
-        uint32_t met = seen;
-        for (uint32_t base = begin; base < end; base += kWave) {
-            const uint32_t i = base + lane;
-            const uint32_t key = i < end ? get(i) : 0;
-            const bool tie = i < end && key == threshold;
-            const uint64_t tied = __ballot(tie);
-            const bool kept = i < end && (key > threshold || (tie && met + rank_in(tied) < ties));
-            const uint64_t hole = __ballot(i < end && i < budget && !kept);
-            const uint64_t goes = __ballot(kept && i >= budget);
-            if (pass == 1) {
-                if (i < end && i < budget && !kept)
-                    hole_at[holes + rank_in(hole)] = int(i);
-                else if (kept && i >= budget)
-                    source[moved + rank_in(goes)] = int(i);
-            }
-            holes += __popcll(hole);
-            moved += __popcll(goes);
-            met += __popcll(tied);
+        if (ties != 0xffffffffu) {
+            places_of<THREADS, kEach>(flag, place, met, sc);
+#pragma unroll
+            for (int e = 0; e < kEach; e++)
+                kept[e] = kept[e] && (flag[e] == 0 || place[e] < ties);
         }
-        if (pass == 0) {
-            if (lane == 0)
-                sc.wave[wave] = holes, sc.bins[wave] = moved;
-            __syncthreads();
-            if (threadIdx.x == THREADS - kWave)
-                counts[id] = int(moved);
-            holes = moved = 0;
-            for (uint32_t v = 0; v < wave; v++)
-                holes += sc.wave[v], moved += sc.bins[v];
-            if (threadIdx.x == THREADS - kWave)
-                counts[id] += int(moved);
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const uint32_t i = keys.index(segment, e);
+            flag[e] = i >= n ? 0 : i < budget ? !kept[e] : uint32_t(kept[e]) << 16;
         }
+        uint32_t both = 0;
+        places_of<THREADS, kEach>(flag, place, both, sc);
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            if (flag[e] == 1)
+                hole_at[holes + (place[e] & 0xffffu)] = int(keys.index(segment, e));
+            else if (flag[e] != 0)
+                source[moved + (place[e] >> 16)] = int(keys.index(segment, e));
+        }
+        holes += both & 0xffffu;
+        moved += both >> 16;
     }
+    if (threadIdx.x == 0)
+        counts[id] = int(moved);
 }
 
 // A workgroup per (sequence, KV head, 256 entries of its list): a thread an
