@@ -748,29 +748,30 @@ __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs 
     __syncthreads();
     if (group >= groups)
         return;
-    for (uint32_t r = group; r < count; r += 2 * groups) {
-        // two rows in flight
-        uint4 k[2][kSize / 2], v[2][kSize / 2];
-        size_t x[2];
+    typedef uint32_t Piece __attribute__((ext_vector_type(4)));
+    constexpr int kPieces = kSize / 2, kRows = 4; // rows in flight
+    for (uint32_t r = group; r < count; r += kRows * groups) {
+        Piece k[kRows][kPieces], v[kRows][kPieces];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t e = min(r + i * groups, count - 1);
-            const size_t y = there[e] == kNoRow ? 0 : there[e];
-            x[i] = r + i * groups < count ? here[e] : kNoRow;
+        for (int i = 0; i < kRows; i++) {
+            const size_t y = there[min(r + i * groups, count - 1)];
+            const size_t from_row = y == kNoRow ? 0 : y;
 #pragma unroll
-            for (int w = 0; w < int(kSize / 2); w++) {
-                k[i][w] = reinterpret_cast<const uint4 *>(kv.keys + y + column)[w];
-                v[i][w] = reinterpret_cast<const uint4 *>(kv.values + y + column)[w];
+            for (int w = 0; w < kPieces; w++) {
+                k[i][w] = reinterpret_cast<const Piece *>(kv.keys + from_row + column)[w];
+                v[i][w] = reinterpret_cast<const Piece *>(kv.values + from_row + column)[w];
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (x[i] != kNoRow)
+        for (int i = 0; i < kRows; i++) {
+            const size_t x = r + i * groups < count ? here[r + i * groups] : kNoRow;
+            if (x != kNoRow)
 #pragma unroll
-                for (int w = 0; w < int(kSize / 2); w++) {
-                    reinterpret_cast<uint4 *>(kv.keys + x[i] + column)[w] = k[i][w];
-                    reinterpret_cast<uint4 *>(kv.values + x[i] + column)[w] = v[i][w];
+                for (int w = 0; w < kPieces; w++) {
+                    reinterpret_cast<Piece *>(kv.keys + x + column)[w] = k[i][w];
+                    reinterpret_cast<Piece *>(kv.values + x + column)[w] = v[i][w];
                 }
+        }
     }
     if (kv.bounds == nullptr)
         return;
