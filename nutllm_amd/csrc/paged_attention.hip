@@ -483,14 +483,26 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
     // up to 64 components) keep loads in flight. A second tile in registers
     // cost their places: 378 us for 337 where both were measured.
     Tile<TYPE, HD> x;
-    if (wave < tiles)
-        x.template load<FULL, NT>(kv, lds.at + wave * T::kRows, lane);
+    constexpr uint32_t kAll = T::kWide ? 0xffffu : 0xffffffffu;
+    const auto masked = [&](int t) {
+        return uint32_t(__builtin_amdgcn_readfirstlane(
+            gone[t * T::kRows / 32] >> (t * T::kRows % 32) & kAll));
+    };
+    // the wave's next tile; of a selection, which may hold fewer pages than there
+    // is room for, the next one that has a row
+    const auto next = [&](int t) {
+        while (a.selected != nullptr && t < tiles && masked(t) == kAll)
+            t += kWaves;
+        return t;
+    };
+    int t = next(wave);
+    if (t < tiles)
+        x.template load<FULL, NT>(kv, lds.at + t * T::kRows, lane);
     q.convert(a.scale);
-    for (int t = wave; t < tiles;) {
-        const uint32_t word = gone[t * T::kRows / 32] >> (t * T::kRows % 32);
-        attend<TYPE, HD>(x, __builtin_amdgcn_readfirstlane(T::kWide ? word & 0xffffu : word), q, sm,
-                         scores == nullptr ? nullptr : scores + t * T::kRows, lane);
-        t += kWaves;
+    while (t < tiles) {
+        attend<TYPE, HD>(x, masked(t), q, sm, scores == nullptr ? nullptr : scores + t * T::kRows,
+                         lane);
+        t = next(t + kWaves);
         if (t < tiles)
             x.template load<FULL, NT>(kv, lds.at + t * T::kRows, lane);
     }
@@ -737,8 +749,11 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
 {
     const auto aligned = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
     AttentionPlan plan{};
-    const uint32_t group = heads / kv.kv_heads, rows = top == 0 ? seqs.max_length
-                                                                : top * kv.page_size;
+    const uint32_t group = heads / kv.kv_heads;
+    const uint32_t rows = top == 0 ? seqs.max_length : top * kv.page_size;
+    // a selection of more pages than a sequence has is -1 behind them, and tiles
+    // without a row are passed over
+    const uint32_t likely = std::min(rows, seqs.max_length);
     plan.tiles = (group + 15) / 16;
     // Runs as long as leave 512 workgroups: of 32 ragged sequences of up to 2,048
     // bfloat16 rows, 13.5 us in runs of 512 (512 workgroups), 14.2 in runs of 256
@@ -753,7 +768,7 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     // join's launch costs more. One sequence of 64 components, one run and
     // split: 256 fp32 rows 6.9 and 8.6 us, 512 10.3 and 8.6; 512 bfloat16 rows
     // 7.2 and 8.4, 1,000 10.6 and 8.5.
-    if (rows <= kMostRows && uint64_t(rows) * kv.head_dim * paged_element(kv.type) <= 65536)
+    if (rows <= kMostRows && uint64_t(likely) * kv.head_dim * paged_element(kv.type) <= 65536)
         plan.chunk = kMostRows;
     plan.chunks = (rows + plan.chunk - 1) / plan.chunk;
     if (plan.chunks == 1 && !weighted)

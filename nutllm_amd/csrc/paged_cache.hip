@@ -543,7 +543,7 @@ __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSe
     sc.bins[threadIdx.x] = 0;
     if (threadIdx.x < 2)
         sc.any[threadIdx.x] = sc.lacked[threadIdx.x] = 0;
-    const uint32_t n = paged_length(kv, s, b, false);
+    const uint32_t n = paged_length(kv, s, b, threadIdx.x == 0 && h == 0);
     const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
     int *out = selected + (size_t(b) * kv.kv_heads + h) * top;
     if (count <= top) {
@@ -887,8 +887,11 @@ void launch_paged_select(const PagedView &kv, const PagedSeqs &seqs, const float
     const auto run = kv.type == NUT_F32   ? scores_for<NUT_F32>
                      : kv.type == NUT_F16 ? scores_for<NUT_F16>
                                           : scores_for<NUT_BF16>;
-    run(kv, seqs, query, query_stride, heads, scores, stream);
-    check_launch("paged select");
+    // sequences of no more than `top` pages read them all
+    if (pages_of(kv, seqs.max_length) > top) {
+        run(kv, seqs, query, query_stride, heads, scores, stream);
+        check_launch("paged select");
+    }
     hipLaunchKernelGGL(choose_pages_kernel, paged_grid(uint64_t(seqs.batch) * kv.kv_heads, 256),
                        dim3(256), 0, stream, kv, seqs, scores, pages_of(kv, seqs.max_length), top, first, last,
                        selected);

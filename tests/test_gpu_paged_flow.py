@@ -361,3 +361,19 @@ def test_allocates_nothing(gpu):
     case.paged.evict(case.seqs, case.history, case.d["new_lengths"], 50, workspace=space)
     gpu.synchronize()
     assert gpu.device_allocations() == before
+
+
+def test_weights_of_rows_on_a_missing_page(gpu):
+    """Rows on a page that the cache has not gather nothing, whole tiles of
+    them included, whatever the workspace held."""
+    case = Case("bf16", [200], 2, 64, 64, seed=57, max_length=256).upload()
+    table = case.table.copy()
+    table[0, 1] = -1  # rows 64 to 127
+    case.d["table"].upload(table)
+    case.attention(query_of(case, 4), 4, history=case.history)
+    got = case.fetch("weights")
+    assert same(got[0, :, 64:128], case.weights[0, :, 64:128])
+    grown = (got - case.weights)[0, :, :200].sum(1)
+    assert np.all(np.abs(grown - 2) <= 1e-4)  # two heads a KV head, all their weight
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
