@@ -442,6 +442,87 @@ private:
     void *ptr_ = nullptr;
 };
 
+// One layer's paged K/V cache: a nut_paged_kv over device memory that the
+// caller holds (no reference counterpart). Calls are asynchronous on `stream`,
+// allocate nothing, and throw for arguments that the host can judge; check()
+// waits and throws for what only the device saw.
+class PagedKV {
+public:
+    explicit PagedKV(const nut_paged_kv &view) : view_(view) {}
+    const nut_paged_kv &view() const { return view_; }
+
+    // Fp32 rows behind the sequences: rows starts[b] to starts[b + 1] for
+    // sequence b, or row b where starts is null (and max_new 1).
+    void append(const nut_paged_batch &seqs, const float *d_keys, const float *d_values,
+                size_t rows, const int *d_starts = nullptr, size_t max_new = 1,
+                int *d_new_lengths = nullptr, const nut_paged_history *history = nullptr,
+                const int *d_first_positions = nullptr, size_t row_stride = 0,
+                size_t head_stride = 0, void *stream = nullptr) const
+    {
+        check_status(nut_paged_append(&view_, &seqs, d_keys, d_values, rows, row_stride,
+                                      head_stride, d_starts, max_new, history,
+                                      d_first_positions, d_new_lengths, stream));
+    }
+    // Rows [begin, end) of a layer of `source` behind the one sequence of seqs.
+    void append(const nut_paged_batch &seqs, const KVCache &source, size_t layer, size_t begin,
+                size_t end, int *d_new_lengths = nullptr,
+                const nut_paged_history *history = nullptr,
+                const int *d_first_positions = nullptr, void *stream = nullptr) const
+    {
+        check_status(nut_paged_append_cache(&view_, &seqs, source.handle(), layer, begin, end,
+                                            history, d_first_positions, d_new_lengths, stream));
+    }
+    size_t attention_workspace(const nut_paged_batch &seqs, size_t heads, size_t top = 0,
+                               bool weighted = false) const
+    {
+        return bytes(nut_paged_attention_workspace(&view_, &seqs, heads, top, weighted ? 1 : 0));
+    }
+    void attention(const nut_paged_batch &seqs, const float *d_query, size_t heads, float scale,
+                   float *d_out, void *d_workspace, size_t workspace_bytes,
+                   float *d_lse = nullptr, const nut_paged_history *history = nullptr,
+                   const int *d_selected = nullptr, size_t top = 0, size_t query_stride = 0,
+                   void *stream = nullptr) const
+    {
+        check_status(nut_paged_attention(&view_, &seqs, d_query, query_stride, heads, scale,
+                                         d_selected, top, history, d_out, d_lse, d_workspace,
+                                         workspace_bytes, stream));
+    }
+    size_t select_workspace(const nut_paged_batch &seqs, size_t heads, size_t top) const
+    {
+        return bytes(nut_paged_select_workspace(&view_, &seqs, heads, top));
+    }
+    void select(const nut_paged_batch &seqs, const float *d_query, size_t heads, size_t top,
+                size_t first, size_t last, int *d_selected, void *d_workspace,
+                size_t workspace_bytes, size_t query_stride = 0, void *stream = nullptr) const
+    {
+        check_status(nut_paged_select(&view_, &seqs, d_query, query_stride, heads, top, first,
+                                      last, d_selected, d_workspace, workspace_bytes, stream));
+    }
+    size_t evict_workspace(const nut_paged_batch &seqs, size_t budget) const
+    {
+        return bytes(nut_paged_evict_workspace(&view_, &seqs, budget));
+    }
+    void evict(const nut_paged_batch &seqs, const nut_paged_history &history, size_t budget,
+               size_t first, size_t last, int *d_new_lengths, void *d_workspace,
+               size_t workspace_bytes, void *stream = nullptr) const
+    {
+        check_status(nut_paged_evict(&view_, &seqs, &history, budget, first, last, d_new_lengths,
+                                     d_workspace, workspace_bytes, stream));
+    }
+    void check() const { check_status(nut_paged_check(&view_)); }
+
+private:
+    static void check_status(int status) { nutgpu::check(status); }
+    static size_t bytes(size_t count)
+    {
+        if (count == SIZE_MAX)
+            check_status(NUT_EINVAL);
+        return count;
+    }
+
+    nut_paged_kv view_;
+};
+
 inline void matvec_quantized_threaded(const QuantizedMatrix &matrix,
                                       const float *vector, float *output,
                                       size_t thread_count)

@@ -36,7 +36,7 @@ nut::PagedView view_of(const nut_paged_kv *kv)
     v.pages = uint32_t(kv->pages), v.page_size = uint32_t(kv->page_size);
     v.kv_heads = uint32_t(kv->kv_heads), v.head_dim = uint32_t(kv->head_dim);
     v.type = kv->type, v.status = kv->d_status;
-    nut::set_page_division(v);
+    v.division = nut::page_division(v.page_size);
     // Rows are at most 2^93 elements apart by these counts; offsets have to
     // stay below 2^63 bytes.
     const double rows = double(kv->pages) * double(kv->page_size) * double(kv->kv_heads);

@@ -8,40 +8,24 @@
 #include <stdint.h>
 
 #include "nutllm_hip.h"
+#include "paged_index.hpp"
 #include "status.hpp"
 
 namespace nut {
-
-// Bits of a view's status word.
-enum : int { kBadPage = 1, kBadLength = 2, kBadRows = 4 };
 
 // A nut_paged_kv with its strides resolved, in bytes.
 struct PagedView {
     char *keys, *values, *bounds;
     uint32_t pages, page_size, kv_heads, head_dim;
-    uint32_t page_magic, page_shift; // row / page_size, see page_of
+    PageDivision division; // by page_size
     size_t page_stride, head_stride, slot_stride;
     int type;
     int *status;
 };
 
-// Division of rows (below 2^31) by the page size as a multiplication: with
-// 2^(l - 1) < size <= 2^l and magic = floor(2^(31 + l) / size) + 1, the product
-// row magic exceeds row 2^(31 + l) / size by at most row < 2^31, less than
-// what a row's fraction of a page is short of the next one. Size 1: magic 0.
-inline void set_page_division(PagedView &v)
-{
-    uint32_t l = 0;
-    while ((uint64_t(1) << l) < v.page_size)
-        l++;
-    v.page_magic = l == 0 ? 0 : uint32_t((uint64_t(1) << (31 + l)) / v.page_size + 1);
-    v.page_shift = l == 0 ? 0 : l - 1;
-}
-
 inline __host__ __device__ uint32_t page_of(const PagedView &v, uint32_t row)
 {
-    return v.page_magic == 0 ? row
-                             : uint32_t(uint64_t(row) * v.page_magic >> 32) >> v.page_shift;
+    return divide(v.division, row);
 }
 
 struct PagedSeqs {
@@ -68,10 +52,11 @@ inline size_t paged_element(int type) { return type == NUT_F32 ? 4 : 2; }
 
 // How an attention call is split: `chunks` runs of `chunk` rows (of the
 // sequence, or of the selection) a sequence and KV head, `tiles` tiles of 16
-// query heads, and where the pieces of its workspace lie.
+// query heads, and where the pieces of its workspace lie behind the runs'
+// unnormalised results. Raises NUT_EINVAL where a launch does not cover it.
 struct AttentionPlan {
     uint32_t chunk, chunks, tiles;
-    size_t parts, stats, scores; // byte offsets
+    size_t stats, scores; // byte offsets
     size_t bytes;
 };
 AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_t heads,

@@ -461,7 +461,7 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
             paged_flag(kv.status, kBadPage);
         if (i < count && place.index >= 0 &&
             uint64_t(place.index) * kv.page_size + place.slot < n) {
-            out = place.page < 0 || uint32_t(place.page) >= kv.pages;
+            out = !page_in(place.page, kv.pages);
             if (!out)
                 at = size_t(place.page) * kv.page_stride + h * kv.head_stride +
                      place.slot * kv.slot_stride;
@@ -769,8 +769,11 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     // split: 256 fp32 rows 6.9 and 8.6 us, 512 10.3 and 8.6; 512 bfloat16 rows
     // 7.2 and 8.4, 1,000 10.6 and 8.5.
     if (rows <= kMostRows && uint64_t(likely) * kv.head_dim * paged_element(kv.type) <= 65536)
-        plan.chunk = kMostRows;
+        plan.chunk = (rows + 127) / 128 * 128;
     plan.chunks = (rows + plan.chunk - 1) / plan.chunk;
+    require(seqs.batch <= 65535 && uint64_t(kv.kv_heads) * plan.tiles <= 65535, NUT_EINVAL,
+            "paged cache: more rows than one launch covers");
+    paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks, 256);
     if (plan.chunks == 1 && !weighted)
         return plan;
     const size_t runs = size_t(seqs.batch) * heads * plan.chunks;
@@ -796,9 +799,6 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
         a.stats = reinterpret_cast<float2 *>(workspace + plan.stats);
         a.scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
     }
-    paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks, 512);
-    require(seqs.batch <= 65535 && uint64_t(kv.kv_heads) * plan.tiles <= 65535, NUT_EINVAL,
-            "paged cache: more rows than one launch covers");
     const dim3 grid(plan.chunks, kv.kv_heads * plan.tiles, seqs.batch);
     // a wave joins up to 16 runs of a head
     const uint32_t threads = plan.chunks <= 16 ? 64 : 256;

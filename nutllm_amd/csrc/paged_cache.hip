@@ -32,11 +32,9 @@ __global__ __launch_bounds__(256) void append_kernel(
     const int length = s.lengths[b];
     const int64_t from = starts == nullptr ? int64_t(b) * each : starts[b];
     int64_t gain = starts == nullptr ? int64_t(each) : starts[b + 1] - from;
-    int bad = 0;
-    if (from < 0 || gain < 0 || gain > int64_t(max_new) || from + gain > int64_t(rows))
-        bad = kBadRows, gain = 0;
-    else if (length < 0 || length + gain > int64_t(s.max_length))
-        bad = kBadLength, gain = 0;
+    const int bad = append_error(length, from, gain, max_new, rows, s.max_length);
+    if (bad != 0)
+        gain = 0;
     if (leader) {
         if (bad != 0)
             paged_flag(kv.status, bad);
@@ -46,12 +44,10 @@ __global__ __launch_bounds__(256) void append_kernel(
     if (gain == 0)
         return;
 
-    const uint32_t n = uint32_t(length), m = uint32_t(gain), ps = kv.page_size;
-    const uint32_t index = n / ps + c;
-    // 64 bits: the end of the last page may pass 32
-    const uint32_t begin = max(n, index * ps);
-    const uint32_t end = uint32_t(min(uint64_t(n) + m, (uint64_t(index) + 1) * ps));
-    if (uint64_t(index) * ps >= uint64_t(n) + m)
+    const uint32_t n = uint32_t(length), ps = kv.page_size;
+    const AppendSpan span = append_span(n, uint32_t(gain), c, ps, kv.division);
+    const uint32_t index = span.index, begin = span.begin, end = span.end;
+    if (begin == end)
         return;
     constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
     const uint32_t tpr = kv.head_dim / 8, part = threadIdx.x % tpr, group = threadIdx.x / tpr;
@@ -140,7 +136,7 @@ __device__ __forceinline__ uint32_t dpp_bits(uint32_t v, uint32_t fill)
     return uint32_t(__builtin_amdgcn_update_dpp(int(fill), int(v), CTRL, ROWS, 0xF, false));
 }
 
-// Bits that any (all) lanes of the wave have, in lane 63.
+// Bits that any lane of the wave has, in lane 63.
 __device__ __forceinline__ uint32_t any_bits(uint32_t v)
 {
     v |= dpp_bits<kDppQuadSwap1>(v, 0);
@@ -150,8 +146,6 @@ __device__ __forceinline__ uint32_t any_bits(uint32_t v)
     v |= dpp_bits<kDppRowBcast15, 0xA>(v, 0);
     return v | dpp_bits<kDppRowBcast31, 0xC>(v, 0);
 }
-
-__device__ __forceinline__ uint32_t all_bits(uint32_t v) { return ~any_bits(~v); }
 
 // The largest of a wave's values, none below -1, in lane 63.
 __device__ __forceinline__ int largest(int v)
@@ -443,7 +437,7 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     for (uint32_t k = 0; k < kPages; k++) {
         const uint32_t i = k * 256 + threadIdx.x;
         if (i < step * kPages) {
-            const bool good = entry[k] >= 0 && uint32_t(entry[k]) < kv.pages;
+            const bool good = page_in(entry[k], kv.pages);
             if (!good && first + i < count)
                 paged_flag(kv.status, kBadPage);
             pages[i] = good ? entry[k] : -1;
@@ -814,7 +808,7 @@ __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs 
     }
 }
 
-uint32_t pages_of(const PagedView &kv, uint32_t rows) { return (rows - 1) / kv.page_size + 1; }
+uint32_t pages_of(const PagedView &kv, uint32_t rows) { return page_of(kv, rows - 1) + 1; }
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -861,8 +855,7 @@ void launch_paged_append(const PagedView &kv, const PagedSeqs &seqs, const float
                          uint32_t max_new, const PagedHistory &history, const int *firsts,
                          int *new_lengths, hipStream_t stream)
 {
-    // pages that max_new rows can lie in, wherever they begin
-    const uint32_t touched = (max_new - 1 + kv.page_size - 1) / kv.page_size + 1;
+    const uint32_t touched = pages_touched(max_new, kv.page_size);
     const uint32_t most = std::min(kv.page_size, max_new) * (kv.head_dim / 8);
     const uint32_t threads = std::min(256u, (most + kWave - 1) / kWave * kWave);
     const auto kernel = kv.type == NUT_F32   ? append_kernel<NUT_F32>
@@ -876,6 +869,7 @@ void launch_paged_append(const PagedView &kv, const PagedSeqs &seqs, const float
 
 size_t select_workspace(const PagedView &kv, const PagedSeqs &seqs)
 {
+    paged_grid(uint64_t(seqs.batch) * kv.kv_heads, 256);
     return size_t(seqs.batch) * kv.kv_heads * pages_of(kv, seqs.max_length) * sizeof(uint64_t);
 }
 
@@ -901,6 +895,7 @@ void launch_paged_select(const PagedView &kv, const PagedSeqs &seqs, const float
 size_t evict_workspace(const PagedView &kv, const PagedSeqs &seqs, uint32_t budget)
 {
     const size_t heads = size_t(seqs.batch) * kv.kv_heads;
+    paged_grid(heads, 1024);
     return 2 * aligned(heads * budget * sizeof(int)) + aligned(heads * sizeof(int));
 }
 

@@ -17,7 +17,7 @@ __device__ __forceinline__ uint32_t paged_length(const PagedView &kv, const Page
                                                  uint32_t b, bool report)
 {
     const int n = s.lengths[b];
-    if (n >= 0 && uint32_t(n) <= s.max_length)
+    if (length_in(n, s.max_length))
         return uint32_t(n);
     if (report)
         paged_flag(kv.status, kBadLength);
@@ -32,7 +32,7 @@ __device__ __forceinline__ size_t paged_row(const PagedView &kv, const PagedSeqs
                                             uint32_t index, uint32_t slot, uint32_t h)
 {
     const int page = s.table[size_t(b) * s.table_stride + index];
-    if (page < 0 || uint32_t(page) >= kv.pages) {
+    if (!page_in(page, kv.pages)) {
         paged_flag(kv.status, kBadPage);
         return kNoRow;
     }

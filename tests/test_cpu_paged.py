@@ -2,6 +2,8 @@
 on a host without a GPU: each refusal's message, and that the arguments next to
 it come through to the device (and fail there, loudly, where there is none)."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 
@@ -222,3 +224,26 @@ def test_null_views():
     assert L.nut_paged_append(None, None, None, None, 0, 0, 0, None, 1, None, None, None, None) == 1
     assert L.nut_paged_attention(None, None, None, 0, 8, 1.0, None, 0, None, None, None, None, 0,
                                  None) == 1
+
+
+@pytest.mark.parametrize("program", [["paged_index_test"], ["paged_api_test", "--cpu-only"]])
+def test_cpp(program):
+    """Pages, lengths and counts as the kernels judge them, and where rows
+    go; the C++ host API's refusals."""
+    build = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build")
+    binary = os.path.join(build, program[0])
+    assert os.path.exists(binary), "build first: make -C tests/cpp"
+    r = subprocess.run([binary, *program[1:]], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
+
+
+def test_launches_that_one_grid_does_not_cover():
+    big = dict(kv_heads=1 << 20, head_dim=8, page_size=1, pages=4)
+    refused("more rows than one launch covers", paged(**big).attention_workspace,
+            seqs(table_stride=64, batch=8), 1 << 20)
+    refused("more rows than one launch covers", paged(**big).select_workspace,
+            seqs(table_stride=64, batch=128), 1 << 20, 3)
+    refused("more rows than one launch covers", paged(**big).evict_workspace,
+            seqs(table_stride=64, batch=128), 8)
+    refused("more rows than one launch covers", paged(kv_heads=1).attention_workspace,
+            seqs(table_stride=64, batch=65536), 8)

@@ -292,3 +292,67 @@ def test_append_not_a_number_shows_in_the_bounds(gpu):
     for b, d in ((0, 4), (1, 5)):
         nan = np.isnan(case.fetch("bounds")[case.table[b, 0], 0])
         assert np.all(nan[:, d]) and nan.sum() == 2
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(3, 1, 32), (8, 1, 64), (2, 2, 96), (17, 1, 128),
+                                          (5, 1, 256)])
+def test_attention_room_for_long_sequences(gpu, kind, heads, kv, dim):
+    """Calls that allow for millions of rows (and read past the caches) over
+    short sequences: the table's entries behind them are not followed."""
+    case = Case(kind, [700, 0, 33, 1025], kv, dim, 32, seed=59).upload()
+    q = query_of(case, heads)
+    out, lse, _, tol, _ = case.expect_attention(q, heads)
+    most = (256 << 20) // (kv * dim * 2 * (4 if kind == "f32" else 2)) // 4
+    width = -(-most // 32)
+    table = np.full((4, width), -1, np.int32)
+    table[:, :case.width] = case.table
+    A = gpu.DeviceArray
+    d_table = A(like=table)
+    seqs = gpu.PagedBatch(d_table, width, case.d["lengths"], 4, most)
+    need = case.paged.attention_workspace(seqs, heads)
+    work = A(like=np.full(need, 0xff, np.uint8))
+    dq, do, dl = A(like=q), A(out.size * 4), A(lse.size * 4)
+    case.paged.attention(seqs, dq, do, heads, lse=dl, workspace=work)
+    gpu.synchronize()
+    got = do.download(np.float32, out.size).reshape(out.shape)
+    assert np.all(np.abs(got - out) <= tol)
+    case.paged.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_attention_queries_that_are_not_finite(gpu, kind):
+    """A query with a NaN, or with an infinity (whose products with keys of both
+    signs are both infinities), gives no number for its own head alone; one
+    whose scores are all minus infinity gives zeros."""
+    case = Case(kind, [40], 2, 32, 16, seed=61)
+    for h in range(2):
+        for i in range(40):
+            row = decode(case.keys[case.table[0, i // 16], h, i % 16], kind)
+            row[7] = abs(row[7]) + 0.5
+            case.keys[case.table[0, i // 16], h, i % 16] = encode(row, kind)
+    case.upload()
+    q = query_of(case, 8)
+    q[0, 1, 3], q[0, 2, 7], q[0, 5, 7], q[0, 6, 2] = np.nan, np.inf, -np.inf, np.inf
+    got, lse = case.attention(q, 8)
+    plain = [0, 3, 4, 7]
+    out, want, _, tol, _ = case.expect_attention(np.nan_to_num(q, posinf=0, neginf=0), 8)
+    assert np.all(np.abs(got - out)[0, plain] <= tol[0, plain])
+    assert np.all(np.isnan(got[0, [1, 2, 6]]))
+    assert np.all(got[0, 5] == 0) and np.isneginf(lse[0, 5])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_attention_values_that_are_not_finite(gpu, kind):
+    """An infinite or NaN value shows in its component of the KV head's results
+    and nowhere else."""
+    case = Case(kind, [40], 2, 32, 16, seed=63)
+    out, _, _, tol, _ = case.expect_attention(query_of(case, 4), 4)
+    case.values[case.table[0, 1], 1, 2, 9] = encode(np.array(np.inf), kind)
+    case.values[case.table[0, 2], 1, 5, 20] = encode(np.array(np.nan), kind)
+    case.upload()
+    got, _ = case.attention(query_of(case, 4), 4)
+    odd = np.zeros_like(got, bool)
+    odd[0, 2:, [9, 20]] = True
+    assert np.array_equal(~np.isfinite(got), odd)
+    assert np.all(np.abs(got - out)[~odd] <= tol[~odd])

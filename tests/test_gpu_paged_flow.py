@@ -2,6 +2,9 @@
 moved into pages, tokens appended, read, weighed and evicted; in captured
 graphs, on other streams, far into a large pool; and what they do with page
 tables, lengths and row counts that they cannot follow."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 import torch
@@ -377,3 +380,12 @@ def test_weights_of_rows_on_a_missing_page(gpu):
     assert np.all(np.abs(grown - 2) <= 1e-4)  # two heads a KV head, all their weight
     with pytest.raises(gpu.OutOfRange, match="page out of range"):
         case.paged.check()
+
+
+def test_cpp_host_api(gpu):
+    binary = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build",
+                          "paged_api_test")
+    assert os.path.exists(binary), "build first: make -C tests/cpp"
+    r = subprocess.run([binary], capture_output=True, text=True, timeout=60)
+    print(r.stdout, flush=True)
+    assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
