@@ -328,11 +328,6 @@ __device__ __forceinline__ void places_of(const uint32_t (&flag)[EACH], uint32_t
 
 // ---------------------------------------------------------------- select --
 
-// Pages a lane scores: where the query takes many conversions, more (16 long
-// sequences of eight heads 28.3 us, 29.6 with two pages and 29.5 with eight; one of
-// four heads 17.7 us, 18.1 with two).
-template <int GH> constexpr uint32_t kPagesOf = GH <= 4 ? 1 : 4;
-
 // A partner's value among the lanes of a page: for O = 2 and 1 the lane O away,
 // for 8 and 4 the mirror image in 2 O lanes, which lies O away in the bit that
 // counts and has not been told apart in the others yet.
@@ -399,33 +394,34 @@ __device__ __forceinline__ uint64_t score_key(double v)
 
 // Scores of every page: LANES lanes, head_dim / 8 of them with work, hold eight
 // components of a page's bounds each. For one page
-//   2 sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (hi_d + lo_d)
-//                                          + |q_d| (hi_d - lo_d),
-// two multiply-adds a component in 64 bits: the answer is whole numbers, and
-// 32 bits would let rounding choose among near pages. GH heads at a time, one
-// page of a lane after another with the next one's bounds on their way.
-template <int TYPE, int GH, uint32_t LANES>
+//   sum_d max(q_d lo_d, q_d hi_d) = sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d,
+// two multiply-adds a component in 64 bits, of which one adds zero: the answer
+// is whole numbers, and in 32 bits, or with terms that only cancel, rounding
+// would choose among near or equal pages. GH heads at a time, one page of a
+// lane after another with the next one's bounds on their way.
+template <int TYPE, int GH, uint32_t LANES, uint32_t PAGES>
 __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeqs s,
                                                           const float *__restrict__ query,
                                                           size_t query_stride, uint32_t heads,
                                                           uint32_t blocks, uint32_t width,
                                                           uint64_t *__restrict__ scores)
 {
-    constexpr uint32_t kPages = kPagesOf<GH>, kSize = TYPE == NUT_F32 ? 4 : 2;
+    constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
     constexpr int kWords = kSize / 2; // 16-byte words of eight components
     const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
     const uint32_t b = id / blocks / kv.kv_heads;
     constexpr uint32_t step = 256 / LANES;
-    const uint32_t mine = threadIdx.x / LANES, first = c * step * kPages;
+    const uint32_t mine = threadIdx.x / LANES, first = c * step * PAGES;
     const uint32_t group = heads / kv.kv_heads, part = threadIdx.x % LANES;
     const bool works = part * 8 < kv.head_dim;
-    __shared__ int pages[256 * kPages];
+    __shared__ int pages[step * PAGES];
+    __shared__ uint64_t found[step * PAGES];
     // the table beside the length: what lies behind it is not used
-    int entry[kPages];
+    int entry[PAGES];
 #pragma unroll
-    for (uint32_t k = 0; k < kPages; k++) {
+    for (uint32_t k = 0; k < PAGES; k++) {
         const uint32_t i = k * 256 + threadIdx.x;
-        entry[k] = i < step * kPages && first + i < width
+        entry[k] = i < step * PAGES && first + i < width
                        ? s.table[size_t(b) * s.table_stride + first + i]
                        : -1;
     }
@@ -434,9 +430,9 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     if (first >= count)
         return;
 #pragma unroll
-    for (uint32_t k = 0; k < kPages; k++) {
+    for (uint32_t k = 0; k < PAGES; k++) {
         const uint32_t i = k * 256 + threadIdx.x;
-        if (i < step * kPages) {
+        if (i < step * PAGES) {
             const bool good = page_in(entry[k], kv.pages);
             if (!good && first + i < count)
                 paged_flag(kv.status, kBadPage);
@@ -462,7 +458,7 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     for (uint32_t g = 0; g < group; g += GH) {
         uint4 low[kWords], high[kWords], next_low[kWords], next_high[kWords];
         fetch(0, low, high);
-        double q[GH][8];
+        double up[GH][8], down[GH][8]; // max(q, 0) and min(q, 0)
 #pragma unroll
         for (int j = 0; j < GH; j++) {
             float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -472,12 +468,15 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
                                    size_t(h * group + g + j) * kv.head_dim + part * 8),
                                v);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                q[j][i] = double(v[i]);
+            for (int i = 0; i < 8; i++) {
+                // a query component that is not a number stays one
+                up[j][i] = double(v[i] <= 0.0f ? 0.0f : v[i]);
+                down[j][i] = double(v[i] >= 0.0f ? 0.0f : v[i]);
+            }
         }
 #pragma unroll 1
-        for (uint32_t k = 0; k < kPages; k++) {
-            if (k + 1 < kPages)
+        for (uint32_t k = 0; k < PAGES; k++) {
+            if (k + 1 < PAGES)
                 fetch(k + 1, next_low, next_high);
             float lo[8], hi[8];
             load8<TYPE>(reinterpret_cast<const char *>(low), lo);
@@ -488,11 +487,10 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
                 sum[j] = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const double mid = double(hi[i]) + double(lo[i]);
-                const double half = double(hi[i]) - double(lo[i]);
+                const double high_d = hi[i], low_d = lo[i];
 #pragma unroll
                 for (int j = 0; j < GH; j++)
-                    sum[j] = fma(fabs(q[j][i]), half, fma(q[j][i], mid, sum[j]));
+                    sum[j] = fma(down[j][i], low_d, fma(up[j][i], high_d, sum[j]));
             }
             uint32_t head = g;
             sum_lanes<LANES / 2, GH>(sum, part, head);
@@ -505,11 +503,14 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
                     best = key;
             }
             best = best_of_lanes<LANES / 2>(best);
-            if (part == 0 && first + mine + k * step < count) {
-                uint64_t *to = out + k * step;
-                if (pages[mine + k * step] < 0)
-                    best = 0; // below every page that there is
-                *to = g == 0 || best > *to ? best : *to;
+            const uint32_t at = mine + k * step;
+            if (part == 0) {
+                if (g != 0) // by this thread
+                    best = found[at] > best ? found[at] : best;
+                if (g + GH < group)
+                    found[at] = best;
+                else if (first + at < count) // a bad page below all others
+                    out[k * step] = pages[at] < 0 ? 0 : best;
             }
 #pragma unroll
             for (int w = 0; w < kWords; w++)
@@ -812,38 +813,40 @@ uint32_t pages_of(const PagedView &kv, uint32_t rows) { return page_of(kv, rows 
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <int TYPE, int GH, uint32_t LANES>
+template <int TYPE, int GH, uint32_t LANES, uint32_t PAGES>
 void scores_by(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
-    const uint32_t width = pages_of(kv, seqs.max_length);
-    const uint32_t per_block = 256 / LANES * kPagesOf<GH>;
+    const uint32_t width = pages_of(kv, seqs.max_length), per_block = 256 / LANES * PAGES;
     const uint32_t blocks = (width + per_block - 1) / per_block;
-    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH, LANES>),
+    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH, LANES, PAGES>),
                        paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
                        stream, kv, seqs, query, query_stride, heads, blocks, width, scores);
 }
 
-template <int TYPE, int GH>
+template <int TYPE, int GH, uint32_t PAGES>
 void scores_of(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
-    const auto run = kv.head_dim <= 32    ? scores_by<TYPE, GH, 4>
-                     : kv.head_dim <= 64  ? scores_by<TYPE, GH, 8>
-                     : kv.head_dim <= 128 ? scores_by<TYPE, GH, 16>
-                                          : scores_by<TYPE, GH, 32>;
+    const auto run = kv.head_dim <= 32    ? scores_by<TYPE, GH, 4, PAGES>
+                     : kv.head_dim <= 64  ? scores_by<TYPE, GH, 8, PAGES>
+                     : kv.head_dim <= 128 ? scores_by<TYPE, GH, 16, PAGES>
+                                          : scores_by<TYPE, GH, 32, PAGES>;
     run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 
+// More than four heads take turns, and then a lane scores four pages with each
+// four heads' query: 16 long sequences of eight heads 31.1 us, 34.0 with two
+// pages and 34.4 with one. Four heads: one sequence 18.3 us, 20.3 with four pages.
 template <int TYPE>
 void scores_for(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                 size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
     const uint32_t group = heads / kv.kv_heads;
-    const auto run = group == 1   ? scores_of<TYPE, 1>
-                     : group == 2 ? scores_of<TYPE, 2>
-                     : group <= 4 ? scores_of<TYPE, 4>
-                                  : scores_of<TYPE, 8>;
+    const auto run = group == 1   ? scores_of<TYPE, 1, 1>
+                     : group == 2 ? scores_of<TYPE, 2, 1>
+                     : group <= 4 ? scores_of<TYPE, 4, 1>
+                                  : scores_of<TYPE, 4, 4>;
     run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 

@@ -28,7 +28,7 @@ def check_attention(case, heads, query, **kw):
     empty = np.isneginf(lse)
     assert np.array_equal(np.isneginf(got_lse), empty)
     # the logarithm's argument errs as a weight does, and its result is rounded
-    assert np.all(np.abs(got_lse - lse)[~empty] <=
+    assert np.all(np.abs(got_lse[~empty] - lse[~empty]) <=
                   (tol_w + 2.0 ** -22 * (1 + np.abs(lse)))[~empty])
     return weights, tol_w
 
@@ -151,6 +151,24 @@ def test_select_ties_and_many_pages(gpu):
     case.bounds[:] = encode(np.float32(1.0), "bf16")
     case.upload()
     assert np.array_equal(case.select(q, 4, 64, 1, 2), case.expect_select(q, 4, 64, 1, 2))
+
+
+@pytest.mark.parametrize("heads", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_select_equal_scores_of_unequal_pages(gpu, kind, heads):
+    """Pages that agree in the bounds that a query meets, and differ in the
+    others, score alike to the last bit: the lower ones are chosen."""
+    case = Case(kind, [640], 1, 64, 16, seed=65)
+    order = case.rng.permutation(40)
+    best = case.rng.standard_normal(64)
+    for c in order[:25]:
+        case.bounds[case.table[0, c], 0, 1] = encode(best + 3, kind)
+        case.bounds[case.table[0, c], 0, 0] = encode(-3 * case.rng.random(64), kind)
+    case.upload()
+    q = np.abs(query_of(case, heads)) * np.float32(1.1)
+    want = case.expect_select(q, heads, 12, 0, 0)
+    assert want[0, 0].tolist() == sorted(order[:25])[:12]
+    assert np.array_equal(case.select(q, heads, 12, 0, 0), want)
 
 
 def test_select_not_a_number_first(gpu):
