@@ -16,7 +16,9 @@ namespace {
 
 // A workgroup per (sequence, KV head, page that gains rows): it alone touches
 // the page's bounds, so they need no atomics. tpr = head_dim / 8 threads hold
-// a row, eight components (32 bytes of source) each.
+// a row, eight components (32 bytes of source) each. HBM bounds it: prompts of
+// 8 sequences at 32 heads of 128, fp16, 421 MB in 85 us (4.9 TB/s; a 4 GiB copy
+// moves 4.75). One token each of 64 sequences is a launch, 5.4 us.
 template <int TYPE>
 __global__ __launch_bounds__(256) void append_kernel(
     PagedView kv, PagedSeqs s, const float *__restrict__ keys, const float *__restrict__ values,
@@ -392,14 +394,14 @@ __device__ __forceinline__ uint64_t score_key(double v)
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// Scores of every page: LANES lanes, head_dim / 8 of them with work, hold eight
-// components of a page's bounds each. For one page
+// Scores of every page, up to four heads to a KV head: LANES lanes, head_dim / 8
+// of them with work, hold eight components of a page's bounds each. For a page
 //   sum_d max(q_d lo_d, q_d hi_d) = sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d,
 // two multiply-adds a component in 64 bits, of which one adds zero: the answer
 // is whole numbers, and in 32 bits, or with terms that only cancel, rounding
-// would choose among near or equal pages. GH heads at a time, one page of a
-// lane after another with the next one's bounds on their way.
-template <int TYPE, int GH, uint32_t LANES, uint32_t PAGES>
+// would choose among near or equal pages. What bounds it is instructions: 16
+// fp64 ones a head and eight to bring them together, for 64 bytes a lane.
+template <int TYPE, int GH, uint32_t LANES>
 __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeqs s,
                                                           const float *__restrict__ query,
                                                           size_t query_stride, uint32_t heads,
@@ -407,119 +409,168 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
                                                           uint64_t *__restrict__ scores)
 {
     constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
-    constexpr int kWords = kSize / 2; // 16-byte words of eight components
     const uint32_t id = blockIdx.x, c = id % blocks, h = id / blocks % kv.kv_heads;
     const uint32_t b = id / blocks / kv.kv_heads;
-    constexpr uint32_t step = 256 / LANES;
-    const uint32_t mine = threadIdx.x / LANES, first = c * step * PAGES;
-    const uint32_t group = heads / kv.kv_heads, part = threadIdx.x % LANES;
+    const uint32_t index = c * (256 / LANES) + threadIdx.x / LANES, part = threadIdx.x % LANES;
+    const uint32_t group = heads / kv.kv_heads;
     const bool works = part * 8 < kv.head_dim;
-    __shared__ int pages[step * PAGES];
-    __shared__ uint64_t found[step * PAGES];
-    // the table beside the length: what lies behind it is not used
-    int entry[PAGES];
+    // the query and the table beside the length: what lies behind it is not used
+    double up[GH][8], down[GH][8]; // max(q, 0) and min(q, 0)
 #pragma unroll
-    for (uint32_t k = 0; k < PAGES; k++) {
-        const uint32_t i = k * 256 + threadIdx.x;
-        entry[k] = i < step * PAGES && first + i < width
-                       ? s.table[size_t(b) * s.table_stride + first + i]
-                       : -1;
+    for (int j = 0; j < GH; j++) {
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (works && uint32_t(j) < group)
+            load8<NUT_F32>(reinterpret_cast<const char *>(query + b * query_stride +
+                                                          size_t(h * group + j) * kv.head_dim +
+                                                          part * 8),
+                           v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // a query component that is not a number stays one
+            up[j][i] = double(v[i] <= 0.0f ? 0.0f : v[i]);
+            down[j][i] = double(v[i] >= 0.0f ? 0.0f : v[i]);
+        }
     }
+    const int page = index < width ? s.table[size_t(b) * s.table_stride + index] : -1;
     const uint32_t n = paged_length(kv, s, b, threadIdx.x == 0 && h == 0 && c == 0);
     const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
-    if (first >= count)
+    if (index >= count)
         return;
+    const bool good = page_in(page, kv.pages);
+    if (!good && part == 0)
+        paged_flag(kv.status, kBadPage);
+    float lo[8] = {0, 0, 0, 0, 0, 0, 0, 0}, hi[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (good && works) {
+        const char *at = kv.bounds +
+                         (size_t(page) * kv.kv_heads + h) * 2 * kv.head_dim * kSize +
+                         part * 8 * kSize;
+        load8<TYPE>(at, lo);
+        load8<TYPE>(at + kv.head_dim * kSize, hi);
+    }
+    double sum[GH];
 #pragma unroll
-    for (uint32_t k = 0; k < PAGES; k++) {
-        const uint32_t i = k * 256 + threadIdx.x;
-        if (i < step * PAGES) {
-            const bool good = page_in(entry[k], kv.pages);
-            if (!good && first + i < count)
-                paged_flag(kv.status, kBadPage);
-            pages[i] = good ? entry[k] : -1;
+    for (int j = 0; j < GH; j++)
+        sum[j] = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const double high = hi[i], low = lo[i];
+#pragma unroll
+        for (int j = 0; j < GH; j++)
+            sum[j] = fma(down[j][i], low, fma(up[j][i], high, sum[j]));
+    }
+    uint32_t head = 0;
+    sum_lanes<LANES / 2, GH>(sum, part, head);
+    constexpr int kLeft = GH > int(LANES) ? GH / int(LANES) : 1;
+    uint64_t best = 0;
+#pragma unroll
+    for (int j = 0; j < kLeft; j++) {
+        const uint64_t key = score_key(sum[j]);
+        if (head + j < group && key > best)
+            best = key;
+    }
+    best = best_of_lanes<LANES / 2>(best);
+    if (part == 0) // a bad page below all others
+        scores[(size_t(b) * kv.kv_heads + h) * width + index] = good ? best : 0;
+}
+
+// The same for more than four heads to a KV head, on v_mfma_f64_16x16x4f64: a
+// wave takes 16 pages (rows) and 16 heads (columns), and sums over 64
+// components at a time, max(q, 0) hi and min(q, 0) lo apart. Lane 16 j + c
+// loads components 16 j to 16 j + 15 of page c, whose n-th is the j-th of
+// four in step n; the query comes from shared memory, [sign][component][head].
+// Scores of pages 4 i + j and head c come out as element i of that lane. 32
+// steps of 64 cycles a tile bound it: 50,000 pages of 64 components 10.8 us.
+template <int TYPE>
+__global__ __launch_bounds__(256) void page_scores_mfma_kernel(PagedView kv, PagedSeqs s,
+                                                               const float *__restrict__ query,
+                                                               size_t query_stride,
+                                                               uint32_t heads, uint32_t blocks,
+                                                               uint32_t width,
+                                                               uint64_t *__restrict__ scores)
+{
+    typedef double f64x4 __attribute__((ext_vector_type(4)));
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
+    __shared__ double qs[2][64][16];
+    const uint32_t id = blockIdx.x, block = id % blocks, h = id / blocks % kv.kv_heads;
+    const uint32_t b = id / blocks / kv.kv_heads;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t j = lane / 16, c = lane % 16, group = heads / kv.kv_heads;
+    const uint32_t base = block * 64 + wave * 16;
+    // the table beside the length: what lies behind it is not used
+    int page = base + c < width ? s.table[size_t(b) * s.table_stride + base + c] : -1;
+    const float *rows = query + b * query_stride + size_t(h) * group * kv.head_dim;
+    const uint32_t head = threadIdx.x % 16, d = threadIdx.x / 16 * 4;
+    const auto fetch = [&](uint32_t g, uint32_t slab) {
+        return g + head < group && slab + d < kv.head_dim
+                   ? *reinterpret_cast<const f32x4 *>(rows + size_t(g + head) * kv.head_dim +
+                                                      slab + d)
+                   : f32x4{0, 0, 0, 0};
+    };
+    f32x4 x = fetch(0, 0);
+    const uint32_t n = paged_length(kv, s, b, threadIdx.x == 0 && h == 0 && block == 0);
+    asm volatile("" : "+v"(page), "+v"(x));
+    const uint32_t count = n == 0 ? 0 : page_of(kv, n - 1) + 1;
+    if (block * 64 >= count)
+        return;
+    const bool good = page_in(page, kv.pages) && base + c < count;
+    if (!good && base + c < count)
+        paged_flag(kv.status, kBadPage);
+    const uint32_t there = uint32_t(__ballot(good)); // bit c: page c
+    const char *bounds = kv.bounds + (size_t(good ? page : 0) * kv.kv_heads + h) * 2 *
+                                         kv.head_dim * kSize;
+    uint64_t best[4] = {0, 0, 0, 0};
+    for (uint32_t g = 0; g < group; g += 16) {
+        f64x4 above{0, 0, 0, 0}, below{0, 0, 0, 0}; // by hi, by lo
+        for (uint32_t slab = 0; slab < kv.head_dim; slab += 64) {
+            if (g + slab != 0)
+                x = fetch(g, slab);
+            float hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+                float low[8] = {0, 0, 0, 0, 0, 0, 0, 0}, high[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (good && slab + 16 * j + e < kv.head_dim) {
+                    load8<TYPE>(bounds + (slab + 16 * j + e) * kSize, low);
+                    load8<TYPE>(bounds + (kv.head_dim + slab + 16 * j + e) * kSize, high);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    lo[e + i] = low[i], hi[e + i] = high[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // a query component that is not a number stays one
+                qs[0][d + i][head] = double(x[i] <= 0.0f ? 0.0f : x[i]);
+                qs[1][d + i][head] = double(x[i] >= 0.0f ? 0.0f : x[i]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                above = __builtin_amdgcn_mfma_f64_16x16x4f64(double(hi[e]), qs[0][16 * j + e][c],
+                                                             above, 0, 0, 0);
+                below = __builtin_amdgcn_mfma_f64_16x16x4f64(double(lo[e]), qs[1][16 * j + e][c],
+                                                             below, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t key = g + c < group ? score_key(above[i] + below[i]) : 0;
+            best[i] = key > best[i] ? key : best[i];
         }
     }
-    __syncthreads();
-    const char *bounds = kv.bounds + size_t(h) * 2 * kv.head_dim * kSize + part * 8 * kSize;
-    const size_t page_bytes = size_t(kv.kv_heads) * 2 * kv.head_dim * kSize;
-    const auto fetch = [&](uint32_t k, uint4(&low)[kWords], uint4(&high)[kWords]) {
-        const int page = pages[mine + k * step];
-        const bool read = page >= 0 && works && first + mine + k * step < count;
-        const uint4 *at =
-            reinterpret_cast<const uint4 *>(bounds + size_t(read ? page : 0) * page_bytes);
+    uint64_t *out = scores + (size_t(b) * kv.kv_heads + h) * width;
 #pragma unroll
-        for (int w = 0; w < kWords; w++) {
-            low[w] = read ? at[w] : make_uint4(0, 0, 0, 0);
-            high[w] = read ? at[w + kv.head_dim / 8 * kWords] : make_uint4(0, 0, 0, 0);
-        }
-    };
-    uint64_t *out = scores + (size_t(b) * kv.kv_heads + h) * width + first + mine;
-#pragma unroll 1
-    for (uint32_t g = 0; g < group; g += GH) {
-        uint4 low[kWords], high[kWords], next_low[kWords], next_high[kWords];
-        fetch(0, low, high);
-        double up[GH][8], down[GH][8]; // max(q, 0) and min(q, 0)
-#pragma unroll
-        for (int j = 0; j < GH; j++) {
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (works && g + j < group)
-                load8<NUT_F32>(reinterpret_cast<const char *>(
-                                   query + b * query_stride +
-                                   size_t(h * group + g + j) * kv.head_dim + part * 8),
-                               v);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                // a query component that is not a number stays one
-                up[j][i] = double(v[i] <= 0.0f ? 0.0f : v[i]);
-                down[j][i] = double(v[i] >= 0.0f ? 0.0f : v[i]);
-            }
-        }
-#pragma unroll 1
-        for (uint32_t k = 0; k < PAGES; k++) {
-            if (k + 1 < PAGES)
-                fetch(k + 1, next_low, next_high);
-            float lo[8], hi[8];
-            load8<TYPE>(reinterpret_cast<const char *>(low), lo);
-            load8<TYPE>(reinterpret_cast<const char *>(high), hi);
-            double sum[GH];
-#pragma unroll
-            for (int j = 0; j < GH; j++)
-                sum[j] = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const double high_d = hi[i], low_d = lo[i];
-#pragma unroll
-                for (int j = 0; j < GH; j++)
-                    sum[j] = fma(down[j][i], low_d, fma(up[j][i], high_d, sum[j]));
-            }
-            uint32_t head = g;
-            sum_lanes<LANES / 2, GH>(sum, part, head);
-            constexpr int kLeft = GH > int(LANES) ? GH / int(LANES) : 1;
-            uint64_t best = 0;
-#pragma unroll
-            for (int j = 0; j < kLeft; j++) {
-                const uint64_t key = score_key(sum[j]);
-                if (head + j < group && key > best)
-                    best = key;
-            }
-            best = best_of_lanes<LANES / 2>(best);
-            const uint32_t at = mine + k * step;
-            if (part == 0) {
-                if (g != 0) // by this thread
-                    best = found[at] > best ? found[at] : best;
-                if (g + GH < group)
-                    found[at] = best;
-                else if (first + at < count) // a bad page below all others
-                    out[k * step] = pages[at] < 0 ? 0 : best;
-            }
-#pragma unroll
-            for (int w = 0; w < kWords; w++)
-                low[w] = next_low[w], high[w] = next_high[w];
-        }
+    for (int i = 0; i < 4; i++) {
+        const uint64_t key = best_of_lanes<8>(best[i]);
+        const uint32_t p = 4 * i + j;
+        if (c == 0 && base + p < count) // a bad page below all others
+            out[base + p] = there >> p & 1 ? key : 0;
     }
 }
 
-// A workgroup per (sequence, KV head): the `top` best of its pages.
+// A workgroup per (sequence, KV head): the `top` best of its pages. Barriers and
+// the first read bound it: 6.3 us for 1,024 pages each of 64 KV heads.
 __global__ __launch_bounds__(256) void choose_pages_kernel(PagedView kv, PagedSeqs s,
                                                            const uint64_t *__restrict__ scores,
                                                            uint32_t width, uint32_t top,
@@ -601,7 +652,8 @@ __device__ __forceinline__ uint32_t weight_key(float w)
 // A workgroup per (sequence, KV head) decides what stays: to[r] is the r-th
 // row below the budget that goes, from[r] the r-th beyond it that stays, and
 // counts how many there are. Weights and positions of up to eight rows a
-// thread are read once.
+// thread are read once; then barriers bound it: 9 us for 1,040 rows each of 64
+// KV heads, 12 us for 8,192 each of 128.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, PagedSeqs s,
                                                                 PagedHistory history,
@@ -714,7 +766,8 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
 // head_dim / 8 threads a row copy rows. Sources lie beyond the budget and are
 // only read, so the order of workgroups does not matter; the bounds of a page
 // whose entries begin in one workgroup's part and end in another's are the
-// first one's.
+// first one's. HBM bounds it: 205 MB of rows from anywhere to anywhere in 46 us
+// (4.5 TB/s) where 128 KV heads of up to 8,192 rows keep 2,048.
 template <int TYPE>
 __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs s,
                                                         PagedHistory history, uint32_t budget,
@@ -813,40 +866,51 @@ uint32_t pages_of(const PagedView &kv, uint32_t rows) { return page_of(kv, rows 
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <int TYPE, int GH, uint32_t LANES, uint32_t PAGES>
+template <int TYPE, int GH, uint32_t LANES>
 void scores_by(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
-    const uint32_t width = pages_of(kv, seqs.max_length), per_block = 256 / LANES * PAGES;
+    const uint32_t width = pages_of(kv, seqs.max_length), per_block = 256 / LANES;
     const uint32_t blocks = (width + per_block - 1) / per_block;
-    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH, LANES, PAGES>),
+    hipLaunchKernelGGL((page_scores_kernel<TYPE, GH, LANES>),
                        paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
                        stream, kv, seqs, query, query_stride, heads, blocks, width, scores);
 }
 
-template <int TYPE, int GH, uint32_t PAGES>
+template <int TYPE, int GH>
 void scores_of(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
-    const auto run = kv.head_dim <= 32    ? scores_by<TYPE, GH, 4, PAGES>
-                     : kv.head_dim <= 64  ? scores_by<TYPE, GH, 8, PAGES>
-                     : kv.head_dim <= 128 ? scores_by<TYPE, GH, 16, PAGES>
-                                          : scores_by<TYPE, GH, 32, PAGES>;
+    const auto run = kv.head_dim <= 32    ? scores_by<TYPE, GH, 4>
+                     : kv.head_dim <= 64  ? scores_by<TYPE, GH, 8>
+                     : kv.head_dim <= 128 ? scores_by<TYPE, GH, 16>
+                                          : scores_by<TYPE, GH, 32>;
     run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 
-// More than four heads take turns, and then a lane scores four pages with each
-// four heads' query: 16 long sequences of eight heads 31.1 us, 34.0 with two
-// pages and 34.4 with one. Four heads: one sequence 18.3 us, 20.3 with four pages.
+template <int TYPE>
+void scores_mfma(const PagedView &kv, const PagedSeqs &seqs, const float *query,
+                 size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
+{
+    const uint32_t width = pages_of(kv, seqs.max_length), blocks = (width + 63) / 64;
+    hipLaunchKernelGGL(page_scores_mfma_kernel<TYPE>,
+                       paged_grid(uint64_t(seqs.batch) * kv.kv_heads * blocks, 256), dim3(256), 0,
+                       stream, kv, seqs, query, query_stride, heads, blocks, width, scores);
+}
+
 template <int TYPE>
 void scores_for(const PagedView &kv, const PagedSeqs &seqs, const float *query,
                 size_t query_stride, uint32_t heads, uint64_t *scores, hipStream_t stream)
 {
+    // The matrix instruction's 16 columns are worth it from five heads on. Both
+    // calls of a selection, us with its own kernel and with the matrix one: one
+    // head of 128, 4 sequences of 16,000 rows 15.5 and 27.7; two heads 10.4 and
+    // 12.4; four 10.7 and 12.2; eight (four at a time) 14.1 and 11.4.
     const uint32_t group = heads / kv.kv_heads;
-    const auto run = group == 1   ? scores_of<TYPE, 1, 1>
-                     : group == 2 ? scores_of<TYPE, 2, 1>
-                     : group <= 4 ? scores_of<TYPE, 4, 1>
-                                  : scores_of<TYPE, 4, 4>;
+    const auto run = group == 1   ? scores_of<TYPE, 1>
+                     : group == 2 ? scores_of<TYPE, 2>
+                     : group <= 4 ? scores_of<TYPE, 4>
+                                  : scores_mfma<TYPE>;
     run(kv, seqs, query, query_stride, heads, scores, stream);
 }
 
