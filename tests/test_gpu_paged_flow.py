@@ -7,8 +7,8 @@ import subprocess
 
 import numpy as np
 import pytest
-import torch
 
+from hip import Graph, Stream
 from nutllm_amd import workloads as W
 from paged_case import Case, same
 
@@ -24,13 +24,6 @@ def near(case, heads, query, got, **kw):
     out, lse, weights, tol, _ = case.expect_attention(query, heads, **kw)
     assert np.all(np.abs(got - out) <= tol)
     return weights
-
-
-class Tensor:
-    """A torch tensor as a device buffer."""
-
-    def __init__(self, t):
-        self.t, self.ptr, self.nbytes = t, t.data_ptr(), t.numel() * t.element_size()
 
 
 def test_prompt_into_pages(gpu):
@@ -121,52 +114,49 @@ def test_captured_step(gpu):
     with other work between; each replay sees the inputs of its time."""
     heads, budget, top = 4, 100, 3
     case = Case("f16", [90, 130, 60], 2, 64, 16, seed=43, room=8).upload()
-    A, stream, graphs = gpu.DeviceArray, torch.cuda.Stream(), []
-    torch.cuda.synchronize()
-    k, v = (torch.zeros(3, 2, 64, device="cuda") for _ in range(2))
-    q = torch.zeros(3, heads, 64, device="cuda")
+    A, stream, graphs = gpu.DeviceArray, Stream(), []
+    k, v, q = A(4 * 3 * 2 * 64), A(4 * 3 * 2 * 64), A(4 * 3 * heads * 64)
     after = gpu.PagedBatch(case.d["table"], case.width, case.d["new_lengths"], 3, case.max_length)
     cut = A(like=np.zeros(3, np.int32))
     for _ in range(2):
-        sparse = torch.zeros(3, heads, 64, device="cuda")
-        out, chosen = torch.zeros_like(sparse), torch.zeros(3, 2, top, dtype=torch.int32,
-                                                            device="cuda")
+        out, sparse, chosen = A(q.nbytes), A(q.nbytes), A(4 * 3 * 2 * top)
         sizes = (case.paged.attention_workspace(after, heads, weighted=True),
                  case.paged.select_workspace(after, heads, top),
                  case.paged.attention_workspace(after, heads, top=top),
                  case.paged.evict_workspace(after, budget))
-        space = [Tensor(torch.full((max(1, n),), 255, dtype=torch.uint8, device="cuda"))
-                 for n in sizes]
-        torch.cuda.synchronize()
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=stream):
-            at = torch.cuda.current_stream().cuda_stream
-            case.paged.append(case.seqs, Tensor(k), Tensor(v), case.d["new_lengths"],
-                              history=case.history, stream=at)
-            case.paged.attention(after, Tensor(q), Tensor(out), heads, history=case.history,
-                                 workspace=space[0], stream=at)
-            case.paged.select(after, Tensor(q), Tensor(chosen), heads, top, workspace=space[1],
+        space = [A(like=np.full(max(1, n), 255, np.uint8)) for n in sizes]
+
+        def step():
+            at = stream.handle
+            case.paged.append(case.seqs, k, v, case.d["new_lengths"], history=case.history,
                               stream=at)
-            case.paged.attention(after, Tensor(q), Tensor(sparse), heads,
-                                 selected=Tensor(chosen), top=top, workspace=space[2], stream=at)
+            case.paged.attention(after, q, out, heads, history=case.history, workspace=space[0],
+                                 stream=at)
+            case.paged.select(after, q, chosen, heads, top, workspace=space[1], stream=at)
+            case.paged.attention(after, q, sparse, heads, selected=chosen, top=top,
+                                 workspace=space[2], stream=at)
             case.paged.evict(after, case.history, cut, budget, first=1, last=5,
                              workspace=space[3], stream=at)
-        graphs.append((graph, out, chosen, sparse, space))
+
+        gpu.synchronize()
+        graphs.append((Graph(stream, step), out, chosen, sparse, space))
     rng = np.random.default_rng(3)
     for turn in range(6):
         graph, out, chosen, sparse, _ = graphs[turn % 2]
-        new = [torch.from_numpy(rng.standard_normal(t.shape).astype(np.float32)) for t in (k, v, q)]
-        for t, n in zip((k, v, q), new):
-            t.copy_(n)
-        torch.cuda.synchronize()
+        new = [rng.standard_normal(shape).astype(np.float32)
+               for shape in ((3, 2, 64), (3, 2, 64), (3, heads, 64))]
+        for array, x in zip((k, v, q), new):
+            array.upload(x)
+        gpu.synchronize()
         graph.replay()
-        torch.cuda.synchronize()
-        case.lengths = case.expect_append(new[0].numpy(), new[1].numpy(), [1, 1, 1])
-        query = new[2].numpy()
-        near(case, heads, query, out.cpu().numpy())
+        stream.synchronize()
+        case.lengths = case.expect_append(new[0], new[1], [1, 1, 1])
+        query = new[2]
+        near(case, heads, query, out.download(np.float32, query.size).reshape(query.shape))
         want = case.expect_select(query, heads, top, 1, 1)
-        assert np.array_equal(chosen.cpu().numpy(), want)
-        near(case, heads, query, sparse.cpu().numpy(), selected=want)
+        assert np.array_equal(chosen.download(np.int32, want.size).reshape(want.shape), want)
+        near(case, heads, query, sparse.download(np.float32, query.size).reshape(query.shape),
+             selected=want)
         # the weights that decided, from the device: those below the budget
         # moved with their rows, so the plan is made from a copy of the state
         # before the move: the rows beyond the budget are where they were
@@ -192,8 +182,11 @@ def test_captured_step(gpu):
             assert same(case.pool(name), getattr(case, name)), name
         case.lengths = lengths
         case.d["lengths"].upload(lengths)
-        torch.cuda.synchronize()
+        gpu.synchronize()
     case.paged.check()
+    for graph, *_ in graphs:
+        graph.close()
+    stream.close()
 
 
 def test_two_calls_at_once(gpu):
@@ -204,12 +197,13 @@ def test_two_calls_at_once(gpu):
     work = [gpu.DeviceArray(like=np.full(max(1, need), 255, np.uint8)) for _ in q]
     dq = [gpu.DeviceArray(like=x) for x in q]
     out = [gpu.DeviceArray(4 * 2 * 8 * 64) for _ in q]
-    streams = [torch.cuda.Stream() for _ in q]
-    torch.cuda.synchronize()
+    streams = [Stream() for _ in q]
+    gpu.synchronize()
     for _ in range(20):
         for s, a, o, w in zip(streams, dq, out, work):
-            case.paged.attention(case.seqs, a, o, 8, workspace=w, stream=s.cuda_stream)
-    torch.cuda.synchronize()
+            case.paged.attention(case.seqs, a, o, 8, workspace=w, stream=s.handle)
+    for s in streams:
+        s.synchronize()
     for x, o in zip(q, out):
         near(case, 8, x, o.download(np.float32, 2 * 8 * 64).reshape(2, 8, 64))
 
@@ -230,12 +224,10 @@ def test_far_into_a_large_pool(gpu, slot_major):
     attention and eviction with pages at both ends of a 12 GB pool."""
     kv, dim, ps, pages = 2, 64, 16, 1 << 20
     stride = kv * ps * dim + (64 if slot_major else 0)
-    keys, values = (torch.empty(pages * stride, dtype=torch.float32, device="cuda")
-                    for _ in range(2))
-    bounds = torch.zeros(pages, kv, 2, dim, device="cuda")
+    keys, values = (gpu.DeviceArray(4 * pages * stride) for _ in range(2))
+    bounds = gpu.DeviceArray(4 * pages * kv * 2 * dim)
     strides = (stride, dim, kv * dim) if slot_major else (stride, ps * dim, dim)
-    paged = gpu.PagedKV(Tensor(keys), Tensor(values), pages, ps, kv, dim, gpu.F32,
-                        strides=strides, bounds=Tensor(bounds))
+    paged = gpu.PagedKV(keys, values, pages, ps, kv, dim, gpu.F32, strides=strides, bounds=bounds)
     table = np.array([[pages - 1, 0, pages // 2 + 1, pages - 2]], np.int32)
     case = Case("f32", [0], kv, dim, ps, seed=49, max_length=64)
     case.pages, case.table = 4, np.arange(4, dtype=np.int32)[None]
