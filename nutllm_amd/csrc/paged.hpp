@@ -56,6 +56,7 @@ inline size_t paged_element(int type) { return type == NUT_F32 ? 4 : 2; }
 // unnormalised results. Raises NUT_EINVAL where a launch does not cover it.
 struct AttentionPlan {
     uint32_t chunk, chunks, tiles;
+    uint32_t likely; // rows of the longest sequence that are read, but for pages named twice
     size_t stats, scores; // byte offsets
     size_t bytes;
 };

@@ -2,9 +2,10 @@
 // KV cache.
 //
 // A workgroup takes a run of one sequence's rows for one KV head and up to 16
-// of the query heads that share it, and reads each row once. Its four waves
-// take tiles of the run in turn, each with a softmax of its own (running
-// maximum and sum); they are joined at the end, and the runs by join_kernel.
+// of the query heads that share it, and reads each row once. Its waves, four
+// at most, take tiles of the run in turn, each with a softmax of its own
+// (running maximum and sum); they are joined at the end, and the runs by
+// join_kernel.
 //
 // Everything between a tile's loads and its products stays in the lane that
 // it was loaded into. With lane = 16 j + c, the matrix instruction for
@@ -408,22 +409,30 @@ __device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t b, uint3
     return p;
 }
 
-// Waves of a workgroup: their sums have to fit its 64 KB of shared memory.
+// Waves of a workgroup at most: their sums have to fit its 64 KB of shared
+// memory. Runs of one or two tiles have a wave a tile: one that only waits
+// would keep others' registers (bfloat16 rows at 32 KV heads of 128: 61
+// sequences of up to 17 rows 18.6 us with four waves and 7.6 with one, 27 of up
+// to 33 10.4 with four and 6.7 with two). The count is the kernel's type: as an
+// argument it cost 32 sequences of 2,048 rows 14.7 us for 13.6.
 template <int HD> constexpr int kWavesOf = HD == 256 ? 2 : 4;
 
-template <int TYPE, int HD, bool FULL, bool NT>
-__global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
+template <int TYPE, int HD, bool FULL, bool NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
 {
     using T = Tile<TYPE, HD>;
-    constexpr int G = T::G, kWaves = kWavesOf<HD>, kThreads = 64 * kWaves;
+    constexpr int G = T::G, kThreads = 64 * WAVES;
     constexpr int kStride = HD + 4; // of a head's sums: 16 lanes' rows on all banks
+    // with fewer waves than there may be, a tile each
+    constexpr uint32_t kRoom = WAVES == kWavesOf<HD> ? kMostRows : 64;
+    static_assert(WAVES == kWavesOf<HD> || WAVES * T::kRows <= int(kRoom), "rows of a short run");
     // the rows' offsets, and when they are done with the waves' sums
     __shared__ union Shared {
-        size_t at[kMostRows];
-        float o[kWaves][16][kStride];
+        size_t at[kRoom];
+        float o[WAVES][16][kStride];
     } lds;
-    __shared__ float stat[3][kWaves][16];
-    __shared__ uint32_t gone[kMostRows / 32]; // bit per row: masked
+    __shared__ float stat[3][WAVES][16];
+    __shared__ uint32_t gone[kRoom / 32]; // bit per row: masked
     const PagedView &kv = a.kv;
     // A sequence's runs one after another, begun one further for each: workgroups
     // go to the 8 XCDs in turn, and if every sequence's runs began alike, the
@@ -496,7 +505,7 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
     // is room for, the next one that has a row
     const auto next = [&](int t) {
         while (a.selected != nullptr && t < tiles && masked(t) == kAll)
-            t += kWaves;
+            t += WAVES;
         return t;
     };
     int t = next(wave);
@@ -506,7 +515,7 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
     while (t < tiles) {
         attend<TYPE, HD>(x, masked(t), q, sm, scores == nullptr ? nullptr : scores + t * T::kRows,
                          lane);
-        t = next(t + kWaves);
+        t = next(t + WAVES);
         if (t < tiles)
             x.template load<FULL, NT>(kv, lds.at + t * T::kRows, lane);
     }
@@ -537,13 +546,13 @@ __global__ __launch_bounds__(64 * kWavesOf<HD>) void attend_kernel(AttendArgs a)
         const uint32_t head = i / parts, d = i % parts * 4;
         float most = stat[0][0][head];
 #pragma unroll
-        for (int w = 1; w < kWaves; w++)
+        for (int w = 1; w < WAVES; w++)
             most = fmaxf(most, stat[0][w][head]);
         const float ref = most == -INFINITY ? 0.0f : most - Softmax<TYPE, HD>::kShift;
         float sum = 0.0f;
         f32x4 o{0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             // what no row of a finite score reached is zero, or not a number
             const float f = stat[0][w][head] == -INFINITY
                                 ? 1.0f
@@ -724,28 +733,43 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, PagedHistory hi
 // 54 52, 2,097 359 328, fp32 131 32 30, 2,097 372 334.
 constexpr uint64_t kPastCaches = 128ull << 20;
 
-template <int TYPE, int HD>
-void attend_as(const AttendArgs &a, dim3 grid, uint64_t bytes, hipStream_t stream)
+template <int TYPE, int HD, bool FULL, bool NT, int WAVES>
+void attend_by(const AttendArgs &a, dim3 grid, hipStream_t stream)
 {
-    const auto kernel = a.kv.head_dim != HD    ? attend_kernel<TYPE, HD, false, false>
-                        : bytes >= kPastCaches ? attend_kernel<TYPE, HD, true, true>
-                                               : attend_kernel<TYPE, HD, true, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWavesOf<HD>), 0, stream, a);
+    hipLaunchKernelGGL((attend_kernel<TYPE, HD, FULL, NT, WAVES>), grid, dim3(64 * WAVES), 0,
+                       stream, a);
+}
+
+template <int TYPE, int HD>
+void attend_as(const AttendArgs &a, dim3 grid, uint32_t rows, uint64_t bytes, hipStream_t stream)
+{
+    constexpr int kMost = kWavesOf<HD>;
+    const bool full = a.kv.head_dim == HD;
+    const uint32_t tiles = (std::min(a.chunk, rows) - 1) / Tile<TYPE, HD>::kRows + 1;
+    const auto run =
+        full && bytes >= kPastCaches ? attend_by<TYPE, HD, true, true, kMost>
+        : tiles == 1 ? (full ? attend_by<TYPE, HD, true, false, 1>
+                             : attend_by<TYPE, HD, false, false, 1>)
+        : tiles == 2 ? (full ? attend_by<TYPE, HD, true, false, 2>
+                             : attend_by<TYPE, HD, false, false, 2>)
+                     : (full ? attend_by<TYPE, HD, true, false, kMost>
+                             : attend_by<TYPE, HD, false, false, kMost>);
+    run(a, grid, stream);
 }
 
 template <int TYPE>
-void attend_in(const AttendArgs &a, dim3 grid, uint64_t bytes, hipStream_t stream)
+void attend_in(const AttendArgs &a, dim3 grid, uint32_t rows, uint64_t bytes, hipStream_t stream)
 {
     if (a.kv.head_dim <= 32)
-        attend_as<TYPE, 32>(a, grid, bytes, stream);
+        attend_as<TYPE, 32>(a, grid, rows, bytes, stream);
     else if (a.kv.head_dim <= 64)
-        attend_as<TYPE, 64>(a, grid, bytes, stream);
+        attend_as<TYPE, 64>(a, grid, rows, bytes, stream);
     else if (a.kv.head_dim <= 96)
-        attend_as<TYPE, 96>(a, grid, bytes, stream);
+        attend_as<TYPE, 96>(a, grid, rows, bytes, stream);
     else if (a.kv.head_dim <= 128)
-        attend_as<TYPE, 128>(a, grid, bytes, stream);
+        attend_as<TYPE, 128>(a, grid, rows, bytes, stream);
     else
-        attend_as<TYPE, 256>(a, grid, bytes, stream);
+        attend_as<TYPE, 256>(a, grid, rows, bytes, stream);
 }
 
 } // namespace
@@ -759,7 +783,7 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     const uint32_t rows = top == 0 ? seqs.max_length : top * kv.page_size;
     // a selection of more pages than a sequence has is -1 behind them, and tiles
     // without a row are passed over
-    const uint32_t likely = std::min(rows, seqs.max_length);
+    const uint32_t likely = plan.likely = std::min(rows, seqs.max_length);
     plan.tiles = (group + 15) / 16;
     // Runs as long as leave 512 workgroups: of 32 ragged sequences of up to 2,048
     // bfloat16 rows, 13.5 us in runs of 512 (512 workgroups), 14.2 in runs of 256
@@ -811,15 +835,15 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
     const uint32_t blocks = weighted ? (seqs.max_length + 4 * threads - 1) / (4 * threads) : 0;
     const uint64_t joins = uint64_t(seqs.batch) * heads;
     const dim3 join = paged_grid(joins + uint64_t(seqs.batch) * kv.kv_heads * blocks, threads);
-    const uint64_t rows = top == 0 ? seqs.max_length : uint64_t(top) * kv.page_size;
-    const uint64_t bytes = rows * seqs.batch * kv.kv_heads * kv.head_dim * 2 *
+    const uint32_t rows = top == 0 ? seqs.max_length : top * kv.page_size;
+    const uint64_t bytes = uint64_t(plan.likely) * seqs.batch * kv.kv_heads * kv.head_dim * 2 *
                            paged_element(kv.type);
     if (kv.type == NUT_F32)
-        attend_in<NUT_F32>(a, grid, bytes, stream);
+        attend_in<NUT_F32>(a, grid, rows, bytes, stream);
     else if (kv.type == NUT_F16)
-        attend_in<NUT_F16>(a, grid, bytes, stream);
+        attend_in<NUT_F16>(a, grid, rows, bytes, stream);
     else
-        attend_in<NUT_BF16>(a, grid, bytes, stream);
+        attend_in<NUT_BF16>(a, grid, rows, bytes, stream);
     check_launch("paged attention");
     if (!split)
         return;
