@@ -23,8 +23,8 @@ template <int TYPE>
 __global__ __launch_bounds__(256) void append_kernel(
     PagedView kv, PagedSeqs s, const float *__restrict__ keys, const float *__restrict__ values,
     size_t rows, size_t row_stride, size_t head_stride, const int *__restrict__ starts,
-    uint32_t each, uint32_t max_new, PagedHistory history, const int *__restrict__ firsts, int *new_lengths,
-    uint32_t touched)
+    uint32_t each, uint32_t max_new, PagedHistory history, const int *__restrict__ firsts,
+    int *new_lengths, uint32_t touched)
 {
     const uint32_t id = blockIdx.x;
     const uint32_t c = id % touched, h = id / touched % kv.kv_heads;
@@ -923,14 +923,13 @@ void launch_paged_append(const PagedView &kv, const PagedSeqs &seqs, const float
                          int *new_lengths, hipStream_t stream)
 {
     const uint32_t touched = pages_touched(max_new, kv.page_size);
-    const uint32_t most = std::min(kv.page_size, max_new) * (kv.head_dim / 8);
-    const uint32_t threads = std::min(256u, (most + kWave - 1) / kWave * kWave);
+    const uint32_t threads = append_threads(kv.page_size, max_new, kv.head_dim);
     const auto kernel = kv.type == NUT_F32   ? append_kernel<NUT_F32>
                         : kv.type == NUT_F16 ? append_kernel<NUT_F16>
                                              : append_kernel<NUT_BF16>;
     hipLaunchKernelGGL(kernel, paged_grid(uint64_t(seqs.batch) * kv.kv_heads * touched, threads),
-                       dim3(threads), 0, stream, kv, seqs, keys, values, rows, row_stride, head_stride, starts, each,
-                       max_new, history, firsts, new_lengths, touched);
+                       dim3(threads), 0, stream, kv, seqs, keys, values, rows, row_stride,
+                       head_stride, starts, each, max_new, history, firsts, new_lengths, touched);
     check_launch("paged append");
 }
 

@@ -69,6 +69,15 @@ NUT_HOST_DEVICE uint32_t pages_touched(uint32_t gain, uint32_t page_size)
     return (gain - 1 + page_size - 1) / page_size + 1;
 }
 
+// Threads of an append's workgroup: head_dim / 8 a row, as many rows as a page
+// gains at most, in whole waves up to 256 (and never fewer than one row's).
+NUT_HOST_DEVICE uint32_t append_threads(uint32_t page_size, uint32_t max_new, uint32_t head_dim)
+{
+    const uint32_t rows = page_size < max_new ? page_size : max_new;
+    const uint64_t threads = (uint64_t(rows) * (head_dim / 8) + 63) / 64 * 64;
+    return threads < 256 ? uint32_t(threads) : 256;
+}
+
 // The rows [begin, end) that an append of m rows behind n puts into the c-th
 // page it touches, page `index` of the sequence; begin = end for none.
 struct AppendSpan {

@@ -2,6 +2,7 @@
 // the kernels use it, on the host: every row lands in its page and slot, an
 // append's workgroups cover its rows once, and pages, lengths and counts that
 // a call cannot follow are refused before anything is read or written.
+#include <algorithm>
 #include <climits>
 #include <cstdio>
 #include <cstdlib>
@@ -64,6 +65,18 @@ static void spans()
     expect(append_span(n, 5, 3, 48, d).begin == append_span(n, 5, 3, 48, d).end, "behind it");
 }
 
+static void threads()
+{
+    for (uint32_t dim = 8; dim <= 256; dim += 8)
+        for (uint32_t size : {1u, 3u, 16u, 1u << 26, 1u << 27, 1u << 28, 0x7fffffffu})
+            for (uint32_t max_new : {1u, 2u, 64u, 1u << 27, 1u << 28, 1u << 29, 0x7fffffffu}) {
+                const uint32_t t = append_threads(size, max_new, dim);
+                const uint64_t rows = std::min(size, max_new), all = rows * (dim / 8);
+                expect(t % 64 == 0 && t <= 256 && t >= dim / 8, "append threads", dim, size, t);
+                expect(t == 256 || (t >= all && t < all + 64), "a page's rows", dim, size, t);
+            }
+}
+
 static void refusals()
 {
     for (int page : {0, 1, 9})
@@ -92,6 +105,7 @@ int main()
 {
     division();
     spans();
+    threads();
     refusals();
     std::printf("all passed\n");
     return 0;
