@@ -274,10 +274,11 @@ typedef struct nut_paged_history {
  * d_starts is NULL. Rows are rounded to the cache's type (to nearest, ties
  * to even), the page bounds widened, and where history is given the rows'
  * weights set to 0 and their positions to d_first_positions[b] onwards (NULL:
- * d_lengths[b] onwards). d_new_lengths (may be NULL, must not be d_lengths)
- * gets the lengths with the new rows; max_length is the most that it may
- * say. A sequence that would pass max_length gets no row and keeps its
- * length. No two sequences may append to one page. */
+ * d_lengths[b] onwards). d_new_lengths (may be NULL; apart from d_lengths,
+ * d_starts and d_first_positions) gets the lengths with the new rows;
+ * max_length is the most that it may say. A sequence that would pass
+ * max_length gets no row and keeps its length. No two sequences may append
+ * to one page. */
 int nut_paged_append(const nut_paged_kv *kv, const nut_paged_batch *seqs,
                      const float *d_keys, const float *d_values, size_t rows,
                      size_t row_stride, size_t head_stride,
@@ -349,7 +350,7 @@ int nut_paged_select(const nut_paged_kv *kv, const nut_paged_batch *seqs,
  * all others. Rows that stay beyond the budget move, with their weights and
  * positions, into the places of rows that go, both in ascending order;
  * nothing else moves. The bounds of a page that rows move into are widened.
- * d_new_lengths (must not be d_lengths) gets min(length, budget). Positions
+ * d_new_lengths (apart from d_lengths) gets min(length, budget). Positions
  * are distinct and not negative. Pages that hold rows below the budget must
  * not be shared. The workspace (16-byte aligned) needs
  * nut_paged_evict_workspace bytes. */

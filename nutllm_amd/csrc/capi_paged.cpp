@@ -132,6 +132,14 @@ void check_workspace(const void *workspace, size_t bytes, size_t need)
     require(aligned16(workspace), NUT_EINVAL, "paged cache: workspace must be 16-byte aligned");
 }
 
+// New lengths are written while other workgroups still read a call's inputs.
+bool apart(const int *written, const int *read, size_t batch, size_t count)
+{
+    const uintptr_t a = reinterpret_cast<uintptr_t>(written), b = reinterpret_cast<uintptr_t>(read);
+    return written == nullptr || read == nullptr || a + batch * sizeof(int) <= b ||
+           b + count * sizeof(int) <= a;
+}
+
 // The bytes that `body` finds, or (size_t)-1 where it refuses its arguments.
 template <typename Body> size_t bytes_or_error(Body &&body)
 {
@@ -149,7 +157,7 @@ void append(const nut_paged_kv *kv, const nut_paged_batch *seqs, const float *ke
     const nut::PagedSeqs s = seqs_of(v, seqs);
     const nut::PagedHistory h = history_of(s, history);
     require(keys != nullptr && values != nullptr, NUT_EINVAL, "paged cache: null pointer");
-    require(new_lengths != seqs->d_lengths, NUT_EINVAL,
+    require(apart(new_lengths, s.lengths, s.batch, s.batch), NUT_EINVAL,
             "paged cache: new lengths must not be the lengths");
     require(max_new != 0 && max_new <= kMost && rows <= kMost, NUT_EINVAL,
             "paged append: invalid row count");
@@ -164,6 +172,9 @@ void append(const nut_paged_kv *kv, const nut_paged_batch *seqs, const float *ke
             NUT_EINVAL, "paged cache: rows must start at multiples of 16 bytes");
     require(row_stride < (size_t(1) << 31) && head_stride < (size_t(1) << 31), NUT_EINVAL,
             "paged append: invalid strides");
+    require(apart(new_lengths, starts, s.batch, size_t(s.batch) + 1) &&
+                apart(new_lengths, firsts, s.batch, s.batch),
+            NUT_EINVAL, "paged append: new lengths must not be the starts or first positions");
     nut::ensure_device();
     // a sequence that gained more than max_length rows would be refused
     nut::launch_paged_append(v, s, keys, values, rows, row_stride, head_stride, starts,
@@ -287,7 +298,7 @@ int nut_paged_evict(const nut_paged_kv *kv, const nut_paged_batch *seqs,
         require(first <= budget && last <= budget - first, NUT_EINVAL,
                 "paged evict: first and last rows exceed the budget");
         require(d_new_lengths != nullptr, NUT_EINVAL, "paged cache: null pointer");
-        require(d_new_lengths != seqs->d_lengths, NUT_EINVAL,
+        require(apart(d_new_lengths, s.lengths, s.batch, s.batch), NUT_EINVAL,
                 "paged cache: new lengths must not be the lengths");
         check_workspace(d_workspace, workspace_bytes,
                         nut::evict_workspace(v, s, uint32_t(budget)));

@@ -194,6 +194,23 @@ def test_append_arguments():
         append(keys=At(nbytes=4 * 2 * 64 * 3), new_lengths=None)
 
 
+def test_new_lengths_that_overlap_an_input():
+    """The lengths are at 8192: three integers."""
+    for call in (append, evict):
+        for at in (8184, 8188, 8196, 8200):
+            refused("must not be the lengths", call, new_lengths=At(at))
+        for at in (8180, 8204):
+            with pytest.raises(nut.DeviceError):
+                call(new_lengths=At(at))
+    for at in (12280, 12288, 12300):  # four starts
+        refused("starts or first positions", append, starts=At(12288), new_lengths=At(at))
+    for at in (12280, 12288, 12296):
+        refused("starts or first positions", append, first_positions=At(12288),
+                new_lengths=At(at))
+    with pytest.raises(nut.DeviceError):
+        append(starts=At(12288), first_positions=At(12304), new_lengths=At(12276))
+
+
 def test_append_from_a_cache_refuses():
     L, kv, s = nut.lib(), paged(), seqs(batch=1)
     assert L.nut_paged_append_cache(kv.ref, s.ref, None, 0, 0, 1, None, None, None, None) == 1
