@@ -650,15 +650,16 @@ __device__ __forceinline__ uint32_t weight_key(float w)
 }
 
 // A workgroup per (sequence, KV head) decides what stays: to[r] is the r-th
-// row below the budget that goes, from[r] the r-th beyond it that stays, and
-// counts how many there are. Weights and positions of up to eight rows a
+// row below the budget that goes, from[r] the r-th beyond it that stays (`list`
+// at most), and counts how many there are. Weights and positions of up to eight rows a
 // thread are read once; then barriers bound it: 9 us for 1,040 rows each of 64
 // KV heads, 12 us for 8,192 each of 128.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, PagedSeqs s,
                                                                 PagedHistory history,
                                                                 uint32_t budget, uint32_t first,
-                                                                uint32_t last, int *new_lengths,
+                                                                uint32_t last, uint32_t list,
+                                                                int *new_lengths,
                                                                 int *__restrict__ to,
                                                                 int *__restrict__ from,
                                                                 int *__restrict__ counts)
@@ -723,7 +724,7 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
     // holes in the lower halves of words, rows to move in the upper ones: each
     // segment has at most 2^13 of them
     uint32_t met = 0, holes = 0, moved = 0;
-    int *hole_at = to + size_t(id) * budget, *source = from + size_t(id) * budget;
+    int *hole_at = to + size_t(id) * list, *source = from + size_t(id) * list;
     for (uint32_t segment = 0; segment < n; segment += keys.kSegment) {
         keys.open(segment);
         uint32_t flag[kEach], place[kEach];
@@ -770,7 +771,7 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
 // (4.5 TB/s) where 128 KV heads of up to 8,192 rows keep 2,048.
 template <int TYPE>
 __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs s,
-                                                        PagedHistory history, uint32_t budget,
+                                                        PagedHistory history, uint32_t list,
                                                         uint32_t blocks,
                                                         const int *__restrict__ to,
                                                         const int *__restrict__ from,
@@ -780,13 +781,13 @@ __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs 
     const uint32_t id = blockIdx.x, c = id % blocks, row = id / blocks;
     const uint32_t h = row % kv.kv_heads, b = row / kv.kv_heads;
     const size_t at = row * history.stride;
-    to += size_t(row) * budget, from += size_t(row) * budget;
+    to += size_t(row) * list, from += size_t(row) * list;
     const uint32_t tpr = kv.head_dim / 8, part = threadIdx.x % tpr, group = threadIdx.x / tpr;
     const uint32_t groups = 256 / tpr, column = part * 8 * kSize;
     __shared__ size_t here[256], there[256];
     const uint32_t first = c * 256, r0 = first + threadIdx.x;
     // the list beside its length: what lies behind it is not used
-    int dst = r0 < budget ? to[r0] : 0, src = r0 < budget ? from[r0] : 0;
+    int dst = r0 < list ? to[r0] : 0, src = r0 < list ? from[r0] : 0;
     const uint32_t total = uint32_t(counts[row]);
     asm volatile("" : "+v"(dst), "+v"(src));
     if (first >= total)
@@ -958,11 +959,19 @@ void launch_paged_select(const PagedView &kv, const PagedSeqs &seqs, const float
     check_launch("paged select");
 }
 
+// Rows of a sequence and KV head that move at most: into the budget's places,
+// from behind them.
+static uint32_t most_moved(const PagedSeqs &seqs, uint32_t budget)
+{
+    return budget < seqs.max_length ? std::min(budget, seqs.max_length - budget) : 0;
+}
+
 size_t evict_workspace(const PagedView &kv, const PagedSeqs &seqs, uint32_t budget)
 {
     const size_t heads = size_t(seqs.batch) * kv.kv_heads;
     paged_grid(heads, 1024);
-    return 2 * aligned(heads * budget * sizeof(int)) + aligned(heads * sizeof(int));
+    return 2 * aligned(heads * most_moved(seqs, budget) * sizeof(int)) +
+           aligned(heads * sizeof(int));
 }
 
 void launch_paged_evict(const PagedView &kv, const PagedSeqs &seqs, const PagedHistory &history,
@@ -970,24 +979,25 @@ void launch_paged_evict(const PagedView &kv, const PagedSeqs &seqs, const PagedH
                         char *workspace, hipStream_t stream)
 {
     const uint64_t heads = uint64_t(seqs.batch) * kv.kv_heads;
-    const size_t list = aligned(heads * budget * sizeof(int));
+    const uint32_t list = most_moved(seqs, budget);
+    const size_t bytes = aligned(heads * list * sizeof(int));
     int *to = reinterpret_cast<int *>(workspace);
-    int *from = reinterpret_cast<int *>(workspace + list);
-    int *counts = reinterpret_cast<int *>(workspace + 2 * list);
+    int *from = reinterpret_cast<int *>(workspace + bytes);
+    int *counts = reinterpret_cast<int *>(workspace + 2 * bytes);
     // eight rows a thread of the smaller workgroup
     const uint32_t threads = seqs.max_length <= 2048 ? 256 : 1024;
     hipLaunchKernelGGL(threads == 256 ? plan_eviction_kernel<256> : plan_eviction_kernel<1024>,
                        paged_grid(heads, threads), dim3(threads), 0, stream, kv, seqs, history,
-                       budget, first, last, new_lengths, to, from, counts);
+                       budget, first, last, list, new_lengths, to, from, counts);
     check_launch("paged evict");
-    if (budget >= seqs.max_length)
+    if (list == 0)
         return;
-    const uint32_t most = std::min(budget, seqs.max_length - budget), blocks = (most + 255) / 256;
+    const uint32_t blocks = (list + 255) / 256;
     const auto kernel = kv.type == NUT_F32   ? move_rows_kernel<NUT_F32>
                         : kv.type == NUT_F16 ? move_rows_kernel<NUT_F16>
                                              : move_rows_kernel<NUT_BF16>;
     hipLaunchKernelGGL(kernel, paged_grid(heads * blocks, 256), dim3(256), 0, stream, kv, seqs,
-                       history, budget, blocks, to, from, counts);
+                       history, list, blocks, to, from, counts);
     check_launch("paged evict");
 }
 

@@ -229,6 +229,12 @@ def test_workspaces_of_refused_calls():
     refused("invalid budget", kv.evict_workspace, s, 0)
 
 
+def test_eviction_workspace_grows_with_the_rows_that_can_move():
+    """One that keeps all but one row, or every row, of 64 needs little."""
+    sizes = [paged().evict_workspace(seqs(), budget) for budget in (63, 64, 1 << 30)]
+    assert max(sizes) <= 768 and paged().evict_workspace(seqs(), 32) > 768
+
+
 def test_check_needs_a_status_word():
     refused("no status word", paged().check)
 

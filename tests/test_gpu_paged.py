@@ -45,6 +45,27 @@ def test_attention(gpu, kind, heads, kv, dim, page, slot_major):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 16), (3, 1, 40), (8, 8, 64), (34, 2, 96),
+                                          (2, 2, 128), (5, 1, 136), (4, 2, 256)])
+@pytest.mark.parametrize("most", [1, 3, 16, 17, 32, 33, 48, 64, 65])
+def test_attention_short(gpu, kind, heads, kv, dim, most):
+    """Sequences of one tile, two and more: with weights, and of a selection."""
+    lengths = [most, 0, 1, max(1, most - 1), most // 2]
+    case = Case(kind, lengths, kv, dim, 8, seed=most, max_length=most).upload()
+    q = query_of(case, heads)
+    check_attention(case, heads, q)
+    check_attention(case, heads, q, history=case.history)
+    pages = (most + 7) // 8
+    top = min(pages, 4)
+    selected = np.full((5, kv, top), -1, np.int32)
+    for b, n in enumerate(lengths):
+        for h in range(kv):
+            there = case.rng.permutation((n + 7) // 8)[:top]
+            selected[b, h, :len(there)] = there
+    check_attention(case, heads, q, selected=selected, top=top)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("lengths", [[1500], [2049, 1, 0, 1024, 1023, 1025], [5000, 4097]])
 def test_attention_split_lengths(gpu, kind, lengths):
     case = Case(kind, lengths, 1, 64, 48, seed=3).upload()
@@ -232,6 +253,16 @@ def test_evict_ties_and_not_numbers(gpu):
     case.weights[1, 1, 1::5] = -np.inf
     case.weights[1, 1, 2::5] = -0.0
     check_evict(case, 300, 2, 10)
+
+
+@pytest.mark.parametrize("more", [1, 3, 257])
+def test_evict_a_few_of_many(gpu, more):
+    """Budgets just below the longest sequence, and above every one."""
+    lengths = [700 + more, 700, 699 + more, 12]
+    case = Case("bf16", lengths, 2, 16, 16, seed=more, max_length=700 + more)
+    case.weights[:] = np.exp(case.rng.standard_normal(case.weights.shape))
+    check_evict(case, 700, 1, 5)
+    check_evict(case, 1 << 30, 1, 5)
 
 
 def test_evict_long(gpu):
