@@ -221,8 +221,8 @@ int nut_kv_write_positions(nut_kvcache *kv, size_t begin, size_t end,
  * call only launches kernels on `stream` (so it can be captured into a
  * graph), and every workspace is the caller's: calls that may run at the
  * same time, or graphs that may be replayed at the same time, need
- * workspaces of their own. Device pointers are the device's that
- * nut_set_device selected.
+ * workspaces of their own. What a call only writes must not overlap what it
+ * reads. Device pointers are the device's that nut_set_device selected.
  *
  * Arguments that the host sees are checked (NUT_EINVAL). What only the
  * device sees is checked in the kernels: a page outside [0, pages), or a
@@ -287,7 +287,8 @@ int nut_paged_append(const nut_paged_kv *kv, const nut_paged_batch *seqs,
                      const int *d_first_positions, int *d_new_lengths,
                      void *stream);
 /* nut_paged_append from a nut_kvcache, such as nut_prefill leaves: its rows
- * [begin, end) of `layer` go behind the one sequence of `seqs`. */
+ * [begin, end) of `layer` go behind the one sequence of `seqs`. The source
+ * must not change, or be destroyed, before `stream` has come past the call. */
 int nut_paged_append_cache(const nut_paged_kv *kv,
                            const nut_paged_batch *seqs,
                            const nut_kvcache *source, size_t layer,
@@ -303,7 +304,8 @@ int nut_paged_append_cache(const nut_paged_kv *kv,
  * b query_stride (0: packed; a multiple of 4). d_lse (may be NULL) gets the
  * log of each softmax's denominator, [batch][heads]. A sequence without rows,
  * or a head whose scores are all minus infinity, gets zeros and minus
- * infinity.
+ * infinity. Where a value that counts has an infinite component, that
+ * component of out is infinite or not a number.
  *
  * history (may be NULL): every row's weight grows by its attention weight,
  * summed over the heads that share its KV head; the positions are not read.

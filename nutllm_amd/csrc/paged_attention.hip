@@ -73,8 +73,7 @@ __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c)
                                                       __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// The limbs of eight fp32 values as matrix operands. A value that is not
-// finite is its first limb alone.
+// The limbs of eight finite fp32 values as matrix operands.
 template <int TYPE, int LIMBS>
 __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&limb)[LIMBS])
 {
