@@ -57,6 +57,12 @@ struct AttendArgs {
     uint32_t top;
     float *out, *lse;
     uint32_t chunk, chunks, tiles;
+    uint32_t turn; // runs begin one further every 2^turn heads
+    // A selection of more pages than a sequence has: runs without any end early,
+    // which costs the others a barrier (64 pages of 128 rows, 33 sequences of up
+    // to 537 rows, 32 KV heads of 128: 83 us with it and 115 without; where no run
+    // is empty, 32 of 501 pages, 18.1 and 17.7).
+    bool loose;
     float *parts;  // [batch][heads][chunks][head_dim], unnormalised
     float2 *stats; // [batch][heads][chunks]: exponent they refer to, sum
     float *scores; // [batch][heads][chunks * chunk], base 2; nullptr: not kept
@@ -383,28 +389,27 @@ __device__ __forceinline__ void attend(Tile<TYPE, HD> &tile, uint32_t gone,
     }
 }
 
-// Where row i of a run lies: page `index` of the sequence (-1: none, -2: one
-// that no table row has), and what the table says of it.
+// Where a row lies: page `index` of the sequence (-1: none, -2: one that no
+// table row has), and what the table says of it.
 struct Place {
     int index, page;
     uint32_t slot;
 };
 
+// Row i of the run at `begin`, before the table is asked.
 __device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t b, uint32_t h, uint32_t i,
-                                          uint32_t most, uint32_t pages)
+                                          uint32_t begin, uint32_t most, uint32_t pages)
 {
     Place p{-1, -1, 0};
-    if (i >= most)
+    if (i >= a.chunk || begin + i >= most)
         return p;
-    p.index = int(page_of(a.kv, i));
-    p.slot = i - uint32_t(p.index) * a.kv.page_size;
+    p.index = int(page_of(a.kv, begin + i));
+    p.slot = begin + i - uint32_t(p.index) * a.kv.page_size;
     if (a.selected != nullptr) {
         p.index = a.selected[(size_t(b) * a.kv.kv_heads + h) * a.top + p.index];
         if (p.index < -1 || p.index >= int(pages))
             p.index = -2;
     }
-    if (p.index >= 0)
-        p.page = a.s.table[size_t(b) * a.s.table_stride + p.index];
     return p;
 }
 
@@ -433,12 +438,16 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
     __shared__ float stat[3][WAVES][16];
     __shared__ uint32_t gone[kRoom / 32]; // bit per row: masked
     const PagedView &kv = a.kv;
-    // A sequence's runs one after another, begun one further for each: workgroups
-    // go to the 8 XCDs in turn, and if every sequence's runs began alike, the
-    // late runs, which short sequences have not, would all be one XCD's.
+    // A sequence's runs one after another, begun one further every 2^turn: the
+    // workgroups go to 8 XCDs in turn, and on each to 4 groups of its CUs. If
+    // runs began alike, or moved on where these 32 have not been through, some
+    // would get all of the late runs, which short sequences, and selections of
+    // few pages, have not (33 sequences of up to 537 fp16 rows, 32 KV heads of
+    // 128, in the first of four runs of a selection: 144 us when runs moved on
+    // every two heads, 79 every eight).
     const uint32_t b = blockIdx.z, h = a.tiles == 1 ? blockIdx.y : blockIdx.y / a.tiles;
     const uint32_t tile16 = blockIdx.y - h * a.tiles;
-    uint32_t c = (blockIdx.x + blockIdx.y + gridDim.y * b) % a.chunks;
+    const uint32_t c = (blockIdx.x + ((blockIdx.y + gridDim.y * b) >> a.turn)) % a.chunks;
     const uint32_t begin = c * a.chunk;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -451,22 +460,46 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
     q.fetch(a.query + b * a.query_stride + (mine - size_t(b) * a.heads) * kv.head_dim, valid,
             kv.head_dim, lane);
 
-    // Where the run's rows begin, so that pages need not fit tiles. The first
-    // entries of the table are fetched beside the length, not after it: what
-    // lies behind the length is not used.
+    // Where the run's rows begin, so that pages need not fit tiles. The entries
+    // of the table are fetched together, and beside the length, not after it:
+    // what lies behind the length is not used.
     const uint32_t most = a.selected == nullptr ? a.s.max_length : a.top * kv.page_size;
     const uint32_t pages = page_of(kv, a.s.max_length - 1) + 1;
-    Place place = place_of(a, b, h, begin + threadIdx.x, most, pages);
+    constexpr int kEach = (kRoom + kThreads - 1) / kThreads;
+    Place places[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+        places[e] = place_of(a, b, h, e * kThreads + threadIdx.x, begin, most, pages);
+    if (a.loose) {
+        bool some = false;
+#pragma unroll
+        for (int e = 0; e < kEach; e++)
+            some = some || places[e].index != -1;
+        if (!__syncthreads_or(some)) { // no row: the join passes it over
+            if (threadIdx.x < here)
+                a.stats[(row + threadIdx.x) * a.chunks + c] = make_float2(-INFINITY, 0.0f);
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+        if (places[e].index >= 0)
+            places[e].page = a.s.table[size_t(b) * a.s.table_stride + places[e].index];
     const uint32_t n = paged_length(kv, a.s, b, threadIdx.x == 0 && c == 0 && h == 0);
-    asm volatile("" : "+v"(place.page));
+#pragma unroll
+    for (int e = 0; e < kEach; e++)
+        asm volatile("" : "+v"(places[e].page));
     const uint32_t total = a.selected == nullptr ? n : most;
     if (begin >= total && c != 0)
         return;
     const uint32_t count = min(total - begin, a.chunk);
     const int tiles = int((count + T::kRows - 1) / T::kRows);
-    for (uint32_t i = threadIdx.x; i < (count + kWave - 1) / kWave * kWave; i += kThreads) {
-        if (i >= kThreads)
-            place = place_of(a, b, h, begin + i, most, pages);
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const uint32_t i = e * kThreads + threadIdx.x;
+        if (i >= (count + kWave - 1) / kWave * kWave)
+            break;
+        const Place place = places[e];
         size_t at = 0;
         bool out = true;
         if (i < count && place.index < -1)
@@ -784,14 +817,16 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     // without a row are passed over
     const uint32_t likely = plan.likely = std::min(rows, seqs.max_length);
     plan.tiles = (group + 15) / 16;
-    // Runs as long as leave 512 workgroups: of 32 ragged sequences of up to 2,048
-    // bfloat16 rows, 13.5 us in runs of 512 (512 workgroups), 14.2 in runs of 256
-    // and 16.0 in runs of 1,024; of 7 of up to 5,001 fp32 rows 20.0 in runs of 128
-    // and 20.9 in runs of 256 and 512 (210 workgroups).
+    // Runs as long as leave 512 workgroups with rows: of 32 ragged sequences of up
+    // to 2,048 bfloat16 rows, 13.2 us in runs of 512 (512 workgroups), 14.1 in runs
+    // of 256 and 15.6 in runs of 1,024; of 7 of up to 5,001 fp32 rows 19.6 in runs
+    // of 256 (700 workgroups) and of 128, 21.1 in runs of 512. A selection of 124
+    // pages of 128 rows from 1,149 fp32 rows: 33 us by the rows that there are, 64
+    // by the places.
     plan.chunk = kMostRows;
-    while (plan.chunk > 128 && uint64_t(seqs.batch) * kv.kv_heads * plan.tiles *
-                                       ((rows + plan.chunk - 1) / plan.chunk) <
-                                   512)
+    const uint64_t columns = uint64_t(seqs.batch) * kv.kv_heads * plan.tiles;
+    while (likely > 128 && plan.chunk > 128 &&
+           columns * ((likely + plan.chunk - 1) / plan.chunk) < 512)
         plan.chunk /= 2;
     // Keys of up to 64 KB are one run whatever the number of workgroups: the
     // join's launch costs more. One sequence of 64 components, one run and
@@ -822,8 +857,10 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
     const bool split = plan.bytes != 0;
     AttendArgs a{kv, seqs, query, query_stride, heads, heads / kv.kv_heads,
                  scale * 1.4426950408889634f, selected, top, out, lse, plan.chunk, plan.chunks,
-                 plan.tiles, nullptr, nullptr, nullptr};
+                 plan.tiles, 5 - std::min(5u, uint32_t(__builtin_ctz(plan.chunks))), false, nullptr,
+                 nullptr, nullptr};
     if (split) {
+        a.loose = top > page_of(kv, seqs.max_length - 1) + 1;
         a.parts = reinterpret_cast<float *>(workspace);
         a.stats = reinterpret_cast<float2 *>(workspace + plan.stats);
         a.scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
