@@ -159,6 +159,30 @@ def test_select_and_sparse_attention(gpu, kind, heads, kv, dim, page, top, first
     check_attention(case, heads, q, selected=got, top=top)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (3, 3, 128), (34, 1, 40), (2, 2, 256)])
+def test_selection_of_more_pages_than_there_are(gpu, kind, heads, kv, dim):
+    """Runs of -1 before, between and behind the pages of a sequence, or only
+    those; a page that no table has is reported from a run without others."""
+    top = 260
+    case = Case(kind, [300, 0, 17, 160, 299, 300], kv, dim, 16, seed=dim).upload()
+    q = query_of(case, heads)
+    chosen = case.select(q, heads, top, 1, 2)
+    assert np.array_equal(chosen, case.expect_select(q, heads, top, 1, 2))
+    check_attention(case, heads, q, selected=chosen, top=top)
+    chosen[3] = np.roll(chosen[3], 200, axis=-1)
+    for h in range(kv):
+        chosen[4, h] = chosen[4, h][case.rng.permutation(top)]
+    chosen[5] = -1
+    check_attention(case, heads, q, selected=chosen, top=top)
+    case.paged.check()
+    chosen[5, kv - 1, 230] = 19  # one behind the last
+    out, lse = case.attention(q, heads, selected=chosen, top=top)
+    assert np.all(out[5] == 0) and np.all(np.isneginf(lse[5]))
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+
+
 def test_select_ties_and_many_pages(gpu):
     """Pages of equal bounds go by their index; more pages than threads."""
     case = Case("bf16", [9000, 777], 2, 16, 1, seed=17)
