@@ -476,6 +476,8 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
         for (int e = 0; e < kEach; e++)
             some = some || places[e].index != -1;
         if (!__syncthreads_or(some)) { // no row: the join passes it over
+            if (c == 0 && h == 0)
+                (void)paged_length(kv, a.s, b, threadIdx.x == 0); // but reports a bad length
             if (threadIdx.x < here)
                 a.stats[(row + threadIdx.x) * a.chunks + c] = make_float2(-INFINITY, 0.0f);
             return;

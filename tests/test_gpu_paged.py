@@ -183,6 +183,17 @@ def test_selection_of_more_pages_than_there_are(gpu, kind, heads, kv, dim):
         case.paged.check()
 
 
+@pytest.mark.parametrize("top", [4, 260])
+def test_bad_length_beside_a_selection_of_nothing(gpu, top):
+    case = Case("bf16", [100, 100], 2, 64, 16, seed=67)
+    case.lengths[1] = 101
+    case.upload()
+    out, lse = case.attention(query_of(case, 4), 4, selected=np.full((2, 2, top), -1), top=top)
+    assert np.all(out == 0) and np.all(np.isneginf(lse))
+    with pytest.raises(gpu.OutOfRange, match="length out of range"):
+        case.paged.check()
+
+
 def test_select_ties_and_many_pages(gpu):
     """Pages of equal bounds go by their index; more pages than threads."""
     case = Case("bf16", [9000, 777], 2, 16, 1, seed=17)
