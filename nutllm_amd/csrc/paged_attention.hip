@@ -13,8 +13,12 @@
 // (j, c) and leaves the scores of keys 4 j + i (i = 0..3) and head c there.
 // The one for O^T = V^T P^T sums over keys in an order of our choice, so lane
 // (j, c) supplies exactly those keys: P needs no exchange, and lane (j, c)
-// loads V rows 4 j + i, components c G .. c G + G - 1 (G = head dim / 16),
-// whose t-th is row c of output tile t. Only the running maximum crosses lanes.
+// loads V rows 4 j + i, in pieces of E components (up to 16 bytes) that lie
+// beside the other lanes', from 16 E w + E c on for w = 0, 1, ..: the t-th
+// component that it holds is row c of output tile t. With a lane's pieces one
+// after another instead, loads ask for lines by halves: 24 sequences of 6,000
+// fp32 rows of 96, 128 components 172, 218 us for 153, 196. Only the running
+// maximum crosses lanes.
 //
 // Products are exact. fp32 rows run on v_mfma_f32_16x16x4f32; 16-bit rows on
 // the 16x16x32 forms, with the fp32 operand (the query, the weights) split
@@ -156,6 +160,9 @@ template <int TYPE, int HD> struct Tile {
     static constexpr int kScores = kRows / 4;            // of a lane
     static constexpr int kKeys = kWide ? HD / 16 : HD / 16; // 16-byte pieces of K
     static constexpr int kWords = kWide ? G : G / 2;     // of a V row
+    // pieces of a power of two words divide a row of 8 n components
+    static constexpr int kPiece = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;
+    static constexpr int kEach = kWide ? kPiece : 2 * kPiece; // components of a piece
     u32x4 k[kKeys];
     uint32_t v[kScores][kWords];
 
@@ -179,18 +186,18 @@ template <int TYPE, int HD> struct Tile {
             for (int n = 0; n < kParts; n++) {
                 const uint32_t byte = n * 64 + j * 16;
                 const bool in = FULL || byte < kv.head_dim * kSize;
-                const u32x4 x = fetch<NT, u32x4>(p + (in ? byte : 0));
-                k[sub * kParts + n] = in ? x : u32x4{0, 0, 0, 0};
+                u32x4 x{0, 0, 0, 0};
+                if (in)
+                    x = fetch<NT, u32x4>(p + byte);
+                k[sub * kParts + n] = x;
             }
         }
 #pragma unroll
         for (int r = 0; r < kScores; r++) {
             const char *p = kv.values + at[16 * (r / 4) + 4 * j + r % 4];
-            // pieces of a power of two words divide a row of 8 n components
-            constexpr int kPiece = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;
 #pragma unroll
             for (int w = 0; w < kWords; w += kPiece) {
-                const uint32_t byte = (c * kWords + w) * 4;
+                const uint32_t byte = (16 * w + c * kPiece) * 4;
                 const char *q = p + (FULL || byte < kv.head_dim * kSize ? byte : 0);
                 if constexpr (kPiece == 1) {
                     v[r][w] = fetch<NT, uint32_t>(q);
@@ -562,17 +569,21 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
         stat[0][wave][column] = sm.most, stat[1][wave][column] = sm.ref,
         stat[2][wave][column] = sm.sum;
     {
-        float flat[HD / 4]; // components 4 j G .. 4 j G + 4 G - 1 of the lane's head
+        constexpr int E = T::kEach;
 #pragma unroll
-        for (int t = 0; t < G; t++)
+        for (int p = 0; p < G; p += E) {
+            float flat[4 * E]; // components 16 p + 4 j E .. of the lane's head
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                flat[i * G + t] = sm.o[t][i];
-        float *to = lds.o[wave][column] + j * (HD / 4);
+            for (int t = 0; t < E; t++)
 #pragma unroll
-        for (int d = 0; d < HD / 4; d += 4)
-            *reinterpret_cast<f32x4 *>(to + d) =
-                f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
+                for (int i = 0; i < 4; i++)
+                    flat[i * E + t] = sm.o[p + t][i];
+            float *to = lds.o[wave][column] + 16 * p + 4 * j * E;
+#pragma unroll
+            for (int d = 0; d < 4 * E; d += 4)
+                *reinterpret_cast<f32x4 *>(to + d) =
+                    f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
+        }
     }
     __syncthreads();
     const uint32_t parts = FULL ? HD / 4 : kv.head_dim / 4;
@@ -764,7 +775,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, PagedHistory hi
 // is there when the next call comes, and HBM is read faster without it. Three
 // caches in turn, us a call without and with, by MB of a call's rows: bfloat16
 // 33 15.3 16.3, 66 19.8 21.7, 131 33.3 30.6, 524 108 96, fp16 131 32.9 33.4, 262
-// 54 52, 2,097 359 328, fp32 131 32 30, 2,097 372 334.
+// 54 52, 2,097 359 328, fp32 131 32 30, 2,097 372 334. Not where sixteen pieces
+// are less than a line, nor of rows shorter than HD, whose lines' ends would be
+// fetched again: 16-bit rows of 96 components 86 without and 92 with (orders of
+// slots first 95 and 112), fp32 rows of 80 52 and 55.
 constexpr uint64_t kPastCaches = 128ull << 20;
 
 template <int TYPE, int HD, bool FULL, bool NT, int WAVES>
@@ -780,14 +794,15 @@ void attend_as(const AttendArgs &a, dim3 grid, uint32_t rows, uint64_t bytes, hi
     constexpr int kMost = kWavesOf<HD>;
     const bool full = a.kv.head_dim == HD;
     const uint32_t tiles = (std::min(a.chunk, rows) - 1) / Tile<TYPE, HD>::kRows + 1;
-    const auto run =
-        full && bytes >= kPastCaches ? attend_by<TYPE, HD, true, true, kMost>
-        : tiles == 1 ? (full ? attend_by<TYPE, HD, true, false, 1>
-                             : attend_by<TYPE, HD, false, false, 1>)
-        : tiles == 2 ? (full ? attend_by<TYPE, HD, true, false, 2>
-                             : attend_by<TYPE, HD, false, false, 2>)
-                     : (full ? attend_by<TYPE, HD, true, false, kMost>
-                             : attend_by<TYPE, HD, false, false, kMost>);
+    auto run = tiles == 1   ? (full ? attend_by<TYPE, HD, true, false, 1>
+                                    : attend_by<TYPE, HD, false, false, 1>)
+               : tiles == 2 ? (full ? attend_by<TYPE, HD, true, false, 2>
+                                    : attend_by<TYPE, HD, false, false, 2>)
+                            : (full ? attend_by<TYPE, HD, true, false, kMost>
+                                    : attend_by<TYPE, HD, false, false, kMost>);
+    if constexpr (Tile<TYPE, HD>::kPiece >= 2)
+        if (full && bytes >= kPastCaches)
+            run = attend_by<TYPE, HD, true, true, kMost>;
     run(a, grid, stream);
 }
 
