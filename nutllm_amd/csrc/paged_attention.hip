@@ -158,7 +158,7 @@ template <int TYPE, int HD> struct Tile {
     static constexpr bool kWide = TYPE == NUT_F32;
     static constexpr int kRows = kWide ? 16 : 32;
     static constexpr int kScores = kRows / 4;            // of a lane
-    static constexpr int kKeys = kWide ? HD / 16 : HD / 16; // 16-byte pieces of K
+    static constexpr int kKeys = HD / 16;                // 16-byte pieces of K
     static constexpr int kWords = kWide ? G : G / 2;     // of a V row
     // pieces of a power of two words divide a row of 8 n components
     static constexpr int kPiece = kWords % 4 == 0 ? 4 : kWords % 2 == 0 ? 2 : 1;
