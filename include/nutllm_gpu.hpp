@@ -444,7 +444,7 @@ private:
 
 // One layer's paged K/V cache: a nut_paged_kv over device memory that the
 // caller holds (no reference counterpart). Calls are asynchronous on `stream`,
-// allocate nothing, and throw for arguments that the host can judge; check()
+// allocate nothing, and throw for arguments that the host can see; check()
 // waits and throws for what only the device saw.
 class PagedKV {
 public:
