@@ -453,6 +453,9 @@ public:
 
     // Fp32 rows behind the sequences: rows starts[b] to starts[b + 1] for
     // sequence b, or row b where starts is null (and max_new 1).
+    // With history, d_first_positions holds the place in the text of each
+    // sequence's first new row (null: the lengths, right only for sequences
+    // that evict has not cut).
     void append(const nut_paged_batch &seqs, const float *d_keys, const float *d_values,
                 size_t rows, const int *d_starts = nullptr, size_t max_new = 1,
                 int *d_new_lengths = nullptr, const nut_paged_history *history = nullptr,

@@ -273,12 +273,17 @@ typedef struct nut_paged_history {
  * source rows that no sequence names are left out), or one row, row b, where
  * d_starts is NULL. Rows are rounded to the cache's type (to nearest, ties
  * to even), the page bounds widened, and where history is given the rows'
- * weights set to 0 and their positions to d_first_positions[b] onwards (NULL:
- * d_lengths[b] onwards). d_new_lengths (may be NULL; apart from d_lengths,
- * d_starts and d_first_positions) gets the lengths with the new rows;
- * max_length is the most that it may say. A sequence that would pass
- * max_length gets no row and keeps its length. No two sequences may append
- * to one page. */
+ * weights set to 0 and their positions to d_first_positions[b] onwards.
+ * d_new_lengths (may be NULL; apart from d_lengths, d_starts and
+ * d_first_positions) gets the lengths with the new rows; max_length is the
+ * most that it may say. A sequence that would pass max_length gets no row and
+ * keeps its length. No two sequences may append to one page.
+ *
+ * d_first_positions NULL stands for d_lengths: right until nut_paged_evict
+ * has cut a sequence. From then on its length is not its next token's place in
+ * the text: such positions repeat, and lie below those of kept rows, so that
+ * the next eviction takes the new rows for old ones. A program that evicts
+ * counts each sequence's text and passes the counts. */
 int nut_paged_append(const nut_paged_kv *kv, const nut_paged_batch *seqs,
                      const float *d_keys, const float *d_values, size_t rows,
                      size_t row_stride, size_t head_stride,

@@ -108,6 +108,52 @@ def test_serving_loop(gpu, kind):
     case.paged.check()
 
 
+@pytest.mark.parametrize("prompts", [[40, 23], [90, 48]])
+def test_new_tokens_stay_through_evictions(gpu, prompts):
+    """Append, weigh and evict for more steps than the budget has rows, with the
+    text's positions: what stays is the host's choice by the device's weights,
+    the newest `last` tokens of every sequence are always there, and no position
+    repeats."""
+    budget, first, last, heads, kv, dim = 48, 2, 12, 4, 2, 16
+    case = Case("f32", [0, 0], kv, dim, 8, seed=71, max_length=100)
+    case.bounds[:] = 0
+    case.upload()
+    rng, A = np.random.default_rng(72), gpu.DeviceArray
+    counts, text = prompts, np.zeros(2, np.int32)
+    positions = A(like=text)
+    for step in range(budget + 12):
+        k, v = (rng.standard_normal((sum(counts), kv, dim)).astype(np.float32) for _ in range(2))
+        starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        positions.upload(text)
+        new = case.expect_append(k, v, counts, firsts=text)
+        case.paged.append(case.seqs, A(like=k), A(like=v), case.d["new_lengths"],
+                          starts=A(like=starts) if step == 0 else None, max_new=max(counts),
+                          history=case.history, first_positions=positions)
+        gpu.synchronize()
+        text += np.array(counts, np.int32)
+        case.lengths = new
+        case.d["lengths"].upload(new)
+        case.attention(query_of(case, heads, step), heads, history=case.history)
+        case.weights = case.fetch("weights")
+        new = case.expect_evict(budget, first, last)
+        case.evict(budget, first, last)
+        assert np.array_equal(case.new_lengths(), new)
+        case.lengths = new
+        case.d["lengths"].upload(new)
+        for name in ("weights", "positions", "bounds"):
+            assert same(case.fetch(name), getattr(case, name)), name
+        for name in ("keys", "values"):
+            assert same(case.pool(name), getattr(case, name)), name
+        at = case.fetch("positions")
+        for b in range(2):
+            for h in range(kv):
+                there = set(at[b, h, :new[b]].tolist())
+                assert len(there) == new[b]
+                assert there >= set(range(max(0, text[b] - last), text[b])), (step, b, h)
+        counts = [1, 1]
+    case.paged.check()
+
+
 def test_captured_step(gpu):
     """A decode step (append, weighted attention, selection, attention over
     it, eviction) in two graphs with workspaces of their own, replayed in turn
