@@ -42,3 +42,9 @@ class Graph:
 
     def close(self):
         _call("hipGraphExecDestroy", self.handle)
+
+
+def copy(to, source, stream):
+    """All of `source` into `to`, device buffers of one size, on a stream."""
+    _call("hipMemcpyAsync", to.ptr, source.ptr, C.c_size_t(source.nbytes), C.c_int(3),
+          stream.handle)

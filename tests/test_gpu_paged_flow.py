@@ -8,7 +8,7 @@ import subprocess
 import numpy as np
 import pytest
 
-from hip import Graph, Stream
+from hip import Graph, Stream, copy
 from nutllm_amd import workloads as W
 from paged_case import Case, same
 
@@ -232,6 +232,73 @@ def test_captured_step(gpu):
     case.paged.check()
     for graph, *_ in graphs:
         graph.close()
+    stream.close()
+
+
+def test_captured_step_against_the_host(gpu):
+    """A decode step captured with the text's positions and a copy of the
+    weights between attention and eviction, replayed with other work between:
+    positions, weights, bounds and rows are the host's choice by that copy, and
+    the newest `last` tokens are there. Without first and last the same."""
+    heads, budget, kv, dim = 4, 100, 2, 64
+    A, stream = gpu.DeviceArray, Stream()
+    rng = np.random.default_rng(74)
+    for first, last in ((1, 5), (0, 0)):
+        case = Case("f16", [90, 130, 60], kv, dim, 16, seed=73, room=8).upload()
+        k, v, q = A(4 * 3 * kv * dim), A(4 * 3 * kv * dim), A(4 * 3 * heads * dim)
+        after = gpu.PagedBatch(case.d["table"], case.width, case.d["new_lengths"], 3,
+                               case.max_length)
+        text = np.array([90, 130, 60], np.int32)
+        positions, cut = A(like=text), A(like=np.zeros(3, np.int32))
+        out, held = A(q.nbytes), A(like=case.weights)
+        sizes = (case.paged.attention_workspace(after, heads, weighted=True),
+                 case.paged.evict_workspace(after, budget))
+        space = [A(like=np.full(max(1, n), 255, np.uint8)) for n in sizes]
+
+        def step():
+            at = stream.handle
+            case.paged.append(case.seqs, k, v, case.d["new_lengths"], history=case.history,
+                              first_positions=positions, stream=at)
+            case.paged.attention(after, q, out, heads, history=case.history, workspace=space[0],
+                                 stream=at)
+            copy(held, case.d["weights"], stream)
+            case.paged.evict(after, case.history, cut, budget, first=first, last=last,
+                             workspace=space[1], stream=at)
+
+        gpu.synchronize()
+        graph = Graph(stream, step)
+        for turn in range(6):
+            new = [rng.standard_normal(shape).astype(np.float32)
+                   for shape in ((3, kv, dim), (3, kv, dim), (3, heads, dim))]
+            for array, x in zip((k, v, q, positions), (*new, text)):
+                array.upload(x)
+            gpu.synchronize()
+            graph.replay()
+            stream.synchronize()
+            case.lengths = case.expect_append(new[0], new[1], [1, 1, 1], firsts=text)
+            grown = near(case, heads, new[2],
+                         out.download(np.float32, new[2].size).reshape(new[2].shape))
+            text += 1
+            weights = held.download(np.float32, case.weights.size).reshape(case.weights.shape)
+            assert np.allclose(weights, case.weights + grown, rtol=1e-4, atol=1e-6)
+            case.weights = weights
+            case.lengths = case.expect_evict(budget, first, last)
+            lengths = cut.download(np.int32, 3)
+            assert np.array_equal(lengths, case.lengths)
+            for name in ("weights", "positions", "bounds"):
+                assert same(case.fetch(name), getattr(case, name)), name
+            for name in ("keys", "values"):
+                assert same(case.pool(name), getattr(case, name)), name
+            at = case.fetch("positions")
+            for b in range(3):
+                for h in range(kv):
+                    there = set(at[b, h, :lengths[b]].tolist())
+                    assert len(there) == lengths[b]
+                    assert there >= set(range(text[b] - last, text[b]))
+            case.d["lengths"].upload(lengths)
+            gpu.synchronize()
+        graph.close()
+        case.paged.check()
     stream.close()
 
 
