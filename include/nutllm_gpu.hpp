@@ -452,7 +452,8 @@ public:
     const nut_paged_kv &view() const { return view_; }
 
     // Fp32 rows behind the sequences: rows starts[b] to starts[b + 1] for
-    // sequence b, or row b where starts is null (and max_new 1).
+    // sequence b, or row b where starts is null (and max_new 1). A stride of 0
+    // is that of [rows][kv_heads][head_dim].
     // With history, d_first_positions holds the place in the text of each
     // sequence's first new row (null: the lengths, right only for sequences
     // that evict has not cut).

@@ -268,7 +268,8 @@ typedef struct nut_paged_history {
 
 /* Puts new rows behind the rows that the sequences hold. d_keys and d_values
  * hold `rows` fp32 rows: row r's head h at element r row_stride +
- * h head_stride (multiples of 4; 0, 0: packed [rows][kv_heads][head_dim]).
+ * h head_stride (multiples of 4). Each stride of 0 has a default of its own,
+ * that of [rows][kv_heads][head_dim]; rows and heads must not overlap.
  * Sequence b gets rows d_starts[b] to d_starts[b + 1] (at most max_new;
  * source rows that no sequence names are left out), or one row, row b, where
  * d_starts is NULL. Rows are rounded to the cache's type (to nearest, ties

@@ -562,13 +562,17 @@ class PagedKV:
                head_stride=0, stream=None):
         """nut_paged_append: fp32 rows [rows][kv_heads][head_dim] behind the
         sequences, rows starts[b] to starts[b + 1] for sequence b (one each
-        without starts). With history, first_positions holds the place in the
+        without starts). row_stride and head_stride, in elements, are packed
+        ones where they are 0, each on its own. With history, first_positions holds the place in the
         text of each sequence's first new row (None: the lengths, right only
         for sequences that evict has not cut)."""
         row = row_stride or self.kv_heads * self.head_dim or 1
         used = (self.kv_heads - 1) * (head_stride or self.head_dim) + self.head_dim
         held = min(keys.nbytes, values.nbytes) // 4
         rows = (held - used) // row + 1 if held >= used else 0
+        if self.kv_heads > 1 and 0 < row_stride < head_stride:
+            # heads before rows: what the buffer has behind a head's rows is not one
+            rows = min(rows, (head_stride - self.head_dim) // row_stride + 1)
         check(lib().nut_paged_append(
             self.ref, seqs.ref, _raw(keys), _raw(values), rows, row_stride,
             head_stride, _raw(starts), max_new, _ref(history),

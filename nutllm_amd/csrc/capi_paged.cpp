@@ -17,6 +17,29 @@ hipStream_t as_stream(void *stream) { return static_cast<hipStream_t>(stream); }
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+struct Axis {
+    size_t stride, count;
+};
+
+// Elements that rows of head_dim span along these axes. The strides, widest
+// first, each have to clear what lies inside them.
+template <size_t N> double extent(size_t head_dim, const Axis (&axes)[N])
+{
+    Axis axis[N];
+    std::copy(axes, axes + N, axis);
+    std::sort(axis, axis + N, [](const Axis &a, const Axis &b) {
+        return a.stride != b.stride ? a.stride < b.stride : a.count < b.count;
+    });
+    double inside = double(head_dim);
+    for (const Axis &a : axis) {
+        if (a.count <= 1)
+            continue;
+        require(double(a.stride) >= inside, NUT_EINVAL, "paged cache: rows overlap");
+        inside += double(a.stride) * double(a.count - 1);
+    }
+    return inside;
+}
+
 nut::PagedView view_of(const nut_paged_kv *kv)
 {
     require(kv != nullptr && kv->d_keys != nullptr && kv->d_values != nullptr, NUT_EINVAL,
@@ -47,22 +70,9 @@ nut::PagedView view_of(const nut_paged_kv *kv)
         v.head_stride = kv->page_size * v.slot_stride;
         v.page_stride = kv->kv_heads * v.head_stride;
     } else {
-        // the strides, widest first, each have to clear what lies inside it
-        struct { size_t stride, count; } axis[3] = {{kv->page_stride, kv->pages},
-                                                    {kv->head_stride, kv->kv_heads},
-                                                    {kv->slot_stride, kv->page_size}};
-        for (int i = 0; i < 3; i++)
-            for (int j = i + 1; j < 3; j++)
-                if (axis[j].stride < axis[i].stride ||
-                    (axis[j].stride == axis[i].stride && axis[j].count < axis[i].count))
-                    std::swap(axis[i], axis[j]);
-        double inside = double(kv->head_dim);
-        for (const auto &a : axis) {
-            if (a.count == 1)
-                continue;
-            require(double(a.stride) >= inside, NUT_EINVAL, "paged cache: rows overlap");
-            inside += double(a.stride) * double(a.count - 1);
-        }
+        const double inside = extent(kv->head_dim, {Axis{kv->page_stride, kv->pages},
+                                                    Axis{kv->head_stride, kv->kv_heads},
+                                                    Axis{kv->slot_stride, kv->page_size}});
         require(inside * double(size) < 9e18 && kv->page_stride < (size_t(1) << 60) &&
                     kv->head_stride < (size_t(1) << 60) && kv->slot_stride < (size_t(1) << 60),
                 NUT_EINVAL, "paged cache: invalid dimensions");
@@ -164,14 +174,15 @@ void append(const nut_paged_kv *kv, const nut_paged_batch *seqs, const float *ke
     require(starts != nullptr || (max_new == std::max(each, size_t(1)) &&
                                   rows / std::max(each, size_t(1)) >= s.batch) || each == 0,
             NUT_EINVAL, "paged append: one row a sequence without starts");
-    if (row_stride == 0 && head_stride == 0) {
+    if (head_stride == 0)
         head_stride = v.head_dim;
+    if (row_stride == 0)
         row_stride = size_t(v.kv_heads) * v.head_dim;
-    }
     require(aligned16(keys) && aligned16(values) && row_stride % 4 == 0 && head_stride % 4 == 0,
             NUT_EINVAL, "paged cache: rows must start at multiples of 16 bytes");
     require(row_stride < (size_t(1) << 31) && head_stride < (size_t(1) << 31), NUT_EINVAL,
             "paged append: invalid strides");
+    extent(v.head_dim, {Axis{row_stride, rows}, Axis{head_stride, v.kv_heads}});
     require(apart(new_lengths, starts, s.batch, size_t(s.batch) + 1) &&
                 apart(new_lengths, firsts, s.batch, s.batch),
             NUT_EINVAL, "paged append: new lengths must not be the starts or first positions");

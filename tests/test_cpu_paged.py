@@ -194,6 +194,33 @@ def test_append_arguments():
         append(keys=At(nbytes=4 * 2 * 64 * 3), new_lengths=None)
 
 
+def test_append_strides():
+    """Each stride of 0 is that of packed rows, whatever the other one is;
+    source rows or heads that overlap are refused."""
+    # three sequences' rows of two heads of 64, alone and among others
+    for strides in (dict(row_stride=384), dict(head_stride=64), dict(row_stride=128),
+                    dict(row_stride=64, head_stride=192), dict(row_stride=384, head_stride=128),
+                    dict()):
+        with pytest.raises(nut.DeviceError):
+            append(keys=At(nbytes=4 * (2 * (strides.get("row_stride") or 128) +
+                                       (strides.get("head_stride") or 64) + 64)), **strides)
+    for strides in (dict(head_stride=192), dict(head_stride=128), dict(row_stride=64),
+                    dict(row_stride=124), dict(row_stride=192, head_stride=192),
+                    dict(row_stride=384, head_stride=32)):
+        refused("rows overlap", append, **strides)
+    # heads before rows: as many rows as there are before the next head
+    refused("one row a sequence", append, row_stride=64, head_stride=128)
+    for head_stride in (192, 200, 6400):
+        with pytest.raises(nut.DeviceError):
+            append(row_stride=64, head_stride=head_stride)
+    # one row, or one head, has nothing to overlap with
+    one = seqs(batch=1)
+    with pytest.raises(nut.DeviceError):
+        append(s=one, keys=At(nbytes=4 * (192 + 64)), head_stride=192)
+    with pytest.raises(nut.DeviceError):
+        append(paged(kv_heads=1), head_stride=4)
+
+
 def test_new_lengths_that_overlap_an_input():
     """The lengths are at 8192: three integers."""
     for call in (append, evict):

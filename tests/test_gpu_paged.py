@@ -366,6 +366,36 @@ def test_append_tokens(gpu, kind, kv, dim):
     check_append(case, new)
 
 
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("kv,dim,row_stride,head_stride", [
+    (3, 32, 3 * 3 * 32, 0), (3, 32, 0, 32), (4, 64, 4 * 64 + 8, 0), (3, 32, 32, 160),
+    (1, 64, 0, 8), (2, 16, 0, 0)])
+def test_append_strides(gpu, kv, dim, row_stride, head_stride, ragged):
+    """One stride without the other, heads before rows, and heads of one."""
+    counts = [1, 2, 2] if ragged else [1, 1, 1]
+    case = Case("f32", [0, 7, 16], kv, dim, 16, seed=75, room=2).upload()
+    rows = sum(counts)
+    row, head = row_stride or kv * dim, head_stride or dim
+    flat = case.rng.standard_normal(2 * (rows * row + kv * head)).astype(np.float32)
+    at = (np.arange(rows)[:, None, None] * row + np.arange(kv)[:, None] * head + np.arange(dim))
+    k, v = flat[at], flat[at + 4]
+    new = case.expect_append(k, v, counts)
+    A = gpu.DeviceArray
+    whole = A(like=flat)
+
+    class Part:
+        def __init__(self, first):
+            self.ptr = whole.ptr.value + 4 * first
+            self.nbytes = 4 * (flat.size - first)
+
+    starts = A(like=np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+    case.paged.append(case.seqs, Part(0), Part(4), case.d["new_lengths"],
+                      starts=starts if ragged else None, max_new=max(counts),
+                      history=case.history, row_stride=row_stride, head_stride=head_stride)
+    gpu.synchronize()
+    check_append(case, new)
+
+
 def test_append_not_a_number_shows_in_the_bounds(gpu):
     case = Case("f32", [3, 0], 1, 16, 8, seed=33, room=2).upload()
     k = np.ones((2, 1, 16), np.float32)
