@@ -340,7 +340,8 @@ int nut_paged_attention(const nut_paged_kv *kv, const nut_paged_batch *seqs,
  * `top` in all (first + last <= top), in ascending order, then -1. A page's
  * score is the largest, over the heads that share the KV head, of
  * sum_d max(q_d lo_d, q_d hi_d): no row of the page has a larger q . k. Sums
- * in 64 bits, ties to the lower page; a score that is not a number ranks
+ * in 64 bits, ties to the lower page; a score that is not a number (of a NaN,
+ * of infinite bounds met with both signs, or of one where q_d is 0) ranks
  * first. The workspace (16-byte aligned) needs nut_paged_select_workspace
  * bytes. */
 size_t nut_paged_select_workspace(const nut_paged_kv *kv,

@@ -403,13 +403,42 @@ __device__ __forceinline__ uint64_t score_key(double v)
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
+// A component's part of a page's score, max(q lo, q hi), of finite or infinite
+// bounds; not a number where a product is not (one of them, of a query of 0 and
+// an infinite bound).
+__device__ __forceinline__ double score_part(float q, float lo, float hi)
+{
+    const double a = double(q) * double(lo), b = double(q) * double(hi);
+    return a > b || a != a ? a : b;
+}
+
+// Eight components' part.
+template <int TYPE>
+__device__ __forceinline__ double score_of(const float *query, const char *bounds,
+                                           uint32_t head_dim)
+{
+    constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
+    float q[8], lo[8], hi[8];
+    load8<NUT_F32>(reinterpret_cast<const char *>(query), q);
+    load8<TYPE>(bounds, lo);
+    load8<TYPE>(bounds + head_dim * kSize, hi);
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        sum += score_part(q[i], lo[i], hi[i]);
+    return sum;
+}
+
 // Scores of every page, up to four heads to a KV head: LANES lanes, head_dim / 8
 // of them with work, hold eight components of a page's bounds each. For a page
 //   sum_d max(q_d lo_d, q_d hi_d) = sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d,
 // two multiply-adds a component in 64 bits, of which one adds zero: the answer
 // is whole numbers, and in 32 bits, or with terms that only cancel, rounding
-// would choose among near or equal pages. What bounds it is instructions: 16
-// fp64 ones a head and eight to bring them together, for 64 bytes a lane.
+// would choose among near or equal pages. An infinite bound that the query does
+// not meet makes the term that adds zero no number: such sums are made anew from
+// the definition, the same additions without those terms. What bounds it is
+// instructions: 16 fp64 ones a head and eight to bring them together, for 64
+// bytes a lane.
 template <int TYPE, int GH, uint32_t LANES>
 __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeqs s,
                                                           const float *__restrict__ query,
@@ -423,16 +452,14 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     const uint32_t index = c * (256 / LANES) + threadIdx.x / LANES, part = threadIdx.x % LANES;
     const uint32_t group = heads / kv.kv_heads;
     const bool works = part * 8 < kv.head_dim;
+    const float *own = query + b * query_stride + size_t(h) * group * kv.head_dim + part * 8;
     // the query and the table beside the length: what lies behind it is not used
     double up[GH][8], down[GH][8]; // max(q, 0) and min(q, 0)
 #pragma unroll
     for (int j = 0; j < GH; j++) {
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (works && uint32_t(j) < group)
-            load8<NUT_F32>(reinterpret_cast<const char *>(query + b * query_stride +
-                                                          size_t(h * group + j) * kv.head_dim +
-                                                          part * 8),
-                           v);
+            load8<NUT_F32>(reinterpret_cast<const char *>(own + size_t(j) * kv.head_dim), v);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             // a query component that is not a number stays one
@@ -449,10 +476,9 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
     if (!good && part == 0)
         paged_flag(kv.status, kBadPage);
     float lo[8] = {0, 0, 0, 0, 0, 0, 0, 0}, hi[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const char *at = kv.bounds + (size_t(good ? page : 0) * kv.kv_heads + h) * 2 * kv.head_dim *
+                                     kSize + part * 8 * kSize;
     if (good && works) {
-        const char *at = kv.bounds +
-                         (size_t(page) * kv.kv_heads + h) * 2 * kv.head_dim * kSize +
-                         part * 8 * kSize;
         load8<TYPE>(at, lo);
         load8<TYPE>(at + kv.head_dim * kSize, hi);
     }
@@ -467,6 +493,18 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
         for (int j = 0; j < GH; j++)
             sum[j] = fma(down[j][i], low, fma(up[j][i], high, sum[j]));
     }
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < GH; j++)
+        odd = odd || sum[j] != sum[j];
+    if (odd) // the query and the bounds once more: held till here, they cost waves
+#pragma unroll
+        for (int j = 0; j < GH; j++) {
+            const double x = works && uint32_t(j) < group
+                                 ? score_of<TYPE>(own + size_t(j) * kv.head_dim, at, kv.head_dim)
+                                 : 0.0;
+            sum[j] = sum[j] != sum[j] ? x : sum[j];
+        }
     uint32_t head = 0;
     sum_lanes<LANES / 2, GH>(sum, part, head);
     constexpr int kLeft = GH > int(LANES) ? GH / int(LANES) : 1;
@@ -482,13 +520,79 @@ __global__ __launch_bounds__(256) void page_scores_kernel(PagedView kv, PagedSeq
         scores[(size_t(b) * kv.kv_heads + h) * width + index] = good ? best : 0;
 }
 
+// What a page's infinite bounds add to its score: infinities, and no number
+// where they meet a query of 0.
+template <int TYPE>
+__device__ __forceinline__ double unbounded_part(const float *query, const char *bounds,
+                                                 uint32_t head_dim)
+{
+    constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
+    double sum = 0.0;
+#pragma unroll 1
+    for (uint32_t d = 0; d < head_dim; d += 8) {
+        float q[8], lo[8], hi[8];
+        load8<NUT_F32>(reinterpret_cast<const char *>(query + d), q);
+        load8<TYPE>(bounds + d * kSize, lo);
+        load8<TYPE>(bounds + (head_dim + d) * kSize, hi);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const double part = score_part(q[i], lo[i], hi[i]);
+            if (fmaxf(fabsf(lo[i]), fabsf(hi[i])) == INFINITY && !(fabs(part) < INFINITY))
+                sum += part;
+        }
+    }
+    return sum;
+}
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// The sums of page_scores_mfma_kernel anew, product by product, with infinite
+// bounds left out; whether the lane's components of its page have one. `own` is
+// the query of the lane's head.
+template <int TYPE>
+__device__ __forceinline__ bool bounded_sums(const float *own, bool valid, const char *bounds,
+                                             bool good, uint32_t head_dim, f64x4 &above,
+                                             f64x4 &below)
+{
+    constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
+    const uint32_t j = (threadIdx.x & (kWave - 1)) / 16;
+    bool unbounded = false;
+    above = below = f64x4{0, 0, 0, 0};
+#pragma unroll 1
+    for (uint32_t step = 0; step < (head_dim + 63) / 64 * 2; step++) {
+        const uint32_t d = step / 2 * 64 + 16 * j + step % 2 * 8;
+        float q[8] = {0, 0, 0, 0, 0, 0, 0, 0}, lo[8] = {0, 0, 0, 0, 0, 0, 0, 0},
+              hi[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (valid && d < head_dim)
+            load8<NUT_F32>(reinterpret_cast<const char *>(own + d), q);
+        if (good && d < head_dim) {
+            load8<TYPE>(bounds + d * kSize, lo);
+            load8<TYPE>(bounds + (head_dim + d) * kSize, hi);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool low = fabsf(lo[i]) == INFINITY, high = fabsf(hi[i]) == INFINITY;
+            unbounded = unbounded || low || high;
+            above = __builtin_amdgcn_mfma_f64_16x16x4f64(
+                double(high ? 0.0f : hi[i]), double(q[i] <= 0.0f ? 0.0f : q[i]), above, 0, 0, 0);
+            below = __builtin_amdgcn_mfma_f64_16x16x4f64(
+                double(low ? 0.0f : lo[i]), double(q[i] >= 0.0f ? 0.0f : q[i]), below, 0, 0, 0);
+        }
+    }
+    return unbounded;
+}
+
 // The same for more than four heads to a KV head, on v_mfma_f64_16x16x4f64: a
 // wave takes 16 pages (rows) and 16 heads (columns), and sums over 64
 // components at a time, max(q, 0) hi and min(q, 0) lo apart. Lane 16 j + c
 // loads components 16 j to 16 j + 15 of page c, whose n-th is the j-th of
 // four in step n; the query comes from shared memory, [sign][component][head].
 // Scores of pages 4 i + j and head c come out as element i of that lane. 32
-// steps of 64 cycles a tile bound it: 50,000 pages of 64 components 10.8 us.
+// steps of 64 cycles a tile bound it: 50,000 pages of 64 components 10.8 us. A
+// tile with a sum that is no number is summed anew without infinite bounds,
+// which a query of the other sign would make one, and what they add is found
+// from the definition.
 template <int TYPE>
 __global__ __launch_bounds__(256) void page_scores_mfma_kernel(PagedView kv, PagedSeqs s,
                                                                const float *__restrict__ query,
@@ -497,8 +601,6 @@ __global__ __launch_bounds__(256) void page_scores_mfma_kernel(PagedView kv, Pag
                                                                uint32_t width,
                                                                uint64_t *__restrict__ scores)
 {
-    typedef double f64x4 __attribute__((ext_vector_type(4)));
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
     constexpr uint32_t kSize = TYPE == NUT_F32 ? 4 : 2;
     __shared__ double qs[2][64][16];
     const uint32_t id = blockIdx.x, block = id % blocks, h = id / blocks % kv.kv_heads;
@@ -560,6 +662,28 @@ __global__ __launch_bounds__(256) void page_scores_mfma_kernel(PagedView kv, Pag
                                                              above, 0, 0, 0);
                 below = __builtin_amdgcn_mfma_f64_16x16x4f64(double(lo[e]), qs[1][16 * j + e][c],
                                                              below, 0, 0, 0);
+            }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            odd = odd || above[i] + below[i] != above[i] + below[i];
+        if (__any(odd)) {
+            const float *own = rows + size_t(g + c < group ? g + c : 0) * kv.head_dim;
+            const uint64_t lanes = __ballot(
+                bounded_sums<TYPE>(own, g + c < group, bounds, good, kv.head_dim, above, below));
+            const uint32_t which = uint32_t(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48);
+#pragma unroll 1
+            for (uint32_t p = j; p < 16; p += 4) {
+                const int its = __shfl(page, int(p));
+                double more = 0.0;
+                if (which >> p & 1 && g + c < group)
+                    more = unbounded_part<TYPE>(
+                        own, kv.bounds + (size_t(its) * kv.kv_heads + h) * 2 * kv.head_dim * kSize,
+                        kv.head_dim);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++)
+                    above[i] += i == p / 4 ? more : 0.0;
             }
         }
 #pragma unroll

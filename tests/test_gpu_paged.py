@@ -235,6 +235,101 @@ def test_select_not_a_number_first(gpu):
     assert got.tolist() == [[[7, 19]]]
 
 
+def select_by_definition(case, query, heads, top):
+    """[batch][kv][top] from max(q lo, q hi) as written, no numbers first."""
+    got = np.full((case.batch, case.kv, top), -1, np.int32)
+    group, q = heads // case.kv, np.asarray(query, np.float64)
+    for b, n in enumerate(case.lengths):
+        count = -(-int(n) // case.page)
+        for h in range(case.kv):
+            bound = decode(case.bounds[case.table[b, :count], h], case.kind)
+            mine = q[b, h * group:(h + 1) * group, None]
+            with np.errstate(invalid="ignore"):
+                score = np.maximum(mine * bound[:, 0], mine * bound[:, 1]).sum(-1)
+            odd = np.isnan(score).any(0)
+            best = np.where(np.isnan(score), -np.inf, score).max(0)
+            rank = sorted(range(count), key=lambda c: (not odd[c], 0 if odd[c] else -best[c], c))
+            chosen = sorted(rank[:top])
+            got[b, h, :len(chosen)] = chosen
+    return got
+
+
+@pytest.mark.parametrize("heads,dim", [(1, 64), (2, 16), (3, 128), (4, 256), (5, 64), (8, 40),
+                                       (16, 128), (20, 256)])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_select_infinite_bounds(gpu, kind, heads, dim):
+    """An infinite bound counts where the query meets it and nowhere else: by
+    the definition with queries of both signs, met from both sides (no number),
+    by a component of 0 (no number), and beside a NaN."""
+    case = Case(kind, [640, 170], 2, dim, 16, seed=77)
+    inf = np.float32(np.inf)
+    for b, n in enumerate(case.lengths):
+        for c in range(-(-int(n) // 16)):
+            for h in range(2):
+                at = (case.table[b, c], h)
+                d = case.rng.integers(dim, size=3)
+                if c % 5 == 1:
+                    case.bounds[(*at, 1, d[0])] = encode(inf, kind)
+                if c % 5 == 2:
+                    case.bounds[(*at, 0, d[0])] = encode(-inf, kind)
+                if c % 10 == 3:
+                    case.bounds[(*at, 0, d[:2])] = encode(-inf, kind)
+                    case.bounds[(*at, 1, d[1:])] = encode(inf, kind)
+                if c % 10 == 8:
+                    case.bounds[(*at, slice(None), d[2])] = encode(-inf if h else inf, kind)
+    case.bounds[case.table[1, 4], 1, 1, 5] = encode(np.float32(np.nan), kind)
+    case.upload()
+    for sign in (1, -1, 0):
+        q = query_of(case, 2 * heads, seed=5 + sign)
+        q = np.abs(q) * np.float32(sign) if sign else q
+        if sign == 0:
+            q[0, ::2, :3] = 0.0
+        for top in (1, 3, 9, 20, 33):
+            want = select_by_definition(case, q, 2 * heads, top)
+            assert np.array_equal(case.select(q, 2 * heads, top, 0, 0), want), (sign, top)
+
+
+@pytest.mark.parametrize("heads", [1, 4, 5, 8])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_select_bounds_that_the_query_does_not_meet(gpu, kind, heads):
+    """Pages that agree in the bounds that a query meets score alike to the last
+    bit, their others being infinite or not: the lower ones are chosen."""
+    case = Case(kind, [640], 1, 64, 16, seed=79)
+    order = case.rng.permutation(40)
+    best = np.abs(case.rng.standard_normal(64))  # no upper bound below a lower one
+    for i, c in enumerate(order[:25]):
+        lo = -3 * case.rng.random(64)
+        lo[case.rng.random(64) < 0.1 * (i % 3)] = -np.inf
+        case.bounds[case.table[0, c], 0, 1] = encode(best + 3, kind)
+        case.bounds[case.table[0, c], 0, 0] = encode(lo, kind)
+    case.upload()
+    q = np.abs(query_of(case, heads)) * np.float32(1.1)
+    want = select_by_definition(case, q, heads, 12)
+    assert want[0, 0].tolist() == sorted(order[:25])[:12]
+    assert np.array_equal(case.select(q, heads, 12, 0, 0), want)
+
+
+@pytest.mark.parametrize("heads", [2, 8])
+def test_select_keys_beyond_the_type(gpu, heads):
+    """Keys that the cache's type rounds to infinity, where the query has the
+    other sign: the page's score is finite and not the best one."""
+    case = Case("f16", [0], 1, 32, 8, seed=81, max_length=80).upload()
+    k = case.rng.standard_normal((80, 1, 32)).astype(np.float32)
+    k[20, 0, 4] = 70000.0  # page 2
+    k[51] += 4.0           # page 6
+    A = gpu.DeviceArray
+    case.lengths = case.expect_append(k, k, [80])
+    case.paged.append(case.seqs, A(like=k), A(like=k), None,
+                      starts=A(like=np.array([0, 80], np.int32)), max_new=80)
+    case.d["lengths"].upload(case.lengths)
+    q = np.abs(query_of(case, heads)) + np.float32(0.1)
+    q[..., 4] *= -1
+    want = select_by_definition(case, q, heads, 3)
+    assert 2 not in want[0, 0, :1] and 6 in want[0, 0]
+    assert np.array_equal(case.select(q, heads, 3, 0, 0), want)
+    assert np.array_equal(case.select(-q, heads, 1, 0, 0), [[[2]]])
+
+
 def test_sparse_attention_of_a_callers_selection(gpu):
     """A page twice counts twice; -1 anywhere, and pages behind the sequence's
     end, count nothing; a page no table row has is reported."""
