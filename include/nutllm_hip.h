@@ -310,8 +310,9 @@ int nut_paged_append_cache(const nut_paged_kv *kv,
  * b query_stride (0: packed; a multiple of 4). d_lse (may be NULL) gets the
  * log of each softmax's denominator, [batch][heads]. A sequence without rows,
  * or a head whose scores are all minus infinity, gets zeros and minus
- * infinity. Where a value that counts has an infinite component, that
- * component of out is infinite or not a number.
+ * infinity. Where a row that weighs something has a value with an infinite
+ * component, that component of out is infinite or not a number; where a row of
+ * weight 0 beside others has one, or a NaN, it may be not a number.
  *
  * history (may be NULL): every row's weight grows by its attention weight,
  * summed over the heads that share its KV head; the positions are not read.

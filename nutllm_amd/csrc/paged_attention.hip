@@ -614,8 +614,9 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
             if (d == 0)
                 a.stats[at * a.chunks + c] = make_float2(sum == 0.0f ? -INFINITY : ref, sum);
         } else {
-            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-            *reinterpret_cast<f32x4 *>(a.out + at * kv.head_dim + d) = o * f;
+            // no weight: zeros, whatever the values are
+            *reinterpret_cast<f32x4 *>(a.out + at * kv.head_dim + d) =
+                sum == 0.0f ? f32x4{0, 0, 0, 0} : o * (1.0f / sum);
             if (d == 0 && a.lse != nullptr)
                 a.lse[at] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
         }

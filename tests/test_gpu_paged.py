@@ -124,6 +124,39 @@ def test_attention_infinite_keys(gpu, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [32, 128])
+@pytest.mark.parametrize("length", [1, 20, 40, 100, 2500])
+def test_attention_of_no_weight_over_odd_values(gpu, kind, dim, length):
+    """A head whose scores are all minus infinity gets zeros and minus infinity
+    whatever its rows' values are, in one run and in several, and its rows no
+    weight; the other KV head gets what it would."""
+    case = Case(kind, [length, 33], 2, dim, 16, seed=83)
+    q = np.abs(query_of(case, 4)) + np.float32(0.1)
+    out, _, weights, tol, tol_w = case.expect_attention(q, 4)
+    for i in range(length):
+        at = (case.table[0, i // 16], 1, i % 16)
+        case.keys[at][3] = encode(np.array(-np.inf), kind)
+        case.values[at][i % dim] = encode(np.array((np.inf, -np.inf, np.nan)[i % 3]), kind)
+    before = case.weights.copy()
+    case.upload()
+    for history in (None, case.history):
+        got, lse = case.attention(q, 4, history=history)
+        assert np.all(got[0, 2:] == 0) and np.all(np.isneginf(lse[0, 2:]))
+        assert np.all(np.abs(got - out)[0, :2] <= tol[0, :2])
+        assert np.all(np.abs(got - out)[1] <= tol[1])
+    grown = case.fetch("weights") - before
+    assert np.all(grown[0, 1] == 0)
+    assert np.all(np.abs(grown - weights)[0, 0, :length] <=
+                  weights[0, 0, :length] * tol_w[0, :2].max() + 2.0 ** -22)
+    pages = np.arange(-(-length // 16))
+    chosen = np.full((2, 2, max(3, len(pages))), -1, np.int32)
+    chosen[0, :, :len(pages)], chosen[1] = pages, np.r_[0:3, [-1] * (chosen.shape[2] - 3)]
+    got, lse = case.attention(q, 4, selected=chosen, top=chosen.shape[2])
+    assert np.all(got[0, 2:] == 0) and np.all(np.isneginf(lse[0, 2:]))
+    assert np.all(np.abs(got - out)[0, :2] <= tol[0, :2])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 64, 16), (3, 3, 128, 32), (34, 2, 24, 9)])
 def test_attention_gathers_weights(gpu, kind, heads, kv, dim, page):
     lengths = [0, 1, 33, 128, 700, 1300]
