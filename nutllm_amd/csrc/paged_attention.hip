@@ -258,8 +258,16 @@ template <int TYPE, int HD> struct Query {
                     x[n][0][e] = __float_as_uint(v[n][e]);
         } else {
             if constexpr (TYPE == NUT_F16) {
+                if (__any(most == INFINITY)) { // the finite ones have to fit limbs all the same
+                    most = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < kParts; n++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            most = fabsf(v[n][e]) < INFINITY ? fmaxf(most, fabsf(v[n][e])) : most;
+                }
                 most = max_over_rows(most);
-                if (most > 0.0f && most < INFINITY)
+                if (most > 0.0f)
                     exponent = ilogbf(most) - 13;
 #pragma unroll
                 for (int n = 0; n < kParts; n++)

@@ -585,6 +585,27 @@ def test_attention_queries_that_are_not_finite(gpu, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [1.0, 1e5, 1e9, 1e30])
+def test_attention_infinite_queries_of_any_size(gpu, kind, size):
+    """An infinite component decides whatever the size of the finite ones."""
+    case = Case(kind, [40, 300], 2, 64, 16, seed=85)
+    rows = decode(case.keys, kind)
+    rows[..., 7] = np.abs(rows[..., 7]) + 0.5
+    case.keys[:] = encode(rows, kind)
+    case.upload()
+    q = query_of(case, 4) * np.float32(size)
+    q[0, 0, 7], q[1, 1, 7], q[0, 3, 7] = -np.inf, -np.inf, np.inf
+    got, lse = case.attention(q, 4)
+    for b, h in ((0, 0), (1, 1)):
+        assert np.all(got[b, h] == 0) and np.isneginf(lse[b, h])
+    assert np.all(np.isnan(got[0, 3]))
+    rest = [(0, 1), (0, 2), (1, 0), (1, 2), (1, 3)]
+    out, _, _, tol, _ = case.expect_attention(np.nan_to_num(q, posinf=0, neginf=0), 4)
+    for b, h in rest:
+        assert np.all(np.abs(got - out)[b, h] <= tol[b, h])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_attention_values_that_are_not_finite(gpu, kind):
     """An infinite or NaN value shows in its component of the KV head's results
     and nowhere else."""
