@@ -20,12 +20,17 @@
 // fp32 rows of 96, 128 components 172, 218 us for 153, 196. Only the running
 // maximum crosses lanes.
 //
-// Products are exact. fp32 rows run on v_mfma_f32_16x16x4f32; 16-bit rows on
-// the 16x16x32 forms, with the fp32 operand (the query, the weights) split
-// into limbs of the rows' type whose sum it is: three bfloat16 limbs (8 bits
-// each, all 24), or two fp16 limbs (22 bits and more, the query scaled by a
-// power of two so that its largest component lies in [2^13, 2^14), weights in
-// [0, 2^14]). Accumulation is fp32.
+// fp32 rows run on v_mfma_f32_16x16x4f32; 16-bit rows on the 16x16x32 forms,
+// with the fp32 operand (the query, the weights) split into limbs of the rows'
+// type, whose products with a row are exact. Three bfloat16 limbs of 8 bits are
+// all 24 bits of it. Two fp16 limbs are 23, a rounding of 2^-23 of a component's
+// size, down to fp16's smallest step: the query is scaled by a power of two so
+// that its largest component lies in [2^13, 2^14), and weights lie in [0, 2^14],
+// so that what is left out of a query's component is at most 2^-38 of the
+// largest one besides, of a weight 2^-39 of the largest. That shows in
+// components 2^15 and more below the largest, and in scores only where a row is
+// near zero in the large ones; a third limb would not reach lower, and cost
+// half as many products again. Accumulation is fp32.
 //
 // HBM bounds long calls: 2.0 GB of fp16 rows (4 sequences of up to 32,768, 32
 // heads of 128) in 304 us, 6.4 TB/s. 32 sequences of up to 2,048 bfloat16 rows

@@ -97,6 +97,37 @@ def test_attention_large_and_small_values(gpu, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("power", [0, 10, 16, 20, 25, 40])
+def test_attention_one_large_query_component(gpu, kind, power):
+    """A component 2^power above the others that the rows do not have, or have
+    in part. An fp16 row's query component is held to 2^-23 of itself and 2^-38
+    of the largest one, its weight to 2^-23 and 2^-39 of the largest: a score
+    errs by scale sum (2^-23 |q_d| + 2^-38 max |q|) |k_d| more, and a result,
+    whose largest weight is 1 before the division by z >= 1, by
+    sum (2^-23 p + 2^-39) |v| / z."""
+    case = Case(kind, [30, 250], 2, 64, 16, seed=87)
+    rows = decode(case.keys, kind)
+    rows[..., 11] = 0.0
+    rows[case.table[1], 1, :, 11] = 2.0 ** -min(power, 14)
+    case.keys[:] = encode(rows, kind)
+    case.upload()
+    q = query_of(case, 4)
+    q[..., 11] = np.float32(2.0 ** power)
+    out, _, _, tol, _ = case.expect_attention(q, 4)
+    if kind == "f16":
+        for b, n in enumerate(case.lengths):
+            for h in range(4):
+                k, v = (np.abs(case.rows(p, b, h // 2)) for p in (case.keys, case.values))
+                size = np.abs(q[b, h].astype(np.float64))
+                ds = (k @ (2.0 ** -23 * size + 2.0 ** -38 * size.max())).max() / 8
+                # both parts of the quotient err by ds of each weight
+                tol[b, h] += (2 * ds + 2.0 ** -23 + n * 2.0 ** -39) * v.max(0)
+    got, _ = case.attention(q, 4)
+    print(f"worst error {(np.abs(got - out) / tol).max():.3f} of its bound", flush=True)
+    assert np.all(np.abs(got - out) <= tol)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_attention_infinite_keys(gpu, kind):
     """Rows whose score is minus infinity weigh nothing, a sequence of such
     rows alone gives zeros; a NaN key shows in its own KV head only."""
