@@ -57,6 +57,7 @@ inline size_t paged_element(int type) { return type == NUT_F32 ? 4 : 2; }
 struct AttentionPlan {
     uint32_t chunk, chunks, tiles;
     uint32_t likely; // rows of the longest sequence that are read, but for pages named twice
+    uint32_t join_threads, weigh_blocks; // of the second launch
     size_t stats, scores; // byte offsets
     size_t bytes;
 };

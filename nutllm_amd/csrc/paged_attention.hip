@@ -871,6 +871,11 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     paged_grid(uint64_t(seqs.batch) * kv.kv_heads * plan.tiles * plan.chunks, 256);
     if (plan.chunks == 1 && !weighted)
         return plan;
+    // a wave joins up to 16 runs of a head
+    plan.join_threads = plan.chunks <= 16 ? 64 : 256;
+    plan.weigh_blocks = weighted ? (seqs.max_length - 1) / (4 * plan.join_threads) + 1 : 0;
+    paged_grid(uint64_t(seqs.batch) * (heads + uint64_t(kv.kv_heads) * plan.weigh_blocks),
+               plan.join_threads);
     const size_t runs = size_t(seqs.batch) * heads * plan.chunks;
     plan.stats = aligned(runs * kv.head_dim * sizeof(float));
     plan.scores = plan.stats + aligned(runs * sizeof(float2));
@@ -897,11 +902,6 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
         a.scores = weighted ? reinterpret_cast<float *>(workspace + plan.scores) : nullptr;
     }
     const dim3 grid(plan.chunks, kv.kv_heads * plan.tiles, seqs.batch);
-    // a wave joins up to 16 runs of a head
-    const uint32_t threads = plan.chunks <= 16 ? 64 : 256;
-    const uint32_t blocks = weighted ? (seqs.max_length + 4 * threads - 1) / (4 * threads) : 0;
-    const uint64_t joins = uint64_t(seqs.batch) * heads;
-    const dim3 join = paged_grid(joins + uint64_t(seqs.batch) * kv.kv_heads * blocks, threads);
     const uint32_t rows = top == 0 ? seqs.max_length : top * kv.page_size;
     const uint64_t bytes = uint64_t(plan.likely) * seqs.batch * kv.kv_heads * kv.head_dim * 2 *
                            paged_element(kv.type);
@@ -914,8 +914,9 @@ void launch_paged_attention(const PagedView &kv, const PagedSeqs &seqs, const fl
     check_launch("paged attention");
     if (!split)
         return;
-    hipLaunchKernelGGL(join_kernel, join, dim3(threads), 0, stream, a, history, uint32_t(joins),
-                       blocks);
+    const uint32_t joins = seqs.batch * heads;
+    hipLaunchKernelGGL(join_kernel, dim3(joins + seqs.batch * kv.kv_heads * plan.weigh_blocks),
+                       dim3(plan.join_threads), 0, stream, a, history, joins, plan.weigh_blocks);
     check_launch("paged attention");
 }
 

@@ -1099,10 +1099,14 @@ static uint32_t most_moved(const PagedSeqs &seqs, uint32_t budget)
     return budget < seqs.max_length ? std::min(budget, seqs.max_length - budget) : 0;
 }
 
+// Workgroups that move the rows of a list.
+static uint32_t move_blocks(uint32_t list) { return (list + 255) / 256; }
+
 size_t evict_workspace(const PagedView &kv, const PagedSeqs &seqs, uint32_t budget)
 {
     const size_t heads = size_t(seqs.batch) * kv.kv_heads;
     paged_grid(heads, 1024);
+    paged_grid(heads * move_blocks(most_moved(seqs, budget)), 256);
     return 2 * aligned(heads * most_moved(seqs, budget) * sizeof(int)) +
            aligned(heads * sizeof(int));
 }
@@ -1125,7 +1129,7 @@ void launch_paged_evict(const PagedView &kv, const PagedSeqs &seqs, const PagedH
     check_launch("paged evict");
     if (list == 0)
         return;
-    const uint32_t blocks = (list + 255) / 256;
+    const uint32_t blocks = move_blocks(list);
     const auto kernel = kv.type == NUT_F32   ? move_rows_kernel<NUT_F32>
                         : kv.type == NUT_F16 ? move_rows_kernel<NUT_F16>
                                              : move_rows_kernel<NUT_BF16>;

@@ -297,3 +297,23 @@ def test_launches_that_one_grid_does_not_cover():
             seqs(table_stride=64, batch=128), 8)
     refused("more rows than one launch covers", paged(kv_heads=1).attention_workspace,
             seqs(table_stride=64, batch=65536), 8)
+
+
+def test_second_launches_that_one_grid_does_not_cover():
+    """The launches behind a call's first are looked at with it, so that nothing
+    runs of a call that is refused, and its workspace is refused too."""
+    # 2^21 heads whose lists of 1,000 to 3,000 moved rows take 4 to 12 workgroups each
+    many = dict(kv_heads=64, head_dim=8, page_size=64, pages=4)
+    s = dict(table_stride=100, batch=1 << 15, max_length=6000)
+    paged(**many).evict_workspace(seqs(**s), 1000)
+    refused("more rows than one launch covers", paged(**many).evict_workspace, seqs(**s), 3000)
+    refused("more rows than one launch covers", evict, paged(**many), seqs(**s), budget=3000,
+            history=history(6000), workspace=At(nbytes=1 << 60), new_lengths=At(1 << 40))
+    # 2^26 query heads of two runs each, joined by a wave a head
+    wide = dict(kv_heads=1, head_dim=8, page_size=64, pages=4)
+    s = dict(table_stride=64, batch=1 << 15, max_length=2049)
+    paged(**wide).attention_workspace(seqs(**s), 1 << 10)
+    refused("more rows than one launch covers", paged(**wide).attention_workspace, seqs(**s),
+            1 << 11)
+    refused("more rows than one launch covers", attention, paged(**wide), seqs(**s), heads=1 << 11,
+            workspace=At(nbytes=1 << 60))
