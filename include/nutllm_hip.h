@@ -278,7 +278,9 @@ typedef struct nut_paged_history {
  * d_new_lengths (may be NULL; apart from d_lengths, d_starts and
  * d_first_positions) gets the lengths with the new rows; max_length is the
  * most that it may say. A sequence that would pass max_length gets no row and
- * keeps its length. No two sequences may append to one page.
+ * keeps its length. Rows for a page outside [0, pages) are reported and
+ * dropped, but counted: new lengths and history are as if they were there. No
+ * two sequences may append to one page.
  *
  * d_first_positions NULL stands for d_lengths: right until nut_paged_evict
  * has cut a sequence. From then on its length is not its next token's place in
@@ -362,8 +364,17 @@ int nut_paged_select(const nut_paged_kv *kv, const nut_paged_batch *seqs,
  * nothing else moves. The bounds of a page that rows move into are widened.
  * d_new_lengths (apart from d_lengths) gets min(length, budget). Positions
  * are distinct and not negative. Pages that hold rows below the budget must
- * not be shared. The workspace (16-byte aligned) needs
- * nut_paged_evict_workspace bytes. */
+ * not be shared. A row does not move from or to a page outside [0, pages); its
+ * weight and position do. The workspace (16-byte aligned) needs
+ * nut_paged_evict_workspace bytes.
+ *
+ * Behind an eviction a sequence's rows do not lie in the order of the text:
+ * the newest are where there were holes, and the `last` pages of
+ * nut_paged_select are the last by place alone. A page's bounds hold for its
+ * rows, and for rows that went too: they become narrower only when an append
+ * begins the page anew. Rows that no attention with history has weighed, such
+ * as a prompt's from nut_paged_append_cache, all have weight 0, of which the
+ * lower ones stay. */
 size_t nut_paged_evict_workspace(const nut_paged_kv *kv,
                                  const nut_paged_batch *seqs, size_t budget);
 int nut_paged_evict(const nut_paged_kv *kv, const nut_paged_batch *seqs,

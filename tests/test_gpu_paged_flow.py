@@ -422,6 +422,47 @@ def test_pages_that_the_cache_has_not(gpu, bad):
         case.paged.check()
 
 
+def test_append_counts_rows_of_a_page_that_the_cache_has_not(gpu):
+    """Rows on it are dropped; the new lengths, weights and positions are as if
+    they were there, rows on the pages beside it arrive, and attention passes
+    the missing ones over."""
+    case = Case("f32", [10, 3], 2, 32, 16, seed=89, max_length=64).upload()
+    k, v = (case.rng.standard_normal((45, 2, 32)).astype(np.float32) for _ in range(2))
+    table = case.table.copy()
+    table[0, 1] = case.pages  # rows 16 to 31
+    case.d["table"].upload(table)
+    missing = case.table[0, 1]
+    before = [getattr(case, name)[missing].copy() for name in ("keys", "values", "bounds")]
+    new = case.expect_append(k, v, [40, 5], firsts=[70, 7])
+    for name, old in zip(("keys", "values", "bounds"), before):
+        getattr(case, name)[missing] = old
+    A = gpu.DeviceArray
+    case.paged.append(case.seqs, A(like=k), A(like=v), case.d["new_lengths"],
+                      starts=A(like=np.array([0, 40, 45], np.int32)), max_new=40,
+                      history=case.history, first_positions=A(like=np.array([70, 7], np.int32)))
+    gpu.synchronize()
+    assert np.array_equal(case.new_lengths(), new)
+    for name in ("weights", "positions", "bounds"):
+        assert same(case.fetch(name), getattr(case, name)), name
+    for name in ("keys", "values"):
+        assert same(case.pool(name), getattr(case, name)), name
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+    case.lengths = new
+    case.d["lengths"].upload(new)
+    q = query_of(case, 4)
+    got, _ = case.attention(q, 4)
+    rows = np.r_[0:16, 32:50]
+    for h in range(4):
+        x, y = (case.rows(p, 0, h // 2)[rows] for p in (case.keys, case.values))
+        s = x @ q[0, h].astype(np.float64) * 32 ** -0.5
+        p = np.exp(s - s.max())
+        # a score errs by (dim + 4) 2^-24 sum |q k|, below 2^-14; both parts by as much
+        assert np.all(np.abs(got[0, h] - (p / p.sum()) @ y) <= 2.0 ** -12 * np.abs(y).max())
+    with pytest.raises(gpu.OutOfRange, match="page out of range"):
+        case.paged.check()
+
+
 def test_lengths_and_counts_out_of_range(gpu):
     """A length below zero or over max_length holds no rows; appends that do
     not fit leave a sequence as it is."""
