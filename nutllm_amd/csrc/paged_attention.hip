@@ -546,9 +546,11 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a)
                         : nullptr;
     Softmax<TYPE, HD> sm;
     __syncthreads();
-    // One tile in registers a wave: the other waves of the SIMD (four and more
-    // up to 64 components) keep loads in flight. A second tile in registers
-    // cost their places: 378 us for 337 where both were measured.
+    // One tile in registers a wave: in long calls the other waves of the SIMD (four
+    // and more up to 64 components) keep loads in flight, and a second tile in
+    // registers cost their places: 378 us for 337 where both were measured. Short
+    // calls have little more than a wave a SIMD (308 workgroups with rows), and
+    // wait for each tile; a second one cost them too (13.2 to 14.4 us).
     Tile<TYPE, HD> x;
     constexpr uint32_t kAll = T::kWide ? 0xffffu : 0xffffffffu;
     const auto masked = [&](int t) {
@@ -848,12 +850,14 @@ AttentionPlan plan_attention(const PagedView &kv, const PagedSeqs &seqs, uint32_
     // without a row are passed over
     const uint32_t likely = plan.likely = std::min(rows, seqs.max_length);
     plan.tiles = (group + 15) / 16;
-    // Runs as long as leave 512 workgroups with rows: of 32 ragged sequences of up
-    // to 2,048 bfloat16 rows, 13.2 us in runs of 512 (512 workgroups), 14.1 in runs
-    // of 256 and 15.6 in runs of 1,024; of 7 of up to 5,001 fp32 rows 19.6 in runs
-    // of 256 (700 workgroups) and of 128, 21.1 in runs of 512. A selection of 124
-    // pages of 128 rows from 1,149 fp32 rows: 33 us by the rows that there are, 64
-    // by the places.
+    // Runs as long as make 512 workgroups, or down to 128 rows, by the longest
+    // length (shorter sequences leave some without rows: 308 of 512 have any in
+    // the first of these): 32 ragged sequences of up to 2,048 bfloat16 rows, four
+    // KV heads, 13.2 us in runs of 512 (512 workgroups), 14.1 in runs of 256 and
+    // 15.6 in runs of 1,024; 7 of up to 5,001 fp32 rows, three KV heads, 19.6 in
+    // runs of 256 (420 workgroups, 252 with rows) and of 128 (840 and 501), 21.1
+    // in runs of 512. A selection of 124 pages of 128 rows from 1,149 fp32 rows:
+    // 33 us by the rows that there are, 64 by the places.
     plan.chunk = kMostRows;
     const uint64_t columns = uint64_t(seqs.batch) * kv.kv_heads * plan.tiles;
     while (likely > 128 && plan.chunk > 128 &&

@@ -588,11 +588,15 @@ __device__ __forceinline__ bool bounded_sums(const float *own, bool valid, const
 // components at a time, max(q, 0) hi and min(q, 0) lo apart. Lane 16 j + c
 // loads components 16 j to 16 j + 15 of page c, whose n-th is the j-th of
 // four in step n; the query comes from shared memory, [sign][component][head].
-// Scores of pages 4 i + j and head c come out as element i of that lane. 32
-// steps of 64 cycles a tile bound it: 50,000 pages of 64 components 10.8 us. A
-// tile with a sum that is no number is summed anew without infinite bounds,
-// which a query of the other sign would make one, and what they add is found
-// from the definition.
+// Scores of pages 4 i + j and head c come out as element i of that lane. 49,140
+// pages of 64 components and 8 heads take 10.9 us, which neither their 12.6 MB
+// (2.0 us) nor their matrix instructions (32 of 64 cycles a tile, 3 tiles a
+// SIMD: 2.7 us of pipe by its counter) bound: all waves are there at once, four
+// to a SIMD, and wait for the length, the bounds and the staged query before
+// any of them multiplies. No bank of shared memory is asked for twice (counter
+// 0). A tile with a sum that is no number is summed anew without infinite
+// bounds, which a query of the other sign would make one, and what they add is
+// found from the definition.
 template <int TYPE>
 __global__ __launch_bounds__(256) void page_scores_mfma_kernel(PagedView kv, PagedSeqs s,
                                                                const float *__restrict__ query,
@@ -901,7 +905,10 @@ __global__ __launch_bounds__(THREADS) void plan_eviction_kernel(PagedView kv, Pa
 // only read, so the order of workgroups does not matter; the bounds of a page
 // whose entries begin in one workgroup's part and end in another's are the
 // first one's. HBM bounds it: 205 MB of rows from anywhere to anywhere in 46 us
-// (4.5 TB/s) where 128 KV heads of up to 8,192 rows keep 2,048.
+// (4.5 TB/s) where 128 KV heads of up to 8,192 rows keep 2,048. With bounds it
+// does not: the threads of a page read its entries, the table and the keys once
+// more, one row after another, and the whole call takes 315 us for 64.5 (16.8
+// for 14.0 where 64 heads are up to 16 rows over 1,024).
 template <int TYPE>
 __global__ __launch_bounds__(256) void move_rows_kernel(PagedView kv, PagedSeqs s,
                                                         PagedHistory history, uint32_t list,
