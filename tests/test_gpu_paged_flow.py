@@ -154,6 +154,140 @@ def test_new_tokens_stay_through_evictions(gpu, prompts):
     case.paged.check()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page,order", [
+    (6, 2, 72, 16, "phs"), (12, 4, 104, 8, "psh"), (5, 5, 200, 32, "hps"), (40, 2, 16, 64, "sph"),
+])
+def test_views_with_room_between(gpu, kind, heads, kv, dim, page, order):
+    """Rows with gaps between them, heads, slots and pages in any order, tables,
+    queries and histories wider than they have to be, a table that two
+    sequences of one length share: append, weigh, select, read and evict, what
+    lies between left as it was."""
+    lengths = [130, 1, 0, 77, 64]
+    case = Case(kind, lengths, kv, dim, page, seed=91, room=3)
+    # element strides, innermost axis last, each with room of 8 to 24 elements
+    count, stride, at = dict(p=case.pages, h=kv, s=page), {}, dim + 8
+    for i, axis in enumerate(reversed([a for a in order if a in count])):
+        stride[axis], at = at, at * count[axis] + 8 * (i + 1)
+    index = (np.arange(case.pages)[:, None, None, None] * stride["p"] +
+             np.arange(kv)[:, None, None] * stride["h"] +
+             np.arange(page)[:, None] * stride["s"] + np.arange(dim))
+    A, flat = gpu.DeviceArray, {}
+    for name in ("keys", "values"):
+        flat[name] = np.full(at, 9, getattr(case, name).dtype)
+        flat[name][index] = getattr(case, name)
+    wide, span = case.width + 3, case.max_length + 5
+    table = np.full((5, wide), -1, np.int32)
+    table[:, :case.width] = case.table
+    weights, positions = np.full((5, kv, span), 5.0, np.float32), np.full((5, kv, span), 6, np.int32)
+    weights[..., :case.max_length], positions[..., :case.max_length] = case.weights, case.positions
+    d = {name: A(like=x) for name, x in flat.items()}
+    d.update(bounds=A(like=case.bounds), table=A(like=table), lengths=A(like=case.lengths),
+             new=A(4 * 5), weights=A(like=weights), positions=A(like=positions),
+             status=A(like=np.zeros(1, np.int32)))
+    paged = gpu.PagedKV(d["keys"], d["values"], case.pages, page, kv, dim,
+                        {"f32": gpu.F32, "f16": gpu.F16, "bf16": gpu.BF16}[kind],
+                        strides=tuple(stride[a] for a in "phs"), bounds=d["bounds"],
+                        status=d["status"])
+    before, after = (gpu.PagedBatch(d["table"], wide, d[n], 5, case.max_length)
+                     for n in ("lengths", "new"))
+    history = gpu.PagedHistory(d["weights"], d["positions"], span)
+
+    def compare():
+        gpu.synchronize()
+        for name in ("keys", "values"):
+            flat[name][index] = getattr(case, name)
+            assert same(d[name].download(flat[name].dtype, at), flat[name]), name
+        assert same(d["bounds"].download(case.bounds.dtype, case.bounds.size),
+                    case.bounds.reshape(-1))
+        for name, want in (("weights", weights), ("positions", positions)):
+            want[..., :case.max_length] = getattr(case, name)
+            assert same(d[name].download(want.dtype, want.size).reshape(want.shape), want), name
+
+    rows, counts, firsts = 8, [1, 3, 0, 2, 2], np.array([400, 1, 0, 77, 90], np.int32)
+    k, v = (case.rng.standard_normal((rows, kv, dim)).astype(np.float32) for _ in range(2))
+    starts = A(like=np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+    case.lengths = case.expect_append(k, v, counts, firsts=firsts)
+    paged.append(before, A(like=k), A(like=v), d["new"], starts=starts, max_new=3, history=history,
+                 first_positions=A(like=firsts))
+    compare()
+    room = heads * dim + 12
+    query = np.full((5, room), np.nan, np.float32)
+    query[:, :heads * dim] = query_of(case, heads).reshape(5, -1)
+    q, out, space = A(like=query), A(4 * 5 * heads * dim), A(1 << 22)
+    q64 = query[:, :heads * dim].reshape(5, heads, dim)
+
+    def result():
+        gpu.synchronize()
+        return out.download(np.float32, 5 * heads * dim).reshape(5, heads, dim)
+
+    assert paged.attention_workspace(after, heads, weighted=True) <= space.nbytes
+    paged.attention(after, q, out, heads, query_stride=room, history=history, workspace=space)
+    grown = near(case, heads, q64, result())
+    got = d["weights"].download(np.float32, weights.size).reshape(weights.shape)
+    assert np.allclose(got[..., :case.max_length], case.weights + grown, rtol=1e-4, atol=1e-6)
+    case.weights = got[..., :case.max_length].copy()
+    top, chosen = 3, A(4 * 5 * kv * 3)
+    paged.select(after, q, chosen, heads, top, query_stride=room, workspace=space)
+    want = case.expect_select(q64, heads, top, 1, 1)
+    gpu.synchronize()
+    assert np.array_equal(chosen.download(np.int32, want.size).reshape(want.shape), want)
+    paged.attention(after, q, out, heads, query_stride=room, selected=chosen, top=top,
+                    workspace=space)
+    near(case, heads, q64, result(), selected=want)
+    case.lengths = case.expect_evict(70, 2, 9)
+    paged.evict(after, history, d["lengths"], 70, first=2, last=9, workspace=space)
+    compare()
+    assert np.array_equal(d["lengths"].download(np.int32, 5), case.lengths)
+    paged.attention(before, q, out, heads, query_stride=room, workspace=space)
+    near(case, heads, q64, result())
+    # sequences that share pages which are only read
+    table[1:] = table[0]
+    d["table"].upload(table)
+    case.table = np.tile(case.table[:1], (5, 1))
+    case.lengths = np.array([70, 70, 30, 1, 0], np.int32)
+    d["lengths"].upload(case.lengths)
+    paged.attention(before, q, out, heads, query_stride=room, workspace=space)
+    near(case, heads, q64, result())
+    paged.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_many_short_sequences(gpu, kind):
+    """A batch of 40,000 sequences, most of them of a row or none."""
+    batch = 40000
+    lengths = np.zeros(batch, np.int32)
+    lengths[::37], lengths[5::1001], lengths[-1] = 1, 19, 19
+    case = Case(kind, lengths[-1:], 1, 16, 8, seed=93, max_length=20)
+    width, A = 3, gpu.DeviceArray
+    # every sequence over the same three pages, which are only read
+    seqs_table, d_lengths = A(like=np.tile(case.table, (batch, 1))), A(like=lengths)
+    case.upload()
+    seqs = gpu.PagedBatch(seqs_table, width, d_lengths, batch, 20)
+    q = np.random.default_rng(4).standard_normal((batch, 2, 16)).astype(np.float32)
+    dq, out, lse = A(like=q), A(q.nbytes), A(4 * batch * 2)
+    chosen, space = A(4 * batch * 2), A(1 << 22)
+    assert max(case.paged.attention_workspace(seqs, 2), case.paged.select_workspace(seqs, 2, 2)) \
+        <= space.nbytes
+    case.paged.attention(seqs, dq, out, 2, lse=lse, workspace=space)
+    case.paged.select(seqs, dq, chosen, 2, 2, first=0, last=0, workspace=space)
+    gpu.synchronize()
+    got = out.download(np.float32, q.size).reshape(q.shape)
+    none = lengths == 0
+    assert np.all(got[none] == 0)
+    assert np.all(np.isneginf(lse.download(np.float32, 2 * batch).reshape(batch, 2)[none]))
+    value = case.rows(case.values, 0, 0)[0]
+    # one row: its weight is 1, and 1 / 1
+    assert np.all(np.abs(got[lengths == 1] - value) <= 2.0 ** -22 * np.abs(value))
+    pages = chosen.download(np.int32, 2 * batch).reshape(batch, 2)
+    assert np.all(pages[none] == -1) and np.all(pages[lengths == 1] == [0, -1])
+    for b in np.flatnonzero(lengths == 19):
+        one = Case(kind, [19], 1, 16, 8, seed=93, max_length=20)
+        near(one, 2, q[b:b + 1], got[b:b + 1])
+        assert np.array_equal(pages[b:b + 1, None], one.expect_select(q[b:b + 1], 2, 2, 0, 0))
+    case.paged.check()
+
+
 def test_captured_step(gpu):
     """A decode step (append, weighted attention, selection, attention over
     it, eviction) in two graphs with workspaces of their own, replayed in turn
