@@ -563,9 +563,9 @@ class PagedKV:
         """nut_paged_append: fp32 rows [rows][kv_heads][head_dim] behind the
         sequences, rows starts[b] to starts[b + 1] for sequence b (one each
         without starts). row_stride and head_stride, in elements, are packed
-        ones where they are 0, each on its own. With history, first_positions holds the place in the
-        text of each sequence's first new row (None: the lengths, right only
-        for sequences that evict has not cut)."""
+        ones where they are 0, each on its own. With history, first_positions
+        holds the place in the text of each sequence's first new row (None:
+        the lengths, right only for sequences that evict has not cut)."""
         row = row_stride or self.kv_heads * self.head_dim or 1
         used = (self.kv_heads - 1) * (head_stride or self.head_dim) + self.head_dim
         held = min(keys.nbytes, values.nbytes) // 4
