@@ -384,8 +384,212 @@ int nut_paged_evict(const nut_paged_kv *kv, const nut_paged_batch *seqs,
 
 /* Waits for the device, then raises what the view's status word holds
  * (NUT_EOUTOFRANGE: "paged cache: page out of range", "paged cache: length
- * out of range", "paged cache: rows out of range") and clears it. */
+ * out of range", "paged cache: rows out of range", "draft tree: parent out of
+ * range", "page pool: parent out of range", "page pool: out of pages") and
+ * clears it. */
 int nut_paged_check(const nut_paged_kv *kv);
+/* The same of a status word that several views share. */
+int nut_status_check(int *d_status);
+
+/* -------------------------------------------------------- draft trees -- */
+
+/* Tokens that a draft proposes behind each sequence, as a tree: node i of
+ * sequence b is row d_starts[b] + i of the arrays [total] (d_starts NULL:
+ * `most` nodes each, total = batch most), its parent the node d_parents[..],
+ * a number below i within the sequence's own tree, -1 for none. Node 0 is
+ * the token that the sequence goes on with for certain; the others are
+ * guesses. At most `most` (up to 1,024) nodes a sequence; one may have none.
+ * Starts that this does not hold for are reported, and the sequence taken to
+ * have no nodes. The nodes' keys and values are the rows behind the rows
+ * that the sequence holds, where nut_paged_append with these starts puts
+ * them. Rows of `total` that no sequence names are left as they are. */
+typedef struct nut_draft {
+    const int *d_starts;
+    size_t total, most, batch;
+    const int *d_parents; /* read by nut_draft_mask and nut_draft_accept */
+    /* [total][mask_stride] words: bit j % 32 of word j / 32 of node i: i
+     * sees node j. nut_draft_mask writes the tree's; nut_paged_tree_attention
+     * follows any. mask_stride >= ceil(most / 32). */
+    unsigned *d_mask;
+    size_t mask_stride;
+    int *d_status; /* as a nut_paged_kv's, and it may be the same word */
+} nut_draft;
+
+/* Each node's mask, itself and its ancestors (words below ceil(most / 32)),
+ * and its depth (d_depths may be NULL), 0 for a node without a parent: its
+ * place in the text is the sequence's next one plus the depth. A parent that
+ * is not below its node is reported and taken for none. */
+int nut_draft_mask(const nut_draft *draft, int *d_depths, void *stream);
+
+/* Attention of every node over its sequence's rows and the nodes that its
+ * mask names: head h of `heads` of node i (query row at d_query +
+ * (d_starts[b] + i) query_stride, 0: packed; a multiple of 4) reads the
+ * d_lengths[b] rows that the sequence holds and those of the rows behind them
+ * whose bit is set; d_out [total][heads][head_dim], d_lse [total][heads] (may
+ * be NULL), as nut_paged_attention. max_length bounds rows and nodes together.
+ * What a node does not see has no part in its result, infinite or not a
+ * number though it be. A node that sees no row, and every node of a sequence
+ * whose length is out of range, gets zeros and minus infinity. */
+size_t nut_paged_tree_attention_workspace(const nut_paged_kv *kv,
+                                          const nut_paged_batch *seqs,
+                                          const nut_draft *draft,
+                                          size_t heads);
+int nut_paged_tree_attention(const nut_paged_kv *kv,
+                             const nut_paged_batch *seqs,
+                             const nut_draft *draft, const float *d_query,
+                             size_t query_stride, size_t heads, float scale,
+                             float *d_out, float *d_lse, void *d_workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* The path of a tree that the model agrees with: node 0, then of each kept
+ * node the lowest child whose token (d_tokens [total]) is the one that the
+ * model chose behind that node (d_chosen [total]), as long as there is one.
+ * d_path [batch][path_stride] (path_stride >= most) gets the path's nodes, in
+ * ascending order; entries behind it stay. d_counts [batch] gets their number,
+ * 0 for a sequence without nodes, d_last [batch] (may be NULL; left where the
+ * count is 0) the model's choice behind the last of them, with which the next
+ * tree begins, and d_new_lengths [batch] (may be NULL; apart from d_lengths)
+ * the lengths with the path's rows. A sequence whose rows and nodes pass
+ * max_length is reported and keeps none. */
+int nut_draft_accept(const nut_draft *draft, const nut_paged_batch *seqs,
+                     const int *d_tokens, const int *d_chosen, int *d_path,
+                     size_t path_stride, int *d_counts, int *d_last,
+                     int *d_new_lengths, void *stream);
+
+/* Keeps the path's rows, in every layer at once: row d_lengths[b] +
+ * d_path[b path_stride + k] moves to row d_lengths[b] + k, for k below
+ * d_counts[b] (at most path_stride). The bounds of a page that rows move
+ * into are widened. Path entries ascend; from one on that does not, or whose
+ * row is not below max_length, the path is reported and not followed. Rows
+ * from or to a page outside [0, pages) do not move. Weights and positions of
+ * a nut_paged_history stay right as nut_paged_append left them: the k-th node
+ * of a path is the k-th new token. The layers are views of one shape, 64 to a
+ * launch; pages that the rows lie in must not be shared. */
+int nut_paged_keep(const nut_paged_kv *layers, size_t count,
+                   const nut_paged_batch *seqs, const int *d_path,
+                   size_t path_stride, const int *d_counts, void *stream);
+
+/* --------------------------------------------------------- page pools -- */
+
+/* Who holds the pages that a cache's layers have in common: d_refs[p] counts
+ * the table entries that name page p, and a page of 0 is free. The caller
+ * zeroes the counts once; from then on the calls below keep them. */
+typedef struct nut_page_pool {
+    int *d_refs; /* [pages] */
+    size_t pages, page_size;
+    int *d_status; /* as a nut_paged_kv's, and it may be the same word */
+} nut_page_pool;
+
+/* Sequences and the pages that they hold: sequence b holds d_lengths[b] rows
+ * and the first d_held[b] entries of its row of d_pages [batch][stride],
+ * ceil(length / page_size) of them or, ahead of rows to come, more. A
+ * nut_paged_batch views the same table and lengths. */
+typedef struct nut_page_table {
+    int *d_pages;
+    size_t stride;
+    int *d_lengths, *d_held; /* [batch] */
+    size_t batch;
+} nut_page_table;
+
+/* From one table to the next: sequence i of `to` goes on with sequence
+ * d_parents[i] of `from`, as long as that is, or is new and empty (-1), and
+ * gets pages for d_gains[i] (`gain` each where d_gains is NULL) rows more.
+ * This forks a sequence (several with one parent), drops it (none), admits
+ * one (-1), lets it grow (itself) and gives back what it holds ahead, all of
+ * it in one call that covers every sequence of `from`.
+ *
+ * Pages full of rows are shared. The page that the next row goes to, and
+ * pages held ahead, stay with the parent's first continuation as far as it
+ * needs them, unless something else holds them; every other one gets a fresh
+ * page, and d_copies [to.batch][3] the copy to be made in every layer
+ * ({page, fresh page, rows}, {-1, -1, -1} for none; nut_paged_copy). So no two
+ * sequences ever append to one page. Fresh pages are the lowest that were free
+ * before the call, handed out in order; where none is left the entry is -1,
+ * which is reported. Pages that nothing holds any more are free from the next
+ * call on. Entries of `to` behind d_held stay.
+ *
+ * `to` shares no memory with `from`. A parent outside `from`, a sequence
+ * whose length its pages or `to` do not hold, is reported, and what goes on
+ * with it is empty and holds nothing; a gain that is negative or too large is
+ * reported and taken for 0. Sequences that hold more than their table's row
+ * are reported and give nothing back. The workspace (16-byte aligned) needs
+ * nut_pages_reorder_workspace bytes. */
+size_t nut_pages_reorder_workspace(const nut_page_pool *pool,
+                                   const nut_page_table *from,
+                                   const nut_page_table *to);
+int nut_pages_reorder(const nut_page_pool *pool, const nut_page_table *from,
+                      const nut_page_table *to, const int *d_parents,
+                      const int *d_gains, size_t gain, int *d_copies,
+                      void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* Moves pages out of the upper part of a cache: the k-th lowest page from
+ * `limit` on that the table alone holds becomes the k-th lowest free page
+ * below it, for as many as there are of both, and `copies` at most. The table
+ * and the counts follow, and d_copies [copies][3] gets the copies to be made
+ * in every layer, whole pages, then {-1, -1, -1}. A page that something else
+ * holds too stays. The workspace (16-byte aligned) needs
+ * nut_pages_compact_workspace bytes. */
+size_t nut_pages_compact_workspace(const nut_page_pool *pool,
+                                   const nut_page_table *table);
+int nut_pages_compact(const nut_page_pool *pool, const nut_page_table *table,
+                      size_t limit, int *d_copies, size_t copies,
+                      void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* Copies pages in every layer at once: of each {from, to, rows} of d_copies
+ * [copies][3] the first `rows` rows of page `from` of every KV head, keys and
+ * values, and the page's bounds, to page `to`. Negative `from`: none. A page
+ * outside [0, pages), or more rows than a page has, is reported and not
+ * copied. No page is copied to twice, or copied to and from. The layers are
+ * views of one shape, 64 to a launch. */
+int nut_paged_copy(const nut_paged_kv *layers, size_t count,
+                   const int *d_copies, size_t copies, void *stream);
+
+/* -------------------------------------------------------- beam search -- */
+
+/* Beams of several requests, [requests][beams] each: the sum of a beam's
+ * log-probabilities (minus infinity: no beam), its tokens, and whether it has
+ * ended (not 0). d_lengths and d_ended may be NULL. */
+typedef struct nut_beams {
+    float *d_scores;
+    int *d_lengths, *d_ended;
+    size_t requests, beams; /* beams up to 64 */
+} nut_beams;
+
+/* One step of beam search: of each request's candidates, beam i of `from`
+ * with token v, scored s = score_i + logit_iv - log sum_w exp(logit_iw), the
+ * to.beams best, best first, become the beams of `to`. A beam that has ended
+ * has one candidate, token `eos` with the score as it is. Candidates rank by
+ * s / max(1, length)^power, length counting the new token (power 0: by s, and
+ * lengths may be NULL); of equal ranks by the lower beam, then the larger
+ * logit, then the lower token. Candidates of minus infinity, or of a score
+ * that is not a number, are none; where fewer than to.beams are left, parent
+ * and token are -1, the score minus infinity, the length 0 and the beam ended
+ * as little as one can be (0).
+ *
+ * Beam i's logits are [vocab] elements of `type` (vocab up to 262,144) at
+ * element (request beams + i) row_stride (0: vocab). d_parents and d_tokens
+ * are [requests][to.beams]; a parent is numbered over all requests, as
+ * nut_pages_reorder and nut_beam_gather take it. A beam that chooses `eos`
+ * (-1: none) has ended, where the states keep that; both do or neither, and
+ * likewise lengths. Exponentials are 32-bit, sums and ranks 64. The workspace
+ * (16-byte aligned) needs nut_beam_select_workspace bytes. */
+size_t nut_beam_select_workspace(const nut_beams *from, const nut_beams *to,
+                                 size_t vocab);
+int nut_beam_select(const nut_beams *from, const nut_beams *to,
+                    const void *d_logits, int type, size_t row_stride,
+                    size_t vocab, int eos, float power, int *d_parents,
+                    int *d_tokens, void *d_workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* State that goes with beams or sequences (texts, a nut_paged_history): row i
+ * of `rows` rows at d_to + i to_stride gets the row_bytes bytes of the source
+ * row d_parents[i], of `sources`, from d_from on (strides in bytes, 0:
+ * row_bytes; all multiples of 4, rows apart). A row without a parent (-1)
+ * stays; one outside [0, sources) is reported in d_status (may be NULL). */
+int nut_beam_gather(const void *d_from, size_t from_stride, size_t sources,
+                    void *d_to, size_t to_stride, size_t rows,
+                    size_t row_bytes, const int *d_parents, int *d_status,
+                    void *stream);
 
 /* -------------------------------------------------------- token loop -- */
 

@@ -173,6 +173,24 @@ _SIGS = {
     "nut_paged_evict": (C.c_int, [_P, _P, _P, _SZ, _SZ, _SZ, _P, _P, _SZ,
                                   _P]),
     "nut_paged_check": (C.c_int, [_P]),
+    "nut_status_check": (C.c_int, [_P]),
+    "nut_draft_mask": (C.c_int, [_P, _P, _P]),
+    "nut_draft_accept": (C.c_int, [_P, _P, _P, _P, _P, _SZ, _P, _P, _P, _P]),
+    "nut_paged_tree_attention_workspace": (_SZ, [_P, _P, _P, _SZ]),
+    "nut_paged_tree_attention": (C.c_int, [_P, _P, _P, _P, _SZ, _SZ,
+                                           C.c_float, _P, _P, _P, _SZ, _P]),
+    "nut_paged_keep": (C.c_int, [_P, _SZ, _P, _P, _SZ, _P, _P]),
+    "nut_pages_reorder_workspace": (_SZ, [_P, _P, _P]),
+    "nut_pages_reorder": (C.c_int, [_P, _P, _P, _P, _P, _SZ, _P, _P, _SZ,
+                                    _P]),
+    "nut_pages_compact_workspace": (_SZ, [_P, _P]),
+    "nut_pages_compact": (C.c_int, [_P, _P, _SZ, _P, _SZ, _P, _SZ, _P]),
+    "nut_paged_copy": (C.c_int, [_P, _SZ, _P, _SZ, _P]),
+    "nut_beam_select_workspace": (_SZ, [_P, _P, _SZ]),
+    "nut_beam_select": (C.c_int, [_P, _P, _P, C.c_int, _SZ, _SZ, C.c_int,
+                                  C.c_float, _P, _P, _P, _SZ, _P]),
+    "nut_beam_gather": (C.c_int, [_P, _SZ, _SZ, _P, _SZ, _SZ, _SZ, _P, _P,
+                                  _P]),
 }
 
 
@@ -628,10 +646,188 @@ class PagedKV:
             _raw(new_lengths), _raw(workspace),
             0 if workspace is None else workspace.nbytes, stream))
 
+    def tree_attention_workspace(self, seqs, draft, heads):
+        return _bytes(lib().nut_paged_tree_attention_workspace(
+            self.ref, seqs.ref, draft.ref, heads))
+
+    def tree_attention(self, seqs, draft, query, out, heads, *, scale=None,
+                       query_stride=0, lse=None, workspace=None, stream=None):
+        """nut_paged_tree_attention: attention of every node of a DraftTree
+        over its sequence's rows and the nodes that its mask names, fp32 query
+        and out [total][heads][head_dim]."""
+        check(lib().nut_paged_tree_attention(
+            self.ref, seqs.ref, draft.ref, _raw(query), query_stride, heads,
+            self._scale if scale is None else scale, _raw(out), _raw(lse),
+            _raw(workspace), 0 if workspace is None else workspace.nbytes,
+            stream))
+
     def check(self):
         """nut_paged_check: waits, then raises OutOfRange for a page, length
         or row that an earlier call could not follow."""
         check(lib().nut_paged_check(self.ref))
+
+
+def check_status(status):
+    """nut_status_check: waits, then raises OutOfRange for what earlier calls
+    with this status word could not follow."""
+    check(lib().nut_status_check(_raw(status)))
+
+
+class _Draft(C.Structure):
+    _fields_ = [("d_starts", _P), ("total", _SZ), ("most", _SZ),
+                ("batch", _SZ), ("d_parents", _P), ("d_mask", _P),
+                ("mask_stride", _SZ), ("d_status", _P)]
+
+
+class _PagePool(C.Structure):
+    _fields_ = [("d_refs", _P), ("pages", _SZ), ("page_size", _SZ),
+                ("d_status", _P)]
+
+
+class _PageTable(C.Structure):
+    _fields_ = [("d_pages", _P), ("stride", _SZ), ("d_lengths", _P),
+                ("d_held", _P), ("batch", _SZ)]
+
+
+class _Beams(C.Structure):
+    _fields_ = [("d_scores", _P), ("d_lengths", _P), ("d_ended", _P),
+                ("requests", _SZ), ("beams", _SZ)]
+
+
+class DraftTree:
+    """Drafted tokens behind each sequence, as trees (nut_draft): int32
+    parents [total] and masks [total][mask_stride] (0: ceil(most / 32)) of at
+    most `most` nodes a sequence, nodes starts[b] to starts[b + 1] for
+    sequence b (`most` each without starts)."""
+
+    def __init__(self, parents, mask, most, total, batch, *, starts=None,
+                 mask_stride=0, status=None):
+        self._keep = (parents, mask, starts, status)
+        self.most, self.total, self.batch = int(most), int(total), int(batch)
+        self.view = _Draft(_raw(starts), total, most, batch, _raw(parents),
+                           _raw(mask), mask_stride or (self.most + 31) // 32,
+                           _raw(status))
+        self.ref = C.addressof(self.view)
+
+    def build(self, *, depths=None, stream=None):
+        """nut_draft_mask: every node's mask, itself and its ancestors, and
+        its depth, int32 [total]."""
+        check(lib().nut_draft_mask(self.ref, _raw(depths), stream))
+
+    def accept(self, seqs, tokens, chosen, path, counts, *, path_stride=0,
+               last=None, new_lengths=None, stream=None):
+        """nut_draft_accept: the nodes that the model agrees with, int32 path
+        [batch][path_stride] (0: most) and counts [batch], from the nodes'
+        tokens and the model's choices behind them, int32 [total]."""
+        check(lib().nut_draft_accept(
+            self.ref, seqs.ref, _raw(tokens), _raw(chosen), _raw(path),
+            path_stride or self.most, _raw(counts), _raw(last),
+            _raw(new_lengths), stream))
+
+
+class PagedLayers:
+    """The PagedKV views of a cache's layers, all of one shape: what one call
+    does in every layer."""
+
+    def __init__(self, layers):
+        self._keep = tuple(layers)
+        self.views = (_PagedKV * len(self._keep))(*(l.view for l in self._keep))
+        self.ref = C.addressof(self.views)
+
+    def keep(self, seqs, path, path_stride, counts, *, stream=None):
+        """nut_paged_keep: the rows of accepted nodes, path [batch][path_stride]
+        and counts [batch], move behind their sequences' rows."""
+        check(lib().nut_paged_keep(self.ref, len(self._keep), seqs.ref,
+                                   _raw(path), path_stride, _raw(counts),
+                                   stream))
+
+    def copy(self, copies, count, *, stream=None):
+        """nut_paged_copy: the first `rows` rows of pages, int32 copies
+        [count][3] of (from, to, rows)."""
+        check(lib().nut_paged_copy(self.ref, len(self._keep), _raw(copies),
+                                   count, stream))
+
+
+class PageTable:
+    """Sequences and the pages that they hold (nut_page_table): int32 device
+    buffers pages [batch][stride], lengths [batch] and held [batch]."""
+
+    def __init__(self, pages, stride, lengths, held, batch):
+        self._keep = (pages, lengths, held)
+        self.batch, self.stride = int(batch), int(stride)
+        self.view = _PageTable(_raw(pages), stride, _raw(lengths), _raw(held),
+                               batch)
+        self.ref = C.addressof(self.view)
+
+
+class PagePool:
+    """Who holds a cache's pages (nut_page_pool): int32 counts refs [pages], 0
+    for a free page, zeroed by the caller once."""
+
+    def __init__(self, refs, pages, page_size, status=None):
+        self._keep = (refs, status)
+        self.view = _PagePool(_raw(refs), pages, page_size, _raw(status))
+        self.ref = C.addressof(self.view)
+
+    def reorder_workspace(self, old, new):
+        return _bytes(lib().nut_pages_reorder_workspace(self.ref, old.ref,
+                                                        new.ref))
+
+    def reorder(self, old, new, parents, copies, *, gains=None, gain=0,
+                workspace=None, stream=None):
+        """nut_pages_reorder: sequence i of the table `new` goes on with
+        sequence parents[i] of `old` (-1: none) and gets pages for gains[i]
+        (or `gain`) more rows; copies [new.batch][3] for PagedLayers.copy."""
+        check(lib().nut_pages_reorder(
+            self.ref, old.ref, new.ref, _raw(parents), _raw(gains), gain,
+            _raw(copies), _raw(workspace),
+            0 if workspace is None else workspace.nbytes, stream))
+
+    def compact_workspace(self, table):
+        return _bytes(lib().nut_pages_compact_workspace(self.ref, table.ref))
+
+    def compact(self, table, limit, copies, count, *, workspace=None,
+                stream=None):
+        """nut_pages_compact: pages from `limit` on move to free ones below it;
+        copies [count][3] for PagedLayers.copy."""
+        check(lib().nut_pages_compact(
+            self.ref, table.ref, limit, _raw(copies), count, _raw(workspace),
+            0 if workspace is None else workspace.nbytes, stream))
+
+
+class BeamState:
+    """Beams of several requests (nut_beams): fp32 scores, int32 lengths and
+    ended, device buffers [requests][beams]."""
+
+    def __init__(self, scores, requests, beams, *, lengths=None, ended=None):
+        self._keep = (scores, lengths, ended)
+        self.requests, self.beams = int(requests), int(beams)
+        self.view = _Beams(_raw(scores), _raw(lengths), _raw(ended), requests,
+                           beams)
+        self.ref = C.addressof(self.view)
+
+
+def beam_select_workspace(old, new, vocab):
+    return _bytes(lib().nut_beam_select_workspace(old.ref, new.ref, vocab))
+
+
+def beam_select(old, new, logits, vocab, parents, tokens, *, dtype=F32,
+                row_stride=0, eos=-1, power=0.0, workspace=None, stream=None):
+    """nut_beam_select: the new.beams best continuations of each request's
+    beams by logits [requests][old.beams][vocab]; parents (numbered over all
+    requests) and tokens, int32 [requests][new.beams]."""
+    check(lib().nut_beam_select(
+        old.ref, new.ref, _raw(logits), dtype, row_stride, vocab, eos, power,
+        _raw(parents), _raw(tokens), _raw(workspace),
+        0 if workspace is None else workspace.nbytes, stream))
+
+
+def beam_gather(source, to, row_bytes, parents, *, rows, sources,
+                from_stride=0, to_stride=0, status=None, stream=None):
+    """nut_beam_gather: row i of `to` gets row parents[i] of `source`."""
+    check(lib().nut_beam_gather(_raw(source), from_stride, sources, _raw(to),
+                                to_stride, rows, row_bytes, _raw(parents),
+                                _raw(status), stream))
 
 
 class DeviceModel:

@@ -1,0 +1,387 @@
+// beam.hip — beam search: the best continuations of every request's beams, and
+// the state that goes with them.
+//
+// Two launches. In the first a wave takes a part of a beam's logits into
+// registers: their largest, the sum of their exponentials, and the K largest in
+// order. In the second a workgroup per request joins a beam's parts to its K
+// best tokens and its log-sum, and then the beams to the request's K best. Only
+// the logits' order matters within a beam, so that ranks are worked out for K
+// candidates a beam, in 64 bits.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "device.hpp"
+#include "paged_device.hpp"
+#include "runtime.hpp"
+#include "serving.hpp"
+
+namespace nut {
+
+namespace {
+
+constexpr uint32_t kMostParts = 64;   // of a beam's logits: a lane each
+constexpr uint32_t kMostListed = 2112; // keys of a beam's parts: 33 parts of 64
+
+struct Part {
+    float most; // minus infinity: no finite one
+    uint32_t unused;
+    double sum; // of exp(logit - most); not a number after one that is none
+};
+
+struct BeamArgs {
+    BeamsView from, to;
+    const void *logits;
+    size_t row_stride;
+    uint32_t vocab, parts;
+    int eos;
+    float power;
+    int *parents, *tokens;
+    Part *stats;    // [requests][beams][parts]
+    uint64_t *best; // [requests][beams][parts][to.beams]: keys in descending order, then 0
+};
+
+// An order of 64-bit keys: the larger logit, then the lower token. 0: none.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t token)
+{
+    const uint32_t u = __float_as_uint(v + 0.0f); // -0 is 0
+    const uint32_t order = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return uint64_t(order) << 32 | uint32_t(~token);
+}
+__device__ __forceinline__ float logit_of(uint64_t key)
+{
+    const uint32_t order = uint32_t(key >> 32);
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~uint32_t(key); }
+
+// Ranks as keys in the same order; 0 for minus infinity and what is no number.
+__device__ __forceinline__ uint64_t rank_key(double v)
+{
+    if (!(v > -INFINITY))
+        return 0;
+    const uint64_t u = uint64_t(__double_as_longlong(v + 0.0));
+    return u >> 63 ? ~u : u | (uint64_t(1) << 63);
+}
+
+__device__ __forceinline__ uint64_t wave_most(uint64_t v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t x = uint64_t(__shfl_xor((unsigned long long)v, o));
+        v = x > v ? x : v;
+    }
+    return v;
+}
+
+// exp(d), d <= 0: the exponent in base 2 in two pieces, so that the error is
+// that of the instruction, a unit in the last place, however large d is.
+__device__ __forceinline__ float exp_below(float d)
+{
+    const float t = d * 1.44269504f;
+    const float rest = fmaf(d, 1.44269504f, -t) + d * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, rest * 0.69314718f, e);
+}
+
+// EACH logits a lane, in runs of 16 bytes: run r of the wave's part is lane r % 64's.
+template <int TYPE, int EACH>
+__global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
+{
+    constexpr int kRun = TYPE == NUT_F32 ? 4 : 8, kRuns = EACH / kRun;
+    constexpr uint32_t kPart = kWave * EACH;
+    const uint32_t lane = threadIdx.x, part = blockIdx.x, row = blockIdx.y + gridDim.y * blockIdx.z;
+    if (row >= a.from.requests * a.from.beams)
+        return;
+    if (!(a.from.scores[row] > -INFINITY) || (a.from.ended != nullptr && a.from.ended[row] != 0))
+        return; // no beam, or one that needs no logits
+    constexpr int kSize = TYPE == NUT_F32 ? 4 : 2;
+    const char *logits = static_cast<const char *>(a.logits) + row * a.row_stride * kSize;
+    // runs at multiples of 16 bytes: the first may begin before the row
+    const uint32_t lead = uint32_t(reinterpret_cast<uintptr_t>(logits) % 16 / kSize);
+    float v[EACH];
+#pragma unroll
+    for (int r = 0; r < kRuns; r++) {
+        const int64_t at = int64_t(part) * kPart + (r * kWave + lane) * kRun - lead;
+        if (at >= 0 && at + kRun <= int64_t(a.vocab)) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(logits + at * kSize);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < kRun; e++)
+                v[r * kRun + e] = TYPE == NUT_F32 ? __uint_as_float(w[e % 4])
+                                  : TYPE == NUT_BF16
+                                      ? from_bf16(w[e / 2 % 4] >> (e % 2 * 16) & 0xffffu)
+                                      : from_f16(w[e / 2 % 4] >> (e % 2 * 16) & 0xffffu);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kRun; e++) {
+                float x = -INFINITY;
+                if (at + e >= 0 && at + e < int64_t(a.vocab)) {
+                    const char *p = logits + (at + e) * kSize;
+                    x = TYPE == NUT_F32    ? *reinterpret_cast<const float *>(p)
+                        : TYPE == NUT_BF16 ? from_bf16(*reinterpret_cast<const uint16_t *>(p))
+                                           : from_f16(*reinterpret_cast<const uint16_t *>(p));
+                }
+                v[r * kRun + e] = x;
+            }
+        }
+    }
+    float most = v[0];
+#pragma unroll
+    for (int e = 1; e < EACH; e++)
+        most = fmaxf(most, v[e]);
+    const float top = wave_max(most);
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        // all of the part minus infinity: no sum, but for what is no number
+        const float d = top == -INFINITY && v[e] == -INFINITY ? -INFINITY : v[e] - top;
+        sum += double(exp_below(d < -200.0f ? -200.0f : d)); // that is 0 in 32 bits
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        sum += __shfl_xor(sum, o);
+    const size_t slot = size_t(row) * a.parts + part;
+    if (lane == 0)
+        a.stats[slot] = Part{top, 0, sum};
+
+    // The keep largest, one after another: each lane's largest left, and the wave's.
+    const uint32_t keep = a.to.beams;
+    uint64_t mine = 0;
+    const auto largest_below = [&](uint64_t bound) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int64_t at = int64_t(part) * kPart + (e / kRun * kWave + lane) * kRun + e % kRun -
+                               lead;
+            const uint64_t key = key_of(v[e], uint32_t(at));
+            if (at >= 0 && at < int64_t(a.vocab) && key < bound && key > best)
+                best = key;
+        }
+        return best;
+    };
+    mine = largest_below(~uint64_t(0));
+    uint64_t kept = 0; // the lane-th largest
+    for (uint32_t k = 0; k < keep; k++) {
+        const uint64_t now = wave_most(mine);
+        if (now == 0)
+            break;
+        if (lane == k)
+            kept = now;
+        if (mine == now)
+            mine = largest_below(now);
+    }
+    if (lane < keep)
+        a.best[slot * keep + lane] = kept;
+}
+
+// exp and power in 64 bits: a few for each request.
+__global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
+{
+    extern __shared__ uint64_t lists[]; // a wave's parts [parts][keep]
+    __shared__ uint64_t best[kMostBeams][kMostBeams];
+    __shared__ double base[kMostBeams], divisor[kMostBeams];
+    __shared__ int grown[kMostBeams];
+    const uint32_t request = blockIdx.x, beams = a.from.beams, keep = a.to.beams;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t waves = blockDim.x / kWave;
+    uint64_t *list = lists + size_t(wave) * room;
+    for (uint32_t i = wave; i < beams; i += waves) {
+        const size_t row = size_t(request) * beams + i;
+        const float score = a.from.scores[row];
+        const bool ended = a.from.ended != nullptr && a.from.ended[row] != 0;
+        const int length = a.from.lengths == nullptr ? 0 : a.from.lengths[row];
+        if (lane == 0) {
+            grown[i] = ended ? length : length + 1;
+            divisor[i] = a.power == 0.0f ? 1.0 : pow(double(max(grown[i], 1)), double(a.power));
+        }
+        if (!(score > -INFINITY)) {
+            if (lane < keep)
+                best[i][lane] = 0;
+            continue;
+        }
+        if (ended) {
+            if (lane < keep)
+                best[i][lane] = lane == 0 ? key_of(0.0f, uint32_t(a.eos)) : 0;
+            if (lane == 0)
+                base[i] = double(score);
+            continue;
+        }
+        Part part{-INFINITY, 0, 0.0};
+        if (lane < a.parts)
+            part = a.stats[row * a.parts + lane];
+        for (uint32_t k = lane; k < a.parts * keep; k += kWave)
+            list[k] = a.best[row * a.parts * keep + k];
+        const float top = wave_max(part.most);
+        double sum = part.most == -INFINITY ? part.sum
+                                            : part.sum * exp(double(part.most) - double(top));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            sum += __shfl_xor(sum, o);
+        if (lane == 0)
+            base[i] = double(score) - (double(top) + log(sum));
+        // the wave's lanes read what its other lanes wrote
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // the heads of the parts' lists, a lane a part
+        uint32_t at = 0;
+        uint64_t head = lane < a.parts ? list[lane * keep] : 0, kept = 0;
+        for (uint32_t k = 0; k < keep; k++) {
+            const uint64_t now = wave_most(head);
+            if (now == 0)
+                break;
+            if (lane == k)
+                kept = now;
+            if (head == now)
+                head = ++at < keep ? list[lane * keep + at] : 0;
+        }
+        if (lane < keep)
+            best[i][lane] = kept;
+    }
+    __syncthreads();
+    if (wave != 0)
+        return;
+    // the beams' lists, a lane a beam
+    const auto rank = [&](uint32_t at) {
+        if (lane >= beams || at >= keep || best[lane][at] == 0)
+            return uint64_t(0);
+        return rank_key((base[lane] + double(logit_of(best[lane][at]))) / divisor[lane]);
+    };
+    uint32_t at = 0;
+    uint64_t head = rank(0);
+    for (uint32_t k = 0; k < keep; k++) {
+        const uint64_t now = wave_most(head);
+        const uint64_t same = __ballot(head == now);
+        const uint32_t beam = uint32_t(__builtin_ctzll(same));
+        const size_t to = size_t(request) * keep + k;
+        if (lane == beam) {
+            const bool live = now != 0;
+            const uint64_t key = live ? best[beam][at] : 0;
+            const size_t row = size_t(request) * beams + beam;
+            const bool over = live && a.from.ended != nullptr && a.from.ended[row] != 0;
+            a.parents[to] = live ? int(row) : -1;
+            a.tokens[to] = live ? int(token_of(key)) : -1;
+            a.to.scores[to] = live ? float(base[beam] + double(logit_of(key))) : -INFINITY;
+            if (a.to.lengths != nullptr)
+                a.to.lengths[to] = live ? grown[beam] : 0;
+            if (a.to.ended != nullptr)
+                a.to.ended[to] = over || (live && int(token_of(key)) == a.eos) ? 1 : 0;
+            head = live ? rank(++at) : 0;
+        }
+    }
+}
+
+template <typename Word>
+__global__ __launch_bounds__(256) void gather_kernel(const char *source, size_t from_stride,
+                                                     uint32_t sources, char *to, size_t to_stride,
+                                                     size_t words, const int *__restrict__ parents,
+                                                     int *status, uint32_t blocks)
+{
+    const uint32_t i = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const int parent = parents[i];
+    if (parent == -1)
+        return;
+    if (parent < 0 || uint32_t(parent) >= sources) {
+        if (threadIdx.x == 0 && block == 0)
+            status_flag(status, kBadParent);
+        return;
+    }
+    const Word *x = reinterpret_cast<const Word *>(source + size_t(parent) * from_stride);
+    Word *y = reinterpret_cast<Word *>(to + size_t(i) * to_stride);
+    for (size_t w = size_t(block) * 256 + threadIdx.x; w < words; w += size_t(blocks) * 256)
+        y[w] = x[w];
+}
+
+// A row may begin up to 7 elements into its first run.
+uint32_t parts_of(uint32_t vocab, uint32_t each)
+{
+    return (vocab + 7 + each * kWave - 1) / (each * kWave);
+}
+
+// Logits a lane holds, 16 to 128: the fewest whose parts fit a wave, and their
+// lists its shared memory. 128 do for kMostVocab.
+uint32_t each_of(uint32_t vocab, uint32_t keep)
+{
+    uint32_t each = 16;
+    while (each < 128 && (parts_of(vocab, each) > kMostParts ||
+                          parts_of(vocab, each) * keep > kMostListed))
+        each *= 2;
+    return each;
+}
+
+size_t carve(BeamArgs &a, char *base)
+{
+    const auto aligned = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    a.parts = parts_of(a.vocab, each_of(a.vocab, a.to.beams));
+    const size_t parts = size_t(a.from.requests) * a.from.beams * a.parts;
+    a.stats = reinterpret_cast<Part *>(base);
+    a.best = reinterpret_cast<uint64_t *>(base + aligned(parts * sizeof(Part)));
+    return aligned(parts * sizeof(Part)) + aligned(parts * a.to.beams * sizeof(uint64_t));
+}
+
+template <int TYPE> void scan_as(const BeamArgs &a, dim3 grid, hipStream_t stream)
+{
+    const uint32_t each = each_of(a.vocab, a.to.beams);
+    const auto run = each == 16   ? scan_kernel<TYPE, 16>
+                     : each == 32 ? scan_kernel<TYPE, 32>
+                     : each == 64 ? scan_kernel<TYPE, 64>
+                                  : scan_kernel<TYPE, 128>;
+    hipLaunchKernelGGL(run, grid, dim3(kWave), 0, stream, a);
+}
+
+} // namespace
+
+size_t beam_workspace(const BeamsView &from, const BeamsView &to, uint32_t vocab)
+{
+    BeamArgs a{};
+    a.from = from, a.to = to, a.vocab = vocab;
+    const size_t bytes = carve(a, nullptr);
+    paged_grid(uint64_t(from.requests) * from.beams * a.parts, kWave);
+    paged_grid(from.requests, 1024);
+    return bytes;
+}
+
+void launch_beam_select(const BeamsView &from, const BeamsView &to, const void *logits, int type,
+                        size_t row_stride, uint32_t vocab, int eos, float power, int *parents,
+                        int *tokens, char *workspace, hipStream_t stream)
+{
+    BeamArgs a{};
+    a.from = from, a.to = to, a.logits = logits, a.row_stride = row_stride, a.vocab = vocab;
+    a.eos = eos, a.power = power, a.parents = parents, a.tokens = tokens;
+    carve(a, workspace);
+    const uint32_t rows = from.requests * from.beams, y = std::min(rows, 32768u);
+    const dim3 grid(a.parts, y, (rows + y - 1) / y);
+    if (type == NUT_F32)
+        scan_as<NUT_F32>(a, grid, stream);
+    else if (type == NUT_F16)
+        scan_as<NUT_F16>(a, grid, stream);
+    else
+        scan_as<NUT_BF16>(a, grid, stream);
+    check_launch("beam select");
+    const uint32_t room = a.parts * to.beams;
+    const uint32_t waves = std::min({from.beams, 16u, kMostListed / room});
+    hipLaunchKernelGGL(choose_kernel, dim3(from.requests), dim3(waves * kWave),
+                       size_t(waves) * room * sizeof(uint64_t), stream, a, room);
+    check_launch("beam select");
+}
+
+void launch_beam_gather(const char *source, size_t from_stride, uint32_t sources, char *to,
+                        size_t to_stride, uint32_t rows, size_t row_bytes, const int *parents,
+                        int *status, hipStream_t stream)
+{
+    const uintptr_t all = reinterpret_cast<uintptr_t>(source) | reinterpret_cast<uintptr_t>(to) |
+                          from_stride | to_stride | row_bytes;
+    const bool wide = all % 16 == 0;
+    const size_t words = row_bytes / (wide ? 16 : 4);
+    // 4 words a thread, as far as one launch covers them
+    const uint64_t most = 0xffffffffull / 256 / rows;
+    require(most != 0, NUT_EINVAL, "beam gather: more rows than one launch covers");
+    const uint32_t blocks = uint32_t(std::min<uint64_t>((words + 1023) / 1024, most));
+    hipLaunchKernelGGL(wide ? gather_kernel<uint4> : gather_kernel<uint32_t>, dim3(rows * blocks),
+                       dim3(256), 0, stream, source, from_stride, sources, to, to_stride, words,
+                       parents, status, blocks);
+    check_launch("beam gather");
+}
+
+} // namespace nut

@@ -14,7 +14,8 @@
 namespace nut {
 
 // Bits of a view's status word.
-enum : int { kBadPage = 1, kBadLength = 2, kBadRows = 4 };
+enum : int { kBadPage = 1, kBadLength = 2, kBadRows = 4, kBadTree = 8, kBadParent = 16,
+             kNoPages = 32 };
 
 // Division of rows (below 2^31) by the page size as a multiplication: with
 // 2^(l - 1) < size <= 2^l and magic = floor(2^(31 + l) / size) + 1, the product
@@ -61,6 +62,41 @@ NUT_HOST_DEVICE int append_error(int length, int64_t from, int64_t gain, uint32_
     if (length < 0 || length + gain > int64_t(max_length))
         return kBadLength;
     return 0;
+}
+
+// Rows [from, end) of `total` that are at most `most`.
+NUT_HOST_DEVICE bool span_in(int from, int end, uint32_t most, uint32_t total)
+{
+    return from >= 0 && end >= from && uint32_t(end) <= total && uint32_t(end - from) <= most;
+}
+
+// Whether `more` rows fit behind `length` ones.
+NUT_HOST_DEVICE bool length_with(int length, uint32_t more, uint32_t most)
+{
+    return length >= 0 && uint64_t(length) + more <= most;
+}
+
+// A parent that node i of a draft tree may have; -1: none.
+NUT_HOST_DEVICE bool parent_in(int parent, uint32_t i)
+{
+    return parent == -1 || (parent >= 0 && uint32_t(parent) < i);
+}
+
+// The 32 bits from bit `at` on of a mask of `words` words; bits below 0 are
+// set, bits behind the words are not.
+template <typename Word>
+NUT_HOST_DEVICE uint32_t mask_bits(int64_t at, uint32_t words, Word &&word)
+{
+    if (at <= -32)
+        return ~0u;
+    if (at < 0) {
+        const uint32_t low = uint32_t(-at), first = words > 0 ? word(0) : 0;
+        return ((1u << low) - 1) | (first << low);
+    }
+    const uint32_t w = uint32_t(at >> 5), shift = uint32_t(at) & 31;
+    const uint64_t lo = uint64_t(w) < words ? word(w) : 0;
+    const uint64_t hi = uint64_t(w) + 1 < words ? word(w + 1) : 0;
+    return uint32_t((hi << 32 | lo) >> shift);
 }
 
 // Pages that `gain` rows (one or more) can lie in, wherever they begin.
