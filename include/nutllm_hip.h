@@ -505,8 +505,9 @@ typedef struct nut_page_table {
  * ({page, fresh page, rows}, {-1, -1, -1} for none; nut_paged_copy). So no two
  * sequences ever append to one page. Fresh pages are the lowest that were free
  * before the call, handed out in order; where none is left the entry is -1,
- * which is reported. Pages that nothing holds any more are free from the next
- * call on. Entries of `to` behind d_held stay.
+ * which is reported (an entry of -1 then goes on as one). Pages that nothing
+ * holds any more are free from the next call on. Entries of `to` behind d_held
+ * stay.
  *
  * `to` shares no memory with `from`. A parent outside `from`, a sequence
  * whose length its pages or `to` do not hold, is reported, and what goes on

@@ -21,7 +21,7 @@ namespace nut {
 namespace {
 
 constexpr uint32_t kMostParts = 64;   // of a beam's logits: a lane each
-constexpr uint32_t kMostListed = 2112; // keys of a beam's parts: 33 parts of 64
+constexpr uint32_t kMostListed = 2048; // keys of a beam's parts: 32 parts of 64
 
 struct Part {
     float most; // minus infinity: no finite one
@@ -84,6 +84,11 @@ __device__ __forceinline__ float exp_below(float d)
     return fmaf(e, rest * 0.69314718f, e);
 }
 
+// 16 bytes of a row, which may begin at any element.
+template <int TYPE> struct __attribute__((packed, aligned(TYPE == NUT_F32 ? 4 : 2))) Run {
+    uint32_t w[4];
+};
+
 // EACH logits a lane, in runs of 16 bytes: run r of the wave's part is lane r % 64's.
 template <int TYPE, int EACH>
 __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
@@ -97,27 +102,26 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
         return; // no beam, or one that needs no logits
     constexpr int kSize = TYPE == NUT_F32 ? 4 : 2;
     const char *logits = static_cast<const char *>(a.logits) + row * a.row_stride * kSize;
-    // runs at multiples of 16 bytes: the first may begin before the row
-    const uint32_t lead = uint32_t(reinterpret_cast<uintptr_t>(logits) % 16 / kSize);
+    // Runs by token, not by address: beams with the same logits have the same sums,
+    // to the last bit, wherever their rows begin.
     float v[EACH];
 #pragma unroll
     for (int r = 0; r < kRuns; r++) {
-        const int64_t at = int64_t(part) * kPart + (r * kWave + lane) * kRun - lead;
-        if (at >= 0 && at + kRun <= int64_t(a.vocab)) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(logits + at * kSize);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const uint32_t at = part * kPart + (r * kWave + lane) * kRun;
+        if (at + kRun <= a.vocab) {
+            const Run<TYPE> x = *reinterpret_cast<const Run<TYPE> *>(logits + size_t(at) * kSize);
 #pragma unroll
             for (int e = 0; e < kRun; e++)
-                v[r * kRun + e] = TYPE == NUT_F32 ? __uint_as_float(w[e % 4])
+                v[r * kRun + e] = TYPE == NUT_F32 ? __uint_as_float(x.w[e % 4])
                                   : TYPE == NUT_BF16
-                                      ? from_bf16(w[e / 2 % 4] >> (e % 2 * 16) & 0xffffu)
-                                      : from_f16(w[e / 2 % 4] >> (e % 2 * 16) & 0xffffu);
+                                      ? from_bf16(x.w[e / 2 % 4] >> (e % 2 * 16) & 0xffffu)
+                                      : from_f16(x.w[e / 2 % 4] >> (e % 2 * 16) & 0xffffu);
         } else {
 #pragma unroll
             for (int e = 0; e < kRun; e++) {
                 float x = -INFINITY;
-                if (at + e >= 0 && at + e < int64_t(a.vocab)) {
-                    const char *p = logits + (at + e) * kSize;
+                if (at + e < a.vocab) {
+                    const char *p = logits + size_t(at + e) * kSize;
                     x = TYPE == NUT_F32    ? *reinterpret_cast<const float *>(p)
                         : TYPE == NUT_BF16 ? from_bf16(*reinterpret_cast<const uint16_t *>(p))
                                            : from_f16(*reinterpret_cast<const uint16_t *>(p));
@@ -152,10 +156,9 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
         uint64_t best = 0;
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const int64_t at = int64_t(part) * kPart + (e / kRun * kWave + lane) * kRun + e % kRun -
-                               lead;
-            const uint64_t key = key_of(v[e], uint32_t(at));
-            if (at >= 0 && at < int64_t(a.vocab) && key < bound && key > best)
+            const uint32_t at = part * kPart + (e / kRun * kWave + lane) * kRun + e % kRun;
+            const uint64_t key = key_of(v[e], at);
+            if (at < a.vocab && key < bound && key > best)
                 best = key;
         }
         return best;
@@ -180,7 +183,8 @@ __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
 {
     extern __shared__ uint64_t lists[]; // a wave's parts [parts][keep]
     __shared__ uint64_t best[kMostBeams][kMostBeams];
-    __shared__ double base[kMostBeams], divisor[kMostBeams];
+    __shared__ double score_of[kMostBeams], top_of[kMostBeams], log_of[kMostBeams];
+    __shared__ double divisor[kMostBeams];
     __shared__ int grown[kMostBeams];
     const uint32_t request = blockIdx.x, beams = a.from.beams, keep = a.to.beams;
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
             if (lane < keep)
                 best[i][lane] = lane == 0 ? key_of(0.0f, uint32_t(a.eos)) : 0;
             if (lane == 0)
-                base[i] = double(score);
+                score_of[i] = double(score), top_of[i] = log_of[i] = 0.0;
             continue;
         }
         Part part{-INFINITY, 0, 0.0};
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
         for (int o = 32; o > 0; o >>= 1)
             sum += __shfl_xor(sum, o);
         if (lane == 0)
-            base[i] = double(score) - (double(top) + log(sum));
+            score_of[i] = double(score), top_of[i] = double(top), log_of[i] = log(sum);
         // the wave's lanes read what its other lanes wrote
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -243,10 +247,14 @@ __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
     if (wave != 0)
         return;
     // the beams' lists, a lane a beam
+    // the difference to the largest logit first: it is small, or says that nothing is
+    const auto scored = [&](uint32_t i, uint64_t key) {
+        return score_of[i] + (double(logit_of(key)) - top_of[i] - log_of[i]);
+    };
     const auto rank = [&](uint32_t at) {
         if (lane >= beams || at >= keep || best[lane][at] == 0)
             return uint64_t(0);
-        return rank_key((base[lane] + double(logit_of(best[lane][at]))) / divisor[lane]);
+        return rank_key(scored(lane, best[lane][at]) / divisor[lane]);
     };
     uint32_t at = 0;
     uint64_t head = rank(0);
@@ -262,7 +270,7 @@ __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
             const bool over = live && a.from.ended != nullptr && a.from.ended[row] != 0;
             a.parents[to] = live ? int(row) : -1;
             a.tokens[to] = live ? int(token_of(key)) : -1;
-            a.to.scores[to] = live ? float(base[beam] + double(logit_of(key))) : -INFINITY;
+            a.to.scores[to] = live ? float(scored(beam, key)) : -INFINITY;
             if (a.to.lengths != nullptr)
                 a.to.lengths[to] = live ? grown[beam] : 0;
             if (a.to.ended != nullptr)
@@ -293,10 +301,9 @@ __global__ __launch_bounds__(256) void gather_kernel(const char *source, size_t 
         y[w] = x[w];
 }
 
-// A row may begin up to 7 elements into its first run.
 uint32_t parts_of(uint32_t vocab, uint32_t each)
 {
-    return (vocab + 7 + each * kWave - 1) / (each * kWave);
+    return (vocab + each * kWave - 1) / (each * kWave);
 }
 
 // Logits a lane holds, 16 to 128: the fewest whose parts fit a wave, and their

@@ -266,7 +266,8 @@ __device__ __forceinline__ void fill_entries(const ReorderArgs &a, uint32_t i, u
     for (uint32_t c = threadIdx.x; c < step.full; c += kWave) {
         int page = old[c];
         if (!page_in(page, a.pool.pages)) {
-            status_flag(a.pool.status, kBadPage);
+            if (page != -1) // -1: none was free for it
+                status_flag(a.pool.status, kBadPage);
             page = -1;
         }
         entries[c] = page;
@@ -298,7 +299,7 @@ __device__ __forceinline__ void fill_entries(const ReorderArgs &a, uint32_t i, u
             const int source = old[c];
             if (page_in(source, a.pool.pages))
                 copy[0] = source, copy[1] = page, copy[2] = rows;
-            else
+            else if (source != -1)
                 status_flag(a.pool.status, kBadPage);
         }
     }
@@ -332,7 +333,7 @@ __device__ __forceinline__ void settle(const ReorderArgs &a, uint32_t p)
             continue;
         const int page = old[c];
         if (!page_in(page, a.pool.pages)) {
-            if (page != -1) // -1: none was free for it
+            if (page != -1)
                 status_flag(a.pool.status, kBadPage);
             continue;
         }
