@@ -45,12 +45,14 @@ struct BeamsView {
     uint32_t requests, beams;
 };
 
-// How a tree attention call is split: `blocks` blocks of query rows (nodes
-// times the heads that share a KV head), `runs` runs of `run` rows.
+// How a tree attention call is split. Few query rows (nodes times the heads that
+// share a KV head): `runs` runs of `run` rows of a sequence. Many: `shares`
+// workgroups that share out blocks of 64 query rows and stages of rows.
 struct TreePlan {
-    uint32_t queries; // 16-row tiles of queries of a block
-    uint32_t blocks, run, runs;
-    size_t stats; // byte offset of the runs' sums
+    bool staged, past; // past the caches
+    uint32_t waves; // of a workgroup that hold different query rows
+    uint32_t blocks, run, runs, shares;
+    size_t stats, before; // byte offsets of the parts' sums, of the stages before each sequence
     size_t bytes;
 };
 TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &draft,

@@ -19,7 +19,7 @@ namespace nut {
 
 namespace {
 
-constexpr uint32_t kPiece = 1024; // rows whose offsets are in shared memory at once
+constexpr uint32_t kPieceRows = 1024; // rows whose offsets are in shared memory at once
 
 struct TreeArgs {
     PagedView kv;
@@ -30,7 +30,10 @@ struct TreeArgs {
     uint32_t heads, group;
     float scale; // times log2(e)
     float *out, *lse;
-    uint32_t blocks, run, runs, units;
+    uint32_t blocks, run, runs, units; // of tree_kernel
+    uint32_t shares;                   // of staged_kernel
+    bool past;                         // rows go past the caches' replacement
+    uint64_t *before; // [batch + 1]: stages before each sequence
     float *parts;  // [total][heads][runs][head_dim], unnormalised
     float2 *stats; // [total][heads][runs]: exponent they refer to, sum
 };
@@ -184,18 +187,19 @@ __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *
 
 template <int HD> constexpr int kTreeWaves = HD == 256 ? 2 : 4;
 
-template <int TYPE, int HD, bool FULL, int QT>
+template <int TYPE, int HD, bool FULL, int QT, int WQ>
 __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
 {
     using T = Tile<TYPE, HD>;
     constexpr int G = T::G, WAVES = kTreeWaves<HD>, kThreads = 64 * WAVES;
+    constexpr int WK = WAVES / WQ;
     constexpr int kStride = HD + 4;
     __shared__ union Shared {
-        size_t at[kPiece];
+        size_t at[kPieceRows];
         float o[WAVES][16][kStride];
     } lds;
     __shared__ float stat[3][WAVES][16];
-    __shared__ uint32_t gone[kPiece / 32];
+    __shared__ uint32_t gone[kPieceRows / 32];
     const PagedView &kv = a.kv;
     // Workgroups go to the 8 XCDs in turn: the blocks that read the same rows
     // follow one another on one of them.
@@ -207,8 +211,8 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
     const uint32_t b = unit / a.runs / kv.kv_heads;
     const bool leader = threadIdx.x == 0 && c == 0 && h == 0 && block == 0;
     const NodeSpan nodes = nodes_of(a.d, b, leader);
-    const uint32_t queries = nodes.count * a.group, first = block * QT * 16;
-    if (first >= queries)
+    const uint32_t queries = nodes.count * a.group, begins = block * QT * 16 * WQ;
+    if (begins >= queries)
         return;
     uint32_t held;
     const uint32_t total = rows_of(a, b, nodes.count, held, leader);
@@ -220,14 +224,16 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int j = lane >> 4, column = lane & 15;
+    const int wq = wave % WQ, wk = wave / WQ;
+    const uint32_t first = begins + wq * QT * 16; // of the wave's query rows
     Query<TYPE, HD> q[QT];
     const uint32_t *mask[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const uint32_t row = first + t * 16 + column;
         const bool valid = row < queries;
-        const uint32_t node = nodes.from + (valid ? row : first) / a.group;
-        const uint32_t head = h * a.group + (valid ? row : first) % a.group;
+        const uint32_t node = nodes.from + (valid ? row : begins) / a.group;
+        const uint32_t head = h * a.group + (valid ? row : begins) % a.group;
         q[t].fetch(a.query + node * a.query_stride + size_t(head) * kv.head_dim, valid,
                    kv.head_dim, lane);
         mask[t] = a.d.mask + node * a.d.mask_stride;
@@ -238,8 +244,8 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
         q[t].convert(a.scale);
 
     Softmax<TYPE, HD> sm[QT];
-    for (uint32_t piece = 0; piece < count; piece += kPiece) {
-        const uint32_t rows = min(count - piece, kPiece);
+    for (uint32_t piece = 0; piece < count; piece += kPieceRows) {
+        const uint32_t rows = min(count - piece, kPieceRows);
         if (piece != 0)
             __syncthreads();
         for (uint32_t i = threadIdx.x; i < (rows + 63) / 64 * 64; i += kThreads) {
@@ -258,8 +264,8 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
         }
         __syncthreads();
         constexpr uint32_t kAll = T::kWide ? 0xffffu : 0xffffffffu;
-        const int tiles = int((rows + T::kRows - 1) / T::kRows);
-        for (int t = wave; t < tiles; t += WAVES) {
+        const int tiles = first >= queries ? 0 : int((rows + T::kRows - 1) / T::kRows);
+        for (int t = wk; t < tiles; t += WK) {
             Tile<TYPE, HD> x;
             x.template load<FULL, false>(kv, lds.at + t * T::kRows, lane);
             const uint32_t none = uint32_t(__builtin_amdgcn_readfirstlane(
@@ -277,12 +283,12 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
         }
     }
 
-    // The waves' sums side by side, a tile of query rows at a time; then a thread
-    // per four components adds them.
+    // The waves' sums side by side, a tile of each one's query rows at a time; then a
+    // thread per four components adds those of the same rows.
     const uint32_t parts = FULL ? HD / 4 : kv.head_dim / 4;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        if (first + t * 16 >= queries)
+        if (begins + t * 16 >= queries)
             break;
         sm[t].sum += __shfl_xor(sm[t].sum, 16);
         sm[t].sum += __shfl_xor(sm[t].sum, 32);
@@ -306,29 +312,31 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
                     f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
         }
         __syncthreads();
-        const uint32_t here = min(16u, queries - first - t * 16);
-        for (uint32_t i = threadIdx.x; i < here * parts; i += kThreads) {
-            const uint32_t k = i / parts, d = i % parts * 4;
-            float most = stat[0][0][k];
+        for (uint32_t i = threadIdx.x; i < WQ * 16 * parts; i += kThreads) {
+            const uint32_t k = i / parts, d = (i - k * parts) * 4, of = k / 16, c16 = k % 16;
+            const uint32_t row = begins + of * QT * 16 + t * 16 + c16;
+            if (row >= queries)
+                continue;
+            float most = stat[0][of][c16];
 #pragma unroll
-            for (int w = 1; w < WAVES; w++)
-                most = fmaxf(most, stat[0][w][k]);
+            for (int w = 1; w < WK; w++)
+                most = fmaxf(most, stat[0][of + w * WQ][c16]);
             const float ref = most == -INFINITY ? 0.0f : most - Softmax<TYPE, HD>::kShift;
             float sum = 0.0f;
             f32x4 o{0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) {
+            for (int w = 0; w < WK; w++) {
+                const int from = of + w * WQ;
                 // what no row of a finite score reached is zero, or not a number
-                const float f = stat[0][w][k] == -INFINITY
+                const float f = stat[0][from][c16] == -INFINITY
                                     ? 1.0f
-                                    : __builtin_amdgcn_exp2f(stat[1][w][k] - ref);
-                sum = fmaf(stat[2][w][k], f, sum);
-                const f32x4 y = *reinterpret_cast<const f32x4 *>(&lds.o[w][k][d]);
+                                    : __builtin_amdgcn_exp2f(stat[1][from][c16] - ref);
+                sum = fmaf(stat[2][from][c16], f, sum);
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(&lds.o[from][c16][d]);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     o[e] = fmaf(y[e], f, o[e]);
             }
-            const uint32_t row = first + t * 16 + k;
             const size_t at = size_t(nodes.from + row / a.group) * a.heads + h * a.group +
                               row % a.group;
             if (a.parts != nullptr) {
@@ -342,6 +350,733 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
                     a.lse[at] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
             }
         }
+    }
+}
+
+// ---------------------------------------------------------------- staged --
+
+// Many query rows: the four waves hold QT tiles each and share every tile of rows,
+// staged in shared memory. 16-bit rows come by DMA, the next stage while this one
+// is multiplied; fp32 rows come through registers and are kept as three bfloat16
+// limbs, whose six largest products with the query's limbs leave out 2^-21 of a
+// product at most and 2^-24 in the mean: 2.7 times the rate of the fp32
+// instruction. Keys are read as they lie; values by the transposing read, of the
+// keys that the lane's weights are of, so that those need no exchange.
+template <int TYPE, int HD> struct Stage {
+    static constexpr int kPlanes = TYPE == NUT_F32 ? 3 : 1;
+    static constexpr int kType = TYPE == NUT_F32 ? NUT_BF16 : TYPE; // of the planes
+    static constexpr int kRows = HD <= 64 && TYPE != NUT_F32 ? 64 : 32;
+    static constexpr int kChunks = HD <= 32 ? 4 : HD <= 64 ? 8 : HD <= 128 ? 16 : 32; // of a row
+    static constexpr int kUsed = HD / 8;
+    // The stage at work and, of 16-bit rows, the one that is fetched beside it. (Two
+    // fetched ahead, at a row of 128 components, read no faster: 418 us for 408 of
+    // four sequences of up to 32,768 fp16 rows, 32 KV heads.)
+    static constexpr int kBuffers = TYPE == NUT_F32 ? 1 : 2;
+    static constexpr int kBytes = kPlanes * kRows * kChunks * 16; // of keys, or of values
+    // Chunks of 16 bytes trade places within 128, by the row: 16 rows of one chunk
+    // lie on all banks.
+    static constexpr int kShift = kChunks < 8 ? 3 : kChunks == 8 ? 3 : kChunks == 16 ? 4 : 5;
+    static __device__ __forceinline__ uint32_t place(uint32_t i) { return i ^ (i >> kShift & 7); }
+    static __device__ __forceinline__ uint32_t offset(uint32_t row, uint32_t chunk)
+    {
+        return place(row * kChunks + chunk) * 16;
+    }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// BYTES (16 or 4) for each lane, from `source` to shared memory, lane after lane.
+// As asm: the compiler would wait for all of it before it reads shared memory.
+template <int BYTES = 16, bool NT = false>
+__device__ __forceinline__ void stage_dma(const void *source, const void *to)
+{
+    const uint32_t at = __builtin_amdgcn_readfirstlane(uint32_t(
+        reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)to)));
+    if constexpr (BYTES == 16 && NT)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt"
+                     :
+                     : "v"(source), "s"(at)
+                     : "memory", "m0");
+    else if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                     :
+                     : "v"(source), "s"(at)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+                     :
+                     : "v"(source), "s"(at)
+                     : "memory", "m0");
+}
+
+// A compiler that has the loads before this does not put them off behind it.
+__device__ __forceinline__ void keep_loads() { asm volatile("" ::: "memory"); }
+
+// A stage against QT tiles of query rows; the other arguments as attend_tree's,
+// a word for 32 rows. `odd`: rows some of whose values are not finite and were
+// staged as 0; they are added one by one. Shared memory answers after 100 cycles
+// and a product after 30, so that everything that can be is asked for together:
+// all keys of a plane, the values before the softmax, and products in turn that do
+// not wait for one another.
+template <int TYPE, int HD, bool FULL, int QT>
+__device__ __forceinline__ void
+attend_stage(const char *keys, const char *values, const size_t *at,
+             const uint32_t (&gone)[Stage<TYPE, HD>::kRows / 32], bool drafted,
+             const uint32_t (&odd)[Stage<TYPE, HD>::kRows / 32],
+             const uint32_t (&seen)[QT][Stage<TYPE, HD>::kRows / 32],
+             const Query<Stage<TYPE, HD>::kType, HD> (&q)[QT],
+             Softmax<Stage<TYPE, HD>::kType, HD> (&sm)[QT], const PagedView &kv, int lane)
+{
+    using S = Stage<TYPE, HD>;
+    constexpr int G = HD / 16, kParts = HD / 32, kType = S::kType, kPlanes = S::kPlanes;
+    constexpr int kLimbs = Query<kType, HD>::kLimbs, kSubs = S::kRows / 16, kHalves = kSubs / 2;
+    const uint32_t j = lane >> 4, c = lane & 15;
+    const auto key = [&](int p, int sub, int n) {
+        return *reinterpret_cast<const u32x4 *>(
+            keys + S::offset(p * S::kRows + sub * 16 + c, n * 4 + j));
+    };
+    f32x4 acc[QT][kSubs];
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++)
+            acc[t][sub] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int p = kPlanes - 1; p >= 0; p--) {
+        u32x4 k[kSubs][kParts];
+#pragma unroll
+        for (int n = 0; n < kParts; n++)
+#pragma unroll
+            for (int sub = 0; sub < kSubs; sub++)
+                k[sub][n] = key(p, sub, n);
+        keep_loads();
+#pragma unroll
+        for (int n = 0; n < kParts; n++)
+#pragma unroll
+            for (int l = kLimbs - 1; l >= 0; l--)
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int sub = 0; sub < kSubs; sub++)
+                        if (kPlanes == 1 || p + l < 3)
+                            acc[t][sub] = product<kType>(k[sub][n], q[t].x[n][l], acc[t][sub]);
+    }
+    // Values of plane p, kGroup tiles of 16 components from tile g0 on: of rows
+    // 4 j + c / 4 (then 16 further), components 16 g + 4 (c % 4) onwards, transposed.
+    constexpr int kGroup = kHalves * G <= 8 ? G : G / 2;
+    u32x4 v[kHalves][kGroup];
+    const auto load_values = [&](int p, int g0) {
+#pragma unroll
+        for (int g = 0; g < kGroup; g++)
+#pragma unroll
+            for (int half = 0; half < kHalves; half++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t row = p * S::kRows + half * 32 + 16 * e + 4 * j + c / 4;
+                    const char *from =
+                        values + S::offset(row, 2 * (g0 + g) + (c & 3) / 2) + (c & 1) * 8;
+                    const u32x2 z = __builtin_bit_cast(
+                        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)from));
+                    v[half][g][2 * e] = z[0], v[half][g][2 * e + 1] = z[1];
+                }
+        keep_loads();
+    };
+    load_values(kPlanes - 1, 0);
+    float s[QT][kHalves][8];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        float all = 0.0f; // not a number after one that is none
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                all += acc[t][sub][i];
+        if (__any(all != all)) {
+            // An infinite key: the first limbs' product has the sum's sign, later ones
+            // of zero, or of the other sign, make it no number. (So do sums of both
+            // infinities, which are none in the end either.)
+#pragma unroll
+            for (int sub = 0; sub < kSubs; sub++) {
+                f32x4 first{0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < kParts; n++)
+                    first = product<kType>(key(0, sub, n), q[t].x[n][0], first);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[t][sub][i] = acc[t][sub][i] != acc[t][sub][i] ? first[i] : acc[t][sub][i];
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < kHalves; half++)
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const float x = acc[t][2 * half + r / 4][r % 4];
+                s[t][half][r] = kType == NUT_F16 ? ldexpf(x, q[t].exponent) : x;
+            }
+    }
+    bool masked = drafted;
+#pragma unroll
+    for (int half = 0; half < kHalves; half++)
+        masked = masked || gone[half] != 0;
+    if (masked)
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int half = 0; half < kHalves; half++) {
+                const uint32_t mine = (seen[t][half] & ~gone[half]) >> (4 * j);
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+                    s[t][half][r] = mine >> (16 * (r / 4) + r % 4) & 1 ? s[t][half][r] : -INFINITY;
+            }
+    u32x4 limb[QT][kHalves][kLimbs];
+    float p[QT][kHalves][8];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        float most = s[t][0][0];
+#pragma unroll
+        for (int half = 0; half < kHalves; half++)
+#pragma unroll
+            for (int r = 0; r < 8; r++)
+                most = fmaxf(most, s[t][half][r]);
+        sm[t].raise(max_over_rows(most));
+        float sum[kHalves][2] = {};
+#pragma unroll
+        for (int half = 0; half < kHalves; half++) {
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                p[t][half][r] = __builtin_amdgcn_exp2f(s[t][half][r] - sm[t].ref);
+                sum[half][r % 2] += p[t][half][r];
+            }
+            split<kType, kLimbs>(p[t][half], limb[t][half]);
+            sm[t].sum += sum[half][0] + sum[half][1];
+        }
+    }
+#pragma unroll
+    for (int half = 0; half < kHalves; half++)
+        for (uint32_t left = odd[half]; left != 0; left &= left - 1) {
+            const int row = __builtin_ctz(left), own = row % 16 / 4;
+            const char *from = kv.values + at[half * 32 + row];
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float weight = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+                    if (16 * (r / 4) + r % 4 == row - 4 * own)
+                        weight = p[t][half][r];
+                weight = __shfl(weight, 16 * own + c);
+                for (int g = 0; g < G; g++) // rare: not unrolled but for the sums
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t d = 16 * g + 4 * j + i;
+                        const float x = FULL || d < kv.head_dim ? component<TYPE>(from, d) : 0.0f;
+                        const bool adds = weight != 0.0f && !(fabsf(x) < INFINITY);
+#pragma unroll
+                        for (int k = 0; k < G; k++)
+                            if (k == g && adds)
+                                sm[t].o[k][i] = fmaf(weight, x, sm[t].o[k][i]);
+                    }
+            }
+        }
+#pragma unroll
+    for (int pl = kPlanes - 1; pl >= 0; pl--)
+#pragma unroll
+        for (int g0 = 0; g0 < G; g0 += kGroup) {
+            if (pl != kPlanes - 1 || g0 != 0)
+                load_values(pl, g0);
+#pragma unroll
+            for (int half = 0; half < kHalves; half++)
+#pragma unroll
+                for (int l = kLimbs - 1; l >= 0; l--)
+#pragma unroll
+                    for (int t = 0; t < QT; t++)
+#pragma unroll
+                        for (int g = 0; g < kGroup; g++)
+                            if (kPlanes == 1 || pl + l < 3)
+                                sm[t].o[g0 + g] = product<kType>(v[half][g], limb[t][half][l],
+                                                                 sm[t].o[g0 + g]);
+        }
+}
+
+constexpr uint32_t kBlock = 64;        // query rows of a workgroup
+constexpr uint32_t kLeast = 2;         // stages that a workgroup takes at least
+
+// How the work is shared out. An item is a block of a sequence's query rows and a
+// KV head, its work the stages of the sequence's rows; items follow one another
+// by sequence, KV head and block, and `shares` workgroups take equal parts of all
+// stages, wherever that cuts an item: lengths and trees are known to the device
+// alone, and parts by the longest would leave most of the chip without work (16
+// sequences of 1 to 2,048 rows: 47 us, of which a CU worked half).
+struct Item {
+    NodeSpan nodes;
+    uint32_t held, total, blocks, stages;
+};
+
+template <int R>
+__device__ __forceinline__ Item item_of(const TreeArgs &a, uint32_t b, bool report)
+{
+    Item it;
+    it.nodes = nodes_of(a.d, b, report);
+    it.total = rows_of(a, b, it.nodes.count, it.held, report && it.nodes.count != 0);
+    it.blocks = (it.nodes.count * a.group + kBlock - 1) / kBlock;
+    it.stages = max((it.total + R - 1) / R, 1u); // a sequence out of range gets zeros
+    return it;
+}
+
+struct Shares {
+    uint64_t all; // stages
+    uint32_t count;
+    __device__ __forceinline__ uint64_t begin(uint32_t i) const { return all * i / count; }
+    // The share that stage x, below `all`, is of.
+    __device__ __forceinline__ uint32_t of(uint64_t x) const
+    {
+        uint32_t i = uint32_t(x * count / all);
+        while (i + 1 < count && begin(i + 1) <= x)
+            i++;
+        while (begin(i) > x)
+            i--;
+        return i;
+    }
+};
+
+__device__ __forceinline__ uint32_t share_count(uint64_t all, uint32_t most)
+{
+    return uint32_t(max(min((all + kLeast - 1) / kLeast, uint64_t(most)), uint64_t(1)));
+}
+
+// The stages before each sequence: a thread sums those of `each` sequences, and
+// then the threads' sums are summed. Returns the share-out, and in `before` the
+// stages before this thread's first sequence. 256 threads.
+template <int R>
+__device__ __forceinline__ Shares share_out(const TreeArgs &a, uint32_t each, bool report,
+                                            uint64_t &before)
+{
+    __shared__ uint64_t sums[4];
+    uint64_t mine = 0;
+    for (uint32_t k = 0; k < each; k++) {
+        const uint32_t b = threadIdx.x * each + k;
+        if (b >= a.s.batch)
+            break;
+        const Item it = item_of<R>(a, b, report);
+        mine += uint64_t(it.blocks) * it.stages;
+    }
+    mine *= a.kv.kv_heads;
+    uint64_t upto = mine;
+    const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const uint64_t x = uint64_t(__shfl_up((unsigned long long)upto, o));
+        upto += lane >= uint32_t(o) ? x : 0;
+    }
+    if (lane == kWave - 1)
+        sums[wave] = upto;
+    __syncthreads();
+    Shares shares{0, 1};
+    before = upto - mine;
+    for (uint32_t w = 0; w < 4; w++) {
+        before += w < wave ? sums[w] : 0;
+        shares.all += sums[w];
+    }
+    shares.count = share_count(shares.all, a.shares);
+    return shares;
+}
+
+// Workgroups that a CU holds, by registers and shared memory.
+constexpr int staged_groups(int type, uint32_t head_dim)
+{
+    return head_dim <= 64 ? 3 : head_dim <= 128 ? (type == NUT_F32 ? 2 : 3) : type == NUT_F32 ? 1 : 2;
+}
+
+template <int TYPE, int HD, bool FULL>
+__global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(TreeArgs a)
+{
+    constexpr int QT = 1;
+    using S = Stage<TYPE, HD>;
+    constexpr int G = HD / 16, R = S::kRows;
+    constexpr uint32_t kEach = 4, kPiece = kEach * R; // rows whose offsets are found at once
+    constexpr int kWork = R * S::kChunks / 256; // chunks of a plane a thread
+    static_assert(R * S::kChunks % 256 == 0 || R * S::kChunks < 256, "whole chunks a thread");
+    __shared__ alignas(128) char stage[S::kBuffers][2][S::kBytes];
+    __shared__ size_t offsets[2][kPiece];
+    __shared__ int table[kPiece];
+    __shared__ uint32_t gone[2][kPiece / 32], strange[2][2];
+    __shared__ uint64_t where[2]; // a sequence, and the stages before it
+    const PagedView &kv = a.kv;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t j = lane >> 4, column = lane & 15;
+    const uint32_t used = FULL ? S::kUsed : kv.head_dim / 8;
+    if constexpr (!FULL && TYPE != NUT_F32) // where no chunk of a row comes to
+        for (uint32_t i = threadIdx.x; i < sizeof stage / 16; i += 256)
+            reinterpret_cast<u32x4 *>(stage)[i] = u32x4{0, 0, 0, 0};
+
+    const uint32_t each = (a.s.batch + 255) / 256;
+    uint64_t before;
+    const Shares shares = share_out<R>(a, each, blockIdx.x == 0, before);
+    // Workgroups go to the 8 XCDs in turn: each takes shares that follow one another,
+    // so that the blocks that read the same rows do so through one cache.
+    const uint32_t run_of = (shares.count + 7) / 8;
+    const uint32_t share = blockIdx.x % 8 * run_of + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= run_of || share >= shares.count ||
+        (shares.all == 0 && blockIdx.x != 0))
+        return;
+    uint64_t at_stage = shares.begin(share);
+    const uint64_t end_stage = shares.begin(share + 1);
+    if (blockIdx.x == 0) { // for the join
+        uint64_t upto = before;
+        for (uint32_t k = 0; k < each; k++) {
+            const uint32_t b = threadIdx.x * each + k;
+            if (b >= a.s.batch)
+                break;
+            const Item it = item_of<R>(a, b, false);
+            a.before[b] = upto;
+            upto += uint64_t(it.blocks) * it.stages * kv.kv_heads;
+        }
+        if (threadIdx.x == 0)
+            a.before[a.s.batch] = shares.all;
+    }
+    for (uint32_t k = 0; k < each; k++) { // one thread has the sequence that holds it
+        const uint32_t b = threadIdx.x * each + k;
+        if (b >= a.s.batch || before > at_stage)
+            break;
+        const Item it = item_of<R>(a, b, false);
+        const uint64_t work = uint64_t(it.blocks) * it.stages * kv.kv_heads;
+        if (at_stage < before + work) {
+            where[0] = b, where[1] = before;
+            break;
+        }
+        before += work;
+    }
+    __syncthreads();
+    uint32_t b = uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(where[0])));
+    uint64_t passed = where[1]; // stages before sequence b
+    bool opening = true;
+
+    while (at_stage < end_stage) {
+        const Item it = item_of<R>(a, b, false);
+        const uint64_t work = uint64_t(it.blocks) * it.stages * kv.kv_heads;
+        if (at_stage >= passed + work) {
+            passed += work;
+            b++;
+            continue;
+        }
+        const uint32_t item = uint32_t((at_stage - passed) / it.stages);
+        const uint32_t from_stage = uint32_t(at_stage - passed - uint64_t(item) * it.stages);
+        const uint32_t to_stage =
+            uint32_t(min(uint64_t(it.stages), from_stage + (end_stage - at_stage)));
+        const bool cut = from_stage != 0 || to_stage != it.stages;
+        const uint32_t slot = 2 * share + (opening && from_stage != 0 ? 0 : 1);
+        opening = false;
+        at_stage += to_stage - from_stage;
+        const uint32_t h = item / it.blocks, block = item - h * it.blocks;
+        const NodeSpan nodes = it.nodes;
+        const uint32_t held = it.held;
+        const uint32_t queries = nodes.count * a.group, begins = block * kBlock;
+        const uint32_t begin = from_stage * R, count = min(to_stage * R, it.total) - begin;
+        const uint32_t first = begins + wave * 16; // of the wave's query rows
+        Query<S::kType, HD> q[QT];
+        const uint32_t *mask[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const uint32_t row = first + t * 16 + column;
+            const bool valid = row < queries;
+            const uint32_t node = nodes.from + (valid ? row : begins) / a.group;
+            const uint32_t head = h * a.group + (valid ? row : begins) % a.group;
+            q[t].fetch(a.query + node * a.query_stride + size_t(head) * kv.head_dim, valid,
+                       kv.head_dim, lane);
+            mask[t] = a.d.mask + node * a.d.mask_stride;
+        }
+        const uint32_t words = (nodes.count + 31) / 32;
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+            q[t].convert(a.scale);
+
+        Softmax<S::kType, HD> sm[QT];
+        // a thread's chunks of the next stage of fp32 rows
+        constexpr int kHeld = TYPE == NUT_F32 ? (kWork == 0 ? 1 : kWork) : 1;
+        float ahead[2][kHeld][8];
+
+        // Where the segment's rows lie, kPiece at a time, a thread a row: the table is
+        // asked for a piece while the one before it is multiplied, by DMA, as a load into
+        // registers would have to be waited for, and all that was asked for before it.
+        const auto ask_table = [&](uint32_t piece) {
+            const uint32_t index = page_of(kv, begin + piece * kPiece) + threadIdx.x;
+            if (threadIdx.x < kPiece && index <= page_of(kv, begin + count - 1))
+                stage_dma<4>(a.s.table + size_t(b) * a.s.table_stride + index, table + wave * kWave);
+        };
+        const auto place_rows = [&](uint32_t piece) {
+            const uint32_t i = piece * kPiece + threadIdx.x, row = begin + i;
+            size_t at = kNoRow;
+            if (threadIdx.x >= kPiece) // whole waves
+                return;
+            if (i < count) {
+                const uint32_t index = page_of(kv, row);
+                const int page = table[index - page_of(kv, row - threadIdx.x)];
+                if (page_in(page, kv.pages))
+                    at = size_t(page) * kv.page_stride + h * kv.head_stride +
+                         (row - index * kv.page_size) * kv.slot_stride;
+                else
+                    status_flag(kv.status, kBadPage);
+            }
+            offsets[piece % 2][threadIdx.x] = at;
+            const uint64_t masked = __ballot(at == kNoRow);
+            if (lane % 32 == 0)
+                gone[piece % 2][threadIdx.x / 32] = uint32_t(masked >> lane);
+        };
+        const auto offset_of = [&](uint32_t s) { return offsets[s / kEach % 2] + s % kEach * R; };
+        const auto gone_of = [&](uint32_t s, int half) {
+            return gone[s / kEach % 2][s % kEach * (R / 32) + half];
+        };
+        // Whether there are rows behind the piece of stage s.
+        const auto more = [&](uint32_t s) { return (s / kEach + 1) * kPiece < count; };
+        static_assert(kEach > S::kBuffers, "a piece is placed before its first stage is fetched");
+        const uint32_t stages = (count + R - 1) / R;
+        // Chunk i of a stage: row i / kChunks, as place() lays them. Rows that are none
+        // are zeros.
+        const auto fetch = [&](uint32_t s) {
+            const size_t *rows = offset_of(s);
+            if constexpr (TYPE == NUT_F32) {
+#pragma unroll
+                for (int w = 0; w < kHeld; w++) {
+                    const uint32_t i = w * 256 + threadIdx.x, row = i / S::kChunks;
+                    const uint32_t chunk = i % S::kChunks;
+                    // without a branch, so that the chunks stay in registers
+                    const size_t at = row < uint32_t(R) ? rows[row] : kNoRow;
+                    const bool there = at != kNoRow && chunk < used;
+                    const size_t byte = there ? at + chunk * 32 : 0;
+                    load8<NUT_F32>(kv.keys + byte, ahead[0][w]);
+                    load8<NUT_F32>(kv.values + byte, ahead[1][w]);
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            ahead[x][w][e] = there ? ahead[x][w][e] : 0.0f;
+                }
+            } else {
+                char *keys = stage[s % S::kBuffers][0], *values = stage[s % S::kBuffers][1];
+                for (uint32_t i = wave * kWave; i < uint32_t(R) * S::kChunks; i += 256) {
+                    const uint32_t from = S::place(i + lane), row = from / S::kChunks;
+                    const uint32_t chunk = from % S::kChunks;
+                    const size_t at = rows[row];
+                    if (chunk < used && at != kNoRow && a.past) {
+                        stage_dma<16, true>(kv.keys + at + chunk * 16, keys + i * 16);
+                        stage_dma<16, true>(kv.values + at + chunk * 16, values + i * 16);
+                    } else if (chunk < used && at != kNoRow) {
+                        stage_dma(kv.keys + at + chunk * 16, keys + i * 16);
+                        stage_dma(kv.values + at + chunk * 16, values + i * 16);
+                    } else if (chunk < used) {
+                        const u32x4 zero{0, 0, 0, 0};
+                        *reinterpret_cast<u32x4 *>(keys + (i + lane) * 16) = zero;
+                        *reinterpret_cast<u32x4 *>(values + (i + lane) * 16) = zero;
+                    }
+                }
+            }
+        };
+        __syncthreads(); // the segment before is done with
+        if (stages != 0)
+            ask_table(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        place_rows(0);
+        __syncthreads();
+        if (stages != 0)
+            fetch(0);
+        for (uint32_t s = 0; s < stages; s++) {
+            char *keys = stage[s % S::kBuffers][0], *values = stage[s % S::kBuffers][1];
+            uint32_t *odd_rows = strange[s % 2]; // the other stage's may still be read
+            const uint32_t row = begin + s * R;
+            const bool drafted = row + R > held;
+            if constexpr (TYPE == NUT_F32) {
+                if (s != 0)
+                    __syncthreads(); // the stage before is done with
+                if (threadIdx.x < 2)
+                    odd_rows[threadIdx.x] = 0;
+                if (drafted)
+                    __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kHeld; w++) {
+                    const uint32_t i = w * 256 + threadIdx.x, own = i / S::kChunks;
+                    const bool there = kWork != 0 || own < uint32_t(R);
+                    if (drafted) { // values that are not finite are added one by one
+                        bool odd = false;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const bool is = !(fabsf(ahead[1][w][e]) < INFINITY);
+                            odd = odd || is;
+                            ahead[1][w][e] = is ? 0.0f : ahead[1][w][e];
+                        }
+                        if (odd && there)
+                            atomicOr(&odd_rows[own / 32], 1u << (own % 32));
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        u32x4 limb[3];
+                        split<NUT_BF16, 3>(ahead[x][w], limb);
+                        if (there)
+#pragma unroll
+                            for (int p = 0; p < 3; p++)
+                                *reinterpret_cast<u32x4 *>(
+                                    (x == 0 ? keys : values) +
+                                    S::place(p * R * S::kChunks + i) * 16) = limb[p];
+                    }
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // a table that was asked for
+                __syncthreads();
+                if (s % kEach == 0 && more(s))
+                    ask_table(s / kEach + 1);
+                if (s % kEach == 1 && more(s))
+                    place_rows(s / kEach + 1);
+                if (s + 1 < stages)
+                    fetch(s + 1);
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                if (drafted && threadIdx.x < 2)
+                    odd_rows[threadIdx.x] = 0;
+                __syncthreads(); // the stage is there, the one before done with
+                if (s % kEach == 0 && more(s)) // older than the stage that follows it
+                    ask_table(s / kEach + 1);
+                if (s % kEach == 1 && more(s)) // first read one barrier from here
+                    place_rows(s / kEach + 1);
+                if (s + 1 < stages)
+                    fetch(s + 1);
+                if (drafted) {
+                    for (uint32_t i = threadIdx.x; i < uint32_t(R) * S::kChunks; i += 256) {
+                        const uint32_t from = S::place(i), own = from / S::kChunks;
+                        if (from % S::kChunks >= used) // no chunk of a row: never written
+                            continue;
+                        u32x4 *v = reinterpret_cast<u32x4 *>(values + i * 16);
+                        u32x4 x = *v;
+                        bool odd = false;
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            constexpr uint32_t e = TYPE == NUT_F16 ? 0x7c00u : 0x7f80u;
+                            const bool lo = (x[w] & e) == e, hi = (x[w] >> 16 & e) == e;
+                            odd = odd || lo || hi;
+                            x[w] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                        }
+                        if (odd) {
+                            *v = x;
+                            atomicOr(&odd_rows[own / 32], 1u << (own % 32));
+                        }
+                    }
+                    __syncthreads();
+                }
+            }
+            if (first >= queries)
+                continue;
+            constexpr int kHalves = R / 32;
+            uint32_t none[kHalves], odd[kHalves], seen[QT][kHalves];
+#pragma unroll
+            for (int half = 0; half < kHalves; half++) {
+                none[half] = uint32_t(__builtin_amdgcn_readfirstlane(gone_of(s, half)));
+                odd[half] = drafted ? uint32_t(__builtin_amdgcn_readfirstlane(odd_rows[half])) &
+                                          ~none[half]
+                                    : 0;
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+                    seen[t][half] = !drafted ? ~0u
+                                             : mask_bits(int64_t(row + half * 32) - held, words,
+                                                         [&](uint32_t w) { return mask[t][w]; });
+            }
+            attend_stage<TYPE, HD, FULL, QT>(keys, values, offset_of(s), none, drafted, odd, seen,
+                                             q, sm, kv, lane);
+        }
+
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const uint32_t row = first + t * 16 + column;
+            float sum = sm[t].sum;
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (row >= queries)
+                continue;
+            const size_t at = size_t(nodes.from + row / a.group) * a.heads + h * a.group +
+                              row % a.group;
+            const size_t part = size_t(slot) * kBlock + (row - begins);
+            const float f = cut ? 1.0f : 1.0f / sum;
+            float *to = cut ? a.parts + part * kv.head_dim : a.out + at * kv.head_dim;
+#pragma unroll
+            for (int g = 0; g < G; g++)
+                if (FULL || 16 * g + 4 * j < kv.head_dim)
+                    *reinterpret_cast<f32x4 *>(to + 16 * g + 4 * j) =
+                        !cut && sum == 0.0f ? f32x4{0, 0, 0, 0} : sm[t].o[g] * f;
+            if (j == 0 && cut)
+                a.stats[part] = make_float2(sum == 0.0f ? -INFINITY : sm[t].ref, sum);
+            if (j == 0 && !cut && a.lse != nullptr)
+                a.lse[at] = sum == 0.0f ? -INFINITY
+                                        : (sm[t].ref + log2f(sum)) * 0.69314718055994531f;
+        }
+    }
+}
+
+// The shares of an item joined, where it was cut: a workgroup an item, a thread
+// for four components of a query row.
+template <int R>
+__global__ __launch_bounds__(256) void staged_join_kernel(TreeArgs a)
+{
+    constexpr int kAtOnce = 8; // shares whose loads are in flight together
+    const uint32_t tpr = a.kv.head_dim / 4, at_once = 256 / tpr; // query rows of a workgroup
+    const uint32_t groups = (kBlock + at_once - 1) / at_once;
+    const uint32_t b = blockIdx.y, item = blockIdx.x / groups;
+    const uint64_t start = a.before[b], all = a.before[a.s.batch];
+    const Item it = item_of<R>(a, b, false);
+    const uint32_t h = it.blocks == 0 ? 0 : item / it.blocks;
+    if (it.blocks == 0 || h >= a.kv.kv_heads)
+        return;
+    const Shares shares{all, share_count(all, a.shares)};
+    const uint64_t begin = start + uint64_t(item) * it.stages;
+    const uint32_t first = shares.of(begin), last = shares.of(begin + it.stages - 1);
+    if (first == last)
+        return;
+    const uint32_t begins = (item - h * it.blocks) * kBlock;
+    const uint32_t queries = it.nodes.count * a.group, rows = min(kBlock, queries - begins);
+    const f32x4 *parts = reinterpret_cast<const f32x4 *>(a.parts);
+    const uint32_t own = threadIdx.x / tpr, k = (blockIdx.x - item * groups) * at_once + own;
+    if (own < at_once && k < rows) {
+        const uint32_t part = threadIdx.x - own * tpr;
+        float most = -INFINITY, sum = 0.0f;
+        f32x4 o{0, 0, 0, 0};
+        for (uint32_t r = first; r <= last; r += kAtOnce) {
+            float2 st[kAtOnce];
+            f32x4 x[kAtOnce];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; e++) { // behind the last: the last again, without weight
+                const uint32_t share = min(r + e, last);
+                // a share's second slot is of the item that it ends in
+                const size_t row = size_t(2 * share + (share == first)) * kBlock + k;
+                st[e] = a.stats[row];
+                x[e] = parts[row * tpr + part];
+            }
+            float now = most;
+#pragma unroll
+            for (int e = 0; e < kAtOnce; e++)
+                now = fmaxf(now, st[e].x);
+            if (now == -INFINITY)
+                continue;
+            const float f = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - now);
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+                o[d] *= f;
+            most = now;
+#pragma unroll
+            for (int e = 0; e < kAtOnce; e++) {
+                if (r + e > last || st[e].x == -INFINITY) // no row of a finite score: not summed
+                    continue;
+                const float g = __builtin_amdgcn_exp2f(st[e].x - now);
+                sum = fmaf(st[e].y, g, sum);
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    o[d] = fmaf(x[e][d], g, o[d]);
+            }
+        }
+        const uint32_t row = begins + k;
+        const size_t at = size_t(it.nodes.from + row / a.group) * a.heads + h * a.group +
+                          row % a.group;
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        *reinterpret_cast<f32x4 *>(a.out + at * a.kv.head_dim + part * 4) = o * f;
+        if (part == 0 && a.lse != nullptr)
+            a.lse[at] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
     }
 }
 
@@ -383,39 +1118,44 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a)
         a.lse[at] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
 }
 
-// Query tiles of a block at most, by what fits the registers of two waves a SIMD.
-constexpr uint32_t most_queries(uint32_t head_dim)
+template <int TYPE, int HD, int QT, int WQ>
+void tree_by(const TreeArgs &a, dim3 grid, hipStream_t stream)
 {
-    return head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;
-}
-
-template <int TYPE, int HD>
-void tree_as(const TreeArgs &a, uint32_t queries, dim3 grid, hipStream_t stream)
-{
-    const bool full = a.kv.head_dim == HD;
-    auto run = full ? tree_kernel<TYPE, HD, true, 1> : tree_kernel<TYPE, HD, false, 1>;
-    if constexpr (most_queries(HD) >= 2)
-        if (queries == 2)
-            run = full ? tree_kernel<TYPE, HD, true, 2> : tree_kernel<TYPE, HD, false, 2>;
-    if constexpr (most_queries(HD) >= 4)
-        if (queries == 4)
-            run = full ? tree_kernel<TYPE, HD, true, 4> : tree_kernel<TYPE, HD, false, 4>;
+    const auto run = a.kv.head_dim == HD ? tree_kernel<TYPE, HD, true, QT, WQ>
+                                         : tree_kernel<TYPE, HD, false, QT, WQ>;
     hipLaunchKernelGGL(run, grid, dim3(64 * kTreeWaves<HD>), 0, stream, a);
 }
 
+template <int TYPE, int HD>
+void tree_as(const TreeArgs &a, const TreePlan &plan, dim3 grid, hipStream_t stream)
+{
+    const bool full = a.kv.head_dim == HD;
+    if (plan.staged) {
+        const auto run = full ? staged_kernel<TYPE, HD, true> : staged_kernel<TYPE, HD, false>;
+        const auto join = staged_join_kernel<Stage<TYPE, HD>::kRows>;
+        hipLaunchKernelGGL(run, dim3(plan.shares), dim3(256), 0, stream, a);
+        check_launch("tree attention");
+        hipLaunchKernelGGL(join, grid, dim3(256), 0, stream, a);
+    } else if (plan.waves == 1) {
+        tree_by<TYPE, HD, 1, 1>(a, grid, stream);
+    } else {
+        tree_by<TYPE, HD, 1, 2>(a, grid, stream);
+    }
+}
+
 template <int TYPE>
-void tree_in(const TreeArgs &a, uint32_t queries, dim3 grid, hipStream_t stream)
+void tree_in(const TreeArgs &a, const TreePlan &plan, dim3 grid, hipStream_t stream)
 {
     if (a.kv.head_dim <= 32)
-        tree_as<TYPE, 32>(a, queries, grid, stream);
+        tree_as<TYPE, 32>(a, plan, grid, stream);
     else if (a.kv.head_dim <= 64)
-        tree_as<TYPE, 64>(a, queries, grid, stream);
+        tree_as<TYPE, 64>(a, plan, grid, stream);
     else if (a.kv.head_dim <= 96)
-        tree_as<TYPE, 96>(a, queries, grid, stream);
+        tree_as<TYPE, 96>(a, plan, grid, stream);
     else if (a.kv.head_dim <= 128)
-        tree_as<TYPE, 128>(a, queries, grid, stream);
+        tree_as<TYPE, 128>(a, plan, grid, stream);
     else
-        tree_as<TYPE, 256>(a, queries, grid, stream);
+        tree_as<TYPE, 256>(a, plan, grid, stream);
 }
 
 } // namespace
@@ -426,11 +1166,30 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
     const auto aligned = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
     TreePlan plan{};
     const uint64_t queries = uint64_t(draft.most) * (heads / kv.kv_heads);
-    require(queries <= 0x7fffffff, NUT_EINVAL, "paged cache: more rows than one launch covers");
-    plan.queries = 1;
-    while (plan.queries < most_queries(kv.head_dim) && plan.queries * 16 < queries)
-        plan.queries *= 2;
-    plan.blocks = uint32_t((queries + plan.queries * 16 - 1) / (plan.queries * 16));
+    require(queries * kv.kv_heads <= 0x7fffffff, NUT_EINVAL,
+            "paged cache: more rows than one launch covers");
+    // Workgroups that 16 query rows and 128 rows of a sequence make.
+    const uint64_t small = uint64_t(draft.batch) * kv.kv_heads * ((queries + 15) / 16) *
+                           ((seqs.max_length + 127) / 128);
+    plan.staged = queries > 32 && small > 1024;
+    if (plan.staged) {
+        // as many workgroups as the chip holds at once, by registers and shared memory
+        plan.shares = 256 * staged_groups(kv.type, kv.head_dim);
+        plan.blocks = uint32_t((queries + kBlock - 1) / kBlock);
+        // Rows that are read once, and are more than the caches hold: nothing of them is
+        // there when the next call comes.
+        plan.past = plan.blocks == 1 && uint64_t(seqs.max_length) * draft.batch * kv.kv_heads *
+                                                kv.head_dim * 2 * paged_element(kv.type) >=
+                                            (128ull << 20);
+        require(draft.batch <= 65535, NUT_EINVAL, "paged cache: more rows than one launch covers");
+        paged_grid(uint64_t(draft.batch) * kv.kv_heads * plan.blocks * kBlock, 256);
+        plan.stats = aligned(size_t(plan.shares) * 2 * kBlock * kv.head_dim * sizeof(float));
+        plan.before = plan.stats + aligned(size_t(plan.shares) * 2 * kBlock * sizeof(float2));
+        plan.bytes = plan.before + aligned((size_t(draft.batch) + 1) * sizeof(uint64_t));
+        return plan;
+    }
+    plan.waves = queries > 16 && small > 1024 ? 2 : 1;
+    plan.blocks = uint32_t((queries + 16 * plan.waves - 1) / (16 * plan.waves));
     const uint64_t columns = uint64_t(draft.batch) * kv.kv_heads * plan.blocks;
     // Runs as long as make 1,024 workgroups, or down to 128 rows.
     plan.run = (seqs.max_length + 127) / 128 * 128;
@@ -457,20 +1216,24 @@ void launch_tree_attention(const PagedView &kv, const PagedSeqs &seqs, const Dra
     const uint64_t units = uint64_t(draft.batch) * kv.kv_heads * plan.runs;
     TreeArgs a{kv, seqs, draft, query, query_stride, heads, heads / kv.kv_heads,
                scale * 1.4426950408889634f, out, lse, plan.blocks, plan.run, plan.runs,
-               uint32_t(units), nullptr, nullptr};
-    if (plan.runs > 1) {
+               uint32_t(units), plan.shares, plan.past, nullptr, nullptr, nullptr};
+    if (plan.bytes != 0) {
         a.parts = reinterpret_cast<float *>(workspace);
         a.stats = reinterpret_cast<float2 *>(workspace + plan.stats);
+        a.before = reinterpret_cast<uint64_t *>(workspace + plan.before);
     }
-    const dim3 grid = paged_grid((units + 7) / 8 * 8 * plan.blocks, 256);
+    const uint32_t joined = 256 / (kv.head_dim / 4); // query rows of a workgroup of the join
+    const dim3 grid = plan.staged ? dim3(kv.kv_heads * plan.blocks * ((kBlock + joined - 1) / joined),
+                                         draft.batch)
+                                  : paged_grid((units + 7) / 8 * 8 * plan.blocks, 256);
     if (kv.type == NUT_F32)
-        tree_in<NUT_F32>(a, plan.queries, grid, stream);
+        tree_in<NUT_F32>(a, plan, grid, stream);
     else if (kv.type == NUT_F16)
-        tree_in<NUT_F16>(a, plan.queries, grid, stream);
+        tree_in<NUT_F16>(a, plan, grid, stream);
     else
-        tree_in<NUT_BF16>(a, plan.queries, grid, stream);
+        tree_in<NUT_BF16>(a, plan, grid, stream);
     check_launch("tree attention");
-    if (plan.runs == 1)
+    if (plan.staged || plan.runs == 1)
         return;
     const uint64_t threads = uint64_t(draft.most) * heads * (kv.head_dim / 4);
     hipLaunchKernelGGL(tree_join_kernel, dim3(uint32_t((threads + 255) / 256), draft.batch),
