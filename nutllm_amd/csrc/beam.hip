@@ -21,6 +21,7 @@ namespace nut {
 namespace {
 
 constexpr uint32_t kMostParts = 64;   // of a beam's logits: a lane each
+constexpr int kFound = 64;           // keys that a wave ranks at once
 constexpr uint32_t kMostListed = 2048; // keys of a beam's parts: 32 parts of 64
 
 struct Part {
@@ -64,14 +65,27 @@ __device__ __forceinline__ uint64_t rank_key(double v)
     return u >> 63 ? ~u : u | (uint64_t(1) << 63);
 }
 
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ uint32_t dpp_max(uint32_t v)
+{
+    return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xF, false)));
+}
+
+// The largest of a wave's values, in every lane: 12 moves within the registers, the
+// upper halves first (through shared memory 64-bit values took 600 cycles).
+__device__ __forceinline__ uint32_t wave_most(uint32_t v)
+{
+    v = dpp_max<kDppQuadSwap1>(v);
+    v = dpp_max<kDppQuadSwap2>(v);
+    v = dpp_max<kDppRowHalfMirror>(v);
+    v = dpp_max<kDppRowMirror>(v);
+    v = dpp_max<kDppRowBcast15, 0xA>(v);
+    v = dpp_max<kDppRowBcast31, 0xC>(v);
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+}
 __device__ __forceinline__ uint64_t wave_most(uint64_t v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t x = uint64_t(__shfl_xor((unsigned long long)v, o));
-        v = x > v ? x : v;
-    }
-    return v;
+    const uint32_t hi = wave_most(uint32_t(v >> 32));
+    return uint64_t(hi) << 32 | wave_most(uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
 }
 
 // exp(d), d <= 0: the exponent in base 2 in two pieces, so that the error is
@@ -79,7 +93,7 @@ __device__ __forceinline__ uint64_t wave_most(uint64_t v)
 __device__ __forceinline__ float exp_below(float d)
 {
     const float t = d * 1.44269504f;
-    const float rest = fmaf(d, 1.44269504f, -t) + d * 1.92596299e-8f;
+    const float rest = fmaf(d, 1.92596299e-8f, fmaf(d, 1.44269504f, -t));
     const float e = __builtin_amdgcn_exp2f(t);
     return fmaf(e, rest * 0.69314718f, e);
 }
@@ -130,17 +144,25 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
             }
         }
     }
-    float most = v[0];
+    float most = v[0], odd = v[0]; // `odd`: not a number after one that is none
 #pragma unroll
-    for (int e = 1; e < EACH; e++)
+    for (int e = 1; e < EACH; e++) {
         most = fmaxf(most, v[e]);
+        odd = __builtin_elementwise_maximum(odd, v[e]);
+    }
     const float top = wave_max(most);
     double sum = 0.0;
+    if (__any(odd != odd) || top == INFINITY) {
+        sum = NAN;
+    } else if (top > -INFINITY) {
 #pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        // all of the part minus infinity: no sum, but for what is no number
-        const float d = top == -INFINITY && v[e] == -INFINITY ? -INFINITY : v[e] - top;
-        sum += double(exp_below(d < -200.0f ? -200.0f : d)); // that is 0 in 32 bits
+        for (int e = 0; e < EACH; e += 4) { // four in 32 bits, whose error is an exponential's
+            float four[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                four[k] = exp_below(fmaxf(v[e + k] - top, -200.0f)); // that is 0 in 32 bits
+            sum += double((four[0] + four[1]) + (four[2] + four[3]));
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
@@ -149,30 +171,77 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
     if (lane == 0)
         a.stats[slot] = Part{top, 0, sum};
 
-    // The keep largest, one after another: each lane's largest left, and the wave's.
+    // The keep largest. A bound first: the keep-th largest of the lanes' own largest,
+    // below which none of them is; then all keys from it on, few where the largest are
+    // spread over the lanes, at most keep lanes' where they are not.
     const uint32_t keep = a.to.beams;
-    uint64_t mine = 0;
-    const auto largest_below = [&](uint64_t bound) {
-        uint64_t best = 0;
-#pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const uint32_t at = part * kPart + (e / kRun * kWave + lane) * kRun + e % kRun;
-            const uint64_t key = key_of(v[e], at);
-            if (at < a.vocab && key < bound && key > best)
-                best = key;
-        }
-        return best;
+    const auto at = [&](int e) {
+        return part * kPart + (e / kRun * kWave + lane) * kRun + e % kRun;
     };
-    mine = largest_below(~uint64_t(0));
+    // Logits of minus infinity, and what is behind the vocabulary, are no candidates.
+    const auto key = [&](int e) { return v[e] > -INFINITY ? key_of(v[e], at(e)) : 0; };
+    uint32_t first = 0;
+#pragma unroll
+    for (int e = EACH - 1; e >= 0; e--)
+        first = v[e] == most ? at(e) : first;
+    uint64_t mine = most > -INFINITY ? key_of(most, first) : 0, left = mine, bound = 0;
+    if (keep < uint32_t(kWave)) {
+        for (uint32_t k = 0; k < keep; k++) {
+            bound = wave_most(left);
+            left = left == bound ? 0 : left;
+        }
+    } else {
+        bound = ~wave_most(~mine); // the least of 64
+    }
+    const bool few = bound == 0; // fewer lanes than that have any
+    const float least = few ? -INFINITY : logit_of(bound);
+    __shared__ uint64_t found[kFound];
+    uint32_t count = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        if (!__any(v[e] >= least && (!few || v[e] > -INFINITY)))
+            continue;
+        const uint64_t k = key(e);
+        const bool in = k != 0 && k >= bound;
+        const uint64_t those = __ballot(in);
+        const uint32_t to = count + __popcll(those & ((uint64_t(1) << lane) - 1));
+        if (in && to < uint32_t(kFound))
+            found[to] = k;
+        count += uint32_t(__popcll(those));
+    }
     uint64_t kept = 0; // the lane-th largest
-    for (uint32_t k = 0; k < keep; k++) {
-        const uint64_t now = wave_most(mine);
-        if (now == 0)
-            break;
-        if (lane == k)
-            kept = now;
-        if (mine == now)
-            mine = largest_below(now);
+    if (count <= uint32_t(kWave)) {
+        __syncthreads();
+        const uint64_t own = lane < count ? found[lane] : 0;
+        uint32_t above = 0;
+        for (uint32_t k = 0; k < count; k++) {
+            const uint64_t other =
+                uint64_t(uint32_t(__builtin_amdgcn_readlane(int(own >> 32), k))) << 32 |
+                uint32_t(__builtin_amdgcn_readlane(int(own), k));
+            above += other > own;
+        }
+        __syncthreads();
+        if (lane < count)
+            found[above] = own; // keys differ by their tokens
+        __syncthreads();
+        kept = lane < count ? found[lane] : 0;
+    } else { // one after another: each lane's largest left, and the wave's
+        for (uint32_t k = 0; k < keep; k++) {
+            const uint64_t now = wave_most(mine);
+            if (now == 0)
+                break;
+            if (lane == k)
+                kept = now;
+            if (mine == now) {
+                mine = 0;
+#pragma unroll
+                for (int e = 0; e < EACH; e++) {
+                    const uint64_t x = key(e);
+                    if (x < now && x > mine)
+                        mine = x;
+                }
+            }
+        }
     }
     if (lane < keep)
         a.best[slot * keep + lane] = kept;
@@ -307,12 +376,15 @@ uint32_t parts_of(uint32_t vocab, uint32_t each)
 }
 
 // Logits a lane holds, 16 to 128: the fewest whose parts fit a wave, and their
-// lists its shared memory. 128 do for kMostVocab.
-uint32_t each_of(uint32_t vocab, uint32_t keep)
+// lists its shared memory; 128 do for kMostVocab. 32 rather than 16 where that leaves
+// 8,192 waves: each finds its own largest, and lists them for the second launch (512
+// beams, 100,003 fp16 logits: 59 us of 32, 62 of 64, 121 of 128).
+uint32_t each_of(uint32_t rows, uint32_t vocab, uint32_t keep)
 {
     uint32_t each = 16;
     while (each < 128 && (parts_of(vocab, each) > kMostParts ||
-                          parts_of(vocab, each) * keep > kMostListed))
+                          parts_of(vocab, each) * keep > kMostListed ||
+                          (each < 32 && uint64_t(rows) * parts_of(vocab, each) > 8192)))
         each *= 2;
     return each;
 }
@@ -320,7 +392,7 @@ uint32_t each_of(uint32_t vocab, uint32_t keep)
 size_t carve(BeamArgs &a, char *base)
 {
     const auto aligned = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-    a.parts = parts_of(a.vocab, each_of(a.vocab, a.to.beams));
+    a.parts = parts_of(a.vocab, each_of(a.from.requests * a.from.beams, a.vocab, a.to.beams));
     const size_t parts = size_t(a.from.requests) * a.from.beams * a.parts;
     a.stats = reinterpret_cast<Part *>(base);
     a.best = reinterpret_cast<uint64_t *>(base + aligned(parts * sizeof(Part)));
@@ -329,7 +401,7 @@ size_t carve(BeamArgs &a, char *base)
 
 template <int TYPE> void scan_as(const BeamArgs &a, dim3 grid, hipStream_t stream)
 {
-    const uint32_t each = each_of(a.vocab, a.to.beams);
+    const uint32_t each = each_of(a.from.requests * a.from.beams, a.vocab, a.to.beams);
     const auto run = each == 16   ? scan_kernel<TYPE, 16>
                      : each == 32 ? scan_kernel<TYPE, 32>
                      : each == 64 ? scan_kernel<TYPE, 64>
