@@ -513,6 +513,22 @@ public:
         check_status(nut_paged_evict(&view_, &seqs, &history, budget, first, last, d_new_lengths,
                                      d_workspace, workspace_bytes, stream));
     }
+    size_t tree_attention_workspace(const nut_paged_batch &seqs, const nut_draft &draft,
+                                    size_t heads) const
+    {
+        return bytes(nut_paged_tree_attention_workspace(&view_, &seqs, &draft, heads));
+    }
+    // Attention of every node of a draft tree over its sequence's rows and the nodes
+    // that its mask names.
+    void tree_attention(const nut_paged_batch &seqs, const nut_draft &draft, const float *d_query,
+                        size_t heads, float scale, float *d_out, void *d_workspace,
+                        size_t workspace_bytes, float *d_lse = nullptr, size_t query_stride = 0,
+                        void *stream = nullptr) const
+    {
+        check_status(nut_paged_tree_attention(&view_, &seqs, &draft, d_query, query_stride, heads,
+                                              scale, d_out, d_lse, d_workspace, workspace_bytes,
+                                              stream));
+    }
     void check() const { check_status(nut_paged_check(&view_)); }
 
 private:
@@ -526,6 +542,121 @@ private:
 
     nut_paged_kv view_;
 };
+
+// Waits, then throws for what earlier calls with this status word could not follow.
+inline void check_status_word(int *d_status) { check(nut_status_check(d_status)); }
+
+namespace detail {
+inline size_t workspace_bytes(size_t count)
+{
+    if (count == SIZE_MAX)
+        check(NUT_EINVAL);
+    return count;
+}
+} // namespace detail
+
+// Drafted tokens behind each sequence, as trees: a nut_draft over device memory that
+// the caller holds (no reference counterpart).
+class DraftTree {
+public:
+    explicit DraftTree(const nut_draft &view) : view_(view) {}
+    const nut_draft &view() const { return view_; }
+
+    // Every node's mask, itself and its ancestors, and its depth (may be null).
+    void build(int *d_depths = nullptr, void *stream = nullptr) const
+    {
+        check(nut_draft_mask(&view_, d_depths, stream));
+    }
+    // The nodes that the model agrees with: d_path [batch][path_stride].
+    void accept(const nut_paged_batch &seqs, const int *d_tokens, const int *d_chosen, int *d_path,
+                size_t path_stride, int *d_counts, int *d_last = nullptr,
+                int *d_new_lengths = nullptr, void *stream = nullptr) const
+    {
+        check(nut_draft_accept(&view_, &seqs, d_tokens, d_chosen, d_path, path_stride, d_counts,
+                               d_last, d_new_lengths, stream));
+    }
+
+private:
+    nut_draft view_;
+};
+
+// The views of a cache's layers, all of one shape: what one call does in every layer.
+class PagedLayers {
+public:
+    explicit PagedLayers(std::vector<nut_paged_kv> layers) : layers_(std::move(layers)) {}
+
+    // Rows of accepted nodes move behind their sequences' rows.
+    void keep(const nut_paged_batch &seqs, const int *d_path, size_t path_stride,
+              const int *d_counts, void *stream = nullptr) const
+    {
+        check(nut_paged_keep(layers_.data(), layers_.size(), &seqs, d_path, path_stride, d_counts,
+                             stream));
+    }
+    // The first `rows` rows of pages, d_copies [copies][3] of {from, to, rows}.
+    void copy(const int *d_copies, size_t copies, void *stream = nullptr) const
+    {
+        check(nut_paged_copy(layers_.data(), layers_.size(), d_copies, copies, stream));
+    }
+
+private:
+    std::vector<nut_paged_kv> layers_;
+};
+
+// Who holds a cache's pages: a nut_page_pool over counts that the caller zeroed.
+class PagePool {
+public:
+    explicit PagePool(const nut_page_pool &view) : view_(view) {}
+
+    size_t reorder_workspace(const nut_page_table &from, const nut_page_table &to) const
+    {
+        return detail::workspace_bytes(nut_pages_reorder_workspace(&view_, &from, &to));
+    }
+    // Sequence i of `to` goes on with sequence d_parents[i] of `from` (-1: none), with
+    // pages for d_gains[i], or `gain`, more rows.
+    void reorder(const nut_page_table &from, const nut_page_table &to, const int *d_parents,
+                 const int *d_gains, size_t gain, int *d_copies, void *d_workspace,
+                 size_t workspace_bytes, void *stream = nullptr) const
+    {
+        check(nut_pages_reorder(&view_, &from, &to, d_parents, d_gains, gain, d_copies, d_workspace,
+                                workspace_bytes, stream));
+    }
+    size_t compact_workspace(const nut_page_table &table) const
+    {
+        return detail::workspace_bytes(nut_pages_compact_workspace(&view_, &table));
+    }
+    // Pages from `limit` on move to free ones below it.
+    void compact(const nut_page_table &table, size_t limit, int *d_copies, size_t copies,
+                 void *d_workspace, size_t workspace_bytes, void *stream = nullptr) const
+    {
+        check(nut_pages_compact(&view_, &table, limit, d_copies, copies, d_workspace,
+                                workspace_bytes, stream));
+    }
+
+private:
+    nut_page_pool view_;
+};
+
+// The best continuations of each request's beams.
+inline size_t beam_select_workspace(const nut_beams &from, const nut_beams &to, size_t vocab)
+{
+    return detail::workspace_bytes(nut_beam_select_workspace(&from, &to, vocab));
+}
+inline void beam_select(const nut_beams &from, const nut_beams &to, const void *d_logits, int type,
+                        size_t vocab, int eos, float power, int *d_parents, int *d_tokens,
+                        void *d_workspace, size_t workspace_bytes, size_t row_stride = 0,
+                        void *stream = nullptr)
+{
+    check(nut_beam_select(&from, &to, d_logits, type, row_stride, vocab, eos, power, d_parents,
+                          d_tokens, d_workspace, workspace_bytes, stream));
+}
+// Row i of d_to gets row d_parents[i] of d_from.
+inline void beam_gather(const void *d_from, size_t sources, void *d_to, size_t rows,
+                        size_t row_bytes, const int *d_parents, int *d_status = nullptr,
+                        size_t from_stride = 0, size_t to_stride = 0, void *stream = nullptr)
+{
+    check(nut_beam_gather(d_from, from_stride, sources, d_to, to_stride, rows, row_bytes, d_parents,
+                          d_status, stream));
+}
 
 inline void matvec_quantized_threaded(const QuantizedMatrix &matrix,
                                       const float *vector, float *output,

@@ -455,7 +455,6 @@ void launch_beam_gather(const char *source, size_t from_stride, uint32_t sources
     const size_t words = row_bytes / (wide ? 16 : 4);
     // 4 words a thread, as far as one launch covers them
     const uint64_t most = 0xffffffffull / 256 / rows;
-    require(most != 0, NUT_EINVAL, "beam gather: more rows than one launch covers");
     const uint32_t blocks = uint32_t(std::min<uint64_t>((words + 1023) / 1024, most));
     hipLaunchKernelGGL(wide ? gather_kernel<uint4> : gather_kernel<uint32_t>, dim3(rows * blocks),
                        dim3(256), 0, stream, source, from_stride, sources, to, to_stride, words,

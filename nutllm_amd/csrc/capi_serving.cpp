@@ -228,6 +228,8 @@ int nut_paged_keep(const nut_paged_kv *layers, size_t count, const nut_paged_bat
         require(d_path != nullptr && d_counts != nullptr, NUT_EINVAL, "paged cache: null pointer");
         require(path_stride != 0 && path_stride <= kMost, NUT_EINVAL,
                 "draft tree: paths shorter than the nodes");
+        nut::paged_grid(uint64_t(s.batch) * layers->kv_heads *
+                            std::min<size_t>(count, nut::kMostLayers), 64);
         each_launch(layers, count, [&](const nut::PagedLayers &l) {
             nut::launch_paged_keep(l, s, d_path, path_stride, d_counts, as_stream(stream));
         });
@@ -364,6 +366,8 @@ int nut_beam_gather(const void *d_from, size_t from_stride, size_t sources, void
                  from_stride | to_stride | row_bytes) % 4 == 0,
                 NUT_EINVAL, "beam gather: rows must be multiples of 4 bytes");
         require(to_stride >= row_bytes || rows == 1, NUT_EINVAL, "beam gather: rows overlap");
+        require(rows <= 0xffffffff / 256, NUT_EINVAL,
+                "beam gather: more rows than one launch covers");
         require(disjoint(d_to, double(to_stride) * double(rows - 1) + double(row_bytes), d_from,
                          double(from_stride) * double(sources - 1) + double(row_bytes)),
                 NUT_EINVAL, "beam gather: rows overlap");
