@@ -144,25 +144,19 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
             }
         }
     }
-    float most = v[0], odd = v[0]; // `odd`: not a number after one that is none
+    float most = v[0];
 #pragma unroll
-    for (int e = 1; e < EACH; e++) {
+    for (int e = 1; e < EACH; e++)
         most = fmaxf(most, v[e]);
-        odd = __builtin_elementwise_maximum(odd, v[e]);
-    }
-    const float top = wave_max(most);
+    const float top = wave_max(most), base = top == -INFINITY ? 0.0f : top;
     double sum = 0.0;
-    if (__any(odd != odd) || top == INFINITY) {
-        sum = NAN;
-    } else if (top > -INFINITY) {
 #pragma unroll
-        for (int e = 0; e < EACH; e += 4) { // four in 32 bits, whose error is an exponential's
-            float four[4];
+    for (int e = 0; e < EACH; e += 4) { // four in 32 bits, whose error is an exponential's
+        float four[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                four[k] = exp_below(fmaxf(v[e + k] - top, -200.0f)); // that is 0 in 32 bits
-            sum += double((four[0] + four[1]) + (four[2] + four[3]));
-        }
+        for (int k = 0; k < 4; k++) // exp(-200) is 0 in 32 bits; what is no number stays that
+            four[k] = exp_below(__builtin_elementwise_maximum(v[e + k] - base, -200.0f));
+        sum += double((four[0] + four[1]) + (four[2] + four[3]));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
@@ -180,21 +174,17 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
     };
     // Logits of minus infinity, and what is behind the vocabulary, are no candidates.
     const auto key = [&](int e) { return v[e] > -INFINITY ? key_of(v[e], at(e)) : 0; };
-    uint32_t first = 0;
-#pragma unroll
-    for (int e = EACH - 1; e >= 0; e--)
-        first = v[e] == most ? at(e) : first;
-    uint64_t mine = most > -INFINITY ? key_of(most, first) : 0, left = mine, bound = 0;
+    uint32_t left = most > -INFINITY ? uint32_t(key_of(most, 0) >> 32) : 0, bound = 0;
     if (keep < uint32_t(kWave)) {
-        for (uint32_t k = 0; k < keep; k++) {
+        for (uint32_t k = 0; k < keep; k++) { // equal ones go together: a lower bound then
             bound = wave_most(left);
             left = left == bound ? 0 : left;
         }
     } else {
-        bound = ~wave_most(~mine); // the least of 64
+        bound = ~wave_most(~left); // the least of 64
     }
     const bool few = bound == 0; // fewer lanes than that have any
-    const float least = few ? -INFINITY : logit_of(bound);
+    const float least = few ? -INFINITY : logit_of(uint64_t(bound) << 32);
     __shared__ uint64_t found[kFound];
     uint32_t count = 0;
 #pragma unroll
@@ -202,7 +192,7 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
         if (!__any(v[e] >= least && (!few || v[e] > -INFINITY)))
             continue;
         const uint64_t k = key(e);
-        const bool in = k != 0 && k >= bound;
+        const bool in = k != 0 && uint32_t(k >> 32) >= bound;
         const uint64_t those = __ballot(in);
         const uint32_t to = count + __popcll(those & ((uint64_t(1) << lane) - 1));
         if (in && to < uint32_t(kFound))
@@ -226,12 +216,8 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
         __syncthreads();
         kept = lane < count ? found[lane] : 0;
     } else { // one after another: each lane's largest left, and the wave's
+        uint64_t now = ~uint64_t(0), mine = now;
         for (uint32_t k = 0; k < keep; k++) {
-            const uint64_t now = wave_most(mine);
-            if (now == 0)
-                break;
-            if (lane == k)
-                kept = now;
             if (mine == now) {
                 mine = 0;
 #pragma unroll
@@ -241,6 +227,11 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
                         mine = x;
                 }
             }
+            now = wave_most(mine);
+            if (now == 0)
+                break;
+            if (lane == k)
+                kept = now;
         }
     }
     if (lane < keep)

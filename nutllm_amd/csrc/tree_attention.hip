@@ -2,11 +2,12 @@
 // cache.
 //
 // The query rows of a KV head are its sequence's nodes times the heads that
-// share it, node after node. A workgroup takes a block of them and a run of the
-// sequence's rows; its waves take tiles of the run in turn, as in
-// paged_attention.hip, but multiply a tile in registers with QT tiles of 16
-// query rows, not one. Rows that the sequence held before are seen by every node;
-// of a tile that reaches into the drafted rows each lane takes its node's mask.
+// share it, node after node. Rows that the sequence held before are seen by every
+// node; of a tile that reaches into the drafted rows each lane takes its node's mask.
+// Few query rows, or little work: tree_kernel, whose workgroups take 16 or 32 of
+// them and a run of the sequence's rows, in registers as in paged_attention.hip.
+// Many: staged_kernel, whose workgroups take 64 and share rows in shared memory.
+// A second launch joins the parts of either.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -72,23 +73,19 @@ template <int TYPE> __device__ __forceinline__ float component(const char *row, 
     return TYPE == NUT_BF16 ? from_bf16(bits) : from_f16(bits);
 }
 
-// A tile against QT tiles of query rows. `gone`: rows that no node sees, the
-// same in every lane; `seen`: with `drafted`, the rows that the lane's node of
-// each query tile sees.
-template <int TYPE, int HD, bool FULL, int QT>
+// A tile against 16 query rows. `gone`: rows that no node sees, the same in every
+// lane; `seen`: with `drafted`, the rows that the lane's node sees.
+template <int TYPE, int HD, bool FULL>
 __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *at, uint32_t gone,
-                                            bool drafted, const uint32_t (&seen)[QT],
-                                            const Query<TYPE, HD> (&q)[QT],
-                                            Softmax<TYPE, HD> (&sm)[QT], const PagedView &kv,
-                                            int lane)
+                                            bool drafted, uint32_t seen,
+                                            const Query<TYPE, HD> &q, Softmax<TYPE, HD> &sm,
+                                            const PagedView &kv, int lane)
 {
     using T = Tile<TYPE, HD>;
     constexpr int G = T::G, E = T::kEach;
     const int j = lane >> 4;
-    float s[QT][T::kScores];
-#pragma unroll
-    for (int t = 0; t < QT; t++)
-        score<TYPE, HD>(tile, q[t], s[t]);
+    float s[T::kScores];
+    score<TYPE, HD>(tile, q, s);
     uint32_t odd = 0; // rows with values that are not finite, which not every node may see
     if (gone != 0 || drafted) {
         const uint32_t none = gone >> (4 * j);
@@ -102,9 +99,7 @@ __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *
                 tile.v[r][w] = out ? 0 : tile.v[r][w];
                 strange = strange || odd_word<TYPE>(tile.v[r][w]);
             }
-#pragma unroll
-            for (int t = 0; t < QT; t++)
-                s[t][r] = out || !(seen[t] >> (4 * j) >> bit & 1) ? -INFINITY : s[t][r];
+            s[r] = out || !(seen >> (4 * j) >> bit & 1) ? -INFINITY : s[r];
             if (drafted) {
                 const uint64_t any = __ballot(strange);
 #pragma unroll
@@ -114,19 +109,16 @@ __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *
         }
         odd = __builtin_amdgcn_readfirstlane(odd);
     }
-    float p[QT][8];
+    float p[8];
+    float most = s[0];
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        float most = s[t][0];
+    for (int r = 1; r < T::kScores; r++)
+        most = fmaxf(most, s[r]);
+    sm.raise(max_over_rows(most));
 #pragma unroll
-        for (int r = 1; r < T::kScores; r++)
-            most = fmaxf(most, s[t][r]);
-        sm[t].raise(max_over_rows(most));
-#pragma unroll
-        for (int r = 0; r < T::kScores; r++) {
-            p[t][r] = __builtin_amdgcn_exp2f(s[t][r] - sm[t].ref);
-            sm[t].sum += p[t][r];
-        }
+    for (int r = 0; r < T::kScores; r++) {
+        p[r] = __builtin_amdgcn_exp2f(s[r] - sm.ref);
+        sm.sum += p[r];
     }
     if (odd != 0) {
         // 0 times what is not finite is no number: such rows leave the product,
@@ -134,23 +126,20 @@ __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *
         for (uint32_t left = odd; left != 0; left &= left - 1) {
             const int row = __builtin_ctz(left), own = row % 16 / 4;
             const char *v = kv.values + at[row];
+            float weight = 0.0f;
 #pragma unroll
-            for (int t = 0; t < QT; t++) {
-                float weight = 0.0f;
+            for (int r = 0; r < T::kScores; r++)
+                if (16 * (r / 4) + r % 4 == row - 4 * own)
+                    weight = p[r];
+            weight = __shfl(weight, 16 * own + (lane & 15));
 #pragma unroll
-                for (int r = 0; r < T::kScores; r++)
-                    if (16 * (r / 4) + r % 4 == row - 4 * own)
-                        weight = p[t][r];
-                weight = __shfl(weight, 16 * own + (lane & 15));
+            for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int g = 0; g < G; g++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t d = 16 * (g / E * E) + 4 * j * E + i * E + g % E;
-                        if (weight != 0.0f && (FULL || d < kv.head_dim))
-                            sm[t].o[g][i] = fmaf(weight, component<TYPE>(v, d), sm[t].o[g][i]);
-                    }
-            }
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t d = 16 * (g / E * E) + 4 * j * E + i * E + g % E;
+                    if (weight != 0.0f && (FULL || d < kv.head_dim))
+                        sm.o[g][i] = fmaf(weight, component<TYPE>(v, d), sm.o[g][i]);
+                }
         }
 #pragma unroll
         for (int r = 0; r < T::kScores; r++)
@@ -163,31 +152,25 @@ __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int g = 0; g < G; g++)
-#pragma unroll
-                for (int t = 0; t < QT; t++)
-                    sm[t].o[g] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                        __uint_as_float(tile.v[r][g]), p[t][r], sm[t].o[g], 0, 0, 0);
+                sm.o[g] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    __uint_as_float(tile.v[r][g]), p[r], sm.o[g], 0, 0, 0);
     } else {
         constexpr int kLimbs = Query<TYPE, HD>::kLimbs;
-        u32x4 limb[QT][kLimbs];
-#pragma unroll
-        for (int t = 0; t < QT; t++)
-            split<TYPE, kLimbs>(p[t], limb[t]);
+        u32x4 limb[kLimbs];
+        split<TYPE, kLimbs>(p, limb);
 #pragma unroll
         for (int g = 0; g < G; g++) {
             const u32x4 x = tile.component(g);
 #pragma unroll
             for (int l = kLimbs - 1; l >= 0; l--)
-#pragma unroll
-                for (int t = 0; t < QT; t++)
-                    sm[t].o[g] = product<TYPE>(x, limb[t][l], sm[t].o[g]);
+                sm.o[g] = product<TYPE>(x, limb[l], sm.o[g]);
         }
     }
 }
 
 template <int HD> constexpr int kTreeWaves = HD == 256 ? 2 : 4;
 
-template <int TYPE, int HD, bool FULL, int QT, int WQ>
+template <int TYPE, int HD, bool FULL, int WQ>
 __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
 {
     using T = Tile<TYPE, HD>;
@@ -211,7 +194,7 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
     const uint32_t b = unit / a.runs / kv.kv_heads;
     const bool leader = threadIdx.x == 0 && c == 0 && h == 0 && block == 0;
     const NodeSpan nodes = nodes_of(a.d, b, leader);
-    const uint32_t queries = nodes.count * a.group, begins = block * QT * 16 * WQ;
+    const uint32_t queries = nodes.count * a.group, begins = block * 16 * WQ;
     if (begins >= queries)
         return;
     uint32_t held;
@@ -225,25 +208,18 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int j = lane >> 4, column = lane & 15;
     const int wq = wave % WQ, wk = wave / WQ;
-    const uint32_t first = begins + wq * QT * 16; // of the wave's query rows
-    Query<TYPE, HD> q[QT];
-    const uint32_t *mask[QT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const uint32_t row = first + t * 16 + column;
-        const bool valid = row < queries;
-        const uint32_t node = nodes.from + (valid ? row : begins) / a.group;
-        const uint32_t head = h * a.group + (valid ? row : begins) % a.group;
-        q[t].fetch(a.query + node * a.query_stride + size_t(head) * kv.head_dim, valid,
-                   kv.head_dim, lane);
-        mask[t] = a.d.mask + node * a.d.mask_stride;
-    }
+    const uint32_t first = begins + wq * 16; // of the wave's query rows
+    const bool valid = first + column < queries;
+    const uint32_t query = valid ? first + column : begins;
+    const uint32_t node = nodes.from + query / a.group, head = h * a.group + query % a.group;
+    Query<TYPE, HD> q;
+    q.fetch(a.query + node * a.query_stride + size_t(head) * kv.head_dim, valid, kv.head_dim,
+            lane);
+    const uint32_t *mask = a.d.mask + node * a.d.mask_stride;
     const uint32_t words = (nodes.count + 31) / 32;
-#pragma unroll
-    for (int t = 0; t < QT; t++)
-        q[t].convert(a.scale);
+    q.convert(a.scale);
 
-    Softmax<TYPE, HD> sm[QT];
+    Softmax<TYPE, HD> sm;
     for (uint32_t piece = 0; piece < count; piece += kPieceRows) {
         const uint32_t rows = min(count - piece, kPieceRows);
         if (piece != 0)
@@ -272,91 +248,83 @@ __global__ __launch_bounds__(64 * kTreeWaves<HD>, HD == 256 ? 1 : 2) void tree_k
                 gone[t * T::kRows / 32] >> (t * T::kRows % 32) & kAll));
             const uint32_t row = begin + piece + t * T::kRows;
             const bool drafted = row + T::kRows > held;
-            uint32_t seen[QT];
-#pragma unroll
-            for (int k = 0; k < QT; k++)
-                seen[k] = !drafted ? ~0u
-                                   : mask_bits(int64_t(row) - held, words,
-                                               [&](uint32_t w) { return mask[k][w]; });
-            attend_tree<TYPE, HD, FULL, QT>(x, lds.at + t * T::kRows, none, drafted, seen, q, sm,
-                                            kv, lane);
+            const uint32_t seen = !drafted ? ~0u
+                                           : mask_bits(int64_t(row) - held, words,
+                                                       [&](uint32_t w) { return mask[w]; });
+            attend_tree<TYPE, HD, FULL>(x, lds.at + t * T::kRows, none, drafted, seen, q, sm, kv,
+                                        lane);
         }
     }
 
-    // The waves' sums side by side, a tile of each one's query rows at a time; then a
-    // thread per four components adds those of the same rows.
+    // The waves' sums side by side; then a thread per four components adds those of
+    // the same query rows.
     const uint32_t parts = FULL ? HD / 4 : kv.head_dim / 4;
+    sm.sum += __shfl_xor(sm.sum, 16);
+    sm.sum += __shfl_xor(sm.sum, 32);
+    __syncthreads();
+    if (j == 0)
+        stat[0][wave][column] = sm.most, stat[1][wave][column] = sm.ref,
+        stat[2][wave][column] = sm.sum;
+    constexpr int E = T::kEach;
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        if (begins + t * 16 >= queries)
-            break;
-        sm[t].sum += __shfl_xor(sm[t].sum, 16);
-        sm[t].sum += __shfl_xor(sm[t].sum, 32);
-        __syncthreads();
-        if (j == 0)
-            stat[0][wave][column] = sm[t].most, stat[1][wave][column] = sm[t].ref,
-            stat[2][wave][column] = sm[t].sum;
-        constexpr int E = T::kEach;
+    for (int p = 0; p < G; p += E) {
+        float flat[4 * E]; // components 16 p + 4 j E .. of the lane's query row
 #pragma unroll
-        for (int p = 0; p < G; p += E) {
-            float flat[4 * E]; // components 16 p + 4 j E .. of the lane's query row
+        for (int g = 0; g < E; g++)
 #pragma unroll
-            for (int g = 0; g < E; g++)
+            for (int i = 0; i < 4; i++)
+                flat[i * E + g] = sm.o[p + g][i];
+        float *to = lds.o[wave][column] + 16 * p + 4 * j * E;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    flat[i * E + g] = sm[t].o[p + g][i];
-            float *to = lds.o[wave][column] + 16 * p + 4 * j * E;
+        for (int d = 0; d < 4 * E; d += 4)
+            *reinterpret_cast<f32x4 *>(to + d) =
+                f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < WQ * 16 * parts; i += kThreads) {
+        const uint32_t k = i / parts, d = (i - k * parts) * 4, of = k / 16, c16 = k % 16;
+        const uint32_t row = begins + of * 16 + c16;
+        if (row >= queries)
+            continue;
+        float most = stat[0][of][c16];
 #pragma unroll
-            for (int d = 0; d < 4 * E; d += 4)
-                *reinterpret_cast<f32x4 *>(to + d) =
-                    f32x4{flat[d], flat[d + 1], flat[d + 2], flat[d + 3]};
+        for (int w = 1; w < WK; w++)
+            most = fmaxf(most, stat[0][of + w * WQ][c16]);
+        const float ref = most == -INFINITY ? 0.0f : most - Softmax<TYPE, HD>::kShift;
+        float sum = 0.0f;
+        f32x4 o{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < WK; w++) {
+            const int from = of + w * WQ;
+            // what no row of a finite score reached is zero, or not a number
+            const float f = stat[0][from][c16] == -INFINITY
+                                ? 1.0f
+                                : __builtin_amdgcn_exp2f(stat[1][from][c16] - ref);
+            sum = fmaf(stat[2][from][c16], f, sum);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&lds.o[from][c16][d]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                o[e] = fmaf(y[e], f, o[e]);
         }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < WQ * 16 * parts; i += kThreads) {
-            const uint32_t k = i / parts, d = (i - k * parts) * 4, of = k / 16, c16 = k % 16;
-            const uint32_t row = begins + of * QT * 16 + t * 16 + c16;
-            if (row >= queries)
-                continue;
-            float most = stat[0][of][c16];
-#pragma unroll
-            for (int w = 1; w < WK; w++)
-                most = fmaxf(most, stat[0][of + w * WQ][c16]);
-            const float ref = most == -INFINITY ? 0.0f : most - Softmax<TYPE, HD>::kShift;
-            float sum = 0.0f;
-            f32x4 o{0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < WK; w++) {
-                const int from = of + w * WQ;
-                // what no row of a finite score reached is zero, or not a number
-                const float f = stat[0][from][c16] == -INFINITY
-                                    ? 1.0f
-                                    : __builtin_amdgcn_exp2f(stat[1][from][c16] - ref);
-                sum = fmaf(stat[2][from][c16], f, sum);
-                const f32x4 y = *reinterpret_cast<const f32x4 *>(&lds.o[from][c16][d]);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    o[e] = fmaf(y[e], f, o[e]);
-            }
-            const size_t at = size_t(nodes.from + row / a.group) * a.heads + h * a.group +
-                              row % a.group;
-            if (a.parts != nullptr) {
-                *reinterpret_cast<f32x4 *>(a.parts + (at * a.runs + c) * kv.head_dim + d) = o;
-                if (d == 0)
-                    a.stats[at * a.runs + c] = make_float2(sum == 0.0f ? -INFINITY : ref, sum);
-            } else {
-                *reinterpret_cast<f32x4 *>(a.out + at * kv.head_dim + d) =
-                    sum == 0.0f ? f32x4{0, 0, 0, 0} : o * (1.0f / sum);
-                if (d == 0 && a.lse != nullptr)
-                    a.lse[at] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
-            }
+        const size_t at = size_t(nodes.from + row / a.group) * a.heads + h * a.group +
+                          row % a.group;
+        if (a.parts != nullptr) {
+            *reinterpret_cast<f32x4 *>(a.parts + (at * a.runs + c) * kv.head_dim + d) = o;
+            if (d == 0)
+                a.stats[at * a.runs + c] = make_float2(sum == 0.0f ? -INFINITY : ref, sum);
+        } else {
+            *reinterpret_cast<f32x4 *>(a.out + at * kv.head_dim + d) =
+                sum == 0.0f ? f32x4{0, 0, 0, 0} : o * (1.0f / sum);
+            if (d == 0 && a.lse != nullptr)
+                a.lse[at] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
         }
     }
 }
 
 // ---------------------------------------------------------------- staged --
 
-// Many query rows: the four waves hold QT tiles each and share every tile of rows,
-// staged in shared memory. 16-bit rows come by DMA, the next stage while this one
+// Many query rows: the four waves hold 16 each and share every tile of rows, staged
+// in shared memory. 16-bit rows come by DMA, the next stage while this one
 // is multiplied; fp32 rows come through registers and are kept as three bfloat16
 // limbs, whose six largest products with the query's limbs leave out 2^-21 of a
 // product at most and 2^-24 in the mean: 2.7 times the rate of the fp32
@@ -413,20 +381,20 @@ __device__ __forceinline__ void stage_dma(const void *source, const void *to)
 // A compiler that has the loads before this does not put them off behind it.
 __device__ __forceinline__ void keep_loads() { asm volatile("" ::: "memory"); }
 
-// A stage against QT tiles of query rows; the other arguments as attend_tree's,
-// a word for 32 rows. `odd`: rows some of whose values are not finite and were
+// A stage against 16 query rows; the other arguments as attend_tree's, a word for
+// 32 rows. `odd`: rows some of whose values are not finite and were
 // staged as 0; they are added one by one. Shared memory answers after 100 cycles
 // and a product after 30, so that everything that can be is asked for together:
 // all keys of a plane, the values before the softmax, and products in turn that do
 // not wait for one another.
-template <int TYPE, int HD, bool FULL, int QT>
+template <int TYPE, int HD, bool FULL>
 __device__ __forceinline__ void
 attend_stage(const char *keys, const char *values, const size_t *at,
              const uint32_t (&gone)[Stage<TYPE, HD>::kRows / 32], bool drafted,
              const uint32_t (&odd)[Stage<TYPE, HD>::kRows / 32],
-             const uint32_t (&seen)[QT][Stage<TYPE, HD>::kRows / 32],
-             const Query<Stage<TYPE, HD>::kType, HD> (&q)[QT],
-             Softmax<Stage<TYPE, HD>::kType, HD> (&sm)[QT], const PagedView &kv, int lane)
+             const uint32_t (&seen)[Stage<TYPE, HD>::kRows / 32],
+             const Query<Stage<TYPE, HD>::kType, HD> &q,
+             Softmax<Stage<TYPE, HD>::kType, HD> &sm, const PagedView &kv, int lane)
 {
     using S = Stage<TYPE, HD>;
     constexpr int G = HD / 16, kParts = HD / 32, kType = S::kType, kPlanes = S::kPlanes;
@@ -436,12 +404,10 @@ attend_stage(const char *keys, const char *values, const size_t *at,
         return *reinterpret_cast<const u32x4 *>(
             keys + S::offset(p * S::kRows + sub * 16 + c, n * 4 + j));
     };
-    f32x4 acc[QT][kSubs];
+    f32x4 acc[kSubs];
 #pragma unroll
-    for (int t = 0; t < QT; t++)
-#pragma unroll
-        for (int sub = 0; sub < kSubs; sub++)
-            acc[t][sub] = f32x4{0, 0, 0, 0};
+    for (int sub = 0; sub < kSubs; sub++)
+        acc[sub] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int p = kPlanes - 1; p >= 0; p--) {
         u32x4 k[kSubs][kParts];
@@ -456,11 +422,9 @@ attend_stage(const char *keys, const char *values, const size_t *at,
 #pragma unroll
             for (int l = kLimbs - 1; l >= 0; l--)
 #pragma unroll
-                for (int t = 0; t < QT; t++)
-#pragma unroll
-                    for (int sub = 0; sub < kSubs; sub++)
-                        if (kPlanes == 1 || p + l < 3)
-                            acc[t][sub] = product<kType>(k[sub][n], q[t].x[n][l], acc[t][sub]);
+                for (int sub = 0; sub < kSubs; sub++)
+                    if (kPlanes == 1 || p + l < 3)
+                        acc[sub] = product<kType>(k[sub][n], q.x[n][l], acc[sub]);
     }
     // Values of plane p, kGroup tiles of 16 components from tile g0 on: of rows
     // 4 j + c / 4 (then 16 further), components 16 g + 4 (c % 4) onwards, transposed.
@@ -483,100 +447,89 @@ attend_stage(const char *keys, const char *values, const size_t *at,
         keep_loads();
     };
     load_values(kPlanes - 1, 0);
-    float s[QT][kHalves][8];
+    float s[kHalves][8];
+    float all = 0.0f; // not a number after one that is none
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        float all = 0.0f; // not a number after one that is none
+    for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
-        for (int sub = 0; sub < kSubs; sub++)
+        for (int i = 0; i < 4; i++)
+            all += acc[sub][i];
+    if (__any(all != all)) {
+        // An infinite key: the first limbs' product has the sum's sign, later ones
+        // of zero, or of the other sign, make it no number. (So do sums of both
+        // infinities, which are none in the end either.)
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++) {
+            f32x4 first{0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < kParts; n++)
+                first = product<kType>(key(0, sub, n), q.x[n][0], first);
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                all += acc[t][sub][i];
-        if (__any(all != all)) {
-            // An infinite key: the first limbs' product has the sum's sign, later ones
-            // of zero, or of the other sign, make it no number. (So do sums of both
-            // infinities, which are none in the end either.)
-#pragma unroll
-            for (int sub = 0; sub < kSubs; sub++) {
-                f32x4 first{0, 0, 0, 0};
-#pragma unroll
-                for (int n = 0; n < kParts; n++)
-                    first = product<kType>(key(0, sub, n), q[t].x[n][0], first);
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    acc[t][sub][i] = acc[t][sub][i] != acc[t][sub][i] ? first[i] : acc[t][sub][i];
-            }
+                acc[sub][i] = acc[sub][i] != acc[sub][i] ? first[i] : acc[sub][i];
         }
-#pragma unroll
-        for (int half = 0; half < kHalves; half++)
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const float x = acc[t][2 * half + r / 4][r % 4];
-                s[t][half][r] = kType == NUT_F16 ? ldexpf(x, q[t].exponent) : x;
-            }
     }
+#pragma unroll
+    for (int half = 0; half < kHalves; half++)
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            const float x = acc[2 * half + r / 4][r % 4];
+            s[half][r] = kType == NUT_F16 ? ldexpf(x, q.exponent) : x;
+        }
     bool masked = drafted;
 #pragma unroll
     for (int half = 0; half < kHalves; half++)
         masked = masked || gone[half] != 0;
     if (masked)
 #pragma unroll
-        for (int t = 0; t < QT; t++)
-#pragma unroll
-            for (int half = 0; half < kHalves; half++) {
-                const uint32_t mine = (seen[t][half] & ~gone[half]) >> (4 * j);
-#pragma unroll
-                for (int r = 0; r < 8; r++)
-                    s[t][half][r] = mine >> (16 * (r / 4) + r % 4) & 1 ? s[t][half][r] : -INFINITY;
-            }
-    u32x4 limb[QT][kHalves][kLimbs];
-    float p[QT][kHalves][8];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        float most = s[t][0][0];
-#pragma unroll
-        for (int half = 0; half < kHalves; half++)
+        for (int half = 0; half < kHalves; half++) {
+            const uint32_t mine = (seen[half] & ~gone[half]) >> (4 * j);
 #pragma unroll
             for (int r = 0; r < 8; r++)
-                most = fmaxf(most, s[t][half][r]);
-        sm[t].raise(max_over_rows(most));
-        float sum[kHalves][2] = {};
-#pragma unroll
-        for (int half = 0; half < kHalves; half++) {
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                p[t][half][r] = __builtin_amdgcn_exp2f(s[t][half][r] - sm[t].ref);
-                sum[half][r % 2] += p[t][half][r];
-            }
-            split<kType, kLimbs>(p[t][half], limb[t][half]);
-            sm[t].sum += sum[half][0] + sum[half][1];
+                s[half][r] = mine >> (16 * (r / 4) + r % 4) & 1 ? s[half][r] : -INFINITY;
         }
+    u32x4 limb[kHalves][kLimbs];
+    float p[kHalves][8];
+    float most = s[0][0];
+#pragma unroll
+    for (int half = 0; half < kHalves; half++)
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            most = fmaxf(most, s[half][r]);
+    sm.raise(max_over_rows(most));
+    float sum[kHalves][2] = {};
+#pragma unroll
+    for (int half = 0; half < kHalves; half++) {
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            p[half][r] = __builtin_amdgcn_exp2f(s[half][r] - sm.ref);
+            sum[half][r % 2] += p[half][r];
+        }
+        split<kType, kLimbs>(p[half], limb[half]);
+        sm.sum += sum[half][0] + sum[half][1];
     }
 #pragma unroll
     for (int half = 0; half < kHalves; half++)
         for (uint32_t left = odd[half]; left != 0; left &= left - 1) {
             const int row = __builtin_ctz(left), own = row % 16 / 4;
             const char *from = kv.values + at[half * 32 + row];
+            float weight = 0.0f;
 #pragma unroll
-            for (int t = 0; t < QT; t++) {
-                float weight = 0.0f;
+            for (int r = 0; r < 8; r++)
+                if (16 * (r / 4) + r % 4 == row - 4 * own)
+                    weight = p[half][r];
+            weight = __shfl(weight, 16 * own + c);
+            for (int g = 0; g < G; g++) // rare: not unrolled but for the sums
 #pragma unroll
-                for (int r = 0; r < 8; r++)
-                    if (16 * (r / 4) + r % 4 == row - 4 * own)
-                        weight = p[t][half][r];
-                weight = __shfl(weight, 16 * own + c);
-                for (int g = 0; g < G; g++) // rare: not unrolled but for the sums
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t d = 16 * g + 4 * j + i;
+                    const float x = FULL || d < kv.head_dim ? component<TYPE>(from, d) : 0.0f;
+                    const bool adds = weight != 0.0f && !(fabsf(x) < INFINITY);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t d = 16 * g + 4 * j + i;
-                        const float x = FULL || d < kv.head_dim ? component<TYPE>(from, d) : 0.0f;
-                        const bool adds = weight != 0.0f && !(fabsf(x) < INFINITY);
-#pragma unroll
-                        for (int k = 0; k < G; k++)
-                            if (k == g && adds)
-                                sm[t].o[k][i] = fmaf(weight, x, sm[t].o[k][i]);
-                    }
-            }
+                    for (int k = 0; k < G; k++)
+                        if (k == g && adds)
+                            sm.o[k][i] = fmaf(weight, x, sm.o[k][i]);
+                }
         }
 #pragma unroll
     for (int pl = kPlanes - 1; pl >= 0; pl--)
@@ -589,12 +542,10 @@ attend_stage(const char *keys, const char *values, const size_t *at,
 #pragma unroll
                 for (int l = kLimbs - 1; l >= 0; l--)
 #pragma unroll
-                    for (int t = 0; t < QT; t++)
-#pragma unroll
-                        for (int g = 0; g < kGroup; g++)
-                            if (kPlanes == 1 || pl + l < 3)
-                                sm[t].o[g0 + g] = product<kType>(v[half][g], limb[t][half][l],
-                                                                 sm[t].o[g0 + g]);
+                    for (int g = 0; g < kGroup; g++)
+                        if (kPlanes == 1 || pl + l < 3)
+                            sm.o[g0 + g] =
+                                product<kType>(v[half][g], limb[half][l], sm.o[g0 + g]);
         }
 }
 
@@ -684,13 +635,14 @@ __device__ __forceinline__ Shares share_out(const TreeArgs &a, uint32_t each, bo
 // Workgroups that a CU holds, by registers and shared memory.
 constexpr int staged_groups(int type, uint32_t head_dim)
 {
-    return head_dim <= 64 ? 3 : head_dim <= 128 ? (type == NUT_F32 ? 2 : 3) : type == NUT_F32 ? 1 : 2;
+    if (head_dim <= 64)
+        return 3;
+    return (head_dim <= 128 ? 3 : 2) - (type == NUT_F32 ? 1 : 0);
 }
 
 template <int TYPE, int HD, bool FULL>
 __global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(TreeArgs a)
 {
-    constexpr int QT = 1;
     using S = Stage<TYPE, HD>;
     constexpr int G = HD / 16, R = S::kRows;
     constexpr uint32_t kEach = 4, kPiece = kEach * R; // rows whose offsets are found at once
@@ -774,24 +726,17 @@ __global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(Tr
         const uint32_t queries = nodes.count * a.group, begins = block * kBlock;
         const uint32_t begin = from_stage * R, count = min(to_stage * R, it.total) - begin;
         const uint32_t first = begins + wave * 16; // of the wave's query rows
-        Query<S::kType, HD> q[QT];
-        const uint32_t *mask[QT];
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            const uint32_t row = first + t * 16 + column;
-            const bool valid = row < queries;
-            const uint32_t node = nodes.from + (valid ? row : begins) / a.group;
-            const uint32_t head = h * a.group + (valid ? row : begins) % a.group;
-            q[t].fetch(a.query + node * a.query_stride + size_t(head) * kv.head_dim, valid,
-                       kv.head_dim, lane);
-            mask[t] = a.d.mask + node * a.d.mask_stride;
-        }
+        const bool valid = first + column < queries;
+        const uint32_t query = valid ? first + column : begins;
+        const uint32_t node = nodes.from + query / a.group, head = h * a.group + query % a.group;
+        Query<S::kType, HD> q;
+        q.fetch(a.query + node * a.query_stride + size_t(head) * kv.head_dim, valid, kv.head_dim,
+                lane);
+        const uint32_t *mask = a.d.mask + node * a.d.mask_stride;
         const uint32_t words = (nodes.count + 31) / 32;
-#pragma unroll
-        for (int t = 0; t < QT; t++)
-            q[t].convert(a.scale);
+        q.convert(a.scale);
 
-        Softmax<S::kType, HD> sm[QT];
+        Softmax<S::kType, HD> sm;
         // a thread's chunks of the next stage of fp32 rows
         constexpr int kHeld = TYPE == NUT_F32 ? (kWork == 0 ? 1 : kWork) : 1;
         float ahead[2][kHeld][8];
@@ -802,7 +747,8 @@ __global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(Tr
         const auto ask_table = [&](uint32_t piece) {
             const uint32_t index = page_of(kv, begin + piece * kPiece) + threadIdx.x;
             if (threadIdx.x < kPiece && index <= page_of(kv, begin + count - 1))
-                stage_dma<4>(a.s.table + size_t(b) * a.s.table_stride + index, table + wave * kWave);
+                stage_dma<4>(a.s.table + size_t(b) * a.s.table_stride + index,
+                             table + wave * kWave);
         };
         const auto place_rows = [&](uint32_t piece) {
             const uint32_t i = piece * kPiece + threadIdx.x, row = begin + i;
@@ -965,47 +911,40 @@ __global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(Tr
             if (first >= queries)
                 continue;
             constexpr int kHalves = R / 32;
-            uint32_t none[kHalves], odd[kHalves], seen[QT][kHalves];
+            uint32_t none[kHalves], odd[kHalves], seen[kHalves];
 #pragma unroll
             for (int half = 0; half < kHalves; half++) {
                 none[half] = uint32_t(__builtin_amdgcn_readfirstlane(gone_of(s, half)));
                 odd[half] = drafted ? uint32_t(__builtin_amdgcn_readfirstlane(odd_rows[half])) &
                                           ~none[half]
                                     : 0;
-#pragma unroll
-                for (int t = 0; t < QT; t++)
-                    seen[t][half] = !drafted ? ~0u
-                                             : mask_bits(int64_t(row + half * 32) - held, words,
-                                                         [&](uint32_t w) { return mask[t][w]; });
+                seen[half] = !drafted ? ~0u
+                                      : mask_bits(int64_t(row + half * 32) - held, words,
+                                                  [&](uint32_t w) { return mask[w]; });
             }
-            attend_stage<TYPE, HD, FULL, QT>(keys, values, offset_of(s), none, drafted, odd, seen,
-                                             q, sm, kv, lane);
+            attend_stage<TYPE, HD, FULL>(keys, values, offset_of(s), none, drafted, odd, seen, q,
+                                         sm, kv, lane);
         }
 
+        float sum = sm.sum;
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (!valid)
+            continue;
+        const size_t at = size_t(node) * a.heads + head;
+        const size_t part = size_t(slot) * kBlock + (query - begins);
+        const float f = cut ? 1.0f : 1.0f / sum;
+        float *to = cut ? a.parts + part * kv.head_dim : a.out + at * kv.head_dim;
 #pragma unroll
-        for (int t = 0; t < QT; t++) {
-            const uint32_t row = first + t * 16 + column;
-            float sum = sm[t].sum;
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (row >= queries)
-                continue;
-            const size_t at = size_t(nodes.from + row / a.group) * a.heads + h * a.group +
-                              row % a.group;
-            const size_t part = size_t(slot) * kBlock + (row - begins);
-            const float f = cut ? 1.0f : 1.0f / sum;
-            float *to = cut ? a.parts + part * kv.head_dim : a.out + at * kv.head_dim;
-#pragma unroll
-            for (int g = 0; g < G; g++)
-                if (FULL || 16 * g + 4 * j < kv.head_dim)
-                    *reinterpret_cast<f32x4 *>(to + 16 * g + 4 * j) =
-                        !cut && sum == 0.0f ? f32x4{0, 0, 0, 0} : sm[t].o[g] * f;
-            if (j == 0 && cut)
-                a.stats[part] = make_float2(sum == 0.0f ? -INFINITY : sm[t].ref, sum);
-            if (j == 0 && !cut && a.lse != nullptr)
-                a.lse[at] = sum == 0.0f ? -INFINITY
-                                        : (sm[t].ref + log2f(sum)) * 0.69314718055994531f;
-        }
+        for (int g = 0; g < G; g++)
+            if (FULL || 16 * g + 4 * j < kv.head_dim)
+                *reinterpret_cast<f32x4 *>(to + 16 * g + 4 * j) =
+                    !cut && sum == 0.0f ? f32x4{0, 0, 0, 0} : sm.o[g] * f;
+        if (j == 0 && cut)
+            a.stats[part] = make_float2(sum == 0.0f ? -INFINITY : sm.ref, sum);
+        if (j == 0 && !cut && a.lse != nullptr)
+            a.lse[at] = sum == 0.0f ? -INFINITY
+                                    : (sm.ref + log2f(sum)) * 0.69314718055994531f;
     }
 }
 
@@ -1118,11 +1057,11 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a)
         a.lse[at] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
 }
 
-template <int TYPE, int HD, int QT, int WQ>
+template <int TYPE, int HD, int WQ>
 void tree_by(const TreeArgs &a, dim3 grid, hipStream_t stream)
 {
-    const auto run = a.kv.head_dim == HD ? tree_kernel<TYPE, HD, true, QT, WQ>
-                                         : tree_kernel<TYPE, HD, false, QT, WQ>;
+    const auto run = a.kv.head_dim == HD ? tree_kernel<TYPE, HD, true, WQ>
+                                         : tree_kernel<TYPE, HD, false, WQ>;
     hipLaunchKernelGGL(run, grid, dim3(64 * kTreeWaves<HD>), 0, stream, a);
 }
 
@@ -1137,9 +1076,9 @@ void tree_as(const TreeArgs &a, const TreePlan &plan, dim3 grid, hipStream_t str
         check_launch("tree attention");
         hipLaunchKernelGGL(join, grid, dim3(256), 0, stream, a);
     } else if (plan.waves == 1) {
-        tree_by<TYPE, HD, 1, 1>(a, grid, stream);
+        tree_by<TYPE, HD, 1>(a, grid, stream);
     } else {
-        tree_by<TYPE, HD, 1, 2>(a, grid, stream);
+        tree_by<TYPE, HD, 2>(a, grid, stream);
     }
 }
 
@@ -1223,8 +1162,8 @@ void launch_tree_attention(const PagedView &kv, const PagedSeqs &seqs, const Dra
         a.before = reinterpret_cast<uint64_t *>(workspace + plan.before);
     }
     const uint32_t joined = 256 / (kv.head_dim / 4); // query rows of a workgroup of the join
-    const dim3 grid = plan.staged ? dim3(kv.kv_heads * plan.blocks * ((kBlock + joined - 1) / joined),
-                                         draft.batch)
+    const uint32_t groups = (kBlock + joined - 1) / joined; // of them for an item
+    const dim3 grid = plan.staged ? dim3(kv.kv_heads * plan.blocks * groups, draft.batch)
                                   : paged_grid((units + 7) / 8 * 8 * plan.blocks, 256);
     if (kv.type == NUT_F32)
         tree_in<NUT_F32>(a, plan, grid, stream);
