@@ -52,6 +52,7 @@ struct TreePlan {
     bool staged, past; // past the caches
     uint32_t waves; // of a workgroup that hold different query rows
     uint32_t blocks, run, runs, shares;
+    uint32_t teams; // of the join; 0: none
     size_t stats, before; // byte offsets of the parts' sums, of the stages before each sequence
     size_t bytes;
 };

@@ -33,6 +33,7 @@ struct TreeArgs {
     float *out, *lse;
     uint32_t blocks, run, runs, units; // of tree_kernel
     uint32_t shares;                   // of staged_kernel
+    uint32_t teams;                    // of a query row, of the joins
     bool past;                         // rows go past the caches' replacement
     uint64_t *before; // [batch + 1]: stages before each sequence
     float *parts;  // [total][heads][runs][head_dim], unnormalised
@@ -948,14 +949,96 @@ __global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(Tr
     }
 }
 
-// The shares of an item joined, where it was cut: a workgroup an item, a thread
-// for four components of a query row.
+// Sums of a query row's parts, four components of it.
+struct Joined {
+    float most, sum;
+    f32x4 o;
+};
+
+// Parts `first`, first + step, .. below `end`, whose exponents and sums are at stat(r)
+// and components at part(r); kAtOnce loads in flight together.
+template <typename Stat, typename Part>
+__device__ __forceinline__ Joined join_parts(uint32_t first, uint32_t step, uint32_t end,
+                                             Stat &&stat, Part &&part)
+{
+    constexpr int kAtOnce = 8;
+    Joined to{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+    for (uint32_t r = first; r < end; r += kAtOnce * step) {
+        float2 st[kAtOnce];
+        f32x4 x[kAtOnce];
+#pragma unroll
+        for (int e = 0; e < kAtOnce; e++) { // behind the last: the last again, without weight
+            const uint32_t own = min(r + e * step, end - 1);
+            st[e] = *stat(own);
+            x[e] = *part(own);
+        }
+        float now = to.most;
+#pragma unroll
+        for (int e = 0; e < kAtOnce; e++)
+            now = r + e * step < end ? fmaxf(now, st[e].x) : now;
+        if (now == -INFINITY)
+            continue;
+        const float f = to.most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(to.most - now);
+        to.sum *= f;
+        to.o *= f;
+        to.most = now;
+#pragma unroll
+        for (int e = 0; e < kAtOnce; e++) {
+            if (r + e * step >= end || st[e].x == -INFINITY) // no row of a finite score: not summed
+                continue;
+            const float g = __builtin_amdgcn_exp2f(st[e].x - now);
+            to.sum = fmaf(st[e].y, g, to.sum);
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+                to.o[d] = fmaf(x[e][d], g, to.o[d]);
+        }
+    }
+    return to;
+}
+
+// A workgroup of the joins: threads of `teams` teams to a query row, each a part of the
+// row's parts in turn, tpr threads to a team.
+struct Team {
+    uint32_t row, team, part;
+    bool in;
+};
+__device__ __forceinline__ Team team_of(uint32_t teams, uint32_t tpr)
+{
+    const uint32_t all = threadIdx.x / tpr;
+    return Team{all / teams, all % teams, threadIdx.x - all * tpr, all < 256 / tpr / teams * teams};
+}
+
+// What a query row's teams have summed, written by its first one.
+__device__ __forceinline__ void write_joined(const TreeArgs &a, const Team &t, uint32_t teams,
+                                             uint32_t tpr, Joined own, size_t at, bool valid)
+{
+    __shared__ Joined others[256];
+    if (teams > 1) {
+        others[threadIdx.x] = own;
+        __syncthreads();
+        if (t.team == 0 && valid)
+            own = join_parts(
+                0, 1, teams,
+                [&](uint32_t r) {
+                    return reinterpret_cast<const float2 *>(&others[threadIdx.x + r * tpr].most);
+                },
+                [&](uint32_t r) { return &others[threadIdx.x + r * tpr].o; });
+    }
+    if (!valid || t.team != 0)
+        return;
+    const float f = own.sum == 0.0f ? 0.0f : 1.0f / own.sum;
+    *reinterpret_cast<f32x4 *>(a.out + at * a.kv.head_dim + t.part * 4) = own.o * f;
+    if (t.part == 0 && a.lse != nullptr)
+        a.lse[at] = own.sum == 0.0f ? -INFINITY
+                                    : (own.most + log2f(own.sum)) * 0.69314718055994531f;
+}
+
+// The shares of an item joined, where it was cut: a.joined query rows a workgroup.
 template <int R>
 __global__ __launch_bounds__(256) void staged_join_kernel(TreeArgs a)
 {
-    constexpr int kAtOnce = 8; // shares whose loads are in flight together
-    const uint32_t tpr = a.kv.head_dim / 4, at_once = 256 / tpr; // query rows of a workgroup
-    const uint32_t groups = (kBlock + at_once - 1) / at_once;
+    const uint32_t tpr = a.kv.head_dim / 4, rows = 256 / tpr / a.teams; // of a workgroup
+    const uint32_t groups = (kBlock + rows - 1) / rows;
     const uint32_t b = blockIdx.y, item = blockIdx.x / groups;
     const uint64_t start = a.before[b], all = a.before[a.s.batch];
     const Item it = item_of<R>(a, b, false);
@@ -968,93 +1051,49 @@ __global__ __launch_bounds__(256) void staged_join_kernel(TreeArgs a)
     if (first == last)
         return;
     const uint32_t begins = (item - h * it.blocks) * kBlock;
-    const uint32_t queries = it.nodes.count * a.group, rows = min(kBlock, queries - begins);
-    const f32x4 *parts = reinterpret_cast<const f32x4 *>(a.parts);
-    const uint32_t own = threadIdx.x / tpr, k = (blockIdx.x - item * groups) * at_once + own;
-    if (own < at_once && k < rows) {
-        const uint32_t part = threadIdx.x - own * tpr;
-        float most = -INFINITY, sum = 0.0f;
-        f32x4 o{0, 0, 0, 0};
-        for (uint32_t r = first; r <= last; r += kAtOnce) {
-            float2 st[kAtOnce];
-            f32x4 x[kAtOnce];
-#pragma unroll
-            for (int e = 0; e < kAtOnce; e++) { // behind the last: the last again, without weight
-                const uint32_t share = min(r + e, last);
-                // a share's second slot is of the item that it ends in
-                const size_t row = size_t(2 * share + (share == first)) * kBlock + k;
-                st[e] = a.stats[row];
-                x[e] = parts[row * tpr + part];
-            }
-            float now = most;
-#pragma unroll
-            for (int e = 0; e < kAtOnce; e++)
-                now = fmaxf(now, st[e].x);
-            if (now == -INFINITY)
-                continue;
-            const float f = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - now);
-            sum *= f;
-#pragma unroll
-            for (int d = 0; d < 4; d++)
-                o[d] *= f;
-            most = now;
-#pragma unroll
-            for (int e = 0; e < kAtOnce; e++) {
-                if (r + e > last || st[e].x == -INFINITY) // no row of a finite score: not summed
-                    continue;
-                const float g = __builtin_amdgcn_exp2f(st[e].x - now);
-                sum = fmaf(st[e].y, g, sum);
-#pragma unroll
-                for (int d = 0; d < 4; d++)
-                    o[d] = fmaf(x[e][d], g, o[d]);
-            }
-        }
-        const uint32_t row = begins + k;
-        const size_t at = size_t(it.nodes.from + row / a.group) * a.heads + h * a.group +
-                          row % a.group;
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-        *reinterpret_cast<f32x4 *>(a.out + at * a.kv.head_dim + part * 4) = o * f;
-        if (part == 0 && a.lse != nullptr)
-            a.lse[at] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
-    }
+    const uint32_t queries = min(kBlock, it.nodes.count * a.group - begins);
+    const Team t = team_of(a.teams, tpr);
+    const uint32_t k = (blockIdx.x - item * groups) * rows + t.row, row = begins + k;
+    const bool valid = t.in && k < queries;
+    // a share's second slot is of the item that it ends in
+    const auto slot = [&](uint32_t share) {
+        return size_t(2 * share + (share == first)) * kBlock + k;
+    };
+    Joined own{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+    if (valid)
+        own = join_parts(
+            first + t.team, a.teams, last + 1, [&](uint32_t r) { return a.stats + slot(r); },
+            [&](uint32_t r) {
+                return reinterpret_cast<const f32x4 *>(a.parts) + slot(r) * tpr + t.part;
+            });
+    write_joined(a, t, a.teams, tpr, own,
+                 size_t(it.nodes.from + row / a.group) * a.heads + h * a.group + row % a.group,
+                 valid);
 }
 
-// The runs joined: a thread for four components of a node's head.
+// The runs joined.
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a)
 {
-    const uint32_t b = blockIdx.y, tpr = a.kv.head_dim / 4;
+    const uint32_t b = blockIdx.y, tpr = a.kv.head_dim / 4, rows = 256 / tpr / a.teams;
     const NodeSpan nodes = nodes_of(a.d, b, false);
-    const uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    const uint64_t row = i / tpr;
-    if (row >= uint64_t(nodes.count) * a.heads)
+    const uint64_t all = uint64_t(nodes.count) * a.heads;
+    if (uint64_t(blockIdx.x) * rows >= all)
         return;
     uint32_t held;
     const uint32_t total = rows_of(a, b, nodes.count, held, false);
-    const uint32_t runs = (total + a.run - 1) / a.run, part = uint32_t(i - row * tpr);
+    const uint32_t runs = (total + a.run - 1) / a.run;
+    const Team t = team_of(a.teams, tpr);
+    const uint64_t row = uint64_t(blockIdx.x) * rows + t.row;
+    const bool valid = t.in && row < all;
     const size_t at = size_t(nodes.from) * a.heads + row;
-    const float2 *stats = a.stats + at * a.runs;
-    const f32x4 *parts =
-        reinterpret_cast<const f32x4 *>(a.parts + at * a.runs * a.kv.head_dim) + part;
-    float most = -INFINITY;
-    for (uint32_t r = 0; r < runs; r++)
-        most = fmaxf(most, stats[r].x);
-    float sum = 0.0f;
-    f32x4 o{0, 0, 0, 0};
-    for (uint32_t r = 0; r < runs; r++) {
-        const float2 st = stats[r];
-        const f32x4 x = parts[r * tpr];
-        if (st.x == -INFINITY) // no row of a finite score: not summed
-            continue;
-        const float f = __builtin_amdgcn_exp2f(st.x - most);
-        sum = fmaf(st.y, f, sum);
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            o[e] = fmaf(x[e], f, o[e]);
-    }
-    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<f32x4 *>(a.out + at * a.kv.head_dim + part * 4) = o * f;
-    if (part == 0 && a.lse != nullptr)
-        a.lse[at] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
+    Joined own{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+    if (valid)
+        own = join_parts(
+            t.team, a.teams, runs, [&](uint32_t r) { return a.stats + at * a.runs + r; },
+            [&](uint32_t r) {
+                return reinterpret_cast<const f32x4 *>(a.parts) + (at * a.runs + r) * tpr + t.part;
+            });
+    write_joined(a, t, a.teams, tpr, own, at, valid);
 }
 
 template <int TYPE, int HD, int WQ>
@@ -1097,6 +1136,22 @@ void tree_in(const TreeArgs &a, const TreePlan &plan, dim3 grid, hipStream_t str
         tree_as<TYPE, 256>(a, plan, grid, stream);
 }
 
+// Teams that join a query row of so many parts, eight in flight a team. (Two sequences of
+// 14,283 to 17,791 fp32 rows, 3 KV heads of 80, 3 nodes, 140 runs: the call 139 us where
+// one thread went from run to run, JOINED with teams.)
+uint32_t teams_for(const PagedView &kv, uint64_t parts)
+{
+    uint32_t teams = 1;
+    while (teams * 8 < parts && teams * 2 * (kv.head_dim / 4) <= 256)
+        teams *= 2;
+    return teams;
+}
+// Query rows of a workgroup of the join.
+uint32_t joined_rows(const PagedView &kv, const TreePlan &plan)
+{
+    return 256 / (kv.head_dim / 4) / plan.teams;
+}
+
 } // namespace
 
 TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &draft,
@@ -1120,6 +1175,9 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
         plan.past = plan.blocks == 1 && uint64_t(seqs.max_length) * draft.batch * kv.kv_heads *
                                                 kv.head_dim * 2 * paged_element(kv.type) >=
                                             (128ull << 20);
+        // in the mean, where lengths differ
+        plan.teams =
+            teams_for(kv, plan.shares / (uint64_t(draft.batch) * kv.kv_heads * plan.blocks) + 1);
         require(draft.batch <= 65535, NUT_EINVAL, "paged cache: more rows than one launch covers");
         paged_grid(uint64_t(draft.batch) * kv.kv_heads * plan.blocks * kBlock, 256);
         plan.stats = aligned(size_t(plan.shares) * 2 * kBlock * kv.head_dim * sizeof(float));
@@ -1139,7 +1197,9 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
     paged_grid((units + 7) / 8 * 8 * plan.blocks, 256);
     if (plan.runs == 1)
         return plan;
-    paged_grid((uint64_t(draft.most) * heads * (kv.head_dim / 4) + 255) / 256 * 256, 1);
+    plan.teams = teams_for(kv, plan.runs);
+    const uint32_t joined = joined_rows(kv, plan);
+    paged_grid((uint64_t(draft.most) * heads + joined - 1) / joined, 256);
     require(draft.batch <= 65535, NUT_EINVAL, "paged cache: more rows than one launch covers");
     const size_t parts = size_t(draft.total) * heads * plan.runs;
     plan.stats = aligned(parts * kv.head_dim * sizeof(float));
@@ -1155,14 +1215,14 @@ void launch_tree_attention(const PagedView &kv, const PagedSeqs &seqs, const Dra
     const uint64_t units = uint64_t(draft.batch) * kv.kv_heads * plan.runs;
     TreeArgs a{kv, seqs, draft, query, query_stride, heads, heads / kv.kv_heads,
                scale * 1.4426950408889634f, out, lse, plan.blocks, plan.run, plan.runs,
-               uint32_t(units), plan.shares, plan.past, nullptr, nullptr, nullptr};
+               uint32_t(units), plan.shares, plan.teams, plan.past, nullptr, nullptr, nullptr};
     if (plan.bytes != 0) {
         a.parts = reinterpret_cast<float *>(workspace);
         a.stats = reinterpret_cast<float2 *>(workspace + plan.stats);
         a.before = reinterpret_cast<uint64_t *>(workspace + plan.before);
     }
-    const uint32_t joined = 256 / (kv.head_dim / 4); // query rows of a workgroup of the join
-    const uint32_t groups = (kBlock + joined - 1) / joined; // of them for an item
+    const uint32_t joined = plan.teams == 0 ? 1 : joined_rows(kv, plan);
+    const uint32_t groups = (kBlock + joined - 1) / joined; // workgroups of the join, an item
     const dim3 grid = plan.staged ? dim3(kv.kv_heads * plan.blocks * groups, draft.batch)
                                   : paged_grid((units + 7) / 8 * 8 * plan.blocks, 256);
     if (kv.type == NUT_F32)
@@ -1174,8 +1234,8 @@ void launch_tree_attention(const PagedView &kv, const PagedSeqs &seqs, const Dra
     check_launch("tree attention");
     if (plan.staged || plan.runs == 1)
         return;
-    const uint64_t threads = uint64_t(draft.most) * heads * (kv.head_dim / 4);
-    hipLaunchKernelGGL(tree_join_kernel, dim3(uint32_t((threads + 255) / 256), draft.batch),
+    const uint64_t rows = uint64_t(draft.most) * heads;
+    hipLaunchKernelGGL(tree_join_kernel, dim3(uint32_t((rows + joined - 1) / joined), draft.batch),
                        dim3(256), 0, stream, a);
     check_launch("tree attention");
 }
