@@ -1138,7 +1138,7 @@ void tree_in(const TreeArgs &a, const TreePlan &plan, dim3 grid, hipStream_t str
 
 // Teams that join a query row of so many parts, eight in flight a team. (Two sequences of
 // 14,283 to 17,791 fp32 rows, 3 KV heads of 80, 3 nodes, 140 runs: the call 139 us where
-// one thread went from run to run, JOINED with teams.)
+// one thread went from run to run, 37 with teams.)
 uint32_t teams_for(const PagedView &kv, uint64_t parts)
 {
     uint32_t teams = 1;
