@@ -3,10 +3,9 @@
 //
 // Two launches. In the first a wave takes a part of a beam's logits into
 // registers: their largest, the sum of their exponentials, and the K largest in
-// order. In the second a workgroup per request joins a beam's parts to its K
-// best tokens and its log-sum, and then the beams to the request's K best. Only
-// the logits' order matters within a beam, so that ranks are worked out for K
-// candidates a beam, in 64 bits.
+// order. In the second a workgroup per request joins a beam's parts to its
+// log-sum, and the beams' lists to the request's K best. Only the logits' order
+// matters within a beam, so that ranks are worked out for few candidates, in 64 bits.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,6 +22,7 @@ namespace {
 constexpr uint32_t kMostParts = 64;   // of a beam's logits: a lane each
 constexpr int kFound = 64;           // keys that a wave ranks at once
 constexpr uint32_t kMostListed = 2048; // keys of a beam's parts: 32 parts of 64
+constexpr int kChosen = 512;         // candidates of a request that are ranked at once
 
 struct Part {
     float most; // minus infinity: no finite one
@@ -88,6 +88,21 @@ __device__ __forceinline__ uint64_t wave_most(uint64_t v)
     return uint64_t(hi) << 32 | wave_most(uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
 }
 
+// A lane's value, the same for all.
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, uint32_t lane)
+{
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 |
+           uint32_t(__builtin_amdgcn_readlane(int(v), lane));
+}
+
+// What the wave's lanes wrote to shared memory, its other lanes read.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // exp(d), d <= 0: the exponent in base 2 in two pieces, so that the error is
 // that of the instruction, a unit in the last place, however large d is.
 __device__ __forceinline__ float exp_below(float d)
@@ -104,6 +119,9 @@ template <int TYPE> struct __attribute__((packed, aligned(TYPE == NUT_F32 ? 4 : 
 };
 
 // EACH logits a lane, in runs of 16 bytes: run r of the wave's part is lane r % 64's.
+// 512 beams of 100,003 fp16 logits: 37 us, 2.7 TB/s; exponentials and the search bound it
+// (with the bound searched among 64-bit keys, and a pass of its own for what is no number,
+// 47; with every key found by a reduction of its own 84).
 template <int TYPE, int EACH>
 __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
 {
@@ -204,12 +222,8 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
         __syncthreads();
         const uint64_t own = lane < count ? found[lane] : 0;
         uint32_t above = 0;
-        for (uint32_t k = 0; k < count; k++) {
-            const uint64_t other =
-                uint64_t(uint32_t(__builtin_amdgcn_readlane(int(own >> 32), k))) << 32 |
-                uint32_t(__builtin_amdgcn_readlane(int(own), k));
-            above += other > own;
-        }
+        for (uint32_t k = 0; k < count; k++)
+            above += lane_of(own, k) > own;
         __syncthreads();
         if (lane < count)
             found[above] = own; // keys differ by their tokens
@@ -238,104 +252,172 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
         a.best[slot * keep + lane] = kept;
 }
 
-// exp and power in 64 bits: a few for each request.
+// A request's beams and candidates. exp and power in 64 bits: a few for each request.
+//
+// A part's first key is its best, so that the keep-th best of 64 groups of firsts is
+// a rank that no candidate of the answer is below: the keys from it on are few where
+// logits spread, and each counts those before it. Where there are more (equal
+// logits), a beam's parts are merged first, one key after another, and then the
+// beams. Latency bounds both: 2 requests of 10 beams, 26,160 logits, 18 best 10 us where
+// merging alone took 32; 64 requests of 8 beams, 100,003 logits, 8 best 8.9 for 17.
+struct Found {
+    uint64_t rank, key;
+    uint32_t beam;
+};
+
 __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
 {
-    extern __shared__ uint64_t lists[]; // a wave's parts [parts][keep]
-    __shared__ uint64_t best[kMostBeams][kMostBeams];
+    extern __shared__ uint64_t lists[]; // kMostListed words: places of parts, or a wave's lists
+    __shared__ union {
+        uint64_t first[kMostBeams * kMostParts]; // ranks of the parts' first keys
+        uint64_t best[kMostBeams][kMostBeams];
+    } lds;
+    __shared__ Found found[kChosen];
+    __shared__ uint32_t parts_in, count;
     __shared__ double score_of[kMostBeams], top_of[kMostBeams], log_of[kMostBeams];
     __shared__ double divisor[kMostBeams];
-    __shared__ int grown[kMostBeams];
+    __shared__ int grown[kMostBeams], state[kMostBeams]; // state: 0 none, 1 lives, 2 has ended
     const uint32_t request = blockIdx.x, beams = a.from.beams, keep = a.to.beams;
     const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const uint32_t waves = blockDim.x / kWave;
-    uint64_t *list = lists + size_t(wave) * room;
+    const uint32_t waves = blockDim.x / kWave, firsts = beams * a.parts;
+    // the difference to the largest logit first: it is small, or says that nothing is
+    const auto scored = [&](uint32_t i, uint64_t key) {
+        return score_of[i] + (double(logit_of(key)) - top_of[i] - log_of[i]);
+    };
+    const auto rank_of = [&](uint32_t i, uint64_t key) {
+        return key == 0 ? uint64_t(0) : rank_key(scored(i, key) / divisor[i]);
+    };
+    // An ended beam's only candidate.
+    const uint64_t over = key_of(0.0f, uint32_t(a.eos));
+    if (threadIdx.x == 0)
+        parts_in = count = 0;
     for (uint32_t i = wave; i < beams; i += waves) {
         const size_t row = size_t(request) * beams + i;
         const float score = a.from.scores[row];
         const bool ended = a.from.ended != nullptr && a.from.ended[row] != 0;
         const int length = a.from.lengths == nullptr ? 0 : a.from.lengths[row];
-        if (lane == 0) {
-            grown[i] = ended ? length : length + 1;
-            divisor[i] = a.power == 0.0f ? 1.0 : pow(double(max(grown[i], 1)), double(a.power));
-        }
-        if (!(score > -INFINITY)) {
-            if (lane < keep)
-                best[i][lane] = 0;
-            continue;
-        }
-        if (ended) {
-            if (lane < keep)
-                best[i][lane] = lane == 0 ? key_of(0.0f, uint32_t(a.eos)) : 0;
-            if (lane == 0)
-                score_of[i] = double(score), top_of[i] = log_of[i] = 0.0;
-            continue;
-        }
+        const bool live = score > -INFINITY && !ended, mine = live && lane < a.parts;
         Part part{-INFINITY, 0, 0.0};
-        if (lane < a.parts)
+        uint64_t key = lane == 0 && ended ? over : 0;
+        if (mine) {
             part = a.stats[row * a.parts + lane];
-        for (uint32_t k = lane; k < a.parts * keep; k += kWave)
-            list[k] = a.best[row * a.parts * keep + k];
-        const float top = wave_max(part.most);
+            key = a.best[(row * a.parts + lane) * keep];
+        }
+        const float top = live ? wave_max(part.most) : 0.0f;
         double sum = part.most == -INFINITY ? part.sum
                                             : part.sum * exp(double(part.most) - double(top));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1)
             sum += __shfl_xor(sum, o);
-        if (lane == 0)
-            score_of[i] = double(score), top_of[i] = double(top), log_of[i] = log(sum);
-        // the wave's lanes read what its other lanes wrote
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        // the heads of the parts' lists, a lane a part
-        uint32_t at = 0;
-        uint64_t head = lane < a.parts ? list[lane * keep] : 0, kept = 0;
-        for (uint32_t k = 0; k < keep; k++) {
-            const uint64_t now = wave_most(head);
-            if (now == 0)
-                break;
-            if (lane == k)
-                kept = now;
-            if (head == now)
-                head = ++at < keep ? list[lane * keep + at] : 0;
+        if (lane == 0) {
+            grown[i] = ended ? length : length + 1;
+            divisor[i] = a.power == 0.0f ? 1.0 : pow(double(max(grown[i], 1)), double(a.power));
+            score_of[i] = double(score), top_of[i] = double(top);
+            log_of[i] = live ? log(sum) : 0.0;
+            state[i] = !(score > -INFINITY) ? 0 : ended ? 2 : 1;
+        }
+        wave_fence();
+        if (lane < a.parts)
+            lds.first[i * a.parts + lane] = score > -INFINITY ? rank_of(i, key) : 0;
+    }
+    __syncthreads();
+    // The keep-th largest of 64 groups' largest.
+    uint64_t mine = 0;
+    for (uint32_t f = lane; f < firsts; f += kWave)
+        mine = max(mine, lds.first[f]);
+    uint32_t above = 0;
+#pragma unroll
+    for (int k = 0; k < kWave; k++)
+        above += lane_of(mine, k) > mine;
+    const bool enough = uint32_t(__popcll(__ballot(mine != 0))) >= keep;
+    const uint64_t bound = enough ? ~wave_most(above < keep ? ~mine : uint64_t(0)) : 1;
+    uint16_t *const places = reinterpret_cast<uint16_t *>(lists);
+    for (uint32_t f = threadIdx.x; f < firsts; f += blockDim.x)
+        if (lds.first[f] >= bound)
+            places[atomicAdd(&parts_in, 1u)] = uint16_t(f);
+    __syncthreads();
+    for (uint32_t w = threadIdx.x; w < parts_in * keep; w += blockDim.x) {
+        const uint32_t f = places[w / keep], k = w % keep, i = f / a.parts;
+        const size_t row = size_t(request) * beams + i;
+        const uint64_t key = state[i] == 1 ? a.best[(row * a.parts + f % a.parts) * keep + k]
+                             : k == 0      ? over
+                                           : 0;
+        const uint64_t rank = rank_of(i, key);
+        if (rank >= bound) {
+            const uint32_t to = atomicAdd(&count, 1u);
+            if (to < uint32_t(kChosen))
+                found[to] = Found{rank, key, i};
+        }
+    }
+    __syncthreads();
+    const auto write = [&](uint32_t k, bool live, uint32_t beam, uint64_t key) {
+        const size_t to = size_t(request) * keep + k;
+        a.parents[to] = live ? int(request * beams + beam) : -1;
+        a.tokens[to] = live ? int(token_of(key)) : -1;
+        a.to.scores[to] = live ? float(scored(beam, key)) : -INFINITY;
+        if (a.to.lengths != nullptr)
+            a.to.lengths[to] = live ? grown[beam] : 0;
+        if (a.to.ended != nullptr)
+            a.to.ended[to] = live && (state[beam] == 2 || int(token_of(key)) == a.eos) ? 1 : 0;
+    };
+    if (count <= uint32_t(kChosen)) {
+        if (threadIdx.x < count) {
+            const Found own = found[threadIdx.x];
+            uint32_t before = 0;
+            for (uint32_t k = 0; k < count; k++) {
+                const Found x = found[k];
+                before += x.rank > own.rank ||
+                          (x.rank == own.rank &&
+                           (x.beam < own.beam || (x.beam == own.beam && x.key > own.key)));
+            }
+            if (before < keep)
+                write(before, true, own.beam, own.key);
+        } else if (threadIdx.x < keep) {
+            write(threadIdx.x, false, 0, 0);
+        }
+        return;
+    }
+    const uint32_t merging = min(waves, kMostListed / room);
+    uint64_t *list = lists + size_t(wave) * room;
+    for (uint32_t i = wave; i < beams && wave < merging; i += merging) {
+        const size_t row = size_t(request) * beams + i;
+        uint64_t kept = lane == 0 && state[i] == 2 ? over : 0;
+        if (state[i] == 1) {
+            for (uint32_t k = lane; k < a.parts * keep; k += kWave)
+                list[k] = a.best[row * a.parts * keep + k];
+            wave_fence();
+            // the heads of the parts' lists, a lane a part
+            uint32_t at = 0;
+            uint64_t head = lane < a.parts ? list[lane * keep] : 0;
+            for (uint32_t k = 0; k < keep; k++) {
+                const uint64_t now = wave_most(head);
+                if (now == 0)
+                    break;
+                if (lane == k)
+                    kept = now;
+                if (head == now)
+                    head = ++at < keep ? list[lane * keep + at] : 0;
+            }
+            wave_fence();
         }
         if (lane < keep)
-            best[i][lane] = kept;
+            lds.best[i][lane] = kept;
     }
     __syncthreads();
     if (wave != 0)
         return;
     // the beams' lists, a lane a beam
-    // the difference to the largest logit first: it is small, or says that nothing is
-    const auto scored = [&](uint32_t i, uint64_t key) {
-        return score_of[i] + (double(logit_of(key)) - top_of[i] - log_of[i]);
-    };
     const auto rank = [&](uint32_t at) {
-        if (lane >= beams || at >= keep || best[lane][at] == 0)
-            return uint64_t(0);
-        return rank_key(scored(lane, best[lane][at]) / divisor[lane]);
+        return lane < beams && at < keep ? rank_of(lane, lds.best[lane][at]) : uint64_t(0);
     };
     uint32_t at = 0;
     uint64_t head = rank(0);
     for (uint32_t k = 0; k < keep; k++) {
         const uint64_t now = wave_most(head);
-        const uint64_t same = __ballot(head == now);
-        const uint32_t beam = uint32_t(__builtin_ctzll(same));
-        const size_t to = size_t(request) * keep + k;
+        const uint32_t beam = uint32_t(__builtin_ctzll(__ballot(head == now)));
         if (lane == beam) {
-            const bool live = now != 0;
-            const uint64_t key = live ? best[beam][at] : 0;
-            const size_t row = size_t(request) * beams + beam;
-            const bool over = live && a.from.ended != nullptr && a.from.ended[row] != 0;
-            a.parents[to] = live ? int(row) : -1;
-            a.tokens[to] = live ? int(token_of(key)) : -1;
-            a.to.scores[to] = live ? float(scored(beam, key)) : -INFINITY;
-            if (a.to.lengths != nullptr)
-                a.to.lengths[to] = live ? grown[beam] : 0;
-            if (a.to.ended != nullptr)
-                a.to.ended[to] = over || (live && int(token_of(key)) == a.eos) ? 1 : 0;
-            head = live ? rank(++at) : 0;
+            write(k, now != 0, beam, now != 0 ? lds.best[beam][at] : 0);
+            head = now != 0 ? rank(++at) : 0;
         }
     }
 }
@@ -369,7 +451,8 @@ uint32_t parts_of(uint32_t vocab, uint32_t each)
 // Logits a lane holds, 16 to 128: the fewest whose parts fit a wave, and their
 // lists its shared memory; 128 do for kMostVocab. 32 rather than 16 where that leaves
 // 8,192 waves: each finds its own largest, and lists them for the second launch (512
-// beams, 100,003 fp16 logits: 59 us of 32, 62 of 64, 121 of 128).
+// beams, 100,003 fp16 logits, on an earlier choose_kernel: 59 us of 32, 62 of 64, 121 of
+// 128).
 uint32_t each_of(uint32_t rows, uint32_t vocab, uint32_t keep)
 {
     uint32_t each = 16;
@@ -430,9 +513,10 @@ void launch_beam_select(const BeamsView &from, const BeamsView &to, const void *
         scan_as<NUT_BF16>(a, grid, stream);
     check_launch("beam select");
     const uint32_t room = a.parts * to.beams;
-    const uint32_t waves = std::min({from.beams, 16u, kMostListed / room});
+    // a wave a beam, and threads for kChosen candidates
+    const uint32_t waves = std::min(std::max(from.beams, uint32_t(kChosen / kWave)), 16u);
     hipLaunchKernelGGL(choose_kernel, dim3(from.requests), dim3(waves * kWave),
-                       size_t(waves) * room * sizeof(uint64_t), stream, a, room);
+                       kMostListed * sizeof(uint64_t), stream, a, room);
     check_launch("beam select");
 }
 

@@ -172,6 +172,20 @@ def test_ties_go_to_the_lowest(gpu, kind, vocab):
     Step(gpu, [[-1.0, -1.0, -1.0]], y, min(40, vocab), kind=kind).check()
 
 
+@pytest.mark.parametrize("beams,keep,vocab", [(20, 64, 5000), (64, 64, 2048), (17, 3, 9000),
+                                              (64, 9, 70000), (3, 64, 64), (33, 16, 1030)])
+@pytest.mark.parametrize("levels", [1, 2, 50])
+def test_many_ties(gpu, beams, keep, vocab, levels):
+    """More candidates of one rank than are kept, beside ended beams and beams that are none."""
+    rng = np.random.default_rng(vocab + levels)
+    scores = np.full((3, beams), -2.0, np.float32)
+    scores[:, 1::5] = -np.inf
+    over = rng.random((3, beams)) < 0.2
+    logits = np.broadcast_to(rng.integers(0, levels, (1, 1, vocab)).astype(float), (3, beams, vocab))
+    Step(gpu, scores, logits, keep, lengths=np.full((3, beams), 7), ended=over, eos=2,
+         power=0.5).check()
+
+
 @pytest.mark.parametrize("vocab", [4096, 40000])
 @pytest.mark.parametrize("order", ["falling", "rising"])
 def test_sorted_logits(gpu, vocab, order):
