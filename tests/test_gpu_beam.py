@@ -181,8 +181,8 @@ def test_many_ties(gpu, beams, keep, vocab, levels):
     scores = np.full((3, beams), -2.0, np.float32)
     scores[:, 1::5] = -np.inf
     over = rng.random((3, beams)) < 0.2
-    logits = np.broadcast_to(rng.integers(0, levels, (1, 1, vocab)).astype(float), (3, beams, vocab))
-    Step(gpu, scores, logits, keep, lengths=np.full((3, beams), 7), ended=over, eos=2,
+    row = rng.integers(0, levels, (1, 1, vocab)).astype(float)
+    Step(gpu, scores, np.broadcast_to(row, (3, beams, vocab)), keep, lengths=np.full((3, beams), 7), ended=over, eos=2,
          power=0.5).check()
 
 

@@ -60,7 +60,8 @@ def test_attention_long(gpu):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim", [8, 64, 80, 256])
-@pytest.mark.parametrize("held,counts,heads", [([9000], [3], 2), ([8300, 40, 0, 6000], [64, 1, 0, 9], 4)])
+@pytest.mark.parametrize("held,counts,heads", [([9000], [3], 2),
+                                               ([8300, 40, 0, 6000], [64, 1, 0, 9], 4)])
 def test_attention_many_parts(gpu, kind, dim, held, counts, heads):
     """Few query rows over long sequences, and some beside short ones: a row's parts are
     joined by several threads, which may have none of a short one."""
