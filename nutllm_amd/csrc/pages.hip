@@ -21,6 +21,8 @@ namespace {
 constexpr uint32_t kSegments = 256;     // at most
 constexpr uint32_t kSpan = 4096;        // pages that a workgroup lists at once
 constexpr uint32_t kPlanThreads = 1024;
+constexpr uint32_t kFew = 16384; // entries of a table, and copies, that one workgroup follows
+constexpr uint32_t kFewHeld = 128; // and sequences
 constexpr uint32_t kCounted = 2048;     // old sequences that shared memory counts
 constexpr int kNone = 0x7fffffff;
 
@@ -472,6 +474,66 @@ __global__ __launch_bounds__(kWave) void move_kernel(CompactArgs a)
     copy[0] = from, copy[1] = to, copy[2] = int(a.pool.page_size);
 }
 
+// All of it by one workgroup, which saves three launches: pools of up to kSpan pages,
+// tables of kFew entries and kFewHeld sequences. Counts and lists are in shared memory.
+// Without copies, us, and by four launches: 64 pages, 3 sequences of 20 4.8 and 14.5;
+// 4,096 pages, 64 of 64 7.3 and 14.5, 64 of 256 11.8 and 15.2, 128 of 256 18.9 and 15.5,
+// 512 of 16 26.9 and 14.5.
+__global__ __launch_bounds__(kPlanThreads) void compact_kernel(CompactArgs a)
+{
+    __shared__ int held[kSpan], low_list[kSpan], high_list[kSpan];
+    // threads of a sequence: all, or as few as a wave where there are many
+    uint32_t team = kPlanThreads;
+    while (team > uint32_t(kWave) && kPlanThreads / team < a.table.batch)
+        team /= 2;
+    const uint32_t at = threadIdx.x / team, lane = threadIdx.x % team, teams = kPlanThreads / team;
+    for (uint32_t p = threadIdx.x; p < a.pool.pages; p += kPlanThreads)
+        held[p] = 0;
+    for (uint32_t i = threadIdx.x; i < a.count * 3; i += kPlanThreads)
+        a.copies[i] = -1;
+    __syncthreads();
+    for (uint32_t b = at; b < a.table.batch; b += teams) {
+        const uint32_t entries = held_by(a, b, lane == 0);
+        for (uint32_t c = lane; c < entries; c += team) {
+            const int page = a.table.pages[size_t(b) * a.table.stride + c];
+            if (page_in(page, a.pool.pages))
+                atomicAdd(&held[page], 1);
+            else if (page != -1)
+                status_flag(a.pool.status, kBadPage);
+        }
+    }
+    __syncthreads();
+    const uint32_t low = list_pages<kPlanThreads>(0, a.pool.pages, low_list, [&](uint32_t p) {
+        return p < a.limit && a.pool.refs[p] == 0;
+    });
+    __syncthreads();
+    const uint32_t high = list_pages<kPlanThreads>(0, a.pool.pages, high_list, [&](uint32_t p) {
+        return p >= a.limit && held[p] > 0 && a.pool.refs[p] == held[p];
+    });
+    __syncthreads();
+    for (uint32_t p = threadIdx.x; p < a.pool.pages; p += kPlanThreads)
+        held[p] = -1; // from here on where a page moves to
+    __syncthreads();
+    for (uint32_t r = threadIdx.x; r < min(min(low, high), a.count); r += kPlanThreads) {
+        const int from = high_list[r], to = low_list[r];
+        held[from] = to;
+        a.pool.refs[to] = a.pool.refs[from];
+        a.pool.refs[from] = 0;
+        int *copy = a.copies + size_t(r) * 3;
+        copy[0] = from, copy[1] = to, copy[2] = int(a.pool.page_size);
+    }
+    __syncthreads();
+    for (uint32_t b = at; b < a.table.batch; b += teams) {
+        const uint32_t entries = held_by(a, b, false);
+        int *own = a.table.pages + size_t(b) * a.table.stride;
+        for (uint32_t c = lane; c < entries; c += team) {
+            const int page = own[c];
+            if (page_in(page, a.pool.pages) && held[page] >= 0)
+                own[c] = held[page];
+        }
+    }
+}
+
 // ------------------------------------------------------------------ copy --
 
 // A workgroup per copy, KV head and layer: 59 copies of up to 64 fp16 rows, 32 KV
@@ -592,6 +654,12 @@ void launch_compact(const PoolView &pool, const TableView &table, uint32_t limit
     a.pool = pool, a.table = table, a.limit = limit, a.copies = copies, a.count = count;
     a.segment = segment_of(pool.pages);
     a.segments = uint32_t((uint64_t(pool.pages) + a.segment - 1) / a.segment);
+    if (pool.pages <= kSpan && table.batch <= kFewHeld &&
+        uint64_t(table.batch) * table.stride <= kFew && count <= kFew) {
+        hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
+        check_launch("page compaction");
+        return;
+    }
     carve(a, workspace);
     const uint64_t words = std::max(uint64_t(pool.pages), uint64_t(count) * 3);
     const uint32_t clears = uint32_t(std::min<uint64_t>((words + 255) / 256, 1024));

@@ -363,7 +363,7 @@ def test_null_views():
 
 @pytest.mark.parametrize("program", [["serving_index_test"], ["serving_api_test", "--cpu-only"]])
 def test_cpp(program):
-    """Masks, spans and parents as the kernels judge them; the C++ host API's refusals."""
+    """Masks, spans and parents as the kernels take them; the C++ host API's refusals."""
     build = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build")
     binary = os.path.join(build, program[0])
     assert os.path.exists(binary), "build first: make -C tests/cpp"

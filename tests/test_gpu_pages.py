@@ -230,6 +230,23 @@ def test_compact_at_random(gpu, pages, page, batch, width, seed):
         t.compact(limit, most)
 
 
+@pytest.mark.parametrize("pages,batch,width,most", [(4096, 90, 60, 4096), (4097, 90, 60, 700),
+                                                    (300, 17, 4000, 300), (300, 17, 30, 70000),
+                                                    (4096, 1, 16384, 16384), (4096, 1, 16385, 9),
+                                                    (500, 128, 9, 50), (500, 129, 9, 50),
+                                                    (700, 5, 90, 16385), (1, 1, 1, 1)])
+def test_compact_by_one_workgroup_or_more(gpu, pages, batch, width, most):
+    """Pools, tables and lists at the sizes where one workgroup follows them all, and behind."""
+    rng = np.random.default_rng(pages + width)
+    t = Twin(gpu, pages, 2, batch, width)
+    gains = rng.integers(0, min(width * 2, 2 * pages // batch) + 1, batch)
+    t.reorder([-1] * batch, gains=gains)
+    t.grow(rng.integers(0, t.host.held * 2 + 1))
+    t.reorder(rng.integers(0, batch, batch), gain=1)
+    t.compact(pages // 2, most)
+    t.compact(pages // 3, most)
+
+
 def test_compact_missing_pages(gpu):
     t = Twin(gpu, 12, 4, 2, 4)
     t.reorder([-1, -1], gain=12)
