@@ -422,6 +422,7 @@ __global__ __launch_bounds__(1024) void choose_kernel(BeamArgs a, uint32_t room)
     }
 }
 
+// A workgroup for 1,024 words of a row: 512 rows of 4,000 bytes 4.2 us, a launch.
 template <typename Word>
 __global__ __launch_bounds__(256) void gather_kernel(const char *source, size_t from_stride,
                                                      uint32_t sources, char *to, size_t to_stride,
