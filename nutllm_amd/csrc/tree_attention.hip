@@ -382,6 +382,17 @@ __device__ __forceinline__ void stage_dma(const void *source, const void *to)
                      : "memory", "m0");
 }
 
+// Whether a component of an fp32 row is no number, whatever its bits.
+__device__ __forceinline__ bool no_number(const char *row, uint32_t head_dim)
+{
+    const float *x = reinterpret_cast<const float *>(row);
+    bool found = false;
+#pragma unroll 1
+    for (uint32_t d = 0; d < head_dim; d++)
+        found = found || x[d] != x[d];
+    return found;
+}
+
 // A compiler that has the loads before this does not put them off behind it.
 __device__ __forceinline__ void keep_loads() { asm volatile("" ::: "memory"); }
 
@@ -461,7 +472,8 @@ attend_stage(const char *keys, const char *values, const size_t *at,
     if (__any(all != all)) {
         // An infinite key: the first limbs' product has the sum's sign, later ones
         // of zero, or of the other sign, make it no number. (So do sums of both
-        // infinities, which are none in the end either.)
+        // infinities, which are none in the end either.) A NaN may look infinite in
+        // its upper limb: fp32 keys are read again.
 #pragma unroll
         for (int sub = 0; sub < kSubs; sub++) {
             f32x4 first{0, 0, 0, 0};
@@ -469,8 +481,16 @@ attend_stage(const char *keys, const char *values, const size_t *at,
             for (int n = 0; n < kParts; n++)
                 first = product<kType>(key(0, sub, n), q.x[n][0], first);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                acc[sub][i] = acc[sub][i] != acc[sub][i] ? first[i] : acc[sub][i];
+            for (int i = 0; i < 4; i++) {
+                if (acc[sub][i] == acc[sub][i])
+                    continue;
+                acc[sub][i] = first[i];
+                if constexpr (TYPE == NUT_F32) {
+                    const size_t row = at[16 * sub + 4 * j + i];
+                    if (row != kNoRow && no_number(kv.keys + row, kv.head_dim))
+                        acc[sub][i] = __builtin_nanf("");
+                }
+            }
         }
     }
 #pragma unroll
