@@ -418,7 +418,8 @@ typedef struct nut_draft {
 /* Each node's mask, itself and its ancestors (words below ceil(most / 32)),
  * and its depth (d_depths may be NULL), 0 for a node without a parent: its
  * place in the text is the sequence's next one plus the depth. A parent that
- * is not below its node is reported and taken for none. */
+ * is not below its node is reported and taken for none. Masks and depths share
+ * no memory with starts, parents or one another. */
 int nut_draft_mask(const nut_draft *draft, int *d_depths, void *stream);
 
 /* Attention of every node over its sequence's rows and the nodes that its
@@ -450,7 +451,9 @@ int nut_paged_tree_attention(const nut_paged_kv *kv,
  * count is 0) the model's choice behind the last of them, with which the next
  * tree begins, and d_new_lengths [batch] (may be NULL; apart from d_lengths)
  * the lengths with the path's rows. A sequence whose rows and nodes pass
- * max_length is reported and keeps none. */
+ * max_length is reported and keeps none. What is written shares no memory with
+ * what is read or with one another (d_last may be d_tokens or d_chosen where
+ * `most` is 1). */
 int nut_draft_accept(const nut_draft *draft, const nut_paged_batch *seqs,
                      const int *d_tokens, const int *d_chosen, int *d_path,
                      size_t path_stride, int *d_counts, int *d_last,
@@ -509,7 +512,8 @@ typedef struct nut_page_table {
  * holds any more are free from the next call on. Entries of `to` behind d_held
  * stay.
  *
- * `to` shares no memory with `from`. A parent outside `from`, a sequence
+ * `to` and the copies share no memory with `from`, parents, gains or one
+ * another, nor the counts with any table. A parent outside `from`, a sequence
  * whose length its pages or `to` do not hold, is reported, and what goes on
  * with it is empty and holds nothing; a gain that is negative or too large is
  * reported and taken for 0. Sequences that hold more than their table's row
@@ -528,7 +532,7 @@ int nut_pages_reorder(const nut_page_pool *pool, const nut_page_table *from,
  * below it, for as many as there are of both, and `copies` at most. The table
  * and the counts follow, and d_copies [copies][3] gets the copies to be made
  * in every layer, whole pages, then {-1, -1, -1}. A page that something else
- * holds too stays. The workspace (16-byte aligned) needs
+ * holds too stays. Copies, counts and table share no memory. The workspace (16-byte aligned) needs
  * nut_pages_compact_workspace bytes. */
 size_t nut_pages_compact_workspace(const nut_page_pool *pool,
                                    const nut_page_table *table);
@@ -572,7 +576,8 @@ typedef struct nut_beams {
  * are [requests][to.beams]; a parent is numbered over all requests, as
  * nut_pages_reorder and nut_beam_gather take it. A beam that chooses `eos`
  * (-1: none) has ended, where the states keep that; both do or neither, and
- * likewise lengths. Exponentials are 32-bit, sums and ranks 64. The workspace
+ * likewise lengths. What is written shares no memory with `from`, the logits or
+ * one another. Exponentials are 32-bit, sums and ranks 64. The workspace
  * (16-byte aligned) needs nut_beam_select_workspace bytes. */
 size_t nut_beam_select_workspace(const nut_beams *from, const nut_beams *to,
                                  size_t vocab);
@@ -585,8 +590,9 @@ int nut_beam_select(const nut_beams *from, const nut_beams *to,
 /* State that goes with beams or sequences (texts, a nut_paged_history): row i
  * of `rows` rows at d_to + i to_stride gets the row_bytes bytes of the source
  * row d_parents[i], of `sources`, from d_from on (strides in bytes, 0:
- * row_bytes; all multiples of 4, rows apart). A row without a parent (-1)
- * stays; one outside [0, sources) is reported in d_status (may be NULL). */
+ * row_bytes; all multiples of 4, rows apart, from the parents too). A row
+ * without a parent (-1) stays; one outside [0, sources) is reported in
+ * d_status (may be NULL). */
 int nut_beam_gather(const void *d_from, size_t from_stride, size_t sources,
                     void *d_to, size_t to_stride, size_t rows,
                     size_t row_bytes, const int *d_parents, int *d_status,

@@ -102,27 +102,48 @@ nut::TableView table_of(const nut_page_table *t)
                           uint32_t(t->batch)};
 }
 
-// What a call writes of the new table shares no memory with what it reads.
-void check_apart(const nut::TableView &from, const nut::TableView &to, const int *parents,
-                 const int *gains, const int *copies)
+struct Range {
+    const void *p;
+    double bytes;
+};
+
+// Whether none of what a call writes shares memory with what it reads: workgroups
+// read while others write.
+template <size_t W, size_t R>
+bool apart_from(const Range (&written)[W], const Range (&read)[R])
 {
-    struct Range {
-        const void *p;
-        double bytes;
-    };
-    const double old = from.batch, now = to.batch;
-    const Range read[] = {{from.pages, old * from.stride * 4}, {from.lengths, old * 4},
-                          {from.held, old * 4}, {parents, now * 4}, {gains, now * 4}};
-    const Range written[] = {{to.pages, now * to.stride * 4}, {to.lengths, now * 4},
-                             {to.held, now * 4}, {copies, now * 12}};
     for (const Range &w : written)
         for (const Range &r : read)
-            require(disjoint(w.p, w.bytes, r.p, r.bytes), NUT_EINVAL,
-                    "page pool: the new table overlaps what is read");
+            if (!disjoint(w.p, w.bytes, r.p, r.bytes))
+                return false;
+    return true;
+}
+template <size_t W> bool apart_themselves(const Range (&written)[W])
+{
     for (const Range &w : written)
         for (const Range &x : written)
-            require(&w == &x || disjoint(w.p, w.bytes, x.p, x.bytes), NUT_EINVAL,
-                    "page pool: the new table overlaps itself");
+            if (&w != &x && !disjoint(w.p, w.bytes, x.p, x.bytes))
+                return false;
+    return true;
+}
+
+double entries_bytes(const nut::TableView &t) { return double(t.batch) * t.stride * 4; }
+
+void check_apart(const nut::PoolView &pool, const nut::TableView &from, const nut::TableView &to,
+                 const int *parents, const int *gains, const int *copies)
+{
+    const double old = from.batch, now = to.batch;
+    const Range table[] = {{from.pages, entries_bytes(from)}, {from.lengths, old * 4},
+                           {from.held, old * 4}, {parents, now * 4}};
+    const Range each[] = {{gains, now * 4}};
+    const Range written[] = {{to.pages, entries_bytes(to)}, {to.lengths, now * 4},
+                             {to.held, now * 4}, {copies, now * 12}};
+    require(apart_from(written, table) && apart_from(written, each), NUT_EINVAL,
+            "page pool: the new table overlaps what is read");
+    require(apart_themselves(written), NUT_EINVAL, "page pool: the new table overlaps itself");
+    const Range refs[] = {{pool.refs, double(pool.pages) * 4}};
+    require(apart_from(refs, table) && apart_from(refs, written), NUT_EINVAL,
+            "page pool: the counts overlap a table");
 }
 
 nut::BeamsView beams_of(const nut_beams *b)
@@ -254,7 +275,7 @@ int nut_pages_reorder(const nut_page_pool *pool, const nut_page_table *from,
         require(d_parents != nullptr && d_copies != nullptr, NUT_EINVAL,
                 "page pool: null pointer");
         require(gain <= kMost, NUT_EINVAL, "page pool: invalid gain");
-        check_apart(old, now, d_parents, d_gains, d_copies);
+        check_apart(p, old, now, d_parents, d_gains, d_copies);
         check_workspace(d_workspace, workspace_bytes, nut::reorder_workspace(p, old, now));
         nut::ensure_device();
         nut::launch_reorder(p, old, now, d_parents, d_gains, uint32_t(gain), d_copies,
@@ -277,6 +298,11 @@ int nut_pages_compact(const nut_page_pool *pool, const nut_page_table *table, si
         require(limit <= p.pages, NUT_EINVAL, "page pool: limit beyond the pages");
         require(d_copies != nullptr, NUT_EINVAL, "page pool: null pointer");
         require(copies != 0 && copies <= kMost / 3, NUT_EINVAL, "page pool: invalid copies");
+        const Range read[] = {{t.held, double(t.batch) * 4}};
+        const Range written[] = {{p.refs, double(p.pages) * 4}, {t.pages, entries_bytes(t)},
+                                 {d_copies, double(copies) * 12}};
+        require(apart_from(written, read) && apart_themselves(written), NUT_EINVAL,
+                "page pool: copies, counts and table overlap");
         check_workspace(d_workspace, workspace_bytes, nut::compact_workspace(p, t));
         nut::ensure_device();
         nut::launch_compact(p, t, uint32_t(limit), d_copies, uint32_t(copies),
@@ -331,12 +357,17 @@ int nut_beam_select(const nut_beams *from, const nut_beams *to, const void *d_lo
                 "beam search: no lengths to rank by");
         const double before = double(old.requests) * old.beams * 4;
         const double after = double(now.requests) * now.beams * 4;
-        const void *const read[] = {old.scores, old.lengths, old.ended};
-        const void *const written[] = {now.scores, now.lengths, now.ended, d_parents, d_tokens};
-        for (const void *w : written)
-            for (const void *r : read)
-                require(disjoint(w, after, r, before), NUT_EINVAL,
-                        "beam search: the new state overlaps the old one");
+        const Range read[] = {{old.scores, before}, {old.lengths, before}, {old.ended, before}};
+        const Range rows[] = {{d_logits, (double(row_stride) * (before / 4 - 1) + double(vocab)) *
+                                             double(nut::paged_element(type))}};
+        const Range written[] = {{now.scores, after}, {now.lengths, after}, {now.ended, after},
+                                 {d_parents, after}, {d_tokens, after}};
+        require(apart_from(written, read), NUT_EINVAL,
+                "beam search: the new state overlaps the old one");
+        require(apart_from(written, rows), NUT_EINVAL,
+                "beam search: the new state overlaps the logits");
+        require(apart_themselves(written), NUT_EINVAL,
+                "beam search: the new state overlaps itself");
         check_workspace(d_workspace, workspace_bytes,
                         nut::beam_workspace(old, now, uint32_t(vocab)));
         nut::ensure_device();
@@ -371,6 +402,9 @@ int nut_beam_gather(const void *d_from, size_t from_stride, size_t sources, void
         require(disjoint(d_to, double(to_stride) * double(rows - 1) + double(row_bytes), d_from,
                          double(from_stride) * double(sources - 1) + double(row_bytes)),
                 NUT_EINVAL, "beam gather: rows overlap");
+        require(disjoint(d_to, double(to_stride) * double(rows - 1) + double(row_bytes), d_parents,
+                         double(rows) * 4),
+                NUT_EINVAL, "beam gather: the rows overlap the parents");
         nut::ensure_device();
         nut::launch_beam_gather(static_cast<const char *>(d_from), from_stride, uint32_t(sources),
                                 static_cast<char *>(d_to), to_stride, uint32_t(rows), row_bytes,
