@@ -532,8 +532,8 @@ int nut_pages_reorder(const nut_page_pool *pool, const nut_page_table *from,
  * below it, for as many as there are of both, and `copies` at most. The table
  * and the counts follow, and d_copies [copies][3] gets the copies to be made
  * in every layer, whole pages, then {-1, -1, -1}. A page that something else
- * holds too stays. Copies, counts and table share no memory. The workspace (16-byte aligned) needs
- * nut_pages_compact_workspace bytes. */
+ * holds too stays. Copies, counts and table share no memory. The workspace
+ * (16-byte aligned) needs nut_pages_compact_workspace bytes. */
 size_t nut_pages_compact_workspace(const nut_page_pool *pool,
                                    const nut_page_table *table);
 int nut_pages_compact(const nut_page_pool *pool, const nut_page_table *table,

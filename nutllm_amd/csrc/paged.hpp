@@ -43,7 +43,7 @@ struct PagedHistory {
 // A grid of `workgroups` x `threads` holds at most 2^32 - 1 threads.
 inline dim3 paged_grid(uint64_t workgroups, uint32_t threads)
 {
-    require(workgroups * threads <= 0xffffffffull, NUT_EINVAL,
+    require(workgroups <= 0xffffffffull / threads, NUT_EINVAL, // their product may pass 64 bits
             "paged cache: more rows than one launch covers");
     return dim3(uint32_t(workgroups));
 }
