@@ -512,8 +512,8 @@ typedef struct nut_page_table {
  * holds any more are free from the next call on. Entries of `to` behind d_held
  * stay.
  *
- * `to` and the copies share no memory with `from`, parents, gains or one
- * another, nor the counts with any table. A parent outside `from`, a sequence
+ * `to` has fewer than 2^32 entries; it and the copies share no memory with
+ * `from`, parents, gains or one another, nor the counts with any table. A parent outside `from`, a sequence
  * whose length its pages or `to` do not hold, is reported, and what goes on
  * with it is empty and holds nothing; a gain that is negative or too large is
  * reported and taken for 0. Sequences that hold more than their table's row

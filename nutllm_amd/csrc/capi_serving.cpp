@@ -102,6 +102,15 @@ nut::TableView table_of(const nut_page_table *t)
                           uint32_t(t->batch)};
 }
 
+// Fresh pages are numbered over all entries of a new table, in 32 bits.
+nut::TableView new_table_of(const nut_page_table *t)
+{
+    const nut::TableView v = table_of(t);
+    require(double(v.batch) * v.stride <= double(0xffffffffu), NUT_EINVAL,
+            "page pool: invalid table");
+    return v;
+}
+
 struct Range {
     const void *p;
     double bytes;
@@ -261,7 +270,7 @@ size_t nut_pages_reorder_workspace(const nut_page_pool *pool, const nut_page_tab
                                    const nut_page_table *to)
 {
     return bytes_or_error(
-        [&]() { return nut::reorder_workspace(pool_of(pool), table_of(from), table_of(to)); });
+        [&]() { return nut::reorder_workspace(pool_of(pool), table_of(from), new_table_of(to)); });
 }
 
 int nut_pages_reorder(const nut_page_pool *pool, const nut_page_table *from,
@@ -271,7 +280,7 @@ int nut_pages_reorder(const nut_page_pool *pool, const nut_page_table *from,
 {
     return nut::guarded([&]() {
         const nut::PoolView p = pool_of(pool);
-        const nut::TableView old = table_of(from), now = table_of(to);
+        const nut::TableView old = table_of(from), now = new_table_of(to);
         require(d_parents != nullptr && d_copies != nullptr, NUT_EINVAL,
                 "page pool: null pointer");
         require(gain <= kMost, NUT_EINVAL, "page pool: invalid gain");

@@ -1,6 +1,7 @@
-"""Sizes whose products pass 64 bits: refused before anything is launched, on a host
-without a GPU."""
-from test_cpu_serving import paged, pytestmark, refused, seqs, tree  # noqa: F401
+"""Sizes whose products pass 64 bits, or ranks that pass 32: refused before anything is
+launched, on a host without a GPU."""
+from test_cpu_serving import (At, paged, pool, pytestmark, reaches, refused, reorder,  # noqa: F401
+                              seqs, table, tree)
 
 
 def test_tree_grids_beyond_64_bits():
@@ -11,3 +12,14 @@ def test_tree_grids_beyond_64_bits():
     kv = paged(kv_heads=1 << 26, head_dim=8)
     refused("more rows than one launch covers", kv.tree_attention_workspace,
             seqs(batch=1 << 30), tree(batch=1 << 30, most=1), 1 << 26)
+
+
+def test_tables_whose_entries_pass_32_bits():
+    """Fresh pages are numbered over all entries of the new table."""
+    base, wide = 1 << 40, 1 << 16
+    new = dict(stride=wide, lengths=At(1 << 28), held=At(1 << 29))
+    p = pool(pages=1000)
+    refused("invalid table", reorder, p, None, table(base, batch=wide, **new))
+    refused("invalid table", p.reorder_workspace, table(), table(base, batch=wide, **new))
+    reaches(reorder, p, None, table(base, batch=wide - 1, **new), copies=At(1 << 34))
+    reaches(reorder, p, table(base, batch=wide, **new), None)
