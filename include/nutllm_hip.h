@@ -513,12 +513,12 @@ typedef struct nut_page_table {
  * stay.
  *
  * `to` has fewer than 2^32 entries; it and the copies share no memory with
- * `from`, parents, gains or one another, nor the counts with any table. A parent outside `from`, a sequence
- * whose length its pages or `to` do not hold, is reported, and what goes on
- * with it is empty and holds nothing; a gain that is negative or too large is
- * reported and taken for 0. Sequences that hold more than their table's row
- * are reported and give nothing back. The workspace (16-byte aligned) needs
- * nut_pages_reorder_workspace bytes. */
+ * `from`, parents, gains or one another, nor the counts with any table. A
+ * parent outside `from`, a sequence whose length its pages or `to` do not hold,
+ * is reported, and what goes on with it is empty and holds nothing; a gain that
+ * is negative or too large is reported and taken for 0. Sequences that hold more
+ * than their table's row are reported and give nothing back. The workspace
+ * (16-byte aligned) needs nut_pages_reorder_workspace bytes. */
 size_t nut_pages_reorder_workspace(const nut_page_pool *pool,
                                    const nut_page_table *from,
                                    const nut_page_table *to);

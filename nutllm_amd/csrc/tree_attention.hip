@@ -36,8 +36,10 @@ struct TreeArgs {
     uint32_t teams;                    // of a query row, of the joins
     bool past;                         // rows go past the caches' replacement
     uint64_t *before; // [batch + 1]: stages before each sequence
-    float *parts;  // [total][heads][runs][head_dim], unnormalised
-    float2 *stats; // [total][heads][runs]: exponent they refer to, sum
+    // tree_kernel: [total][heads][runs], of every query row and run; staged_kernel:
+    // [2 shares][kBlock], of the query rows of the items that a share cuts
+    float *parts;  // [head_dim] each, unnormalised
+    float2 *stats; // exponent they refer to, sum
 };
 
 // Rows of the sequence and of its nodes together; 0, reported once, where the
@@ -1062,7 +1064,7 @@ __device__ __forceinline__ void write_joined(const TreeArgs &a, const Team &t, u
                                     : (own.most + log2f(own.sum)) * 0.69314718055994531f;
 }
 
-// The shares of an item joined, where it was cut: a.joined query rows a workgroup.
+// The shares of an item joined, where it was cut; a team takes every a.teams-th of them.
 template <int R>
 __global__ __launch_bounds__(256) void staged_join_kernel(TreeArgs a)
 {
@@ -1199,11 +1201,11 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
         // as many workgroups as the chip holds at once, by registers and shared memory
         plan.shares = 256 * staged_groups(kv.type, kv.head_dim);
         plan.blocks = uint32_t((queries + kBlock - 1) / kBlock);
-        // Rows that are read once, and are more than the caches hold: nothing of them is
-        // there when the next call comes.
-        plan.past = plan.blocks == 1 && uint64_t(seqs.max_length) * draft.batch * kv.kv_heads *
-                                                kv.head_dim * 2 * paged_element(kv.type) >=
-                                            (128ull << 20);
+        // 16-bit rows that are read once, and are more than the caches hold: nothing of
+        // them is there when the next call comes.
+        const uint64_t bytes = uint64_t(seqs.max_length) * draft.batch * kv.kv_heads *
+                               kv.head_dim * 2 * paged_element(kv.type);
+        plan.past = kv.type != NUT_F32 && plan.blocks == 1 && bytes >= (128ull << 20);
         // in the mean, where lengths differ
         plan.teams =
             teams_for(kv, plan.shares / (uint64_t(draft.batch) * kv.kv_heads * plan.blocks) + 1);
