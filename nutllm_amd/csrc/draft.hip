@@ -150,25 +150,29 @@ __global__ __launch_bounds__(kWave) void keep_kernel(PagedLayers layers, PagedSe
             to = paged_row(kv, s, b, index, n + k - index * kv.page_size, h);
         }
         const bool done = moves && from != kNoRow && to != kNoRow;
-        float key[8] = {};
-        uint4 value[TYPE == NUT_F32 ? 2 : 1];
+        constexpr int kPieces = TYPE == NUT_F32 ? 2 : 1;
+        uint4 key[kPieces] = {}, value[kPieces];
         if (done) {
-            load8<TYPE>(keys + from + part * 8 * kSize, key);
 #pragma unroll
-            for (int i = 0; i < (TYPE == NUT_F32 ? 2 : 1); i++)
+            for (int i = 0; i < kPieces; i++) {
+                key[i] = reinterpret_cast<const uint4 *>(keys + from + part * 8 * kSize)[i];
                 value[i] = reinterpret_cast<const uint4 *>(values + from + part * 8 * kSize)[i];
+            }
         }
         __syncthreads(); // every row is loaded before one is stored
         if (done) {
-            store8<TYPE>(keys + to + part * 8 * kSize, key);
 #pragma unroll
-            for (int i = 0; i < (TYPE == NUT_F32 ? 2 : 1); i++)
+            for (int i = 0; i < kPieces; i++) {
+                reinterpret_cast<uint4 *>(keys + to + part * 8 * kSize)[i] = key[i];
                 reinterpret_cast<uint4 *>(values + to + part * 8 * kSize)[i] = value[i];
+            }
         }
         if (kv.bounds != nullptr) {
+            float x[8];
+            load8<TYPE>(reinterpret_cast<const char *>(key), x);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                moved[threadIdx.x][i] = key[i];
+                moved[threadIdx.x][i] = x[i];
             if (group < groups && part == 0)
                 page_at[group] = done && source != index ? index : ~0u;
             __syncthreads();

@@ -67,3 +67,26 @@ def test_keep_in_many_layers(gpu, kind, count, kv, page, dim, order, bounds):
                     for e, f in ((0, np.minimum), (1, np.maximum)):
                         host[2][to, :, e] = encode(f(decode(host[2][to, :, e], kind), row), kind)
         assert all(same(a, b) for a, b in zip(got, host))
+
+
+@pytest.mark.parametrize("kind,bits", [("f32", 0x7f800001), ("f32", 0xffc12345), ("f16", 0x7c01),
+                                       ("f16", 0xfe55), ("bf16", 0x7f81), ("bf16", 0xffd5)])
+@pytest.mark.parametrize("bounds", [True, False])
+def test_keep_moves_bits(gpu, kind, bits, bounds):
+    """Keys that are no numbers arrive as they were; the bounds of their page say so."""
+    rng, pages, page = np.random.default_rng(3), 7, 4
+    layers, hosts, status = _layers(gpu, kind, 2, pages, 2, page, 16, "head", rng, bounds)
+    whole = np.uint32 if kind == "f32" else np.uint16
+    for (host, flat, *_), pool in zip(hosts, (0, 1)):  # keys of one layer, values of the other
+        host[pool].view(whole)[5, 1, 2, 3] = bits
+        flat[pool].upload(host[pool])
+    seqs = gpu.PagedBatch(dev([[2, 5, 1]]), 3, dev([3]), 1, 12)
+    gpu.PagedLayers(layers).keep(seqs, dev([[3]]), 1, dev([1]))  # row 6, on page 5, to 3, on 2
+    gpu.check_status(status)
+    for i, (host, got) in enumerate(_read(hosts, pages, 2, page, 16)):
+        for pool in host[:2]:
+            pool[2, :, 3] = pool[5, :, 2]
+        assert same(got[0], host[0]) and same(got[1], host[1])
+        if bounds:
+            none = np.isnan(decode(got[2], kind))
+            assert none.sum() == (2 if i == 0 else 0) and np.all(none[2, 1, :, 3]) == (i == 0)
