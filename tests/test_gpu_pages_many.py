@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from paged_case import decode, encode, same
-from serving_case import dev
+from serving_case import dev, space
 from test_gpu_pages import Twin, _layers, _read
 
 pytestmark = pytest.mark.gpu
@@ -38,6 +38,32 @@ def test_reorder_forks_one_of_many(gpu, parent):
     t.reorder([parent] * 2500, gain=1)
     assert t.host.refs.max() == 2500
     t.reorder([2499, -1], gain=2)
+
+
+@pytest.mark.parametrize("width,then", [(4, 9), (9, 4), (4, 1030)])
+def test_reorder_to_another_width(gpu, width, then):
+    """The new table's rows are longer, or shorter, than the old one's."""
+    rng = np.random.default_rng(width)
+    t = Twin(gpu, 4000, 4, 1, width)
+    t.reorder([-1] * 9, gains=rng.integers(0, 17, 9))
+    t.grow(rng.integers(0, t.host.held * 4 + 1))
+    h = t.host
+    parents, gains = np.array([3, 3, -1, 8, 0, 3]), np.array([0, 4, 16, 0, 3, 1])
+    gains = np.where(parents < 0, gains, np.minimum(gains, 16 - h.lengths[np.maximum(parents, 0)]))
+    if then > 1000:
+        gains[2] = 4100
+    old, h.width = t.now, then
+    more = np.full((h.batch, max(0, then - width)), -1)
+    h.table = np.concatenate([h.table, more], 1)[:, :max(then, width)]
+    d, new = h.place(np.full((6, then), -1), np.full(6, -9), np.full(6, -9))
+    copies = dev(np.full((6, 3), -9))
+    t.pool.reorder(old, new, dev(parents), copies, gains=dev(gains),
+                   workspace=space(t.pool.reorder_workspace(old, new)))
+    want, short = h.reorder(parents, gains)
+    assert not short and np.array_equal(copies.download(np.int32, 18).reshape(6, 3), want)
+    t.d = d
+    t.check()
+    gpu.check_status(h.status)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])

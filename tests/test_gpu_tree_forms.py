@@ -275,6 +275,29 @@ def test_keys_that_are_no_numbers(gpu, kind, bits, form, dim, heads, row):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dim,heads", [(64, 4), (80, 2), (128, 1), (256, 2), (8, 3)])
+def test_queries_that_are_not_finite(gpu, kind, form, dim, heads):
+    """A query that is no number, one that makes every score minus infinity, one that makes
+    them infinite: their nodes' results alone are none, nothing, and none."""
+    c = bare(kind, form, dim, heads)
+    keys = c.case.keys  # component 2 is below 0 in every key
+    keys[..., 2] = encode(-np.abs(decode(keys[..., 2], kind)) - 0.25, kind)
+    none, nothing, all_of_it = c.starts[0] + 7, c.starts[0] + 20, c.starts[1] + 3
+    out, want_lse, tol, tol_lse = c.expect()
+    c.query.view(np.uint32)[none, heads - 1, 5] = 0x7f800001
+    c.query[nothing, :, 2], c.query[all_of_it, :, 2] = np.inf, -np.inf
+    got, lse = ready(c, form).attention()
+    assert np.all(np.isnan(got[none, heads - 1])) and np.isnan(lse[none, heads - 1])
+    assert np.all(got[nothing] == 0) and np.all(np.isneginf(lse[nothing]))
+    assert np.all(np.isnan(got[all_of_it])) and not np.any(np.isfinite(lse[all_of_it]))
+    rest = np.ones((c.total, heads), bool)
+    rest[none, heads - 1] = rest[nothing] = rest[all_of_it] = False
+    assert np.all((np.abs(got - out) <= tol)[rest])
+    assert np.all((np.abs(lse - want_lse) <= tol_lse)[rest])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim,heads", [(64, 4), (80, 2), (128, 1), (256, 2), (8, 3)])
 @pytest.mark.parametrize("row", [5, 203])
 @pytest.mark.parametrize("what", ["inf", "-inf", "nan"])
 def test_values_that_are_not_finite(gpu, kind, form, dim, heads, row, what):
