@@ -259,7 +259,8 @@ __global__ __launch_bounds__(kWave) void scan_kernel(BeamArgs a)
 // logits spread, and each counts those before it. Where there are more (equal
 // logits), a beam's parts are merged first, one key after another, and then the
 // beams. Latency bounds both: 2 requests of 10 beams, 26,160 logits, 18 best 10 us where
-// merging alone took 32; 64 requests of 8 beams, 100,003 logits, 8 best 8.9 for 17.
+// merging alone took 32; 64 requests of 8 beams, 100,003 logits, 8 best 10.6 (8.6 at
+// least) for 17.
 struct Found {
     uint64_t rank, key;
     uint32_t beam;
@@ -451,9 +452,10 @@ uint32_t parts_of(uint32_t vocab, uint32_t each)
 
 // Logits a lane holds, 16 to 128: the fewest whose parts fit a wave, and their
 // lists its shared memory; 128 do for kMostVocab. 32 rather than 16 where that leaves
-// 8,192 waves: each finds its own largest, and lists them for the second launch (512
-// beams, 100,003 fp16 logits, on an earlier choose_kernel: 59 us of 32, 62 of 64, 121 of
-// 128).
+// 8,192 waves: each finds its own largest, and lists them for the second launch. Calls of
+// 16, 32, 64 and 128, us, fp16: 4 beams of 32,000 logits 14.4, 15.4, 18.6, 23.6, 128 of
+// them 17.2, 18.1, 20.7, 26.7, 512 of them 30.9, 29.9, 33.2, 47.1; 512 of 100,003 (32 at
+// least) 57, 72, 146.
 uint32_t each_of(uint32_t rows, uint32_t vocab, uint32_t keep)
 {
     uint32_t each = 16;

@@ -25,7 +25,7 @@ __device__ __forceinline__ int parent_of(const DraftView &d, uint32_t from, uint
 
 // A workgroup a sequence, a thread a node: it goes up the tree, which names the
 // mask's words from the last to the first, so that each is finished in a
-// register. Latency bounds it: 16 trees of 64 nodes 2.1 to 2.9 us, a launch.
+// register. Latency bounds it: 16 trees of 64 nodes 3.0 us (2.0 at least), a launch.
 __global__ void mask_kernel(DraftView d, int *depths)
 {
     __shared__ int16_t parents[kMostNodes];
@@ -57,7 +57,7 @@ __global__ void mask_kernel(DraftView d, int *depths)
 
 // A workgroup a sequence: every node that its parent's choice names puts itself
 // down as the one to go on with, the lowest staying; then one thread follows.
-// Latency bounds it: 16 trees of 64 nodes 2.7 us, a launch.
+// Latency bounds it: 16 trees of 64 nodes 3.0 us (2.7 at least), a launch.
 __global__ void accept_kernel(DraftView d, PagedSeqs s, const int *__restrict__ tokens,
                               const int *__restrict__ chosen, int *path, size_t path_stride,
                               int *counts, int *last, int *new_lengths)
@@ -101,8 +101,9 @@ __global__ void accept_kernel(DraftView d, PagedSeqs s, const int *__restrict__ 
 // before it stores them; as the path ascends, no later row was stored to. A row
 // stays where it is as long as the path is 0, 1, 2, .. Path, table and rows are read
 // one after another, which bounds it: 16 trees, 22 layers of 4 KV heads of 64 bfloat16
-// components 4.6 to 7.2 us; 32 trees, 32 layers of 32 heads of 128 fp16 ones, four waves
-// after another on a SIMD's place, 15 (four layers a wave were slower).
+// components 6.0 us (4.4 at least); 32 trees, 32 layers of 32 heads of 128 fp16 ones, four
+// waves after another on a SIMD's place, 21.5 (15.5 at least; four layers a wave were
+// slower).
 template <int TYPE>
 __global__ __launch_bounds__(kWave) void keep_kernel(PagedLayers layers, PagedSeqs s,
                                                      const int *__restrict__ path,

@@ -272,7 +272,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a)
 }
 
 // The new table's entries and copies: a wave a sequence. 128 sequences of up to 94 pages
-// 4.1 us, of which the table is a tenth: steps, entries and lists one after another.
+// 4.3 us (2.6 at least), of which the table is a tenth: steps, entries and lists one after another.
 __device__ __forceinline__ void fill_entries(const ReorderArgs &a, uint32_t i, uint32_t *sums)
 {
     const Step step = a.steps[i];
@@ -539,8 +539,11 @@ __global__ __launch_bounds__(kPlanThreads) void compact_kernel(CompactArgs a)
 // ------------------------------------------------------------------ copy --
 
 // A workgroup per copy, KV head and layer: 59 copies of up to 64 fp16 rows, 32 KV
-// heads of 128, 32 layers, 1.9 GB in 412 us (4.7 TB/s, what a large copy reaches).
-// Four layers a workgroup, with their loads in flight together, took 463 us.
+// heads of 128, 32 layers, 1.9 GB in 414 us (393 at least; 4.6 TB/s, near what a large
+// copy reaches). Four layers a workgroup, with their loads in flight together, took 463.
+// Of few rows the start of the workgroups bounds it: 128 entries, 25 of them copies of up
+// to 16 rows, 4 KV heads of 64 bfloat16 components, 22 layers 10.0 us for 2 of bytes, as
+// 9,064 of 11,264 workgroups read an entry without a copy.
 __global__ __launch_bounds__(256) void copy_kernel(PagedLayers layers,
                                                    const int *__restrict__ copies,
                                                    uint32_t pieces, uint32_t bound_pieces)

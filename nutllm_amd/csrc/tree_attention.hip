@@ -173,7 +173,7 @@ __device__ __forceinline__ void attend_tree(Tile<TYPE, HD> &tile, const size_t *
 
 // WQ of a workgroup's waves hold different query rows, and share their rows' offsets;
 // the others take tiles of rows in turn. Latency bounds it: 16 nodes of 32 heads of 64
-// over 211 fp32 rows take 6.7 us, two tiles a wave one after another.
+// over 211 fp32 rows take 7.4 us (6.0 at least), two tiles a wave one after another.
 template <int HD> constexpr int kTreeWaves = HD == 256 ? 2 : 4;
 
 template <int TYPE, int HD, bool FULL, int WQ>
@@ -576,7 +576,10 @@ attend_stage(const char *keys, const char *values, const size_t *at,
 }
 
 constexpr uint32_t kBlock = 64; // query rows of a workgroup
-constexpr uint32_t kLeast = 2;  // stages that a workgroup takes at least
+// Stages that a workgroup takes at least. One, two and four, us: 64 nodes of 32 heads of
+// 64 on 4 KV heads, one sequence of 1,000 bfloat16 rows 20.5, 22.0, 24.6, of fp32 ones
+// 23.7, 22.8, 24.7; 16 sequences of 100 29.6, 26.4, 28.1.
+constexpr uint32_t kLeast = 2;
 
 // How the work is shared out. An item is a block of a sequence's query rows and a
 // KV head, its work the stages of the sequence's rows; items follow one another
@@ -670,8 +673,8 @@ constexpr int staged_groups(int type, uint32_t head_dim)
 // us, a third of them the matrix instructions'; 32 of 4,096 149, 460 TFLOP/s of useful
 // products, three limbs each: between the products stand the softmax and the splitting
 // of its weights. 203 nodes of 24 heads of 80 on 3, fp32, 7 sequences of up to 5,001
-// rows: 207, half of it the rows' splitting into limbs. 32 heads of 128, fp16, 4
-// sequences of 24,000 to 32,768 rows: 390, 5.0 TB/s.
+// rows: 220, half of it the rows' splitting into limbs. 32 heads of 128, fp16, 4
+// sequences of 24,000 to 32,768 rows: 400, 4.9 TB/s.
 template <int TYPE, int HD, bool FULL>
 __global__ __launch_bounds__(256, staged_groups(TYPE, HD)) void staged_kernel(TreeArgs a)
 {
@@ -1193,7 +1196,14 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
     const uint64_t queries = uint64_t(draft.most) * (heads / kv.kv_heads);
     require(queries * kv.kv_heads <= 0x7fffffff, NUT_EINVAL,
             "paged cache: more rows than one launch covers");
-    // Workgroups that 16 query rows and 128 rows of a sequence make.
+    // Rows in shared memory pay for sharing out and joining; from 33 query rows a KV head
+    // on, where 16 of them and 128 rows of a sequence make more than 1,024 workgroups.
+    // tree_kernel and staged_kernel, us, 32 heads of 64 on 4 KV heads. 64 nodes: 16
+    // sequences of 2,000 bfloat16 rows 83 and 57, of 1,000 48 and 43, fp32 146 and 86, 81
+    // and 56; below the bound one of 700 13.8 and 19.0, fp32 16.6 and 20.8. Just above it
+    // 16-bit rows lose: 16 of 500 31 and 34, of 100 17 and 26. 8 nodes: 64 of 8,000 222
+    // and 135, of 1,000 32 and 34, of 200 13 and 21. 4 nodes, 32 query rows: 16 of 4,000
+    // to 8,192 38.6 and 41, though 64 of them 128 and 99.
     const uint64_t small = uint64_t(draft.batch) * kv.kv_heads * ((queries + 15) / 16) *
                            ((seqs.max_length + 127) / 128);
     plan.staged = queries > 32 && small > 1024;
@@ -1202,7 +1212,9 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
         plan.shares = 256 * staged_groups(kv.type, kv.head_dim);
         plan.blocks = uint32_t((queries + kBlock - 1) / kBlock);
         // 16-bit rows that are read once, and are more than the caches hold: nothing of
-        // them is there when the next call comes.
+        // them is there when the next call comes. Through the caches and past them, us,
+        // 64 nodes of 32 fp16 heads of 128: 32 MiB 34 and 36, 64 44 and 45, 128 59 and 57,
+        // 512 150 and 143, 2,044 459 and 444.
         const uint64_t bytes = uint64_t(seqs.max_length) * draft.batch * kv.kv_heads *
                                kv.head_dim * 2 * paged_element(kv.type);
         plan.past = kv.type != NUT_F32 && plan.blocks == 1 && bytes >= (128ull << 20);
@@ -1216,6 +1228,10 @@ TreePlan plan_tree(const PagedView &kv, const PagedSeqs &seqs, const DraftView &
         plan.bytes = plan.before + aligned((size_t(draft.batch) + 1) * sizeof(uint64_t));
         return plan;
     }
+    // Two tiles of query rows read a sequence once for both. One and two, us: 27 nodes of
+    // 32 fp16 heads of 128, 32 sequences of 10 to 64 rows 36 and 24, 4 of 8,000 to 16,000
+    // 234 and 193, though 16 of 500 to 2,048 99 and 104; 4 nodes of 8 heads of 64 a KV
+    // head, 16 of 4,000 to 8,192 bfloat16 rows 44 and 39, of 100 to 512 13.3 and 14.3.
     plan.waves = queries > 16 && small > 1024 ? 2 : 1;
     plan.blocks = uint32_t((queries + 16 * plan.waves - 1) / (16 * plan.waves));
     const uint64_t columns = uint64_t(draft.batch) * kv.kv_heads * plan.blocks;
