@@ -387,11 +387,15 @@ __device__ __forceinline__ void stage_dma(const void *source, const void *to)
 // Whether a component of an fp32 row is no number, whatever its bits.
 __device__ __forceinline__ bool no_number(const char *row, uint32_t head_dim)
 {
-    const float *x = reinterpret_cast<const float *>(row);
     bool found = false;
 #pragma unroll 1
-    for (uint32_t d = 0; d < head_dim; d++)
-        found = found || x[d] != x[d];
+    for (uint32_t d = 0; d < head_dim; d += 8) {
+        float x[8];
+        load8<NUT_F32>(row + d * 4, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            found = found || x[e] != x[e];
+    }
     return found;
 }
 
@@ -475,7 +479,14 @@ attend_stage(const char *keys, const char *values, const size_t *at,
         // An infinite key: the first limbs' product has the sum's sign, later ones
         // of zero, or of the other sign, make it no number. (So do sums of both
         // infinities, which are none in the end either.) A NaN may look infinite in
-        // its upper limb: fp32 keys are read again.
+        // its upper limb: fp32 keys are read again, a lane a row.
+        uint32_t none = 0; // rows of the lane whose keys are no numbers
+        if constexpr (TYPE == NUT_F32) {
+            static_assert(S::kRows == 32, "a bit a row");
+            const size_t row = at[lane % 32];
+            const bool is = row != kNoRow && no_number(kv.keys + row, kv.head_dim);
+            none = uint32_t(__ballot(is)) >> (4 * j);
+        }
 #pragma unroll
         for (int sub = 0; sub < kSubs; sub++) {
             f32x4 first{0, 0, 0, 0};
@@ -484,14 +495,8 @@ attend_stage(const char *keys, const char *values, const size_t *at,
                 first = product<kType>(key(0, sub, n), q.x[n][0], first);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (acc[sub][i] == acc[sub][i])
-                    continue;
-                acc[sub][i] = first[i];
-                if constexpr (TYPE == NUT_F32) {
-                    const size_t row = at[16 * sub + 4 * j + i];
-                    if (row != kNoRow && no_number(kv.keys + row, kv.head_dim))
-                        acc[sub][i] = __builtin_nanf("");
-                }
+                const float x = none >> (16 * sub + i) & 1 ? __builtin_nanf("") : first[i];
+                acc[sub][i] = acc[sub][i] != acc[sub][i] ? x : acc[sub][i];
             }
         }
     }
