@@ -453,7 +453,7 @@ int nut_paged_tree_attention(const nut_paged_kv *kv,
  * the lengths with the path's rows. A sequence whose rows and nodes pass
  * max_length is reported and keeps none. What is written shares no memory with
  * what is read or with one another (d_last may be d_tokens or d_chosen where
- * `most` is 1). */
+ * `most` is 1 and d_starts NULL). */
 int nut_draft_accept(const nut_draft *draft, const nut_paged_batch *seqs,
                      const int *d_tokens, const int *d_chosen, int *d_path,
                      size_t path_stride, int *d_counts, int *d_last,
